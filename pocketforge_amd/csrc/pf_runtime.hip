@@ -20,71 +20,11 @@
 #include <vector>
 
 #include "../../include/pf_gpu.h"
+#include "pf_context.h"
 
 using namespace pf;
 
 // ================================================================ context
-
-struct pf_ctx {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    std::string err;
-    size_t bytes = 0;
-    // growable scratch for the kernel-level entry points
-    void* scratch = nullptr;
-    size_t scratch_bytes = 0;
-};
-
-static pf_status fail(const pf_ctx* c, pf_status s, const std::string& msg) {
-    if (c) const_cast<pf_ctx*>(c)->err = msg;
-    return s;
-}
-
-#define PF_HIP(ctx, call)                                                                        \
-    do {                                                                                         \
-        hipError_t e_ = (call);                                                                  \
-        if (e_ != hipSuccess)                                                                    \
-            return fail(ctx, PF_ERR_HIP, std::string(#call) + " failed: " + hipGetErrorString(e_)); \
-    } while (0)
-
-#define PF_LAUNCHED(ctx) PF_HIP(ctx, hipGetLastError())
-
-static pf_status dalloc(pf_ctx* c, void** p, size_t bytes) {
-    *p = nullptr;
-    if (bytes == 0) bytes = 256;
-    hipError_t e = hipMalloc(p, bytes);
-    if (e != hipSuccess) return fail(c, PF_ERR_HIP, "hipMalloc(" + std::to_string(bytes) + ") failed: " + hipGetErrorString(e));
-    c->bytes += bytes;
-    return PF_OK;
-}
-
-static void dfree(pf_ctx* c, void* p, size_t bytes) {
-    if (!p) return;
-    (void)hipFree(p);
-    if (bytes == 0) bytes = 256;
-    c->bytes -= std::min(c->bytes, bytes);
-}
-
-template <class T>
-static pf_status dalloc_t(pf_ctx* c, T** p, size_t n) {
-    return dalloc(c, reinterpret_cast<void**>(p), n * sizeof(T));
-}
-
-static pf_status ctx_scratch(pf_ctx* c, size_t bytes, void** out) {
-    if (bytes > c->scratch_bytes) {
-        if (c->scratch) {
-            PF_HIP(c, hipStreamSynchronize(c->stream));
-            dfree(c, c->scratch, c->scratch_bytes);
-            c->scratch = nullptr;
-            c->scratch_bytes = 0;
-        }
-        pf_status s = dalloc(c, &c->scratch, bytes);
-        if (s) return s;
-        c->scratch_bytes = bytes;
-    }
-    *out = c->scratch;
-    return PF_OK;
-}
 
 static std::string g_init_error;
 
