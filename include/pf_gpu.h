@@ -174,6 +174,111 @@ uint32_t pf_kv_size(const pf_kv* kv);
 pf_status pf_kv_clear(pf_kv* kv);
 size_t pf_kv_memory_usage(const pf_kv* kv);
 
+/* -------------------------------------------- attention over prompts
+ * (new) The reference attends inside Engine::forward, one token at a time
+ * over its own int8 cache (src/engine.cpp:646-799); these entry points
+ * attend over rows that the caller holds, and over a paged cache that many
+ * sequences share, for schedulers that run their own passes. */
+#define PF_TYPE_F32 0
+#define PF_TYPE_F16 1
+#define PF_TYPE_BF16 2
+#define PF_TYPE_I8 3           /* cache pages: int8 codes and an fp32 scale per row */
+
+typedef struct {
+    int32_t type;              /* PF_TYPE_F32, F16 or BF16: q, k, v and out */
+    uint32_t n_heads, n_kv_heads;   /* query head h reads kv head h / (n_heads / n_kv_heads) */
+    uint32_t head_dim;         /* a multiple of 16, 16 .. 128 */
+    int32_t causal;            /* 1: a query sees keys up to its own position */
+    uint32_t window, sink;     /* window > 0: of the keys up to its own position a query sees the last
+                                  `window` and the first `sink` */
+    float scale;               /* of the scores; 0: 1 / sqrt(head_dim); not negative */
+    uint32_t q_stride, k_stride, v_stride, o_stride;   /* elements from one token's heads to the next
+                                  token's; 0: heads * head_dim */
+} pf_attn_desc;
+
+/* Softmax attention of packed sequences: q and out [sum q_lens][n_heads]
+ * [head_dim], k and v [sum k_lens][n_kv_heads][head_dim].  The queries are
+ * the last q_lens[s] positions of sequence s (query i is at position
+ * k_lens[s] - q_lens[s] + i); k_lens NULL: the same as q_lens.  A query that
+ * sees no key gets zeros.  Lengths are host arrays and may be 0; q_lens may
+ * exceed k_lens.  Buffers and strides are multiples of 16 bytes; out may not
+ * overlap the inputs.  Sums are fp32 whatever the type; fp32 rows (values
+ * below 3.38e38) are multiplied to fp32 accuracy.  An infinity or a NaN in k or v reaches the
+ * queries that see it and no others (fp32 rows: as a NaN).  Asynchronous on
+ * the context's stream; allocates nothing. */
+pf_status pf_prompt_attention(pf_ctx* ctx, const pf_attn_desc* desc, const void* q_dev, const void* k_dev,
+                              const void* v_dev, void* out_dev, const uint32_t* q_lens, const uint32_t* k_lens,
+                              uint32_t n_seq);
+
+/* ----------------------------------------------------- paged KV cache
+ * (new) No counterpart in the reference, whose KVCache holds one sequence
+ * (include/forge/kv_cache.hpp:33-56).  A pool of pages of page_size rows,
+ * and max_seqs sequences (slots 0 .. max_seqs - 1, empty at first) whose
+ * rows lie in pages that may be shared: forked sequences share their pages
+ * until one of them grows into a shared one, which it then copies.  A page
+ * holds the rows of every layer and kv head.  Pages are handed out lowest
+ * number first.  Page tables live on the device and follow the calls in
+ * stream order; no call synchronizes, and only create, destroy and
+ * pf_pages_attention's first call of a larger size (the context's scratch)
+ * allocate.  Every call checks its arguments before it changes anything. */
+typedef struct pf_pages pf_pages;
+typedef struct {
+    int32_t type;              /* PF_TYPE_F16, BF16 or I8 */
+    uint32_t n_layers, n_kv_heads, head_dim;   /* head_dim: a multiple of 16, 16 .. 128 */
+    uint32_t page_size;        /* rows of a page: 16, 32, 64, 128 or 256 */
+    uint32_t n_pages, max_seqs;
+    uint32_t max_context;      /* rows of one sequence at most */
+} pf_pages_config;
+
+pf_status pf_pages_create(pf_ctx* ctx, const pf_pages_config* cfg, pf_pages** out);
+void pf_pages_destroy(pf_pages* p);
+size_t pf_pages_memory_usage(const pf_pages* p);
+uint32_t pf_pages_free_count(const pf_pages* p);
+/* Rows of a sequence (0 for a slot out of range). */
+uint32_t pf_pages_length(const pf_pages* p, uint32_t seq);
+/* Page numbers of n sequences: pages[i * cap ..], -1 past the last, and
+ * their lengths (either may be NULL).  PF_ERR_CAPACITY if one has more. */
+pf_status pf_pages_tables(const pf_pages* p, const uint32_t* seqs, uint32_t n, int64_t* pages, uint32_t cap,
+                          int64_t* lengths);
+/* Device addresses of the pool: k and v [n_layers][n_pages][n_kv_heads]
+ * [page_size][head_dim] of the cache's type; ks, vs the row scales
+ * [n_layers][n_pages][n_kv_heads][page_size] of PF_TYPE_I8, else NULL. */
+pf_status pf_pages_planes(const pf_pages* p, void** k_dev, void** v_dev, float** ks_dev, float** vs_dev);
+/* Begins a pass: sequence seqs[i] (distinct) grows by rows[i] rows (0 is
+ * allowed).  pf_pages_store and pf_pages_attention then work on these rows,
+ * packed in this order, until the next append; the calls below end the pass.
+ * PF_ERR_CAPACITY, with nothing changed, if a sequence would exceed
+ * max_context or the pool has too few free pages. */
+pf_status pf_pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t* rows, uint32_t n);
+/* Writes the pass's key and value rows of one layer: [sum rows][n_kv_heads]
+ * [head_dim] of `type` (F32, F16 or BF16), rounded to the cache's type, or
+ * quantized by KVCache::quantize_row (a row with an infinity or a NaN reads
+ * back as NaN).  Strides as in pf_attn_desc; buffers of 16 bytes. */
+pf_status pf_pages_store(pf_pages* p, uint32_t layer, int32_t type, const void* k_dev, const void* v_dev,
+                         uint32_t k_stride, uint32_t v_stride);
+/* Attention of the pass's rows over their sequences' rows in one layer (store
+ * them first): q and out [sum rows][n_heads][head_dim] of desc->type.  A
+ * 16-bit cache takes rows of its own type, a bf16 or int8 cache fp32 rows
+ * too, an int8 cache all three.  The k and v strides are not used. */
+pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* desc, uint32_t layer, const void* q_dev, void* out_dev);
+/* Reads n sequences' rows of one layer back, packed in this order, as `type`
+ * (F32, F16 or BF16): with pf_prompt_attention, a long pass over a cached
+ * prefix. */
+pf_status pf_pages_gather(pf_pages* p, uint32_t layer, const uint32_t* seqs, uint32_t n, int32_t type, void* k_dev,
+                          void* v_dev, uint32_t k_stride, uint32_t v_stride);
+/* The n empty sequences dst share src's pages. */
+pf_status pf_pages_fork(pf_pages* p, uint32_t src, const uint32_t* dst, uint32_t n);
+/* The n empty sequences dst[i] get copies of src[i]'s pages (whole pages). */
+pf_status pf_pages_copy(pf_pages* p, const uint32_t* src, const uint32_t* dst, uint32_t n);
+/* Shortens n distinct sequences to lengths[i] rows (rejected drafts); pages
+ * that no sequence uses any more are free. */
+pf_status pf_pages_truncate(pf_pages* p, const uint32_t* seqs, const uint32_t* lengths, uint32_t n);
+/* Empties n distinct sequences. */
+pf_status pf_pages_free(pf_pages* p, const uint32_t* seqs, uint32_t n);
+/* Moves used pages so that they are numbers 0 .. used - 1; *moved (may be
+ * NULL) is how many moved. */
+pf_status pf_pages_compact(pf_pages* p, uint32_t* moved);
+
 /* --------------------------------------------------------------- model */
 typedef struct {
     uint32_t n_layers, n_embd, n_heads, head_dim, n_ff, n_vocab, n_mtp;

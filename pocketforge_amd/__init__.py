@@ -20,6 +20,7 @@ FMT_Q4, FMT_Q2, FMT_Q15, FMT_Q8 = 0, 1, 2, 3
 def block_bytes(fmt):
     """Code bytes of one 32-element block in the interchange layout."""
     return {FMT_Q4: 16, FMT_Q8: 32}.get(fmt, 8)
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
 MAT_Q, MAT_K, MAT_V, MAT_O, MAT_GATE, MAT_UP, MAT_DOWN = range(7)
 
 f32p = C.POINTER(C.c_float)
@@ -61,6 +62,18 @@ class SqueezeInfo(C.Structure):
 
 class CacheDesc(C.Structure):
     _fields_ = [(n, C.c_uint32) for n in ("sink_size", "window_size", "pool_block", "max_context")]
+
+
+class AttnDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_heads", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("causal", C.c_int32), ("window", C.c_uint32), ("sink", C.c_uint32), ("scale", C.c_float),
+                ("q_stride", C.c_uint32), ("k_stride", C.c_uint32), ("v_stride", C.c_uint32),
+                ("o_stride", C.c_uint32)]
+
+
+class PagesConfig(C.Structure):
+    _fields_ = [("type", C.c_int32)] + [(n, C.c_uint32) for n in (
+        "n_layers", "n_kv_heads", "head_dim", "page_size", "n_pages", "max_seqs", "max_context")]
 
 
 # Symbol table: name -> (restype, argtypes).  Every entry point of
@@ -142,6 +155,23 @@ SYMBOLS = {
     "pf_engine_attn_stats": (C.c_int32, [vp, u32p, C.POINTER(C.c_double)]),
     "pf_engine_gemv_by_size": (C.c_int32, [vp, C.c_uint32, C.POINTER(C.c_double), u32p, C.POINTER(C.c_double),
                                            u32p]),
+    "pf_prompt_attention": (C.c_int32, [vp, C.POINTER(AttnDesc), vp, vp, vp, vp, vp, vp, C.c_uint32]),
+    "pf_pages_create": (C.c_int32, [vp, C.POINTER(PagesConfig), C.POINTER(vp)]),
+    "pf_pages_destroy": (None, [vp]),
+    "pf_pages_memory_usage": (C.c_size_t, [vp]),
+    "pf_pages_free_count": (C.c_uint32, [vp]),
+    "pf_pages_length": (C.c_uint32, [vp, C.c_uint32]),
+    "pf_pages_tables": (C.c_int32, [vp, vp, C.c_uint32, vp, C.c_uint32, vp]),
+    "pf_pages_planes": (C.c_int32, [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]),
+    "pf_pages_append": (C.c_int32, [vp, vp, vp, C.c_uint32]),
+    "pf_pages_store": (C.c_int32, [vp, C.c_uint32, C.c_int32, vp, vp, C.c_uint32, C.c_uint32]),
+    "pf_pages_attention": (C.c_int32, [vp, C.POINTER(AttnDesc), C.c_uint32, vp, vp]),
+    "pf_pages_gather": (C.c_int32, [vp, C.c_uint32, vp, C.c_uint32, C.c_int32, vp, vp, C.c_uint32, C.c_uint32]),
+    "pf_pages_fork": (C.c_int32, [vp, C.c_uint32, vp, C.c_uint32]),
+    "pf_pages_copy": (C.c_int32, [vp, vp, vp, C.c_uint32]),
+    "pf_pages_truncate": (C.c_int32, [vp, vp, vp, C.c_uint32]),
+    "pf_pages_free": (C.c_int32, [vp, vp, C.c_uint32]),
+    "pf_pages_compact": (C.c_int32, [vp, u32p]),
     "pf_batch_create": (C.c_int32, [vp, C.POINTER(CacheDesc), C.c_uint32, C.POINTER(vp)]),
     "pf_batch_sequences": (C.c_uint32, [vp]),
     "pf_batch_position": (C.c_uint32, [vp, C.c_uint32]),
@@ -221,6 +251,53 @@ class DeviceArray:
             self.free()
         except Exception:
             pass
+
+
+_NUMPY = {TYPE_F32: np.float32, TYPE_F16: np.float16, TYPE_BF16: np.uint16}
+_TYPES = {"float32": TYPE_F32, "float16": TYPE_F16, "bfloat16": TYPE_BF16, "uint16": TYPE_BF16}
+
+
+def _type(t):
+    """Element type of a device array: its dtype, with uint16 for bf16 bits (numpy has no bf16)."""
+    name = str(t.dtype).replace("torch.", "")
+    if name not in _TYPES:
+        raise PFError(f"rows are float32, float16 or bfloat16, not {name}")
+    return _TYPES[name]
+
+
+def _rows(t, what):
+    """(rows, heads, head_dim, elements from one row to the next) of a
+    [rows][heads][head_dim] device array; a torch tensor may be a view whose
+    rows lie apart, as the parts of a fused QKV product do."""
+    if len(t.shape) != 3:
+        raise PFError(f"{what} is [rows][heads][head_dim], not {tuple(t.shape)}")
+    n, h, d = (int(x) for x in t.shape)
+    if isinstance(t, DeviceArray):
+        return n, h, d, h * d
+    s = t.stride()
+    if (d > 1 and s[2] != 1) or (h > 1 and s[1] != d):
+        raise PFError(f"{what}: the heads of a row lie one after another")
+    return n, h, d, (s[0] if n > 1 else h * d)
+
+
+def _u32(a, what):
+    a = np.atleast_1d(np.asarray(a))
+    if a.size and (a.dtype.kind not in "iu" or a.ndim != 1 or a.min() < 0 or a.max() > 0xFFFFFFFF):
+        raise PFError(f"{what} is a list of numbers from 0")
+    return np.ascontiguousarray(a, np.uint32)
+
+
+def _vptr(a):
+    return C.c_void_p(a.ctypes.data)
+
+
+class DevicePlane:
+    """A view of device memory that a PagedCache owns, for libraries that
+    take __cuda_array_interface__ (torch.as_tensor); 16-bit values as int16."""
+
+    def __init__(self, ptr, shape, kind, owner):
+        self.owner = owner
+        self.__cuda_array_interface__ = dict(shape=shape, typestr=kind, data=(ptr, False), version=3, strides=None)
 
 
 # ----------------------------------------------------- host-side weights
@@ -353,6 +430,31 @@ class Context:
         self.synchronize()
         return y
 
+    def prompt_attention(self, q, k, v, q_lens, k_lens=None, causal=True, window=0, sink=0, scale=0.0, out=None):
+        """Attention over packed sequences: q [sum q_lens][heads][head_dim],
+        k and v [sum k_lens][kv heads][head_dim], the queries the last
+        q_lens[s] positions of each sequence.  With `out` the call is
+        asynchronous on the context's stream; without, a new array is
+        returned when it is done."""
+        ql = _u32(q_lens, "q_lens")
+        kl = ql if k_lens is None else _u32(k_lens, "k_lens")
+        nq, H, D, qs = _rows(q, "q")
+        nk, G, _, ks = _rows(k, "k")
+        vs = _rows(v, "v")[3]
+        if tuple(k.shape) != tuple(v.shape) or int(k.shape[2]) != D:
+            raise PFError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are alike, with q's head_dim {D}")
+        if len(kl) != len(ql) or int(ql.sum(dtype=np.int64)) != nq or int(kl.sum(dtype=np.int64)) != nk:
+            raise PFError("q_lens and k_lens name every row of q and of k")
+        y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[_type(q)]) if out is None else out
+        if tuple(y.shape) != (nq, H, D) or len({_type(t) for t in (q, k, v, y)}) != 1:
+            raise PFError("q, k, v and out have one type, q and out one shape")
+        d = AttnDesc(_type(q), H, G, D, int(causal), window, sink, scale, qs, ks, vs, _rows(y, "out")[3])
+        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), _vptr(ql),
+                                             _vptr(kl), len(ql)), "pf_prompt_attention")
+        if out is None:
+            self.synchronize()
+        return y
+
     def gemv_f32(self, W, x):
         M = x.shape[0]
         y = self.empty((M, W.rows), np.float32)
@@ -465,6 +567,146 @@ class KVCache:
     def close(self):
         if self.h:
             lib().pf_kv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+
+class PagedCache:
+    """A pool of key / value pages that many sequences share (pf_pages_*):
+    append() begins a pass of new rows, store() and attention() work on them
+    layer by layer, fork / copy / truncate / free / compact manage the pages.
+    Rows are device arrays [rows][heads][head_dim]."""
+
+    def __init__(self, ctx, n_layers, n_kv_heads, head_dim, n_pages, max_seqs, max_context, page_size=64,
+                 type=TYPE_BF16):
+        self.ctx = ctx
+        self.h = None
+        self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
+        self.page_size, self.n_pages, self.max_seqs, self.type = page_size, n_pages, max_seqs, type
+        self.pass_rows = 0
+        cfg = PagesConfig(type, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_context)
+        h = vp()
+        ctx.check(lib().pf_pages_create(ctx.h, C.byref(cfg), C.byref(h)), "pf_pages_create")
+        self.h = h
+
+    def append(self, seqs, rows):
+        """Begins a pass: sequence seqs[i] grows by rows[i] rows."""
+        s, r = _u32(seqs, "seqs"), _u32(rows, "rows")
+        if len(s) != len(r):
+            raise PFError("seqs and rows have one length")
+        self.ctx.check(lib().pf_pages_append(self.h, _vptr(s), _vptr(r), len(s)), "pf_pages_append")
+        self.pass_rows = int(r.sum(dtype=np.int64))
+
+    def _kv(self, k, v, rows):
+        n, h, d, ks = _rows(k, "k")
+        vs = _rows(v, "v")[3]
+        if tuple(k.shape) != tuple(v.shape) or (n, h, d) != (rows, self.n_kv_heads, self.head_dim):
+            raise PFError(f"k and v are [{rows}][{self.n_kv_heads}][{self.head_dim}], not {tuple(k.shape)}, {tuple(v.shape)}")
+        if _type(k) != _type(v):
+            raise PFError("k and v have one type")
+        return _type(k), ks, vs
+
+    def store(self, layer, k, v):
+        """The pass's new rows of one layer."""
+        t, ks, vs = self._kv(k, v, self.pass_rows)
+        self.ctx.check(lib().pf_pages_store(self.h, layer, t, _dptr(k), _dptr(v), ks, vs), "pf_pages_store")
+
+    def attention(self, layer, q, causal=True, window=0, sink=0, scale=0.0, out=None):
+        """The pass's rows over their sequences.  With `out` asynchronous, as Context.prompt_attention."""
+        n, H, D, qs = _rows(q, "q")
+        y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[_type(q)]) if out is None else out
+        if n != self.pass_rows or tuple(y.shape) != (n, H, D) or _type(y) != _type(q):
+            raise PFError(f"q and out are [{self.pass_rows}][heads][{self.head_dim}] of one type")
+        d = AttnDesc(_type(q), H, self.n_kv_heads, D, int(causal), window, sink, scale, qs, 0, 0, _rows(y, "out")[3])
+        self.ctx.check(lib().pf_pages_attention(self.h, C.byref(d), layer, _dptr(q), _dptr(y)), "pf_pages_attention")
+        if out is None:
+            self.ctx.synchronize()
+        return y
+
+    def gather(self, layer, seqs, out=None, dtype=np.float32):
+        """The sequences' rows of one layer, packed: (k, v)."""
+        s = _u32(seqs, "seqs")
+        n = sum(self.length(i) for i in s)
+        if out is None:
+            k, v = (self.ctx.empty((n, self.n_kv_heads, self.head_dim), dtype) for _ in range(2))
+        else:
+            k, v = out
+        t, ks, vs = self._kv(k, v, n)
+        self.ctx.check(lib().pf_pages_gather(self.h, layer, _vptr(s), len(s), t, _dptr(k), _dptr(v), ks, vs),
+                       "pf_pages_gather")
+        if out is None:
+            self.ctx.synchronize()
+        return k, v
+
+    def fork(self, src, dst):
+        d = _u32(dst, "dst")
+        self.ctx.check(lib().pf_pages_fork(self.h, src, _vptr(d), len(d)), "pf_pages_fork")
+
+    def copy(self, src, dst):
+        s, d = _u32(src, "src"), _u32(dst, "dst")
+        if len(s) != len(d):
+            raise PFError("src and dst have one length")
+        self.ctx.check(lib().pf_pages_copy(self.h, _vptr(s), _vptr(d), len(d)), "pf_pages_copy")
+
+    def truncate(self, seqs, lengths):
+        s, n = _u32(seqs, "seqs"), _u32(lengths, "lengths")
+        if len(s) != len(n):
+            raise PFError("seqs and lengths have one length")
+        self.ctx.check(lib().pf_pages_truncate(self.h, _vptr(s), _vptr(n), len(s)), "pf_pages_truncate")
+
+    def free(self, seqs):
+        s = _u32(seqs, "seqs")
+        self.ctx.check(lib().pf_pages_free(self.h, _vptr(s), len(s)), "pf_pages_free")
+
+    def compact(self):
+        """The number of pages that moved."""
+        n = C.c_uint32(0)
+        self.ctx.check(lib().pf_pages_compact(self.h, C.byref(n)), "pf_pages_compact")
+        return n.value
+
+    def length(self, seq):
+        return lib().pf_pages_length(self.h, int(seq))
+
+    def tables(self, seqs):
+        """Page numbers of the sequences, -1 past their ends, and their lengths."""
+        s = _u32(seqs, "seqs")
+        lens = np.zeros(len(s), np.int64)
+        self.ctx.check(lib().pf_pages_tables(self.h, _vptr(s), len(s), None, 0, _vptr(lens)), "pf_pages_tables")
+        cap = -(-int(lens.max(initial=0)) // self.page_size)
+        pages = np.empty((len(s), cap), np.int64)
+        self.ctx.check(lib().pf_pages_tables(self.h, _vptr(s), len(s), _vptr(pages), cap, None), "pf_pages_tables")
+        return pages, lens
+
+    def planes(self, layer=None):
+        """The pool in device memory: k and v [layers][pages][kv heads][page
+        size][head_dim] and, for int8, their row scales [layers][pages][kv
+        heads][page size][1]; of one layer, without the first dimension."""
+        p = [vp() for _ in range(4)]
+        self.ctx.check(lib().pf_pages_planes(self.h, C.byref(p[0]), C.byref(p[1]), C.byref(p[2]), C.byref(p[3])),
+                       "pf_pages_planes")
+        rows = (self.n_pages, self.n_kv_heads, self.page_size)
+        out = []
+        for i, (ptr, last, size, kind) in enumerate(zip(p, 2 * [self.head_dim] + 2 * [1], 2 * [1 if self.type == TYPE_I8 else 2] + [4, 4],
+                                                        2 * ["|i1" if self.type == TYPE_I8 else "<i2"] + 2 * ["<f4"])):
+            if ptr.value is None:
+                continue
+            shape = rows + (last,)
+            at = ptr.value if layer is None else ptr.value + layer * int(np.prod(shape, dtype=np.int64)) * size
+            out.append(DevicePlane(at, (self.n_layers,) + shape if layer is None else shape, kind, self))
+        return out
+
+    @property
+    def free_pages(self):
+        return lib().pf_pages_free_count(self.h)
+
+    def memory_usage(self):
+        return lib().pf_pages_memory_usage(self.h)
+
+    def close(self):
+        if self.h:
+            lib().pf_pages_destroy(self.h)
             self.h = None
 
     def __del__(self):

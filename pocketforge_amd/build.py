@@ -33,6 +33,9 @@ CXX_FLAGS = ["-O2", "-fPIC", "-std=c++17", "-ffp-contract=off", "-I" + os.path.j
 
 UNITS = [
     ("pf_runtime.hip", "hip"),
+    ("pf_prompt.hip", "hip"),
+    ("pf_paged.hip", "hip"),
+    ("pf_pages.hip", "hip"),
     ("pf_host.cpp", "cxx"),
     ("pf_squeeze.cpp", "cxx"),
 ]

@@ -1,0 +1,429 @@
+// Attention of a pass's rows over their sequences' pages (pf_pages_attention of
+// include/pf_gpu.h): one new token per sequence, a verify pass's few, or more.
+//
+// The mathematics is that of pf_prompt.hip.  A workgroup takes one kv head and
+// a share of one sequence's keys; where there are few sequences the keys are
+// shared among many workgroups, whose partial results (running maximum m, sum
+// l, unnormalised output o) are joined:
+//   M = max_p m_p,  out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.
+#include "pf_paged.h"
+
+#include <algorithm>
+
+using namespace pf;
+
+namespace pf {
+
+// A workgroup: 4 waves, each on 32-key tiles of its own, four tiles apart.
+// A lane's matrix operands of K are 16 bytes of a row as the page holds them,
+// straight from memory; V's rows go through LDS, which transposes them.  The
+// rows of all query heads of the kv head are the columns of the score tile
+// S^T = K Q^T, 16 at a time (NT tiles); exp(S)^T is the operand of O^T = V^T P^T
+// without moving a value between lanes.
+template <int ACT, int CT, int DP, int NT, bool EXACT>
+__global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
+    constexpr bool BF = op_bf<ACT>, I8 = CT == PF_TYPE_I8;
+    constexpr int NP = op_pieces<ACT>, C = DP / 32, DT = DP / 16;
+    constexpr int STR = DP + 16;                 // LDS row stride in values
+    constexpr int VCH = I8 ? DP / 16 : DP / 8;   // 16-byte chunks of a V row
+    constexpr int VL = 32 * VCH / 64;            // V loads of a lane
+    constexpr int KL = I8 ? DP / 64 : C;         // K loads of a lane per 16 keys
+    __shared__ __align__(16) short sv[4][32][STR];
+    __shared__ float s_ml[4][16][2];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+
+    const PageItem it = a.items[blockIdx.x];
+    const uint32_t head0 = blockIdx.y * a.group;
+    const int R = (int)(it.rows * a.group), rt0 = (int)blockIdx.z * 16 * NT;
+    if (rt0 >= R) return;
+    const int len = (int)it.len, p0 = len - (int)it.rows;
+    const PageTiles pt = page_tiles(it.rows, it.len, (uint32_t)a.window, (uint32_t)a.sink);
+    const int lo0 = a.window ? max(0, p0 - a.window + 1) : 0;
+    const int lo1 = a.window ? max(0, len - a.window) : 0;
+
+    s8v qf[NT][NP][C];
+    int hi[NT], lo[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = min(rt0 + n * 16 + col, R - 1), j = r / (int)a.group, h = r - j * (int)a.group;
+        hi[n] = a.causal ? p0 + j : len - 1;
+        lo[n] = a.window ? p0 + j - a.window + 1 : 0;
+        const uint8_t* qp = (const uint8_t*)a.q +
+                            ((size_t)(it.q0 + (uint32_t)j) * a.qs + (size_t)(head0 + (uint32_t)h) * a.dim) * act_size<ACT>;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            // the dims of K's operand: int8 rows give a lane 16 codes at a time
+            const int d = I8 ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
+            float x[8] = {};
+            if (EXACT || d < (int)a.dim) load8<ACT>(qp + (size_t)d * act_size<ACT>, x);
+            s8v t[NP];
+            pieces<BF, NP>(x, t);
+#pragma unroll
+            for (int n2 = 0; n2 < NP; n2++) qf[n][n2][c] = t[n2];
+        }
+    }
+
+    f4v o[NT][DT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; t++) o[n][t] = (f4v)0.0f;
+    }
+
+    const int32_t* table = a.table + (size_t)it.slot * a.table_stride;
+    const int last_page = (len - 1) >> a.page_shift, in_page = (1 << a.page_shift) - 1;
+    const size_t row_bytes = (size_t)a.dim * (I8 ? 1 : 2);
+
+    u4v kr[2][KL], vr[VL];
+    f4v ksc[2], vsc[2];
+    int tile_pos = 0;
+    auto load = [&](int t) {
+        tile_pos = (t < pt.sinks ? t : t - pt.sinks + pt.first) * 32;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int pos = tile_pos + 16 * s;
+            const int pg = table[min(pos >> a.page_shift, last_page)];
+            const size_t row0 = (((size_t)pg * a.kv_heads + blockIdx.y) << a.page_shift) + (size_t)(pos & in_page);
+            const uint8_t* kp = (const uint8_t*)a.k + (row0 + col) * row_bytes;
+#pragma unroll
+            for (int c = 0; c < KL; c++) {
+                const int off = c * 64 + g * 16;
+                kr[s][c] = (EXACT || off < (int)row_bytes) ? *(const u4v*)(kp + off) : (u4v)0u;
+            }
+            const uint8_t* vp = (const uint8_t*)a.v + row0 * row_bytes;
+#pragma unroll
+            for (int i = 0; i < VL / 2; i++) {
+                const int e = i * 64 + lane, r = e / VCH, off = e % VCH * 16;
+                vr[s * (VL / 2) + i] = (EXACT || off < (int)row_bytes) ? *(const u4v*)(vp + (size_t)r * row_bytes + off) : (u4v)0u;
+            }
+            if constexpr (I8) {
+                ksc[s] = *(const f4v*)(a.ks + row0 + 4 * g);
+                vsc[s] = *(const f4v*)(a.vs + row0 + 4 * g);
+            }
+        }
+    };
+
+    int t = (int)it.t0 + wave;
+    if (t < (int)it.t1) load(t);
+    for (; t < (int)it.t1; t += 4) {
+        const int pos0 = tile_pos;
+        const bool whole = pos0 + 31 <= (a.causal ? p0 : len - 1) && (pos0 >= lo1 || pos0 + 32 <= a.sink);
+        // V's rows to LDS; rows that nobody sees (past the end, between sinks and window) as zeros
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < VL; i++) {
+            const int e = i * 64 + lane, r = e / VCH, off = e % VCH;
+            u4v w = vr[i];
+            if (!whole) {
+                const int pos = pos0 + r;
+                if (pos >= len || (pos < lo0 && pos >= a.sink)) w = (u4v)0u;
+            }
+            if constexpr (I8) {
+                float x[8];
+                codes8(w[0], w[1], x);
+                *(s8v*)&sv[wave][r][off * 16] = pack8<BF>(x);
+                codes8(w[2], w[3], x);
+                *(s8v*)&sv[wave][r][off * 16 + 8] = pack8<BF>(x);
+            } else {
+                const s8v x = __builtin_bit_cast(s8v, w);
+                if (!whole) bad |= any_not_finite<BF>(x);
+                *(s8v*)&sv[wave][r][off * 8] = x;
+            }
+        }
+        const bool odd = !I8 && !whole && __any(bad);
+        f4v kscale[2], vscale[2];
+        s8v kf[2][C];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            if constexpr (I8) {
+                kscale[s] = ksc[s];
+                vscale[s] = vsc[s];
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    float x[8];
+                    codes8(kr[s][c >> 1][(c & 1) * 2], kr[s][c >> 1][(c & 1) * 2 + 1], x);
+                    kf[s][c] = pack8<BF>(x);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; c++) kf[s][c] = __builtin_bit_cast(s8v, kr[s][c]);
+            }
+        }
+        f4v sc[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                sc[n][s] = (f4v)0.0f;
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int x = 0; x < NP; x++) sc[n][s] = mfma16<BF>(kf[s][c], qf[n][x][c], sc[n][s]);
+            }
+        if (t + 4 < (int)it.t1) load(t + 4);     // (the next tile's rows are on their way during what follows)
+        s8v pf[NT][NP];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float x[8], top = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float y = sc[n][s][i] * (I8 ? kscale[s][i] * a.scale_log2 : a.scale_log2);
+                    if (!whole && !key_visible(pos0 + 16 * s + 4 * g + i, hi[n], lo[n], a.sink)) y = -INFINITY;
+                    x[4 * s + i] = y;
+                    top = fmaxf(top, y);
+                }
+            if (__any(top > m[n] + MAX_SLACK)) {
+                const float to = fmaxf(m[n], max16(top));
+                const float f = to == -INFINITY ? 1.0f : exp2_fast(m[n] - to);
+                m[n] = to;
+                l[n] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[n][d][i] *= f;
+            }
+            const float ms = m[n] == -INFINITY ? 0.0f : m[n];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float e = exp2_fast(x[i] - ms);
+                l[n] += e;
+                x[i] = e;
+                if constexpr (I8) {
+                    const float w = e * vscale[i / 4][i % 4];
+                    x[i] = !whole && !key_visible(pos0 + 16 * (i / 4) + 4 * g + i % 4, hi[n], lo[n], a.sink) ? 0.0f : w;
+                }
+            }
+            pieces<BF, NP>(x, pf[n]);
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int r = 4 * g + (lane & 15) / 4, c = d * 16 + (lane & 3) * 4;
+            const s4v x0 = lds_read_tr(&sv[wave][r][c]), x1 = lds_read_tr(&sv[wave][r + 16][c]);
+            s8v vf = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+            if (odd) vf = finite_or_zero<BF>(vf);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int x = 0; x < NP; x++) o[n][d] = mfma16<BF>(vf, pf[n][x], o[n][d]);
+        }
+        if (odd) {
+            // infinities and NaN reach the rows that see them, whatever their weight
+            for (int r = 0; r < 32; r++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    if (!key_visible(pos0 + r, hi[n], lo[n], a.sink) || pos0 + r >= len) continue;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const short w = sv[wave][r][d * 16 + 4 * g + i];
+                            if (not_finite<BF>(w)) o[n][d][i] += to_float<BF ? PF_TYPE_BF16 : PF_TYPE_F16>(w);
+                        }
+                }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // the four waves' results meet in LDS, 16 rows at a time
+    float* so = (float*)&sv[0][0][0];            // [4][16][DP]
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float lw = sum16(l[n]);
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DT; d++) *(f4v*)&so[(wave * 16 + col) * DP + d * 16 + 4 * g] = o[n][d];
+        if (g == 0) {
+            s_ml[wave][col][0] = m[n];
+            s_ml[wave][col][1] = lw;
+        }
+        __syncthreads();
+        constexpr int PER = DP / 16;             // dims of a thread
+        const int r = tid >> 4, d0 = (tid & 15) * PER, row = rt0 + n * 16 + r;
+        float M = -INFINITY, L = 0.0f, acc[PER] = {};
+#pragma unroll
+        for (int w = 0; w < 4; w++) M = fmaxf(M, s_ml[w][r][0]);
+        const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = exp2_fast(s_ml[w][r][0] - ms);
+            L += f * s_ml[w][r][1];
+#pragma unroll
+            for (int i = 0; i < PER; i++) acc[i] += f * so[(w * 16 + r) * DP + d0 + i];
+        }
+        if (row >= R || (!EXACT && d0 >= (int)a.dim)) continue;
+        const int j = row / (int)a.group, h = (int)head0 + row - j * (int)a.group;
+        if (it.parts == 1) {
+            const float inv = 1.0f / L;
+            uint8_t* op = (uint8_t*)a.out + ((size_t)(it.q0 + (uint32_t)j) * a.os + (size_t)h * a.dim + d0) * act_size<ACT>;
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = acc[i + e] * inv;
+                if (EXACT || d0 + i < (int)a.dim) store4<ACT>(op + i * act_size<ACT>, x);
+            }
+        } else {
+            const size_t w = (size_t)(it.ws0 + (uint32_t)j) * a.n_heads + (uint32_t)h;
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (EXACT || d0 + i < (int)a.dim) a.ws_o[w * a.dim + d0 + i] = acc[i];
+            if (d0 == 0) {
+                a.ws_ml[2 * w] = M;
+                a.ws_ml[2 * w + 1] = L;
+            }
+        }
+    }
+}
+
+// Joins the parts of the sequences that were cut: one workgroup per (item that
+// begins a sequence, head), its rows one after another.
+template <int ACT>
+__global__ __launch_bounds__(128) void k_paged_join(PagedArgs a) {
+    const PageItem it = a.items[blockIdx.x];
+    if (it.parts == 1 || it.t0 != 0) return;
+    const uint32_t h = blockIdx.y, d = threadIdx.x;
+    for (uint32_t j = blockIdx.z; j < it.rows; j += gridDim.z) {
+        float M = -INFINITY;
+        for (uint32_t p = 0; p < it.parts; p++)
+            M = fmaxf(M, a.ws_ml[2 * ((size_t)(it.ws0 + p * it.rows + j) * a.n_heads + h)]);
+        const float ms = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f, acc = 0.0f;
+        for (uint32_t p = 0; p < it.parts; p++) {
+            const size_t w = (size_t)(it.ws0 + p * it.rows + j) * a.n_heads + h;
+            const float f = exp2_fast(a.ws_ml[2 * w] - ms);
+            L += f * a.ws_ml[2 * w + 1];
+            if (d < a.dim) acc += f * a.ws_o[w * a.dim + d];
+        }
+        if (d >= a.dim) continue;
+        const float y = acc / L;
+        const size_t at = (size_t)(it.q0 + j) * a.os + (size_t)h * a.dim + d;
+        if constexpr (ACT == PF_TYPE_F32) ((float*)a.out)[at] = y;
+        else if constexpr (ACT == PF_TYPE_BF16) ((__bf16*)a.out)[at] = (__bf16)y;
+        else ((_Float16*)a.out)[at] = (_Float16)y;
+    }
+}
+
+}  // namespace pf
+
+// ================================================================== host
+
+template <int ACT, int CT, int DP, bool EXACT>
+static void paged_rows(hipStream_t st, uint32_t items, uint32_t most, const PagedArgs& a) {
+    const uint32_t R = most * a.group;
+    // one tile of 16 rows, or two: the keys are read once for both
+    if (R <= 16)
+        hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, 1, EXACT>), dim3(items, a.kv_heads), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, 2, EXACT>), dim3(items, a.kv_heads, (R + 31) / 32), dim3(256), 0, st, a);
+}
+
+template <int ACT, int CT>
+static void paged_dim(hipStream_t st, uint32_t items, uint32_t most, const PagedArgs& a) {
+    if (a.dim == 128) paged_rows<ACT, CT, 128, true>(st, items, most, a);
+    else if (a.dim == 64) paged_rows<ACT, CT, 64, true>(st, items, most, a);
+    else if (a.dim < 64) paged_rows<ACT, CT, 64, false>(st, items, most, a);
+    else paged_rows<ACT, CT, 128, false>(st, items, most, a);
+}
+
+// Cuts the pass's keys: enough workgroups for every compute unit several times
+// over, none with less than PG_LEAST tiles.
+constexpr uint32_t PG_LEAST = 16;
+static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
+    PageSplit& u = p->cut;
+    if (u.type == d->type && u.window == s.window && u.sink == s.sink && u.heads == d->n_heads) return PF_OK;
+    const uint32_t group = d->n_heads / d->n_kv_heads;
+    uint64_t all = 0;
+    uint32_t most = 0;
+    for (const PageSeq& q : p->pass) {
+        if (!q.rows) continue;
+        all += (uint64_t)page_tiles(q.rows, q.len, s.window, s.sink).count;
+        most = std::max(most, q.rows);
+    }
+    const uint64_t per = (uint64_t)d->n_kv_heads * (((uint64_t)most * group + 31) / 32);
+    const uint32_t chunk = (uint32_t)std::max<uint64_t>(PG_LEAST, (all * per + PG_GROUPS - 1) / PG_GROUPS);
+    std::vector<PageItem> items;
+    PageSplit n;
+    uint64_t ws = 0;
+    for (const PageSeq& q : p->pass) {
+        if (!q.rows) continue;
+        const uint32_t tiles = (uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count;
+        const uint32_t parts = (tiles + chunk - 1) / chunk;
+        for (uint32_t i = 0; i < parts; i++) {
+            items.push_back({q.slot, q.q0, q.rows, q.len, (uint32_t)((uint64_t)tiles * i / parts),
+                             (uint32_t)((uint64_t)tiles * (i + 1) / parts), (uint32_t)ws, parts});
+            if (parts > 1) ws += q.rows;
+        }
+        if (parts > 1) n.split = true;
+    }
+    if (ws * d->n_heads > 0x7FFFFFFFu) return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
+    if (items.size() > p->items_cap) return fail(p->ctx, PF_ERR_STATE, "pages: work list exceeded");
+    if (pf_status st = pages_upload(p, p->items, items.data(), items.size() * sizeof(PageItem))) return st;
+    n.window = s.window; n.sink = s.sink; n.heads = d->n_heads; n.type = d->type;
+    n.n_items = (uint32_t)items.size(); n.ws_rows = (uint32_t)ws; n.most_rows = most;
+    u = n;
+    return PF_OK;
+}
+
+extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint32_t layer, const void* q, void* out) {
+    if (!p || !d) return PF_ERR_ARG;
+    pf_ctx* c = p->ctx;
+    AttnShape s;
+    if (pf_status st = attn_desc_check(c, d, &s)) return st;
+    if (layer >= p->cfg.n_layers) return fail(c, PF_ERR_ARG, "pages: layer out of range");
+    if (d->n_kv_heads != p->cfg.n_kv_heads || d->head_dim != p->cfg.head_dim)
+        return fail(c, PF_ERR_ARG, "pages: n_kv_heads and head_dim are the cache's");
+    const int32_t ct = p->cfg.type;
+    if (ct != PF_TYPE_I8 && ct != d->type && !(ct == PF_TYPE_BF16 && d->type == PF_TYPE_F32))
+        return fail(c, PF_ERR_UNSUPPORTED, "pages: rows of this type over a cache of that type");
+    if (!p->open) return fail(c, PF_ERR_STATE, "pages: no open pass (pf_pages_append begins one)");
+    if (!p->pass_rows) return PF_OK;
+    if (!q || !out) return fail(c, PF_ERR_ARG, "pages: a buffer is NULL");
+    if (!aligned16(q) || !aligned16(out)) return fail(c, PF_ERR_ARG, "pages: buffers start on 16 bytes");
+    const size_t es = d->type == PF_TYPE_F32 ? 4 : 2, qw = (size_t)d->n_heads * d->head_dim;
+    if (overlaps(out, ((size_t)(p->pass_rows - 1) * s.os + qw) * es, q, ((size_t)(p->pass_rows - 1) * s.qs + qw) * es))
+        return fail(c, PF_ERR_ARG, "pages: out overlaps q");
+    DeviceScope on(c);
+    if (pf_status st = no_throw(c, [&] { return paged_cut(p, d, s); })) return st;
+    const PageSplit& u = p->cut;
+    PagedArgs a{};
+    if (u.split) {
+        const size_t rows = (size_t)u.ws_rows * d->n_heads;
+        void* ws = nullptr;
+        if (pf_status st = ctx_scratch(c, rows * (d->head_dim + 2) * 4, &ws)) return st;
+        a.ws_o = (float*)ws;
+        a.ws_ml = a.ws_o + rows * d->head_dim;
+    }
+    a.items = p->items; a.seqs = p->seqs; a.table = p->table; a.table_stride = p->per_seq; a.n_seq = (uint32_t)p->pass.size();
+    a.k = (const uint8_t*)p->k + layer * p->plane; a.v = (const uint8_t*)p->v + layer * p->plane;
+    if (p->ks) { a.ks = p->ks + layer * p->scales; a.vs = p->vs + layer * p->scales; }
+    a.q = q; a.out = out; a.qs = s.qs; a.os = s.os;
+    a.n_heads = d->n_heads; a.kv_heads = d->n_kv_heads; a.group = d->n_heads / d->n_kv_heads; a.dim = d->head_dim;
+    a.page_shift = p->shift;
+    a.causal = d->causal != 0; a.window = (int32_t)s.window; a.sink = (int32_t)s.sink;
+    a.scale_log2 = s.scale_log2;
+    hipStream_t st = c->stream;
+#define PF_PAGED(A, T) paged_dim<A, T>(st, u.n_items, u.most_rows, a)
+    if (ct == PF_TYPE_I8) {
+        if (d->type == PF_TYPE_F32) PF_PAGED(PF_TYPE_F32, PF_TYPE_I8);
+        else if (d->type == PF_TYPE_F16) PF_PAGED(PF_TYPE_F16, PF_TYPE_I8);
+        else PF_PAGED(PF_TYPE_BF16, PF_TYPE_I8);
+    } else if (ct == PF_TYPE_F16) PF_PAGED(PF_TYPE_F16, PF_TYPE_F16);
+    else if (d->type == PF_TYPE_F32) PF_PAGED(PF_TYPE_F32, PF_TYPE_BF16);
+    else PF_PAGED(PF_TYPE_BF16, PF_TYPE_BF16);
+#undef PF_PAGED
+    PF_LAUNCHED(c);
+    if (u.split) {
+        const dim3 grid(u.n_items, d->n_heads, std::min(u.most_rows, 64u));
+        if (d->type == PF_TYPE_F32) hipLaunchKernelGGL(k_paged_join<PF_TYPE_F32>, grid, dim3(128), 0, st, a);
+        else if (d->type == PF_TYPE_F16) hipLaunchKernelGGL(k_paged_join<PF_TYPE_F16>, grid, dim3(128), 0, st, a);
+        else hipLaunchKernelGGL(k_paged_join<PF_TYPE_BF16>, grid, dim3(128), 0, st, a);
+        PF_LAUNCHED(c);
+    }
+    return PF_OK;
+}

@@ -1,0 +1,327 @@
+// Attention over whole prompts: packed sequences, grouped heads, causal and
+// windowed masks (pf_prompt_attention of include/pf_gpu.h).
+//
+// A query row i of a sequence sees keys j with j <= p (causal) and, with a
+// window, j > p - window or j < sink, where p is its position:
+//   out_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i),
+//   s_ij = scale * q_i . k_j,   m_i = max_j s_ij.
+// One pass over the keys: the running maximum m and sum l of a row are
+// corrected when m moves, so nothing of size rows x keys is stored.
+#include "pf_attend.h"
+#include "pf_context.h"
+
+#include <cmath>
+
+using namespace pf;
+
+namespace pf {
+
+constexpr int PR_SEQS = 64;       // sequences of one launch
+constexpr int PR_KEYS = 64;       // keys of a tile
+
+struct PromptArgs {
+    const void *q, *k, *v;
+    void* out;
+    uint32_t n_seq, n_heads, group, dim;
+    uint32_t qs, ks, vs, os;      // row strides in elements
+    int32_t causal, window, sink;
+    float scale_log2;
+    uint32_t tile0[PR_SEQS];      // first query tile of each sequence
+    struct { uint32_t q0, nq, k0, nk; } seq[PR_SEQS];   // first rows and lengths
+};
+
+// A workgroup: 4 waves of 32 query rows of one head.  Scores are formed as
+// S^T = K Q^T, so that a lane holds 16 keys of one row: its maximum and sum
+// need one exchange between two lanes, and exp(S)^T is already the operand
+// of O^T = V^T P^T, whose other operand comes from V's rows in LDS through
+// transposing reads.
+template <int ACT, int DP, bool EXACT>
+__global__ __launch_bounds__(256) void k_prompt_attn(PromptArgs a) {
+    constexpr bool BF = op_bf<ACT>;
+    constexpr int NP = op_pieces<ACT>;
+    constexpr int STR = DP + 16;                 // LDS row stride in values
+    constexpr int C = DP / 16, DT = DP / 32;
+    __shared__ __align__(16) short sk[NP][PR_KEYS][STR];
+    __shared__ __align__(16) short sv[NP][PR_KEYS][STR];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, row = lane & 31, half = lane >> 5;
+
+    // the sequence of this tile: the last one whose first tile is not past it
+    const uint32_t tile = blockIdx.x, head = blockIdx.y;
+    const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= tile);
+    const int seq = 63 - __builtin_clzll(before);
+    const uint32_t q0 = a.seq[seq].q0, k0 = a.seq[seq].k0;
+    const int nq = (int)a.seq[seq].nq, nk = (int)a.seq[seq].nk;
+    const int off = nk - nq, r0 = (int)(tile - a.tile0[seq]) * 128;
+    const int my = r0 + wave * 32 + row;         // this lane's query
+    const int p = off + my;
+    const int hi = a.causal ? p : nk - 1, lo = a.window ? p - a.window + 1 : 0;
+
+    // Q^T: 16 dims of a row per matrix instruction
+    s8v qf[NP][C];
+    {
+        const uint32_t qr = q0 + (uint32_t)min(my, nq - 1);
+        const uint8_t* qp = (const uint8_t*)a.q + ((size_t)qr * a.qs + (size_t)head * a.dim) * act_size<ACT>;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int d = c * 16 + half * 8;
+            float x[8] = {};
+            if (EXACT || d < (int)a.dim) load8<ACT>(qp + (size_t)d * act_size<ACT>, x);
+            s8v t[NP];
+            pieces<BF, NP>(x, t);
+#pragma unroll
+            for (int n = 0; n < NP; n++) qf[n][c] = t[n];
+        }
+    }
+
+    // keys that any row of the workgroup sees
+    const int p0 = off + r0, p1 = off + min(r0 + 128, nq) - 1;
+    const int end = min(nk, a.causal ? p1 + 1 : nk);
+    const int wlo = a.window ? max(0, p0 - a.window + 1) : 0;
+    const int first = wlo / PR_KEYS;
+    const int sinks = min((a.sink + PR_KEYS - 1) / PR_KEYS, first);
+    const int tiles = end <= 0 ? 0 : max(0, (end + PR_KEYS - 1) / PR_KEYS - first) + min(sinks, (end + PR_KEYS - 1) / PR_KEYS);
+
+    f16v o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[t] = (f16v)0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    const size_t kv_head = (size_t)(head / a.group) * a.dim;
+    for (int it = 0; it < tiles; it++) {
+        const int key0 = (it < sinks ? it : it - sinks + first) * PR_KEYS;
+        // a tile that every row of the workgroup sees whole needs no mask
+        const bool whole = key0 + PR_KEYS <= nk && (!a.causal || key0 + PR_KEYS - 1 <= p0) &&
+                           (!a.window || key0 >= p1 - a.window + 1 || key0 + PR_KEYS <= a.sink);
+        __syncthreads();
+        if (tid == 0) s_bad = 0;
+        __syncthreads();
+        bool bad = false;
+#pragma unroll
+        for (int e = tid; e < PR_KEYS * (DP / 8); e += 256) {
+            const int r = e / (DP / 8), d = e % (DP / 8) * 8, key = key0 + r;
+            float xk[8] = {}, xv[8] = {};
+            if (key < nk && (EXACT || d < (int)a.dim)) {
+                const size_t kr = k0 + (uint32_t)key;
+                load8<ACT>((const uint8_t*)a.k + (kr * a.ks + kv_head + d) * act_size<ACT>, xk);
+                load8<ACT>((const uint8_t*)a.v + (kr * a.vs + kv_head + d) * act_size<ACT>, xv);
+            }
+            s8v tk[NP], tv[NP];
+            pieces<BF, NP>(xk, tk);
+            pieces<BF, NP>(xv, tv);
+#pragma unroll
+            for (int n = 0; n < NP; n++) {
+                *(s8v*)&sk[n][r][d] = tk[n];
+                *(s8v*)&sv[n][r][d] = tv[n];
+            }
+            if (!whole) bad |= any_not_finite<BF>(tv[0]);
+        }
+        if (bad) s_bad = 1;
+        __syncthreads();
+        const bool odd = s_bad != 0;             // values that masked rows must not meet
+
+        f16v s[2];
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            s[g] = (f16v)0.0f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                s8v kf[NP];
+#pragma unroll
+                for (int n = 0; n < NP; n++) kf[n] = *(const s8v*)&sk[n][g * 32 + row][c * 16 + half * 8];
+#pragma unroll
+                for (int x = 0; x < NP; x++)
+#pragma unroll
+                    for (int y = 0; y < NP; y++)
+                        if (x + y < 3) s[g] = mfma32<BF>(kf[x], qf[y][c], s[g]);
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float x = s[g][i] * a.scale_log2;
+                if (!whole) {
+                    const int key = key0 + g * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    if (key >= nk || !key_visible(key, hi, lo, a.sink)) x = -INFINITY;
+                }
+                s[g][i] = x;
+                top = fmaxf(top, x);
+            }
+        if (__any(top > m + MAX_SLACK)) {
+            const float to = fmaxf(m, max32(top));
+            const float f = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t][i] *= f;
+        }
+        const float ms = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[g][i] = exp2_fast(s[g][i] - ms);
+                l += s[g][i];
+            }
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {        // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = s[g][8 * h + i];
+                s8v pf[NP];
+                pieces<BF, NP>(x, pf);
+                const int kr = g * 32 + h * 16 + 4 * half + (lane & 15) / 4;
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+                    const int d = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+                    s8v vf[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; n++) {
+                        const s4v x0 = lds_read_tr(&sv[n][kr][d]), x1 = lds_read_tr(&sv[n][kr + 8][d]);
+                        vf[n] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        if (odd) vf[n] = finite_or_zero<BF>(vf[n]);
+                    }
+#pragma unroll
+                    for (int x = 0; x < NP; x++)
+#pragma unroll
+                        for (int y = 0; y < NP; y++)
+                            if (x + y < 3) o[t] = mfma32<BF>(vf[x], pf[y], o[t]);
+                }
+            }
+        if (odd) {
+            // infinities and NaN reach the rows that see them, whatever their weight
+            for (int r = 0; r < PR_KEYS; r++) {
+                const int key = key0 + r;
+                if (key >= nk || !key_visible(key, hi, lo, a.sink)) continue;
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int d = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                        if (!not_finite<BF>(sv[0][r][d])) continue;
+#pragma unroll
+                        for (int n = 0; n < NP; n++) o[t][i] += to_float<BF ? PF_TYPE_BF16 : PF_TYPE_F16>(sv[n][r][d]);
+                    }
+            }
+        }
+    }
+
+    l = sum32(l);
+    if (my >= nq) return;
+    // a row that sees no key is zero; one whose scores are all -infinity is 0 / 0
+    const bool none = !(a.causal ? p >= 0 : nk > 0);
+    const float inv = none ? 0.0f : 1.0f / l;
+    uint8_t* op = (uint8_t*)a.out + ((size_t)(q0 + (uint32_t)my) * a.os + (size_t)head * a.dim) * act_size<ACT>;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = t * 32 + 8 * (i / 4) + 4 * half;
+            if (!EXACT && d >= (int)a.dim) continue;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[t][i + j] * inv;
+            store4<ACT>(op + (size_t)d * act_size<ACT>, x);
+        }
+}
+
+}  // namespace pf
+
+// ================================================================== host
+
+pf_status attn_desc_check(pf_ctx* c, const pf_attn_desc* d, AttnShape* s) {
+    if (d->type != PF_TYPE_F32 && d->type != PF_TYPE_F16 && d->type != PF_TYPE_BF16)
+        return fail(c, PF_ERR_ARG, "attention: type is PF_TYPE_F32, F16 or BF16");
+    if (!d->n_heads || !d->n_kv_heads || d->n_heads % d->n_kv_heads || d->n_heads > 65535)
+        return fail(c, PF_ERR_ARG, "attention: n_heads is a multiple of n_kv_heads");
+    if (!d->head_dim || d->head_dim % 16 || d->head_dim > 128)
+        return fail(c, PF_ERR_UNSUPPORTED, "attention: head_dim is a multiple of 16 up to 128");
+    if (!std::isfinite(d->scale) || d->scale < 0.0f) return fail(c, PF_ERR_ARG, "attention: scale is 0 or positive");
+    s->window = std::min(d->window, SEQ_ROWS);
+    s->sink = std::min(d->sink, SEQ_ROWS);
+    const uint64_t q = (uint64_t)d->n_heads * d->head_dim, k = (uint64_t)d->n_kv_heads * d->head_dim;
+    const uint32_t per16 = d->type == PF_TYPE_F32 ? 4 : 8;
+    const uint32_t given[4] = {d->q_stride, d->k_stride, d->v_stride, d->o_stride};
+    uint32_t* out[4] = {&s->qs, &s->ks, &s->vs, &s->os};
+    for (int i = 0; i < 4; i++) {
+        const uint64_t least = i == 1 || i == 2 ? k : q, st = given[i] ? given[i] : least;
+        if (st < least || st > 0xFFFFFFFFu || st % per16)
+            return fail(c, PF_ERR_ARG, "attention: strides hold every head and are multiples of 16 bytes");
+        *out[i] = (uint32_t)st;
+    }
+    s->scale_log2 = (d->scale == 0.0f ? 1.0f / std::sqrt((float)d->head_dim) : d->scale) * LOG2E;
+    return PF_OK;
+}
+
+template <int ACT, int DP, bool EXACT>
+static void prompt_one(hipStream_t st, uint32_t tiles, const PromptArgs& a) {
+    hipLaunchKernelGGL((k_prompt_attn<ACT, DP, EXACT>), dim3(tiles, a.n_heads), dim3(256), 0, st, a);
+}
+
+template <int ACT>
+static void prompt_dim(hipStream_t st, uint32_t tiles, const PromptArgs& a) {
+    if (a.dim == 128) prompt_one<ACT, 128, true>(st, tiles, a);
+    else if (a.dim == 64) prompt_one<ACT, 64, true>(st, tiles, a);
+    else if (a.dim < 64) prompt_one<ACT, 64, false>(st, tiles, a);
+    else prompt_one<ACT, 128, false>(st, tiles, a);
+}
+
+extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const void* q, const void* k, const void* v,
+                                         void* out, const uint32_t* q_lens, const uint32_t* k_lens, uint32_t n_seq) {
+    if (!c || !d || (n_seq && !q_lens)) return PF_ERR_ARG;
+    AttnShape s;
+    if (pf_status st = attn_desc_check(c, d, &s)) return st;
+    if (!k_lens) k_lens = q_lens;
+    uint64_t nq = 0, nk = 0;
+    for (uint32_t i = 0; i < n_seq; i++) {
+        if (q_lens[i] > SEQ_ROWS || k_lens[i] > SEQ_ROWS) return fail(c, PF_ERR_UNSUPPORTED, "attention: a sequence of over 2^30 rows");
+        nq += q_lens[i];
+        nk += k_lens[i];
+    }
+    if (!nq) return PF_OK;
+    if (nq > 0x7FFFFFFFu || nk > 0x7FFFFFFFu) return fail(c, PF_ERR_UNSUPPORTED, "attention: over 2^31 rows in all");
+    if (!q || !out || (nk && (!k || !v))) return fail(c, PF_ERR_ARG, "attention: a buffer is NULL");
+    if (!aligned16(q) || !aligned16(out) || !aligned16(k) || !aligned16(v))
+        return fail(c, PF_ERR_ARG, "attention: buffers start on 16 bytes");
+    const size_t es = d->type == PF_TYPE_F32 ? 4 : 2;
+    const size_t qw = (size_t)d->n_heads * d->head_dim, kw = (size_t)d->n_kv_heads * d->head_dim;
+    const size_t ob = ((nq - 1) * s.os + qw) * es;
+    if (overlaps(out, ob, q, ((nq - 1) * s.qs + qw) * es) ||
+        (nk && (overlaps(out, ob, k, ((nk - 1) * s.ks + kw) * es) || overlaps(out, ob, v, ((nk - 1) * s.vs + kw) * es))))
+        return fail(c, PF_ERR_ARG, "attention: out overlaps an input");
+    DeviceScope on(c);
+    PromptArgs a{};
+    a.q = q; a.k = k; a.v = v; a.out = out;
+    a.n_heads = d->n_heads; a.group = d->n_heads / d->n_kv_heads; a.dim = d->head_dim;
+    a.qs = s.qs; a.ks = s.ks; a.vs = s.vs; a.os = s.os;
+    a.causal = d->causal != 0; a.window = (int32_t)s.window; a.sink = (int32_t)s.sink;
+    a.scale_log2 = s.scale_log2;
+    uint32_t qa = 0, ka = 0;
+    for (uint32_t b = 0; b < n_seq;) {
+        uint32_t tiles = 0;
+        a.n_seq = 0;
+        for (; b < n_seq && a.n_seq < PR_SEQS; b++) {
+            if (q_lens[b]) {
+                a.tile0[a.n_seq] = tiles;
+                a.seq[a.n_seq++] = {qa, q_lens[b], ka, k_lens[b]};
+                tiles += (q_lens[b] + 127) / 128;
+            }
+            qa += q_lens[b];
+            ka += k_lens[b];
+        }
+        if (!tiles) continue;
+        switch (d->type) {
+            case PF_TYPE_F32: prompt_dim<PF_TYPE_F32>(c->stream, tiles, a); break;
+            case PF_TYPE_F16: prompt_dim<PF_TYPE_F16>(c->stream, tiles, a); break;
+            default: prompt_dim<PF_TYPE_BF16>(c->stream, tiles, a); break;
+        }
+        PF_LAUNCHED(c);
+    }
+    return PF_OK;
+}
