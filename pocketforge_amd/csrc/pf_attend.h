@@ -154,6 +154,36 @@ __device__ __forceinline__ s8v finite_or_zero(s8v v) {
     return v;
 }
 
+// The larger exponents of two operands' values, half by half.
+template <bool BF>
+__device__ __forceinline__ s8v max_exponent(s8v m, s8v v) {
+    const uint32_t mask = BF ? 0x7F807F80u : 0x7C007C00u;
+    const u4v w = __builtin_bit_cast(u4v, v) & mask;
+    typedef uint16_t us8v __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(s8v, __builtin_elementwise_max(__builtin_bit_cast(us8v, m), __builtin_bit_cast(us8v, w)));
+}
+
+// l plus the eight values of an operand: the weights as the products take
+// them, so that a row's weights sum to one whatever they were rounded to.
+template <bool BF>
+__device__ __forceinline__ float sum8(s8v v, float l) {
+    const u4v w = __builtin_bit_cast(u4v, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t two = w[i];
+        if constexpr (BF) {
+            typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+            const b2v one = {(__bf16)1.0f, (__bf16)1.0f};
+            l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2v, two), one, l, false);
+        } else {
+            typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+            const h2v one = {(_Float16)1.0f, (_Float16)1.0f};
+            l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2v, two), one, l, false);
+        }
+    }
+    return l;
+}
+
 // Transposing LDS read: the 16 lanes of a group give the addresses of the 16
 // four-value chunks of a 4 x 16 tile, row by row; lane i gets column i.
 __device__ __forceinline__ s4v lds_read_tr(const short* p) {

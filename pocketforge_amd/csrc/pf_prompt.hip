@@ -11,6 +11,7 @@
 #include "pf_context.h"
 
 #include <cmath>
+#include <type_traits>
 
 using namespace pf;
 
@@ -231,6 +232,209 @@ __global__ __launch_bounds__(256) void k_prompt_attn(PromptArgs a) {
         }
 }
 
+// fp16 and bf16 rows: K and V tiles go from memory straight to LDS, two tiles
+// deep, while the tile before is worked on; a wave whose rows see nothing of a
+// tile leaves it out, and only tiles that some of its rows see in part are
+// masked.
+//
+// LDS rows are not padded (a wave's load writes 1 KiB in a row), so their
+// 16-byte chunks are permuted: K's so that the 16 rows that one read cycle
+// takes chunk c of lie in 16 different places, V's so that the four rows of a
+// transposing read lie in different quarters of the banks.
+template <int DP>
+__device__ __forceinline__ int k_place(int r, int c) {
+    return DP == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+}
+template <int DP>
+__device__ __forceinline__ int v_place(int r, int c) {
+    return DP == 128 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2);
+}
+
+typedef __attribute__((address_space(1))) const void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+
+template <int ACT, int DP, bool EXACT>
+__global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
+    constexpr bool BF = op_bf<ACT>;
+    constexpr int C = DP / 16, DT = DP / 32;
+    constexpr int CH = DP / 8, RPL = 64 / CH;    // chunks of a row, rows of one load of a wave
+    constexpr int LOADS = PR_KEYS / 4 / RPL;     // loads of a wave per tile, K or V
+    __shared__ __align__(16) short sk[2][PR_KEYS * DP];
+    __shared__ __align__(16) short sv[2][PR_KEYS * DP];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, row = lane & 31, half = lane >> 5;
+
+    const uint32_t tile = blockIdx.x, head = blockIdx.y;
+    const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= tile);
+    const int seq = 63 - __builtin_clzll(before);
+    const uint32_t q0 = a.seq[seq].q0, k0 = a.seq[seq].k0;
+    const int nq = (int)a.seq[seq].nq, nk = (int)a.seq[seq].nk;
+    const int off = nk - nq, r0 = (int)(tile - a.tile0[seq]) * 128;
+    const int my = r0 + wave * 32 + row;
+    const int p = off + my;
+    const int hi = a.causal ? p : nk - 1, lo = a.window ? p - a.window + 1 : 0;
+
+    s8v qf[C];
+    {
+        const uint32_t qr = q0 + (uint32_t)min(my, nq - 1);
+        const short* qp = (const short*)a.q + (size_t)qr * a.qs + (size_t)head * a.dim + half * 8;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            qf[c] = (s8v)(short)0;
+            if (EXACT || c * 16 + half * 8 < (int)a.dim) qf[c] = *(const s8v*)(qp + c * 16);
+        }
+    }
+
+    // tiles that any row of the workgroup sees
+    const int p0 = off + r0, p1 = off + min(r0 + 128, nq) - 1;
+    const int end = min(nk, a.causal ? p1 + 1 : nk);
+    const int wlo = a.window ? max(0, p0 - a.window + 1) : 0;
+    const int first = wlo / PR_KEYS, last = (end + PR_KEYS - 1) / PR_KEYS;
+    const int sinks = min((a.sink + PR_KEYS - 1) / PR_KEYS, first);
+    const int tiles = end <= 0 ? 0 : max(0, last - first) + min(sinks, last);
+    // what this wave's rows see
+    const int w0 = p0 + wave * 32, w1 = min(w0 + 31, p1);
+
+    const size_t kv_head = (size_t)(head / a.group) * a.dim;
+    const short* kg = (const short*)a.k + (size_t)k0 * a.ks + kv_head;
+    const short* vg = (const short*)a.v + (size_t)k0 * a.vs + kv_head;
+    const int lr = lane / CH, lc = lane % CH;
+    auto load = [&](int it, int b) {
+        const int key0 = (it < sinks ? it : it - sinks + first) * PR_KEYS;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int r = (wave * LOADS + i) * RPL + lr;
+            const uint32_t kr = (uint32_t)min(key0 + r, nk - 1);   // (rows past the end: masked)
+            int ck = k_place<DP>(r, lc), cv = v_place<DP>(r, lc);
+            if (!EXACT) {                                          // (past head_dim: q's zeros, unused outputs)
+                ck = min(ck, (int)a.dim / 8 - 1);
+                cv = min(cv, (int)a.dim / 8 - 1);
+            }
+            const int at = (wave * LOADS + i) * 64 * 8;
+            __builtin_amdgcn_global_load_lds((gvoid*)(kg + (size_t)kr * a.ks + ck * 8), (lvoid*)&sk[b][at], 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gvoid*)(vg + (size_t)kr * a.vs + cv * 8), (lvoid*)&sv[b][at], 16, 0, 0);
+        }
+    };
+
+    f16v o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++) o[t] = (f16v)0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    // one tile; MASKED: some of this wave's rows do not see all of it
+    auto body = [&](auto masked, int b, int key0) {
+        constexpr bool MASKED = decltype(masked)::value;
+        f16v s[2];
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            s[g] = (f16v)0.0f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const s8v kf = *(const s8v*)&sk[b][(g * 32 + row) * DP + k_place<DP>(row, c * 2 + half) * 8];
+                s[g] = mfma32<BF>(kf, qf[c], s[g]);
+            }
+        }
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = key0 + g * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    if (key >= nk || !key_visible(key, hi, lo, a.sink)) s[g][i] = -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[g][i]);
+        top *= a.scale_log2;
+        if (__any(top > m + MAX_SLACK)) {
+            const float to = fmaxf(m, max32(top));
+            const float f = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t][i] *= f;
+        }
+        const float ms = m == -INFINITY ? 0.0f : m;
+        s8v pf[4];
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = exp2_fast(__builtin_fmaf(s[g][8 * h + i], a.scale_log2, -ms));
+                pf[g * 2 + h] = pack8<BF>(x);
+                l = sum8<BF>(pf[g * 2 + h], l);
+            }
+        s8v seen = (s8v)(short)0;
+#pragma unroll
+        for (int gh = 0; gh < 4; gh++)           // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+                const int r = gh * 16 + 4 * half + (lane & 15) / 4;
+                const int c = t * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                const short* vp = &sv[b][r * DP + v_place<DP>(r, c) * 8 + (lane & 1) * 4];
+                const s4v x0 = lds_read_tr(vp), x1 = lds_read_tr(vp + 8 * DP);
+                s8v vf = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                if constexpr (MASKED) {
+                    seen = max_exponent<BF>(seen, vf);
+                    vf = finite_or_zero<BF>(vf);
+                }
+                o[t] = mfma32<BF>(vf, pf[gh], o[t]);
+            }
+        if (MASKED && __any(any_not_finite<BF>(seen))) {
+            // infinities and NaN reach the rows that see them, whatever their weight
+            for (int r = 0; r < PR_KEYS; r++) {
+                const int key = key0 + r;
+                if (key >= nk || !key_visible(key, hi, lo, a.sink)) continue;
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int d = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                        const short w = sv[b][r * DP + v_place<DP>(r, d / 8) * 8 + d % 8];
+                        if (not_finite<BF>(w)) o[t][i] += to_float<ACT>(w);
+                    }
+            }
+        }
+    };
+
+    if (tiles) load(0, 0);
+    for (int it = 0; it < tiles; it++) {
+        const int b = it & 1, key0 = (it < sinks ? it : it - sinks + first) * PR_KEYS;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                         // this tile is whole, and nobody reads the one before
+        if (it + 1 < tiles) load(it + 1, b ^ 1);
+        if ((a.causal && key0 > w1) || (a.window && key0 + PR_KEYS <= w0 - a.window + 1 && key0 >= a.sink)) continue;
+        const bool whole = key0 + PR_KEYS <= nk && (!a.causal || key0 + PR_KEYS - 1 <= w0) &&
+                           (!a.window || key0 >= w1 - a.window + 1 || key0 + PR_KEYS <= a.sink);
+
+        if (whole) body(std::false_type{}, b, key0);
+        else body(std::true_type{}, b, key0);
+    }
+
+    l = sum32(l);
+    if (my >= nq) return;
+    const bool none = !(a.causal ? p >= 0 : nk > 0);
+    const float inv = none ? 0.0f : 1.0f / l;
+    short* op = (short*)a.out + (size_t)(q0 + (uint32_t)my) * a.os + (size_t)head * a.dim;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = t * 32 + 8 * (i / 4) + 4 * half;
+            if (!EXACT && d >= (int)a.dim) continue;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[t][i + j] * inv;
+            store4<ACT>(op + d, x);
+        }
+}
+
 }  // namespace pf
 
 // ================================================================== host
@@ -261,7 +465,10 @@ pf_status attn_desc_check(pf_ctx* c, const pf_attn_desc* d, AttnShape* s) {
 
 template <int ACT, int DP, bool EXACT>
 static void prompt_one(hipStream_t st, uint32_t tiles, const PromptArgs& a) {
-    hipLaunchKernelGGL((k_prompt_attn<ACT, DP, EXACT>), dim3(tiles, a.n_heads), dim3(256), 0, st, a);
+    if constexpr (ACT == PF_TYPE_F32)
+        hipLaunchKernelGGL((k_prompt_attn<ACT, DP, EXACT>), dim3(tiles, a.n_heads), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_prompt_attn16<ACT, DP, EXACT>), dim3(tiles, a.n_heads), dim3(256), 0, st, a);
 }
 
 template <int ACT>
