@@ -154,30 +154,22 @@ __device__ __forceinline__ s8v finite_or_zero(s8v v) {
     return v;
 }
 
-// The larger exponents of two operands' values, half by half.
+// l plus f times the eight values of an operand.  With f = 1 a row's sum of
+// weights as the products take them, so that they sum to one whatever they were
+// rounded to; with f = 0 a NaN if one of the values is not finite.
 template <bool BF>
-__device__ __forceinline__ s8v max_exponent(s8v m, s8v v) {
-    const uint32_t mask = BF ? 0x7F807F80u : 0x7C007C00u;
-    const u4v w = __builtin_bit_cast(u4v, v) & mask;
-    typedef uint16_t us8v __attribute__((ext_vector_type(8)));
-    return __builtin_bit_cast(s8v, __builtin_elementwise_max(__builtin_bit_cast(us8v, m), __builtin_bit_cast(us8v, w)));
-}
-
-// l plus the eight values of an operand: the weights as the products take
-// them, so that a row's weights sum to one whatever they were rounded to.
-template <bool BF>
-__device__ __forceinline__ float sum8(s8v v, float l) {
+__device__ __forceinline__ float sum8(s8v v, float l, float f = 1.0f) {
     const u4v w = __builtin_bit_cast(u4v, v);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t two = w[i];
         if constexpr (BF) {
             typedef __bf16 b2v __attribute__((ext_vector_type(2)));
-            const b2v one = {(__bf16)1.0f, (__bf16)1.0f};
+            const b2v one = {(__bf16)f, (__bf16)f};
             l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2v, two), one, l, false);
         } else {
             typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-            const h2v one = {(_Float16)1.0f, (_Float16)1.0f};
+            const h2v one = {(_Float16)f, (_Float16)f};
             l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2v, two), one, l, false);
         }
     }
@@ -208,7 +200,12 @@ constexpr float MAX_SLACK = 8.0f;
 // Visibility of a key at position `pos` for a query whose last visible
 // position is hi: the last `window` of the causal range start at lo.
 __device__ __host__ __forceinline__ bool key_visible(int pos, int hi, int lo, int sink) {
-    return pos <= hi && (pos >= lo || pos < sink);
+    return (pos <= hi) & ((pos >= lo) | (pos < sink));
+}
+
+// A word with its first n bits set (none for n <= 0, all from 64 on).
+__device__ __forceinline__ uint64_t first_bits(int n) {
+    return n <= 0 ? 0 : ~0ull >> (64 - min(n, 64));
 }
 
 }  // namespace pf

@@ -27,9 +27,40 @@ struct PromptArgs {
     uint32_t qs, ks, vs, os;      // row strides in elements
     int32_t causal, window, sink;
     float scale_log2;
+    uint32_t tiles;               // query tiles of all sequences
     uint32_t tile0[PR_SEQS];      // first query tile of each sequence
     struct { uint32_t q0, nq, k0, nk; } seq[PR_SEQS];   // first rows and lengths
 };
+
+// The workgroups of a launch.  Workgroup u runs on XCD u mod 8, each with an L2
+// of its own, so the query heads and tiles that read one kv head's rows go to
+// one XCD (8 kv heads or a multiple), or to the 8 / kv_heads XCDs of theirs
+// (1, 2 or 4); within it the query heads of a tile come one after another, and
+// tiles from the last: a causal sequence's last tiles see the most keys, and
+// the short ones fill the end.
+struct PromptUnit {
+    uint32_t head, tile;
+    bool none;
+};
+__host__ __device__ __forceinline__ uint32_t prompt_units(uint32_t tiles, uint32_t kv, uint32_t group) {
+    const uint32_t per = tiles * group;
+    return kv < 8 && 8 % kv == 0 ? 8 * ((per + 8 / kv - 1) / (8 / kv)) : kv * per;
+}
+__device__ __forceinline__ PromptUnit prompt_unit(uint32_t u, uint32_t tiles, uint32_t kv, uint32_t group) {
+    const uint32_t per = tiles * group, x = u % 8, i = u / 8;
+    uint32_t h, j;
+    if (kv % 8 == 0) {
+        h = x + 8 * (i / per);
+        j = i % per;
+    } else if (8 % kv == 0) {
+        h = x % kv;
+        j = i * (8 / kv) + x / kv;
+    } else {
+        h = u % (kv * group) / group;
+        j = u / (kv * group) * group + u % (kv * group) % group;
+    }
+    return {h * group + j % group, tiles - 1 - j / group, j >= per};
+}
 
 // A workgroup: 4 waves of 32 query rows of one head.  Scores are formed as
 // S^T = K Q^T, so that a lane holds 16 keys of one row: its maximum and sum
@@ -48,7 +79,9 @@ __global__ __launch_bounds__(256) void k_prompt_attn(PromptArgs a) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, row = lane & 31, half = lane >> 5;
 
     // the sequence of this tile: the last one whose first tile is not past it
-    const uint32_t tile = blockIdx.x, head = blockIdx.y;
+    const PromptUnit unit = prompt_unit(blockIdx.x, a.tiles, a.n_heads / a.group, a.group);
+    if (unit.none) return;
+    const uint32_t tile = unit.tile, head = unit.head;
     const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= tile);
     const int seq = 63 - __builtin_clzll(before);
     const uint32_t q0 = a.seq[seq].q0, k0 = a.seq[seq].k0;
@@ -263,7 +296,9 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     __shared__ __align__(16) short sv[2][PR_KEYS * DP];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, row = lane & 31, half = lane >> 5;
 
-    const uint32_t tile = blockIdx.x, head = blockIdx.y;
+    const PromptUnit unit = prompt_unit(blockIdx.x, a.tiles, a.n_heads / a.group, a.group);
+    if (unit.none) return;
+    const uint32_t tile = unit.tile, head = unit.head;
     const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= tile);
     const int seq = 63 - __builtin_clzll(before);
     const uint32_t q0 = a.seq[seq].q0, k0 = a.seq[seq].k0;
@@ -323,6 +358,15 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     // one tile; MASKED: some of this wave's rows do not see all of it
     auto body = [&](auto masked, int b, int key0) {
         constexpr bool MASKED = decltype(masked)::value;
+        // weights of zero must not meet infinities: V's values are looked through
+        // first (any of them times zero is a NaN)
+        bool odd = false;
+        if constexpr (MASKED) {
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PR_KEYS * DP / 512; i++) z = sum8<BF>(*(const s8v*)&sv[b][i * 512 + lane * 8], z, 0.0f);
+            odd = __any(z != z);
+        }
         f16v s[2];
 #pragma unroll
         for (int g = 0; g < 2; g++) {
@@ -334,12 +378,17 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
             }
         }
         if constexpr (MASKED) {
+            // one bit per key of the tile
+            const uint64_t see = first_bits(min(hi, nk - 1) + 1 - key0) &
+                                 (~first_bits(lo - key0) | first_bits(a.sink - key0));
+            const uint32_t part[2] = {(uint32_t)see >> (4 * half), (uint32_t)(see >> 32) >> (4 * half)};
 #pragma unroll
             for (int g = 0; g < 2; g++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int key = key0 + g * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                    if (key >= nk || !key_visible(key, hi, lo, a.sink)) s[g][i] = -INFINITY;
+                    const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)part[g], 8 * (i / 4) + i % 4, 1);
+                    const uint32_t x = __builtin_bit_cast(uint32_t, (float)s[g][i]);
+                    s[g][i] = __builtin_bit_cast(float, (x & on) | (0xFF800000u & ~on));   // -infinity
                 }
         }
         float top = s[0][0];
@@ -370,23 +419,24 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
                 pf[g * 2 + h] = pack8<BF>(x);
                 l = sum8<BF>(pf[g * 2 + h], l);
             }
-        s8v seen = (s8v)(short)0;
+        auto weigh = [&](auto clean) {
 #pragma unroll
-        for (int gh = 0; gh < 4; gh++)           // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
+            for (int gh = 0; gh < 4; gh++)       // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
 #pragma unroll
-            for (int t = 0; t < DT; t++) {
-                const int r = gh * 16 + 4 * half + (lane & 15) / 4;
-                const int c = t * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                const short* vp = &sv[b][r * DP + v_place<DP>(r, c) * 8 + (lane & 1) * 4];
-                const s4v x0 = lds_read_tr(vp), x1 = lds_read_tr(vp + 8 * DP);
-                s8v vf = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                if constexpr (MASKED) {
-                    seen = max_exponent<BF>(seen, vf);
-                    vf = finite_or_zero<BF>(vf);
+                for (int t = 0; t < DT; t++) {
+                    const int r = gh * 16 + 4 * half + (lane & 15) / 4;
+                    const int c = t * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                    const short* vp = &sv[b][r * DP + v_place<DP>(r, c) * 8 + (lane & 1) * 4];
+                    const s4v x0 = lds_read_tr(vp), x1 = lds_read_tr(vp + 8 * DP);
+                    s8v vf = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (decltype(clean)::value) vf = finite_or_zero<BF>(vf);
+                    o[t] = mfma32<BF>(vf, pf[gh], o[t]);
                 }
-                o[t] = mfma32<BF>(vf, pf[gh], o[t]);
-            }
-        if (MASKED && __any(any_not_finite<BF>(seen))) {
+        };
+        if (!odd) {
+            weigh(std::false_type{});
+        } else {
+            weigh(std::true_type{});
             // infinities and NaN reach the rows that see them, whatever their weight
             for (int r = 0; r < PR_KEYS; r++) {
                 const int key = key0 + r;
@@ -464,19 +514,20 @@ pf_status attn_desc_check(pf_ctx* c, const pf_attn_desc* d, AttnShape* s) {
 }
 
 template <int ACT, int DP, bool EXACT>
-static void prompt_one(hipStream_t st, uint32_t tiles, const PromptArgs& a) {
+static void prompt_one(hipStream_t st, const PromptArgs& a) {
+    const uint32_t units = prompt_units(a.tiles, a.n_heads / a.group, a.group);
     if constexpr (ACT == PF_TYPE_F32)
-        hipLaunchKernelGGL((k_prompt_attn<ACT, DP, EXACT>), dim3(tiles, a.n_heads), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_prompt_attn<ACT, DP, EXACT>), dim3(units), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((k_prompt_attn16<ACT, DP, EXACT>), dim3(tiles, a.n_heads), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_prompt_attn16<ACT, DP, EXACT>), dim3(units), dim3(256), 0, st, a);
 }
 
 template <int ACT>
-static void prompt_dim(hipStream_t st, uint32_t tiles, const PromptArgs& a) {
-    if (a.dim == 128) prompt_one<ACT, 128, true>(st, tiles, a);
-    else if (a.dim == 64) prompt_one<ACT, 64, true>(st, tiles, a);
-    else if (a.dim < 64) prompt_one<ACT, 64, false>(st, tiles, a);
-    else prompt_one<ACT, 128, false>(st, tiles, a);
+static void prompt_dim(hipStream_t st, const PromptArgs& a) {
+    if (a.dim == 128) prompt_one<ACT, 128, true>(st, a);
+    else if (a.dim == 64) prompt_one<ACT, 64, true>(st, a);
+    else if (a.dim < 64) prompt_one<ACT, 64, false>(st, a);
+    else prompt_one<ACT, 128, false>(st, a);
 }
 
 extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const void* q, const void* k, const void* v,
@@ -523,10 +574,11 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
             ka += k_lens[b];
         }
         if (!tiles) continue;
+        a.tiles = tiles;
         switch (d->type) {
-            case PF_TYPE_F32: prompt_dim<PF_TYPE_F32>(c->stream, tiles, a); break;
-            case PF_TYPE_F16: prompt_dim<PF_TYPE_F16>(c->stream, tiles, a); break;
-            default: prompt_dim<PF_TYPE_BF16>(c->stream, tiles, a); break;
+            case PF_TYPE_F32: prompt_dim<PF_TYPE_F32>(c->stream, a); break;
+            case PF_TYPE_F16: prompt_dim<PF_TYPE_F16>(c->stream, a); break;
+            default: prompt_dim<PF_TYPE_BF16>(c->stream, a); break;
         }
         PF_LAUNCHED(c);
     }
