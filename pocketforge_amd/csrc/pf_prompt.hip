@@ -292,8 +292,9 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     constexpr int C = DP / 16, DT = DP / 32;
     constexpr int CH = DP / 8, RPL = 64 / CH;    // chunks of a row, rows of one load of a wave
     constexpr int LOADS = PR_KEYS / 4 / RPL;     // loads of a wave per tile, K or V
-    __shared__ __align__(16) short sk[2][PR_KEYS * DP];
-    __shared__ __align__(16) short sv[2][PR_KEYS * DP];
+    // (buffers of their own: the compiler lets reads of one pass loads into the other)
+    __shared__ __align__(16) short sk0[PR_KEYS * DP], sk1[PR_KEYS * DP], sv0[PR_KEYS * DP], sv1[PR_KEYS * DP];
+    __shared__ int s_odd;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, row = lane & 31, half = lane >> 5;
 
     const PromptUnit unit = prompt_unit(blockIdx.x, a.tiles, a.n_heads / a.group, a.group);
@@ -319,34 +320,71 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         }
     }
 
-    // tiles that any row of the workgroup sees
+    // tiles that any row of the workgroup sees: sinks, then first .. last - 1;
+    // of those, all rows see wa .. wb - 1 whole.  These come first.
     const int p0 = off + r0, p1 = off + min(r0 + 128, nq) - 1;
     const int end = min(nk, a.causal ? p1 + 1 : nk);
     const int wlo = a.window ? max(0, p0 - a.window + 1) : 0;
-    const int first = wlo / PR_KEYS, last = (end + PR_KEYS - 1) / PR_KEYS;
-    const int sinks = min((a.sink + PR_KEYS - 1) / PR_KEYS, first);
-    const int tiles = end <= 0 ? 0 : max(0, last - first) + min(sinks, last);
-    // what this wave's rows see
-    const int w0 = p0 + wave * 32, w1 = min(w0 + 31, p1);
+    const int first = wlo / PR_KEYS, last = end <= 0 ? 0 : (end + PR_KEYS - 1) / PR_KEYS;
+    const int sinks = min(min((a.sink + PR_KEYS - 1) / PR_KEYS, first), last);
+    const int tiles = max(0, last - first) + sinks;
+    const int wa = a.window ? max(first, (max(0, p1 - a.window + 1) + PR_KEYS - 1) / PR_KEYS) : 0;
+    const int wb = max(wa, min(nk, a.causal ? max(0, p0 + 1) : nk) / PR_KEYS);
+    const int whole = tiles ? wb - wa : 0;
+    auto tile_of = [&](int it) {
+        if (it < whole) return wa + it;
+        it -= whole;
+        if (it < sinks) return it;
+        it += first - sinks;
+        return it < wa ? it : it + whole;
+    };
 
     const size_t kv_head = (size_t)(head / a.group) * a.dim;
     const short* kg = (const short*)a.k + (size_t)k0 * a.ks + kv_head;
     const short* vg = (const short*)a.v + (size_t)k0 * a.vs + kv_head;
+    // a lane's place in a tile's rows as 32-bit offsets from the tile's first row
     const int lr = lane / CH, lc = lane % CH;
-    auto load = [&](int it, int b) {
-        const int key0 = (it < sinks ? it : it - sinks + first) * PR_KEYS;
+    const bool near = (uint64_t)max(a.ks, a.vs) * (PR_KEYS * 2) <= 0xFFFFFFFFull;
+    uint32_t ko[LOADS], vo[LOADS];
+    auto chunks = [&](int r, int* ck, int* cv) {
+        *ck = k_place<DP>(r, lc);
+        *cv = v_place<DP>(r, lc);
+        if (!EXACT) {                            // (past head_dim: q's zeros, unused outputs)
+            *ck = min(*ck, (int)a.dim / 8 - 1);
+            *cv = min(*cv, (int)a.dim / 8 - 1);
+        }
+    };
 #pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            const int r = (wave * LOADS + i) * RPL + lr;
-            const uint32_t kr = (uint32_t)min(key0 + r, nk - 1);   // (rows past the end: masked)
-            int ck = k_place<DP>(r, lc), cv = v_place<DP>(r, lc);
-            if (!EXACT) {                                          // (past head_dim: q's zeros, unused outputs)
-                ck = min(ck, (int)a.dim / 8 - 1);
-                cv = min(cv, (int)a.dim / 8 - 1);
+    for (int i = 0; i < LOADS; i++) {
+        const int r = (wave * LOADS + i) * RPL + lr;
+        int ck, cv;
+        chunks(r, &ck, &cv);
+        ko[i] = (uint32_t)r * a.ks * 2 + (uint32_t)ck * 16;
+        vo[i] = (uint32_t)r * a.vs * 2 + (uint32_t)cv * 16;
+    }
+    auto load = [&](auto buf, int it) {
+        constexpr bool B = decltype(buf)::value;
+        const int key0 = tile_of(it) * PR_KEYS;
+        const uint8_t* kt = (const uint8_t*)(kg + (size_t)(uint32_t)key0 * a.ks);
+        const uint8_t* vt = (const uint8_t*)(vg + (size_t)(uint32_t)key0 * a.vs);
+        short *sk = B ? sk1 : sk0, *sv = B ? sv1 : sv0;
+        if (near && key0 + PR_KEYS <= nk) {
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int at = (wave * LOADS + i) * 64 * 8;
+                __builtin_amdgcn_global_load_lds((gvoid*)(kt + ko[i]), (lvoid*)&sk[at], 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gvoid*)(vt + vo[i]), (lvoid*)&sv[at], 16, 0, 0);
             }
-            const int at = (wave * LOADS + i) * 64 * 8;
-            __builtin_amdgcn_global_load_lds((gvoid*)(kg + (size_t)kr * a.ks + ck * 8), (lvoid*)&sk[b][at], 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gvoid*)(vg + (size_t)kr * a.vs + cv * 8), (lvoid*)&sv[b][at], 16, 0, 0);
+            return;
+        }
+        const int left = nk - 1 - key0;          // (rows past the end: the last one, masked)
+        for (int i = 0; i < LOADS; i++) {
+            const int r = (wave * LOADS + i) * RPL + lr, at = (wave * LOADS + i) * 64 * 8;
+            int ck, cv;
+            chunks(r, &ck, &cv);
+            const size_t kr = (size_t)(uint32_t)min(r, left);
+            __builtin_amdgcn_global_load_lds((gvoid*)(kt + kr * a.ks * 2 + ck * 16), (lvoid*)&sk[at], 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gvoid*)(vt + kr * a.vs * 2 + cv * 16), (lvoid*)&sv[at], 16, 0, 0);
         }
     };
 
@@ -355,28 +393,20 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     for (int t = 0; t < DT; t++) o[t] = (f16v)0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    // one tile; MASKED: some of this wave's rows do not see all of it
-    auto body = [&](auto masked, int b, int key0) {
-        constexpr bool MASKED = decltype(masked)::value;
-        // weights of zero must not meet infinities: V's values are looked through
-        // first (any of them times zero is a NaN)
-        bool odd = false;
-        if constexpr (MASKED) {
-            float z = 0.0f;
-#pragma unroll
-            for (int i = 0; i < PR_KEYS * DP / 512; i++) z = sum8<BF>(*(const s8v*)&sv[b][i * 512 + lane * 8], z, 0.0f);
-            odd = __any(z != z);
-        }
+    // one tile; MASKED: some rows do not see all of it
+    auto body = [&](auto masked, auto buf, int key0) {
+        constexpr bool MASKED = decltype(masked)::value, B = decltype(buf)::value;
+        const short* sk = B ? sk1 : sk0;
+        const short* sv = B ? sv1 : sv0;
         f16v s[2];
+        s[0] = s[1] = (f16v)0.0f;
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            s[g] = (f16v)0.0f;
+        for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                const s8v kf = *(const s8v*)&sk[b][(g * 32 + row) * DP + k_place<DP>(row, c * 2 + half) * 8];
+            for (int g = 0; g < 2; g++) {
+                const s8v kf = *(const s8v*)&sk[(g * 32 + row) * DP + k_place<DP>(row, c * 2 + half) * 8];
                 s[g] = mfma32<BF>(kf, qf[c], s[g]);
             }
-        }
         if constexpr (MASKED) {
             // one bit per key of the tile
             const uint64_t see = first_bits(min(hi, nk - 1) + 1 - key0) &
@@ -409,6 +439,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         }
         const float ms = m == -INFINITY ? 0.0f : m;
         s8v pf[4];
+        float l1 = 0.0f;
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
@@ -417,54 +448,98 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] = exp2_fast(__builtin_fmaf(s[g][8 * h + i], a.scale_log2, -ms));
                 pf[g * 2 + h] = pack8<BF>(x);
-                l = sum8<BF>(pf[g * 2 + h], l);
+                if (h) l = sum8<BF>(pf[g * 2 + h], l);
+                else l1 = sum8<BF>(pf[g * 2 + h], l1);
             }
-        auto weigh = [&](auto clean) {
-#pragma unroll
-            for (int gh = 0; gh < 4; gh++)       // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
-#pragma unroll
-                for (int t = 0; t < DT; t++) {
-                    const int r = gh * 16 + 4 * half + (lane & 15) / 4;
-                    const int c = t * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                    const short* vp = &sv[b][r * DP + v_place<DP>(r, c) * 8 + (lane & 1) * 4];
-                    const s4v x0 = lds_read_tr(vp), x1 = lds_read_tr(vp + 8 * DP);
-                    s8v vf = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    if constexpr (decltype(clean)::value) vf = finite_or_zero<BF>(vf);
-                    o[t] = mfma32<BF>(vf, pf[gh], o[t]);
-                }
+        l += l1;
+        // V^T of 16 keys (a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3) and 32 dims
+        auto v_operand = [&](int gh, int t) {
+            const int r = gh * 16 + 4 * half + (lane & 15) / 4;
+            const int c = t * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+            const short* vp = &sv[r * DP + v_place<DP>(r, c) * 8 + (lane & 1) * 4];
+            const s4v x0 = lds_read_tr(vp), x1 = lds_read_tr(vp + 8 * DP);
+            return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
-        if (!odd) {
-            weigh(std::false_type{});
-        } else {
-            weigh(std::true_type{});
-            // infinities and NaN reach the rows that see them, whatever their weight
-            for (int r = 0; r < PR_KEYS; r++) {
-                const int key = key0 + r;
-                if (key >= nk || !key_visible(key, hi, lo, a.sink)) continue;
+        s8v vf[2][DT];
 #pragma unroll
-                for (int t = 0; t < DT; t++)
+        for (int t = 0; t < DT; t++) vf[0][t] = v_operand(0, t);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int d = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                        const short w = sv[b][r * DP + v_place<DP>(r, d / 8) * 8 + d % 8];
-                        if (not_finite<BF>(w)) o[t][i] += to_float<ACT>(w);
-                    }
-            }
+        for (int gh = 0; gh < 4; gh++) {
+            if (gh < 3)
+#pragma unroll
+                for (int t = 0; t < DT; t++) vf[(gh + 1) & 1][t] = v_operand(gh + 1, t);
+#pragma unroll
+            for (int t = 0; t < DT; t++) o[t] = mfma32<BF>(vf[gh & 1][t], pf[gh], o[t]);
         }
     };
-
-    if (tiles) load(0, 0);
-    for (int it = 0; it < tiles; it++) {
-        const int b = it & 1, key0 = (it < sinks ? it : it - sinks + first) * PR_KEYS;
+    // A tile that some rows see in part: weights of zero must not meet
+    // infinities, so V's values are looked through first (any of them times zero
+    // is a NaN).  Those that are not finite reach the rows that see them,
+    // whatever their weight, and the products find zeros in their places.
+    auto clean = [&](auto buf, int it, int key0) {
+        constexpr bool B = decltype(buf)::value;
+        short* sv = B ? sv1 : sv0;
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) z = sum8<BF>(*(const s8v*)&sv[((wave * LOADS + i) * 64 + lane) * 8], z, 0.0f);
+        if (z != z) s_odd = it;
+        __syncthreads();
+        if (s_odd != it) return;
+        for (int r = 0; r < PR_KEYS; r++) {
+            const int key = key0 + r;
+            if (key >= nk || !key_visible(key, hi, lo, a.sink)) continue;
+#pragma unroll
+            for (int t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int d = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    const short w = sv[r * DP + v_place<DP>(r, d / 8) * 8 + d % 8];
+                    if (not_finite<BF>(w)) o[t][i] += to_float<ACT>(w);
+                }
+        }
+        __syncthreads();
+        for (int i = 0; i < LOADS; i++) {
+            s8v* x = (s8v*)&sv[((wave * LOADS + i) * 64 + lane) * 8];
+            *x = finite_or_zero<BF>(*x);
+        }
+        __syncthreads();
+    };
+    // before a tile: it is whole in LDS, and nobody reads the one before it
+    auto turn = [&] {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                         // this tile is whole, and nobody reads the one before
-        if (it + 1 < tiles) load(it + 1, b ^ 1);
-        if ((a.causal && key0 > w1) || (a.window && key0 + PR_KEYS <= w0 - a.window + 1 && key0 >= a.sink)) continue;
-        const bool whole = key0 + PR_KEYS <= nk && (!a.causal || key0 + PR_KEYS - 1 <= w0) &&
-                           (!a.window || key0 >= w1 - a.window + 1 || key0 + PR_KEYS <= a.sink);
+        __syncthreads();
+    };
+    // this wave's rows see something of the tile
+    auto some = [&](int key0) {
+        const int w0 = p0 + wave * 32, w1 = min(w0 + 31, p1);
+        return !((a.causal && key0 > w1) | (a.window && key0 + PR_KEYS <= w0 - a.window + 1 && key0 >= a.sink));
+    };
+    constexpr std::false_type no{};
+    constexpr std::true_type yes{};
 
-        if (whole) body(std::false_type{}, b, key0);
-        else body(std::true_type{}, b, key0);
+    if (tid == 0) s_odd = -1;
+    if (tiles) load(no, 0);
+    int it = 0;
+    for (; it + 1 < whole; it += 2) {
+        turn();
+        load(yes, it + 1);
+        body(no, no, 0);
+        turn();
+        if (it + 2 < tiles) load(no, it + 2);
+        body(no, yes, 0);
+    }
+    for (; it < tiles; it += 2) {                // (at most one whole tile among these)
+        int key0 = tile_of(it) * PR_KEYS;
+        turn();
+        if (it + 1 < tiles) load(yes, it + 1);
+        clean(no, it, key0);
+        if (some(key0)) body(yes, no, key0);
+        if (it + 1 >= tiles) break;
+        key0 = tile_of(it + 1) * PR_KEYS;
+        turn();
+        if (it + 2 < tiles) load(no, it + 2);
+        clean(yes, it + 1, key0);
+        if (some(key0)) body(yes, yes, key0);
     }
 
     l = sum32(l);
