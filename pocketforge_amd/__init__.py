@@ -254,15 +254,19 @@ class DeviceArray:
 
 
 _NUMPY = {TYPE_F32: np.float32, TYPE_F16: np.float16, TYPE_BF16: np.uint16}
+_TYPE_OF = {}
 _TYPES = {"float32": TYPE_F32, "float16": TYPE_F16, "bfloat16": TYPE_BF16, "uint16": TYPE_BF16}
 
 
 def _type(t):
     """Element type of a device array: its dtype, with uint16 for bf16 bits (numpy has no bf16)."""
-    name = str(t.dtype).replace("torch.", "")
-    if name not in _TYPES:
-        raise PFError(f"rows are float32, float16 or bfloat16, not {name}")
-    return _TYPES[name]
+    try:
+        return _TYPE_OF[t.dtype]
+    except KeyError:
+        name = str(t.dtype).replace("torch.", "")
+        if name not in _TYPES:
+            raise PFError(f"rows are float32, float16 or bfloat16, not {name}") from None
+        return _TYPE_OF.setdefault(t.dtype, _TYPES[name])
 
 
 def _rows(t, what):
@@ -271,20 +275,27 @@ def _rows(t, what):
     rows lie apart, as the parts of a fused QKV product do."""
     if len(t.shape) != 3:
         raise PFError(f"{what} is [rows][heads][head_dim], not {tuple(t.shape)}")
-    n, h, d = (int(x) for x in t.shape)
+    n, h, d = t.shape
     if isinstance(t, DeviceArray):
-        return n, h, d, h * d
-    s = t.stride()
-    if (d > 1 and s[2] != 1) or (h > 1 and s[1] != d):
+        return int(n), int(h), int(d), int(h * d)
+    s, sh, sd = t.stride()
+    if (d > 1 and sd != 1) or (h > 1 and sh != d):
         raise PFError(f"{what}: the heads of a row lie one after another")
-    return n, h, d, (s[0] if n > 1 else h * d)
+    return n, h, d, (s if n > 1 else h * d)
 
 
 def _u32(a, what):
-    a = np.atleast_1d(np.asarray(a))
-    if a.size and (a.dtype.kind not in "iu" or a.ndim != 1 or a.min() < 0 or a.max() > 0xFFFFFFFF):
+    """A list of numbers from 0 as a C array."""
+    if type(a) is list or type(a) is tuple:
+        try:
+            if not a or (min(a) >= 0 and max(a) <= 0xFFFFFFFF):
+                return (C.c_uint32 * len(a))(*a)
+        except TypeError:
+            pass
+    x = np.atleast_1d(np.asarray(a))
+    if x.ndim != 1 or (x.size and (x.dtype.kind not in "iu" or x.min() < 0 or x.max() > 0xFFFFFFFF)):
         raise PFError(f"{what} is a list of numbers from 0")
-    return np.ascontiguousarray(a, np.uint32)
+    return (C.c_uint32 * x.size)(*x.tolist())
 
 
 def _vptr(a):
@@ -439,18 +450,20 @@ class Context:
         ql = _u32(q_lens, "q_lens")
         kl = ql if k_lens is None else _u32(k_lens, "k_lens")
         nq, H, D, qs = _rows(q, "q")
-        nk, G, _, ks = _rows(k, "k")
-        vs = _rows(v, "v")[3]
-        if tuple(k.shape) != tuple(v.shape) or int(k.shape[2]) != D:
+        nk, G, D1, ks = _rows(k, "k")
+        n1, G1, D2, vs = _rows(v, "v")
+        if (n1, G1) != (nk, G) or D1 != D or D2 != D:
             raise PFError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are alike, with q's head_dim {D}")
-        if len(kl) != len(ql) or int(ql.sum(dtype=np.int64)) != nq or int(kl.sum(dtype=np.int64)) != nk:
+        if len(kl) != len(ql) or sum(ql) != nq or sum(kl) != nk:
             raise PFError("q_lens and k_lens name every row of q and of k")
-        y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[_type(q)]) if out is None else out
-        if tuple(y.shape) != (nq, H, D) or len({_type(t) for t in (q, k, v, y)}) != 1:
+        t = _type(q)
+        y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        n2, H2, D3, os = _rows(y, "out")
+        if (n2, H2, D3) != (nq, H, D) or not t == _type(k) == _type(v) == _type(y):
             raise PFError("q, k, v and out have one type, q and out one shape")
-        d = AttnDesc(_type(q), H, G, D, int(causal), window, sink, scale, qs, ks, vs, _rows(y, "out")[3])
-        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), _vptr(ql),
-                                             _vptr(kl), len(ql)), "pf_prompt_attention")
+        d = AttnDesc(t, H, G, D, causal, window, sink, scale, qs, ks, vs, os)
+        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), ql, kl,
+                                             len(ql)), "pf_prompt_attention")
         if out is None:
             self.synchronize()
         return y
@@ -596,17 +609,18 @@ class PagedCache:
         s, r = _u32(seqs, "seqs"), _u32(rows, "rows")
         if len(s) != len(r):
             raise PFError("seqs and rows have one length")
-        self.ctx.check(lib().pf_pages_append(self.h, _vptr(s), _vptr(r), len(s)), "pf_pages_append")
-        self.pass_rows = int(r.sum(dtype=np.int64))
+        self.ctx.check(lib().pf_pages_append(self.h, s, r, len(s)), "pf_pages_append")
+        self.pass_rows = sum(r)
 
     def _kv(self, k, v, rows):
         n, h, d, ks = _rows(k, "k")
-        vs = _rows(v, "v")[3]
-        if tuple(k.shape) != tuple(v.shape) or (n, h, d) != (rows, self.n_kv_heads, self.head_dim):
+        n1, h1, d1, vs = _rows(v, "v")
+        if (n, h, d) != (n1, h1, d1) or (n, h, d) != (rows, self.n_kv_heads, self.head_dim):
             raise PFError(f"k and v are [{rows}][{self.n_kv_heads}][{self.head_dim}], not {tuple(k.shape)}, {tuple(v.shape)}")
-        if _type(k) != _type(v):
+        t = _type(k)
+        if t != _type(v):
             raise PFError("k and v have one type")
-        return _type(k), ks, vs
+        return t, ks, vs
 
     def store(self, layer, k, v):
         """The pass's new rows of one layer."""
@@ -616,10 +630,12 @@ class PagedCache:
     def attention(self, layer, q, causal=True, window=0, sink=0, scale=0.0, out=None):
         """The pass's rows over their sequences.  With `out` asynchronous, as Context.prompt_attention."""
         n, H, D, qs = _rows(q, "q")
-        y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[_type(q)]) if out is None else out
-        if n != self.pass_rows or tuple(y.shape) != (n, H, D) or _type(y) != _type(q):
+        t = _type(q)
+        y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        n1, H1, D1, os = _rows(y, "out")
+        if n != self.pass_rows or (n1, H1, D1) != (n, H, D) or _type(y) != t:
             raise PFError(f"q and out are [{self.pass_rows}][heads][{self.head_dim}] of one type")
-        d = AttnDesc(_type(q), H, self.n_kv_heads, D, int(causal), window, sink, scale, qs, 0, 0, _rows(y, "out")[3])
+        d = AttnDesc(t, H, self.n_kv_heads, D, causal, window, sink, scale, qs, 0, 0, os)
         self.ctx.check(lib().pf_pages_attention(self.h, C.byref(d), layer, _dptr(q), _dptr(y)), "pf_pages_attention")
         if out is None:
             self.ctx.synchronize()
@@ -628,13 +644,15 @@ class PagedCache:
     def gather(self, layer, seqs, out=None, dtype=np.float32):
         """The sequences' rows of one layer, packed: (k, v)."""
         s = _u32(seqs, "seqs")
-        n = sum(self.length(i) for i in s)
+        lens = np.zeros(len(s), np.int64)
+        self.ctx.check(lib().pf_pages_tables(self.h, s, len(s), None, 0, _vptr(lens)), "pf_pages_tables")
+        n = int(lens.sum())
         if out is None:
             k, v = (self.ctx.empty((n, self.n_kv_heads, self.head_dim), dtype) for _ in range(2))
         else:
             k, v = out
         t, ks, vs = self._kv(k, v, n)
-        self.ctx.check(lib().pf_pages_gather(self.h, layer, _vptr(s), len(s), t, _dptr(k), _dptr(v), ks, vs),
+        self.ctx.check(lib().pf_pages_gather(self.h, layer, s, len(s), t, _dptr(k), _dptr(v), ks, vs),
                        "pf_pages_gather")
         if out is None:
             self.ctx.synchronize()
@@ -642,23 +660,23 @@ class PagedCache:
 
     def fork(self, src, dst):
         d = _u32(dst, "dst")
-        self.ctx.check(lib().pf_pages_fork(self.h, src, _vptr(d), len(d)), "pf_pages_fork")
+        self.ctx.check(lib().pf_pages_fork(self.h, src, d, len(d)), "pf_pages_fork")
 
     def copy(self, src, dst):
         s, d = _u32(src, "src"), _u32(dst, "dst")
         if len(s) != len(d):
             raise PFError("src and dst have one length")
-        self.ctx.check(lib().pf_pages_copy(self.h, _vptr(s), _vptr(d), len(d)), "pf_pages_copy")
+        self.ctx.check(lib().pf_pages_copy(self.h, s, d, len(d)), "pf_pages_copy")
 
     def truncate(self, seqs, lengths):
         s, n = _u32(seqs, "seqs"), _u32(lengths, "lengths")
         if len(s) != len(n):
             raise PFError("seqs and lengths have one length")
-        self.ctx.check(lib().pf_pages_truncate(self.h, _vptr(s), _vptr(n), len(s)), "pf_pages_truncate")
+        self.ctx.check(lib().pf_pages_truncate(self.h, s, n, len(s)), "pf_pages_truncate")
 
     def free(self, seqs):
         s = _u32(seqs, "seqs")
-        self.ctx.check(lib().pf_pages_free(self.h, _vptr(s), len(s)), "pf_pages_free")
+        self.ctx.check(lib().pf_pages_free(self.h, s, len(s)), "pf_pages_free")
 
     def compact(self):
         """The number of pages that moved."""
@@ -673,10 +691,10 @@ class PagedCache:
         """Page numbers of the sequences, -1 past their ends, and their lengths."""
         s = _u32(seqs, "seqs")
         lens = np.zeros(len(s), np.int64)
-        self.ctx.check(lib().pf_pages_tables(self.h, _vptr(s), len(s), None, 0, _vptr(lens)), "pf_pages_tables")
+        self.ctx.check(lib().pf_pages_tables(self.h, s, len(s), None, 0, _vptr(lens)), "pf_pages_tables")
         cap = -(-int(lens.max(initial=0)) // self.page_size)
         pages = np.empty((len(s), cap), np.int64)
-        self.ctx.check(lib().pf_pages_tables(self.h, _vptr(s), len(s), _vptr(pages), cap, None), "pf_pages_tables")
+        self.ctx.check(lib().pf_pages_tables(self.h, s, len(s), _vptr(pages), cap, None), "pf_pages_tables")
         return pages, lens
 
     def planes(self, layer=None):

@@ -85,6 +85,7 @@ struct pf_pages {
     std::vector<uint32_t> refs, len;               // per page, per sequence
     std::vector<std::vector<uint32_t>> pages;      // per sequence
     std::vector<uint32_t> heap;                    // free pages, lowest first
+    std::vector<uint32_t> dirty;                   // table entries that the device has not heard of
     std::vector<uint32_t> mark;                    // per sequence: last call that named it
     uint32_t stamp = 0;
 

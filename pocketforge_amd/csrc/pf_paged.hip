@@ -281,31 +281,60 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
     }
 }
 
-// Joins the parts of the sequences that were cut: one workgroup per (item that
-// begins a sequence, head), its rows one after another.
+// Joins the parts of the sequences that were cut: one workgroup per (sequence's
+// first item, head), its rows one after another.  8 groups of 32 threads take
+// every eighth part, 4 dims a thread; then the groups meet in LDS, in order.
 template <int ACT>
-__global__ __launch_bounds__(128) void k_paged_join(PagedArgs a) {
+__global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
     const PageItem it = a.items[blockIdx.x];
     if (it.parts == 1 || it.t0 != 0) return;
-    const uint32_t h = blockIdx.y, d = threadIdx.x;
+    __shared__ float s_f[PG_GROUPS + 1], s_red[2][4];
+    __shared__ __align__(16) float s_o[8][128];
+    const uint32_t h = blockIdx.y, tid = threadIdx.x, grp = tid >> 5, d = (tid & 31) * 4, wave = tid >> 6;
     for (uint32_t j = blockIdx.z; j < it.rows; j += gridDim.z) {
-        float M = -INFINITY;
-        for (uint32_t p = 0; p < it.parts; p++)
-            M = fmaxf(M, a.ws_ml[2 * ((size_t)(it.ws0 + p * it.rows + j) * a.n_heads + h)]);
+        const size_t w0 = (size_t)(it.ws0 + j) * a.n_heads + h, step = (size_t)it.rows * a.n_heads;
+        float M = -INFINITY, L = 0.0f;
+        for (uint32_t p = tid; p < it.parts; p += 256) M = fmaxf(M, a.ws_ml[2 * (w0 + p * step)]);
+#pragma unroll
+        for (int b = 1; b < 64; b <<= 1) M = fmaxf(M, __shfl_xor(M, b));
+        if ((tid & 63) == 0) s_red[0][wave] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
         const float ms = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f, acc = 0.0f;
-        for (uint32_t p = 0; p < it.parts; p++) {
-            const size_t w = (size_t)(it.ws0 + p * it.rows + j) * a.n_heads + h;
-            const float f = exp2_fast(a.ws_ml[2 * w] - ms);
-            L += f * a.ws_ml[2 * w + 1];
-            if (d < a.dim) acc += f * a.ws_o[w * a.dim + d];
+        for (uint32_t p = tid; p < it.parts; p += 256) {
+            const float f = exp2_fast(a.ws_ml[2 * (w0 + p * step)] - ms);
+            L += f * a.ws_ml[2 * (w0 + p * step) + 1];
+            s_f[p] = f;
         }
-        if (d >= a.dim) continue;
-        const float y = acc / L;
-        const size_t at = (size_t)(it.q0 + j) * a.os + (size_t)h * a.dim + d;
-        if constexpr (ACT == PF_TYPE_F32) ((float*)a.out)[at] = y;
-        else if constexpr (ACT == PF_TYPE_BF16) ((__bf16*)a.out)[at] = (__bf16)y;
-        else ((_Float16*)a.out)[at] = (_Float16)y;
+#pragma unroll
+        for (int b = 1; b < 64; b <<= 1) L += __shfl_xor(L, b);
+        if ((tid & 63) == 0) s_red[1][wave] = L;
+        __syncthreads();
+        L = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+        f4v acc = (f4v)0.0f;
+        if (d < a.dim) {
+#pragma unroll 4
+            for (uint32_t p = grp; p < it.parts; p += 8) {
+                const f4v x = *(const f4v*)(a.ws_o + (w0 + p * step) * a.dim + d);
+                const float f = s_f[p];
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[i] += f * x[i];
+            }
+        }
+        *(f4v*)&s_o[grp][d] = acc;
+        __syncthreads();
+        if (tid < 32 && d < a.dim) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float t = 0.0f;
+#pragma unroll
+                for (int g = 0; g < 8; g++) t += s_o[g][d + i];
+                y[i] = t / L;
+            }
+            store4<ACT>((uint8_t*)a.out + ((size_t)(it.q0 + j) * a.os + (size_t)h * a.dim + d) * act_size<ACT>, y);
+        }
+        __syncthreads();
     }
 }
 
@@ -333,7 +362,7 @@ static void paged_dim(hipStream_t st, uint32_t items, uint32_t most, const Paged
 
 // Cuts the pass's keys: enough workgroups for every compute unit several times
 // over, none with less than PG_LEAST tiles.
-constexpr uint32_t PG_LEAST = 16;
+constexpr uint32_t PG_LEAST = 4;
 static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
     PageSplit& u = p->cut;
     if (u.type == d->type && u.window == s.window && u.sink == s.sink && u.heads == d->n_heads) return PF_OK;
@@ -420,9 +449,9 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
     PF_LAUNCHED(c);
     if (u.split) {
         const dim3 grid(u.n_items, d->n_heads, std::min(u.most_rows, 64u));
-        if (d->type == PF_TYPE_F32) hipLaunchKernelGGL(k_paged_join<PF_TYPE_F32>, grid, dim3(128), 0, st, a);
-        else if (d->type == PF_TYPE_F16) hipLaunchKernelGGL(k_paged_join<PF_TYPE_F16>, grid, dim3(128), 0, st, a);
-        else hipLaunchKernelGGL(k_paged_join<PF_TYPE_BF16>, grid, dim3(128), 0, st, a);
+        if (d->type == PF_TYPE_F32) hipLaunchKernelGGL(k_paged_join<PF_TYPE_F32>, grid, dim3(256), 0, st, a);
+        else if (d->type == PF_TYPE_F16) hipLaunchKernelGGL(k_paged_join<PF_TYPE_F16>, grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(k_paged_join<PF_TYPE_BF16>, grid, dim3(256), 0, st, a);
         PF_LAUNCHED(c);
     }
     return PF_OK;

@@ -12,23 +12,33 @@
 
 #include <cstring>
 #include <functional>
-#include <utility>
 
 using namespace pf;
 
 namespace pf {
 
-// Takes a staged message to its places: `words` words to dst, then `pairs`
-// (index, value) pairs into the page table.  One workgroup; the message lies in
-// pinned host memory, which it reads once.
+// Takes a message to its places: `words` words to dst, then `pairs` (index,
+// value) pairs into the page table.  One workgroup.  Small messages come as the
+// kernel's arguments (nothing to keep until it has run), others lie in pinned
+// host memory.
+__device__ __forceinline__ void pages_apply(const uint32_t* msg, uint32_t words, uint32_t* dst, uint32_t pairs,
+                                            int32_t* table) {
+    for (uint32_t i = threadIdx.x; i < words; i += blockDim.x) dst[i] = msg[i];
+    for (uint32_t i = threadIdx.x; i < pairs; i += blockDim.x) table[msg[words + 2 * i]] = (int32_t)msg[words + 2 * i + 1];
+}
 __global__ __launch_bounds__(1024) void k_pages_apply(const uint32_t* msg, uint32_t words, uint32_t* dst, uint32_t pairs,
                                                      int32_t* table) {
-    for (uint32_t i = threadIdx.x; i < words; i += 1024) dst[i] = msg[i];
-    const uint2* pr = (const uint2*)(msg + ((words + 1) & ~1u));
-    for (uint32_t i = threadIdx.x; i < pairs; i += 1024) {
-        const uint2 w = pr[i];
-        table[w.x] = (int32_t)w.y;
-    }
+    pages_apply(msg, words, dst, pairs, table);
+}
+constexpr uint32_t SMALL_WORDS = 896;
+struct SmallMessage {
+    uint32_t* dst;
+    int32_t* table;
+    uint32_t words, pairs;
+    uint32_t msg[SMALL_WORDS];
+};
+__global__ __launch_bounds__(256) void k_pages_apply_small(SmallMessage m) {
+    pages_apply(m.msg, m.words, m.dst, m.pairs, m.table);
 }
 
 // The sequence of a packed row: the last one whose first row is not past it
@@ -163,15 +173,18 @@ __global__ __launch_bounds__(256) void k_pages_gather(GatherArgs a) {
 
 // Copies pages: (from, to, rows) of every layer and head, K and V and the int8
 // scales.  One workgroup takes one (copy, layer) and a share of its heads.
+constexpr uint32_t FEW_MOVES = 256;
 struct MoveArgs {
-    const uint32_t* pairs;        // 3 words each
+    const uint32_t* pairs;        // 3 words each; NULL: these
+    uint32_t few[3 * FEW_MOVES];
     uint8_t *k, *v;
     float *ks, *vs;
     uint32_t kv_heads, page_size, row_bytes;
     size_t plane, scales;         // of one layer
 };
 __global__ __launch_bounds__(256) void k_pages_move(MoveArgs a) {
-    const uint32_t src = a.pairs[3 * blockIdx.x], dst = a.pairs[3 * blockIdx.x + 1], rows = a.pairs[3 * blockIdx.x + 2];
+    const uint32_t* pr = (a.pairs ? a.pairs : a.few) + 3 * blockIdx.x;
+    const uint32_t src = pr[0], dst = pr[1], rows = pr[2];
     const size_t head_bytes = (size_t)a.page_size * a.row_bytes, page = head_bytes * a.kv_heads;
     const uint32_t n16 = rows * a.row_bytes / 16;             // of one head
     for (uint32_t h = blockIdx.z; h < a.kv_heads; h += gridDim.z) {
@@ -229,32 +242,61 @@ static pf_status stage_send(pf_pages* p, const uint32_t* msg, uint32_t words, vo
     return PF_OK;
 }
 
-// Words to device memory, with table changes behind them in the last message.
-typedef std::vector<std::pair<uint32_t, uint32_t>> TableChanges;
-static pf_status stage_all(pf_pages* p, void* dst, const void* src, size_t bytes, const TableChanges* ch) {
+// Words to device memory, and table entries (by index; the values are the
+// host's) behind them.
+static pf_status stage_all(pf_pages* p, void* dst, const void* src, size_t bytes, const std::vector<uint32_t>& changed) {
+    const size_t n = changed.size();
+    const auto value = [&](uint32_t at, uint32_t* v) {
+        const std::vector<uint32_t>& t = p->pages[at / p->per_seq];
+        if (at % p->per_seq >= t.size()) return false;       // dropped since
+        *v = t[at % p->per_seq];
+        return true;
+    };
+    if (!bytes && !n) return PF_OK;
+    if (bytes / 4 + 2 * n <= SMALL_WORDS) {
+        SmallMessage m;
+        m.dst = (uint32_t*)dst; m.table = p->table; m.words = (uint32_t)(bytes / 4); m.pairs = 0;
+        if (bytes) std::memcpy(m.msg, src, bytes);
+        for (uint32_t at : changed) {
+            uint32_t* w = m.msg + m.words + 2 * m.pairs;
+            if (!value(at, w + 1)) continue;
+            w[0] = at;
+            m.pairs++;
+        }
+        hipLaunchKernelGGL(k_pages_apply_small, dim3(1), dim3(256), 0, p->ctx->stream, m);
+        PF_LAUNCHED(p->ctx);
+        return PF_OK;
+    }
     size_t at = 0, c = 0;
-    const size_t n = ch ? ch->size() : 0;
     while (at < bytes || c < n) {
         uint32_t* m = nullptr;
         if (pf_status st = stage_slot(p, &m)) return st;
         const size_t take = std::min(bytes - at, STAGE_BYTES);
         if (take) std::memcpy(m, (const uint8_t*)src + at, take);
-        const uint32_t words = (uint32_t)(take / 4), w2 = (words + 1) & ~1u;
-        const size_t room = (STAGE_BYTES / 4 - std::min<size_t>(w2, STAGE_BYTES / 4)) / 2;
-        const uint32_t pairs = at + take == bytes ? (uint32_t)std::min(n - c, room) : 0;
-        for (uint32_t i = 0; i < pairs; i++) {
-            m[w2 + 2 * i] = (*ch)[c + i].first;
-            m[w2 + 2 * i + 1] = (*ch)[c + i].second;
-        }
+        const uint32_t words = (uint32_t)(take / 4), room = (uint32_t)(STAGE_BYTES / 4 - words) / 2;
+        uint32_t pairs = 0;
+        if (at + take == bytes)
+            for (; c < n && pairs < room; c++) {
+                uint32_t* w = m + words + 2 * pairs;
+                if (!value(changed[c], w + 1)) continue;
+                w[0] = changed[c];
+                pairs++;
+            }
         if (pf_status st = stage_send(p, m, words, dst ? (uint8_t*)dst + at : nullptr, pairs)) return st;
         at += take;
-        c += pairs;
     }
     return PF_OK;
 }
 
 pf_status pages_upload(pf_pages* p, void* dst_dev, const void* src, size_t bytes) {
-    return stage_all(p, dst_dev, src, bytes, nullptr);
+    return stage_all(p, dst_dev, src, bytes, {});
+}
+
+// Table entries that have changed since the device last heard.
+static pf_status tables_to_device(pf_pages* p) {
+    if (pf_status st = stage_all(p, nullptr, nullptr, 0, p->dirty)) return st;
+    p->dirty.clear();
+    return PF_OK;
 }
 
 // ============================================================ page copies
@@ -265,9 +307,15 @@ static pf_status move_pages(pf_pages* p, const std::vector<uint32_t>& moves) {
     const pf_pages_config& g = p->cfg;
     for (size_t at = 0; at < moves.size() / 3; at += MOVE_MOST) {
         const uint32_t n = (uint32_t)std::min(MOVE_MOST, moves.size() / 3 - at);
-        if (pf_status st = pages_upload(p, p->pairs, moves.data() + 3 * at, (size_t)n * 12)) return st;
-        MoveArgs a{};
-        a.pairs = p->pairs; a.k = (uint8_t*)p->k; a.v = (uint8_t*)p->v; a.ks = p->ks; a.vs = p->vs;
+        MoveArgs a;
+        a.pairs = nullptr;
+        if (n <= FEW_MOVES) {
+            std::memcpy(a.few, moves.data() + 3 * at, (size_t)n * 12);
+        } else {
+            if (pf_status st = pages_upload(p, p->pairs, moves.data() + 3 * at, (size_t)n * 12)) return st;
+            a.pairs = p->pairs;
+        }
+        a.k = (uint8_t*)p->k; a.v = (uint8_t*)p->v; a.ks = p->ks; a.vs = p->vs;
         a.kv_heads = g.n_kv_heads; a.page_size = g.page_size; a.row_bytes = (uint32_t)(g.head_dim * p->esize);
         a.plane = p->plane; a.scales = p->scales;
         hipLaunchKernelGGL(k_pages_move, dim3(n, g.n_layers, std::min(g.n_kv_heads, 65535u)), dim3(256), 0, p->ctx->stream, a);
@@ -304,9 +352,12 @@ static void more_pages(pf_pages* p, uint32_t seq, size_t n) {
     std::vector<uint32_t>& t = p->pages[seq];
     if (t.capacity() < n) t.reserve(std::max(n, 2 * t.capacity()));
 }
-static void change(const pf_pages* p, TableChanges* ch, uint32_t seq, uint32_t at) {
-    ch->push_back({seq * p->per_seq + at, p->pages[seq][at]});
+// The device's tables learn of changes with the next pass, or the next call that
+// reads them.  (Room for `n` of them before anything changes.)
+static void more_changes(pf_pages* p, size_t n) {
+    if (p->dirty.capacity() - p->dirty.size() < n) p->dirty.reserve(std::max(p->dirty.size() + n, 2 * p->dirty.capacity()));
 }
+static void change(pf_pages* p, uint32_t seq, uint32_t at) { p->dirty.push_back(seq * p->per_seq + at); }
 
 // In range and named once.
 static pf_status distinct(pf_pages* p, const uint32_t* seqs, uint32_t n) {
@@ -483,9 +534,8 @@ static pf_status pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t*
 
     DeviceScope on(c);
     // (all host memory that the changes need first)
-    TableChanges ch;
     std::vector<uint32_t> moves;
-    ch.reserve(need);
+    more_changes(p, need);
     moves.reserve(3 * copies);
     for (uint32_t i = 0; i < n; i++) more_pages(p, seqs[i], pages_for(p, p->len[seqs[i]] + rows[i]));
     p->pass.clear();
@@ -499,11 +549,11 @@ static pf_status pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t*
             t.back() = take_page(p);
             p->refs[old]--;
             moves.insert(moves.end(), {old, t.back(), used});
-            change(p, &ch, s, (uint32_t)t.size() - 1);
+            change(p, s, (uint32_t)t.size() - 1);
         }
         while (t.size() < pages_for(p, have + rows[i])) {
             t.push_back(take_page(p));
-            change(p, &ch, s, (uint32_t)t.size() - 1);
+            change(p, s, (uint32_t)t.size() - 1);
         }
         p->len[s] = have + rows[i];
         p->pass.push_back({s, q0, rows[i], p->len[s]});
@@ -514,7 +564,8 @@ static pf_status pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t*
     p->uniform = uniform;
     p->cut = PageSplit();
     p->open = false;
-    if (pf_status st = stage_all(p, p->seqs, p->pass.data(), p->pass.size() * sizeof(PageSeq), &ch)) return st;
+    if (pf_status st = stage_all(p, p->seqs, p->pass.data(), p->pass.size() * sizeof(PageSeq), p->dirty)) return st;
+    p->dirty.clear();
     if (pf_status st = move_pages(p, moves)) return st;
     p->open = true;
     return PF_OK;
@@ -605,6 +656,7 @@ extern "C" pf_status pf_pages_gather(pf_pages* p, uint32_t layer, const uint32_t
         if (kst != vst || off < w * es || off > (kst - w) * es) return fail(c, PF_ERR_ARG, "pages: k and v overlap");
     }
     DeviceScope on(c);
+    if (pf_status st = no_throw(c, [&] { return tables_to_device(p); })) return st;
     GatherArgs a{};
     a.table = p->table; a.k = k; a.v = v;
     a.pk = (const uint8_t*)p->k + layer * p->plane; a.pv = (const uint8_t*)p->v + layer * p->plane;
@@ -638,9 +690,7 @@ static pf_status pages_fork(pf_pages* p, uint32_t src, const uint32_t* dst, uint
     if (src >= p->cfg.max_seqs) return fail(p->ctx, PF_ERR_ARG, "pages: sequence out of range");
     if (pf_status st = all_empty(p, dst, n)) return st;
     if (!n || !p->len[src]) return PF_OK;
-    DeviceScope on(p->ctx);
-    TableChanges ch;
-    ch.reserve((size_t)n * p->pages[src].size());
+    more_changes(p, (size_t)n * p->pages[src].size());
     for (uint32_t i = 0; i < n; i++) more_pages(p, dst[i], p->pages[src].size());
     end_pass(p);
     for (uint32_t i = 0; i < n; i++) {
@@ -648,10 +698,10 @@ static pf_status pages_fork(pf_pages* p, uint32_t src, const uint32_t* dst, uint
         p->len[dst[i]] = p->len[src];
         for (uint32_t j = 0; j < p->pages[src].size(); j++) {
             p->refs[p->pages[src][j]]++;
-            change(p, &ch, dst[i], j);
+            change(p, dst[i], j);
         }
     }
-    return stage_all(p, nullptr, nullptr, 0, &ch);
+    return PF_OK;
 }
 extern "C" pf_status pf_pages_fork(pf_pages* p, uint32_t src, const uint32_t* dst, uint32_t n) {
     if (!p) return PF_ERR_ARG;
@@ -668,9 +718,8 @@ static pf_status pages_copy(pf_pages* p, const uint32_t* src, const uint32_t* ds
     }
     if (need > p->heap.size()) return fail(p->ctx, PF_ERR_CAPACITY, "pages: too few free pages");
     DeviceScope on(p->ctx);
-    TableChanges ch;
     std::vector<uint32_t> moves;
-    ch.reserve(need);
+    more_changes(p, need);
     moves.reserve(3 * need);
     for (uint32_t i = 0; i < n; i++) more_pages(p, dst[i], p->pages[src[i]].size());
     end_pass(p);
@@ -681,11 +730,10 @@ static pf_status pages_copy(pf_pages* p, const uint32_t* src, const uint32_t* ds
             const uint32_t page = take_page(p);
             p->pages[dst[i]].push_back(page);
             moves.insert(moves.end(), {from[j], page, p->cfg.page_size});
-            change(p, &ch, dst[i], j);
+            change(p, dst[i], j);
         }
         p->len[dst[i]] = p->len[src[i]];
     }
-    if (pf_status st = stage_all(p, nullptr, nullptr, 0, &ch)) return st;
     return move_pages(p, moves);
 }
 extern "C" pf_status pf_pages_copy(pf_pages* p, const uint32_t* src, const uint32_t* dst, uint32_t n) {
@@ -730,19 +778,23 @@ static pf_status pages_compact(pf_pages* p, uint32_t* moved) {
         moves.insert(moves.end(), {page, hole, p->cfg.page_size});
         to[page - used] = hole++;
     }
-    TableChanges ch;
-    for (uint32_t s = 0; s < p->cfg.max_seqs; s++)
-        for (uint32_t j = 0; j < p->pages[s].size(); j++)
-            if (p->pages[s][j] >= used) ch.push_back({s * p->per_seq + j, to[p->pages[s][j] - used]});
+    size_t named = 0;
+    for (const std::vector<uint32_t>& t : p->pages)
+        for (uint32_t page : t) named += page >= used;
+    more_changes(p, named);
     DeviceScope on(p->ctx);
     end_pass(p);
     if (moves.empty()) return PF_OK;
-    for (const auto& x : ch) p->pages[x.first / p->per_seq][x.first % p->per_seq] = x.second;
+    for (uint32_t s = 0; s < p->cfg.max_seqs; s++)
+        for (uint32_t j = 0; j < p->pages[s].size(); j++)
+            if (p->pages[s][j] >= used) {
+                p->pages[s][j] = to[p->pages[s][j] - used];
+                change(p, s, j);
+            }
     for (size_t i = 0; i < moves.size(); i += 3) std::swap(p->refs[moves[i]], p->refs[moves[i + 1]]);
     for (uint32_t i = 0; i < p->heap.size(); i++) p->heap[i] = used + i;
     if (moved) *moved = (uint32_t)(moves.size() / 3);
-    if (pf_status st = move_pages(p, moves)) return st;
-    return stage_all(p, nullptr, nullptr, 0, &ch);
+    return move_pages(p, moves);
 }
 extern "C" pf_status pf_pages_compact(pf_pages* p, uint32_t* moved) {
     if (!p) return PF_ERR_ARG;
