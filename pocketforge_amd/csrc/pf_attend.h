@@ -30,6 +30,10 @@ constexpr float LOG2E = 1.4426950408889634f;
 // products are the whole product.
 template <int ACT> constexpr bool op_bf = ACT != PF_TYPE_F16;
 template <int ACT> constexpr int op_pieces = ACT == PF_TYPE_F32 ? 3 : 1;
+// Weights over a cache are two pieces of 16-bit rows' type: the matrix core is
+// idle there, and a weight rounded once would add as much error as the result's
+// own rounding.
+template <int ACT> constexpr int weight_pieces = ACT == PF_TYPE_F32 ? 3 : 2;
 template <int ACT> constexpr int act_size = ACT == PF_TYPE_F32 ? 4 : 2;
 
 template <bool BF>
@@ -63,6 +67,12 @@ __device__ __forceinline__ s8v pack8(const float (&x)[8]) {
     }
 }
 
+template <int T>
+__device__ __forceinline__ float to_float(short bits) {
+    if constexpr (T == PF_TYPE_F16) return (float)__builtin_bit_cast(_Float16, bits);
+    else return __builtin_bit_cast(float, (uint32_t)(uint16_t)bits << 16);
+}
+
 // x = hi + mid + lo exactly, each piece the bf16 nearest to what is left (8
 // significant bits each, the remainders signed; below 2^-126 the last bits are
 // lost).  An infinity leaves a NaN.
@@ -82,14 +92,17 @@ __device__ __forceinline__ void split3(const float (&x)[8], s8v (&out)[3]) {
 // Eight floats as NP operand pieces.
 template <bool BF, int NP>
 __device__ __forceinline__ void pieces(const float (&x)[8], s8v (&out)[NP]) {
-    if constexpr (NP == 3) split3(x, out);
-    else out[0] = pack8<BF>(x);
-}
-
-template <int T>
-__device__ __forceinline__ float to_float(short bits) {
-    if constexpr (T == PF_TYPE_F16) return (float)__builtin_bit_cast(_Float16, bits);
-    else return __builtin_bit_cast(float, (uint32_t)(uint16_t)bits << 16);
+    if constexpr (NP == 3) {
+        split3(x, out);
+    } else {
+        out[0] = pack8<BF>(x);
+        if constexpr (NP == 2) {
+            float r[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) r[i] = x[i] - to_float<BF ? PF_TYPE_BF16 : PF_TYPE_F16>(out[0][i]);
+            out[1] = pack8<BF>(r);
+        }
+    }
 }
 
 // Eight int8 codes (two words) as floats.
@@ -201,6 +214,12 @@ constexpr float MAX_SLACK = 8.0f;
 // position is hi: the last `window` of the causal range start at lo.
 __device__ __host__ __forceinline__ bool key_visible(int pos, int hi, int lo, int sink) {
     return (pos <= hi) & ((pos >= lo) | (pos < sink));
+}
+
+// x where `on` is all ones, y where it is 0.
+__device__ __forceinline__ float bits_or(float x, float y, int on) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & (uint32_t)on) |
+                                         (__builtin_bit_cast(uint32_t, y) & ~(uint32_t)on));
 }
 
 // A word with its first n bits set (none for n <= 0, all from 64 on).

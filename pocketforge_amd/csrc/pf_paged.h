@@ -15,13 +15,15 @@ struct PageSeq {
 };
 
 // One workgroup's share of a sequence's keys: tiles t0 .. t1 - 1 of PG_KEYS of
-// the keys that its rows see; its results go to row ws0 of the partial
-// results, or, where parts == 1, to the output.
+// the keys that its rows see.  Part `part` of `parts`; its results go to rows
+// ws0 + part * rows .. of the partial results, or, where parts == 1, to the
+// output.
 struct PageItem {
-    uint32_t slot, q0, rows, len, t0, t1, ws0, parts;
+    uint32_t slot, q0, rows, len, t0, t1, ws0, parts, part, unused;
 };
 constexpr uint32_t PG_KEYS = 32;
-constexpr uint32_t PG_GROUPS = 1536;   // workgroups aimed at
+constexpr uint32_t PG_MOST_PARTS = 1024;   // of one sequence
+constexpr uint32_t PG_MOST_ITEMS = 1024;   // of a pass, or two for each sequence
 
 // How the pass's keys are cut, kept for the layers that follow.
 struct PageSplit {

@@ -9,10 +9,18 @@
 #include "pf_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace pf;
 
 namespace pf {
+
+// Waves of a SIMD (workgroups of a compute unit) that the registers allow: the
+// next tile's rows wait in registers, and fp32 rows take three operands each.
+__host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
+    const bool wide = act == PF_TYPE_F32;
+    return dp == 64 ? (nt == 1 ? (wide ? 3 : 4) : 2) : nt == 1 ? 2 : wide ? 1 : 2;
+}
 
 // A workgroup: 4 waves, each on 32-key tiles of its own, four tiles apart.
 // A lane's matrix operands of K are 16 bytes of a row as the page holds them,
@@ -21,16 +29,16 @@ namespace pf {
 // S^T = K Q^T, 16 at a time (NT tiles); exp(S)^T is the operand of O^T = V^T P^T
 // without moving a value between lanes.
 template <int ACT, int CT, int DP, int NT, bool EXACT>
-__global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
+__global__ __launch_bounds__(256, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
     constexpr bool BF = op_bf<ACT>, I8 = CT == PF_TYPE_I8;
-    constexpr int NP = op_pieces<ACT>, C = DP / 32, DT = DP / 16;
+    constexpr int NP = op_pieces<ACT>, PP = weight_pieces<ACT>, C = DP / 32, DT = DP / 16;
     constexpr int STR = DP + 16;                 // LDS row stride in values
     constexpr int VCH = I8 ? DP / 16 : DP / 8;   // 16-byte chunks of a V row
     constexpr int VL = 32 * VCH / 64;            // V loads of a lane
     constexpr int KL = I8 ? DP / 64 : C;         // K loads of a lane per 16 keys
     __shared__ __align__(16) short sv[4][32][STR];
     __shared__ float s_ml[4][16][2];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
 
     const PageItem it = a.items[blockIdx.x];
     const uint32_t head0 = blockIdx.y * a.group;
@@ -40,6 +48,30 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
     const PageTiles pt = page_tiles(it.rows, it.len, (uint32_t)a.window, (uint32_t)a.sink);
     const int lo0 = a.window ? max(0, p0 - a.window + 1) : 0;
     const int lo1 = a.window ? max(0, len - a.window) : 0;
+    const auto pos_of = [&](int t) { return (t < pt.sinks ? t : t - pt.sinks + pt.first) * 32; };
+
+    // The share's tiles in this wave's order: first those that all rows see whole,
+    // wa .. wb - 1, then the others; the four waves take them in turn.
+    const int t0 = (int)it.t0, t1 = (int)it.t1;
+    const int wa = min(max(pt.sinks + (lo1 + 31) / 32 - pt.first, max(t0, pt.sinks)), t1);
+    const int wb = min(max(pt.sinks + (a.causal ? p0 + 1 : len) / 32 - pt.first, wa), t1);
+    const int n_whole = (wb - wa + 3 - wave) >> 2, n_tiles = n_whole + ((t1 - t0 - (wb - wa) + wave) >> 2);
+    const auto tile_of = [&](int n) {
+        if (n < n_whole) return wa + wave + 4 * n;
+        const int e = t0 + 3 - wave + 4 * (n - n_whole);      // (the waves in the other order)
+        return e < wa ? e : e + wb - wa;
+    };
+
+    // Page numbers of this wave's next 32 tiles, two for each: lane 2 n + s has
+    // the one of tile n's keys 16 s ..
+    const int32_t* table = a.table + (size_t)it.slot * a.table_stride;
+    const int last_page = (len - 1) >> a.page_shift, in_page = (1 << a.page_shift) - 1;
+    int pages = 0;
+    auto look_up = [&](int n) {
+        const int at = tile_of(min(n + (lane >> 1), n_tiles - 1));
+        pages = table[min((pos_of(at) + 16 * (lane & 1)) >> a.page_shift, last_page)];
+    };
+    if (n_tiles) look_up(0);
 
     s8v qf[NT][NP][C];
     int hi[NT], lo[NT];
@@ -73,67 +105,40 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
         for (int t = 0; t < DT; t++) o[n][t] = (f4v)0.0f;
     }
 
-    const int32_t* table = a.table + (size_t)it.slot * a.table_stride;
-    const int last_page = (len - 1) >> a.page_shift, in_page = (1 << a.page_shift) - 1;
-    const size_t row_bytes = (size_t)a.dim * (I8 ? 1 : 2);
+    const uint32_t row_bytes = (EXACT ? DP : a.dim) * (I8 ? 1 : 2);
+    const uint32_t k_off = (uint32_t)col * row_bytes + (uint32_t)g * 16;
+    const uint32_t v_row = (uint32_t)lane / VCH, v_off = v_row * row_bytes + (uint32_t)lane % VCH * 16;
+    constexpr int VR = 64 / VCH;                 // V rows of one load of the wave
 
     u4v kr[2][KL], vr[VL];
     f4v ksc[2], vsc[2];
-    int tile_pos = 0;
-    auto load = [&](int t) {
-        tile_pos = (t < pt.sinks ? t : t - pt.sinks + pt.first) * 32;
+    auto load = [&](int n) {                     // this wave's n-th tile
+        const int pos0 = pos_of(tile_of(n));
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const int pos = tile_pos + 16 * s;
-            const int pg = table[min(pos >> a.page_shift, last_page)];
-            const size_t row0 = (((size_t)pg * a.kv_heads + blockIdx.y) << a.page_shift) + (size_t)(pos & in_page);
-            const uint8_t* kp = (const uint8_t*)a.k + (row0 + col) * row_bytes;
+            const uint32_t pg = (uint32_t)__builtin_amdgcn_readlane(pages, 2 * (n & 31) + s);
+            const size_t row0 = (((size_t)pg * a.kv_heads + blockIdx.y) << a.page_shift) + (size_t)((pos0 + 16 * s) & in_page);
+            const uint8_t *kp = (const uint8_t*)a.k + row0 * row_bytes, *vp = (const uint8_t*)a.v + row0 * row_bytes;
 #pragma unroll
-            for (int c = 0; c < KL; c++) {
-                const int off = c * 64 + g * 16;
-                kr[s][c] = (EXACT || off < (int)row_bytes) ? *(const u4v*)(kp + off) : (u4v)0u;
-            }
-            const uint8_t* vp = (const uint8_t*)a.v + row0 * row_bytes;
+            for (int c = 0; c < KL; c++)
+                kr[s][c] = (EXACT || c * 64 + g * 16 < (int)row_bytes) ? *(const u4v*)(kp + k_off + c * 64) : (u4v)0u;
 #pragma unroll
-            for (int i = 0; i < VL / 2; i++) {
-                const int e = i * 64 + lane, r = e / VCH, off = e % VCH * 16;
-                vr[s * (VL / 2) + i] = (EXACT || off < (int)row_bytes) ? *(const u4v*)(vp + (size_t)r * row_bytes + off) : (u4v)0u;
-            }
+            for (int i = 0; i < VL / 2; i++)
+                vr[s * (VL / 2) + i] = (EXACT || lane % VCH * 16 < (int)row_bytes) ? *(const u4v*)(vp + v_off + i * VR * row_bytes) : (u4v)0u;
             if constexpr (I8) {
-                ksc[s] = *(const f4v*)(a.ks + row0 + 4 * g);
-                vsc[s] = *(const f4v*)(a.vs + row0 + 4 * g);
+                ksc[s] = *(const f4v*)((const uint8_t*)(a.ks + row0) + 16 * g);
+                vsc[s] = *(const f4v*)((const uint8_t*)(a.vs + row0) + 16 * g);
             }
         }
     };
 
-    int t = (int)it.t0 + wave;
-    if (t < (int)it.t1) load(t);
-    for (; t < (int)it.t1; t += 4) {
-        const int pos0 = tile_pos;
-        const bool whole = pos0 + 31 <= (a.causal ? p0 : len - 1) && (pos0 >= lo1 || pos0 + 32 <= a.sink);
-        // V's rows to LDS; rows that nobody sees (past the end, between sinks and window) as zeros
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < VL; i++) {
-            const int e = i * 64 + lane, r = e / VCH, off = e % VCH;
-            u4v w = vr[i];
-            if (!whole) {
-                const int pos = pos0 + r;
-                if (pos >= len || (pos < lo0 && pos >= a.sink)) w = (u4v)0u;
-            }
-            if constexpr (I8) {
-                float x[8];
-                codes8(w[0], w[1], x);
-                *(s8v*)&sv[wave][r][off * 16] = pack8<BF>(x);
-                codes8(w[2], w[3], x);
-                *(s8v*)&sv[wave][r][off * 16 + 8] = pack8<BF>(x);
-            } else {
-                const s8v x = __builtin_bit_cast(s8v, w);
-                if (!whole) bad |= any_not_finite<BF>(x);
-                *(s8v*)&sv[wave][r][off * 8] = x;
-            }
-        }
-        const bool odd = !I8 && !whole && __any(bad);
+    // this wave's n-th tile, already in registers; the next one's loads are under
+    // way while its weights are formed.  MASKED: some rows do not see all of it
+    auto body = [&](auto masked, int n_tile) {
+        const int pos0 = pos_of(tile_of(n_tile));
+        constexpr bool MASKED = decltype(masked)::value;
+        short* sw = &sv[wave][0][0];
+        auto place = [&](int i) { return sw + (i * VR + v_row) * STR + (lane % VCH) * (I8 ? 16 : 8); };
         f4v kscale[2], vscale[2];
         s8v kf[2][C];
 #pragma unroll
@@ -163,20 +168,41 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
 #pragma unroll
                     for (int x = 0; x < NP; x++) sc[n][s] = mfma16<BF>(kf[s][c], qf[n][x][c], sc[n][s]);
             }
-        if (t + 4 < (int)it.t1) load(t + 4);     // (the next tile's rows are on their way during what follows)
-        s8v pf[NT][NP];
+        // V's rows to LDS; rows that nobody sees (past the end, between sinks and window) as zeros
+        const uint32_t any = !MASKED ? 0u : (uint32_t)(first_bits(len - pos0) & (~first_bits(lo0 - pos0) | first_bits(a.sink - pos0)));
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VL; i++) {
+            u4v w = vr[i];
+            if constexpr (MASKED) w &= (uint32_t)-(int)((any >> (i * VR + v_row)) & 1u);
+            if constexpr (I8) {
+                float x[8];
+                codes8(w[0], w[1], x);
+                *(s8v*)place(i) = pack8<BF>(x);
+                codes8(w[2], w[3], x);
+                *(s8v*)(place(i) + 8) = pack8<BF>(x);
+            } else {
+                if constexpr (MASKED) z = sum8<BF>(__builtin_bit_cast(s8v, w), z, 0.0f);
+                *(u4v*)place(i) = w;
+            }
+        }
+        if (n_tile + 1 < n_tiles) {
+            if (((n_tile + 1) & 31) == 0) look_up(n_tile + 1);
+            load(n_tile + 1);
+        }
+        s8v pf[NT][PP];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
+            uint32_t part = ~0u;                 // one bit per key, from 4 g on
+            if constexpr (MASKED)
+                part = (uint32_t)(first_bits(hi[n] + 1 - pos0) & (~first_bits(lo[n] - pos0) | first_bits(a.sink - pos0))) >> (4 * g);
             float x[8], top = -INFINITY;
 #pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float y = sc[n][s][i] * (I8 ? kscale[s][i] * a.scale_log2 : a.scale_log2);
-                    if (!whole && !key_visible(pos0 + 16 * s + 4 * g + i, hi[n], lo[n], a.sink)) y = -INFINITY;
-                    x[4 * s + i] = y;
-                    top = fmaxf(top, y);
-                }
+            for (int e = 0; e < 8; e++) {
+                x[e] = sc[n][e / 4][e % 4] * (I8 ? kscale[e / 4][e % 4] * a.scale_log2 : a.scale_log2);
+                if constexpr (MASKED) x[e] = bits_or(x[e], -INFINITY, __builtin_amdgcn_sbfe((int)part, 16 * (e / 4) + e % 4, 1));
+                top = fmaxf(top, x[e]);
+            }
             if (__any(top > m[n] + MAX_SLACK)) {
                 const float to = fmaxf(m[n], max16(top));
                 const float f = to == -INFINITY ? 1.0f : exp2_fast(m[n] - to);
@@ -189,46 +215,59 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
             }
             const float ms = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float e = exp2_fast(x[i] - ms);
-                l[n] += e;
-                x[i] = e;
+            for (int e = 0; e < 8; e++) {
+                x[e] = exp2_fast(x[e] - ms);
+                l[n] += x[e];
                 if constexpr (I8) {
-                    const float w = e * vscale[i / 4][i % 4];
-                    x[i] = !whole && !key_visible(pos0 + 16 * (i / 4) + 4 * g + i % 4, hi[n], lo[n], a.sink) ? 0.0f : w;
+                    x[e] *= vscale[e / 4][e % 4];
+                    if constexpr (MASKED) x[e] = bits_or(x[e], 0.0f, __builtin_amdgcn_sbfe((int)part, 16 * (e / 4) + e % 4, 1));
                 }
             }
-            pieces<BF, NP>(x, pf[n]);
+            pieces<BF, PP>(x, pf[n]);
         }
         __builtin_amdgcn_wave_barrier();
+        if constexpr (MASKED && !I8) {
+            if (__any(z != z)) {
+                // infinities and NaN reach the rows that see them, whatever their weight,
+                // and the products find zeros in their places
+                for (int r = 0; r < 32; r++)
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const int r = 4 * g + (lane & 15) / 4, c = d * 16 + (lane & 3) * 4;
-            const s4v x0 = lds_read_tr(&sv[wave][r][c]), x1 = lds_read_tr(&sv[wave][r + 16][c]);
-            s8v vf = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-            if (odd) vf = finite_or_zero<BF>(vf);
+                    for (int n = 0; n < NT; n++) {
+                        if (pos0 + r >= len || !key_visible(pos0 + r, hi[n], lo[n], a.sink)) continue;
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const short w = sw[r * STR + d * 16 + 4 * g + i];
+                                if (not_finite<BF>(w)) o[n][d][i] += to_float<BF ? PF_TYPE_BF16 : PF_TYPE_F16>(w);
+                            }
+                    }
+                __builtin_amdgcn_wave_barrier();
+                for (int i = 0; i < VL; i++) *(s8v*)place(i) = finite_or_zero<BF>(*(const s8v*)place(i));
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        auto v_operand = [&](int d) {
+            const short* vp = sw + (4 * g + (lane & 15) / 4) * STR + d * 16 + (lane & 3) * 4;
+            const s4v x0 = lds_read_tr(vp), x1 = lds_read_tr(vp + 16 * STR);
+            return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        s8v vf[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++) vf[d] = v_operand(d);
+#pragma unroll
+        for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int x = 0; x < NP; x++) o[n][d] = mfma16<BF>(vf, pf[n][x], o[n][d]);
-        }
-        if (odd) {
-            // infinities and NaN reach the rows that see them, whatever their weight
-            for (int r = 0; r < 32; r++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    if (!key_visible(pos0 + r, hi[n], lo[n], a.sink) || pos0 + r >= len) continue;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const short w = sv[wave][r][d * 16 + 4 * g + i];
-                            if (not_finite<BF>(w)) o[n][d][i] += to_float<BF ? PF_TYPE_BF16 : PF_TYPE_F16>(w);
-                        }
-                }
-        }
+                for (int x = 0; x < PP; x++) o[n][d] = mfma16<BF>(vf[d], pf[n][x], o[n][d]);
         __builtin_amdgcn_wave_barrier();
-    }
+    };
+
+    if (n_tiles) load(0);
+    int n_tile = 0;
+    for (; n_tile < n_whole; n_tile++) body(std::false_type{}, n_tile);
+    for (; n_tile < n_tiles; n_tile++) body(std::true_type{}, n_tile);
 
     // the four waves' results meet in LDS, 16 rows at a time
     float* so = (float*)&sv[0][0][0];            // [4][16][DP]
@@ -269,7 +308,7 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
                 if (EXACT || d0 + i < (int)a.dim) store4<ACT>(op + i * act_size<ACT>, x);
             }
         } else {
-            const size_t w = (size_t)(it.ws0 + (uint32_t)j) * a.n_heads + (uint32_t)h;
+            const size_t w = (size_t)(it.ws0 + it.part * it.rows + (uint32_t)j) * a.n_heads + (uint32_t)h;
 #pragma unroll
             for (int i = 0; i < PER; i++)
                 if (EXACT || d0 + i < (int)a.dim) a.ws_o[w * a.dim + d0 + i] = acc[i];
@@ -287,8 +326,8 @@ __global__ __launch_bounds__(256) void k_paged_attn(PagedArgs a) {
 template <int ACT>
 __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
     const PageItem it = a.items[blockIdx.x];
-    if (it.parts == 1 || it.t0 != 0) return;
-    __shared__ float s_f[PG_GROUPS + 1], s_red[2][4];
+    if (it.part != 0 || it.parts == 1) return;
+    __shared__ float s_f[PG_MOST_PARTS], s_red[2][4];
     __shared__ __align__(16) float s_o[8][128];
     const uint32_t h = blockIdx.y, tid = threadIdx.x, grp = tid >> 5, d = (tid & 31) * 4, wave = tid >> 6;
     for (uint32_t j = blockIdx.z; j < it.rows; j += gridDim.z) {
@@ -360,35 +399,53 @@ static void paged_dim(hipStream_t st, uint32_t items, uint32_t most, const Paged
     else paged_rows<ACT, CT, 128, false>(st, items, most, a);
 }
 
-// Cuts the pass's keys: enough workgroups for every compute unit several times
-// over, none with less than PG_LEAST tiles.
-constexpr uint32_t PG_LEAST = 4;
+// Cuts the pass's keys: the smallest shares with which one round of workgroups
+// holds them all (two per sequence and head, if that is more: a long sequence
+// beside short ones), but of PG_LEAST tiles, one for each wave.
+constexpr uint32_t PG_LEAST = 4, PG_CUS = 256;
 static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
     PageSplit& u = p->cut;
     if (u.type == d->type && u.window == s.window && u.sink == s.sink && u.heads == d->n_heads) return PF_OK;
     const uint32_t group = d->n_heads / d->n_kv_heads;
+    std::vector<uint32_t> tiles;
+    tiles.reserve(p->pass.size());
     uint64_t all = 0;
-    uint32_t most = 0;
+    uint32_t most = 0, longest = 0;
     for (const PageSeq& q : p->pass) {
         if (!q.rows) continue;
-        all += (uint64_t)page_tiles(q.rows, q.len, s.window, s.sink).count;
+        tiles.push_back((uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count);
+        all += tiles.back();
+        longest = std::max(longest, tiles.back());
         most = std::max(most, q.rows);
     }
-    const uint64_t per = (uint64_t)d->n_kv_heads * (((uint64_t)most * group + 31) / 32);
-    const uint32_t chunk = (uint32_t)std::max<uint64_t>(PG_LEAST, (all * per + PG_GROUPS - 1) / PG_GROUPS);
+    const uint64_t R = (uint64_t)most * group, per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
+    const uint64_t round = (uint64_t)PG_CUS * paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
+    const uint64_t budget = std::max<uint64_t>(round / per, 2 * tiles.size());
+    const auto items_of = [&](uint32_t chunk) {
+        uint64_t n = 0;
+        for (uint32_t t : tiles) n += (t + chunk - 1) / chunk;
+        return n;
+    };
+    uint32_t chunk = std::max<uint32_t>(PG_LEAST, (longest + PG_MOST_PARTS - 1) / PG_MOST_PARTS), high = std::max(chunk, longest);
+    while (chunk < high) {                       // (the fewest tiles that the budget allows)
+        const uint32_t mid = chunk + (high - chunk) / 2;
+        if (items_of(mid) <= budget) high = mid;
+        else chunk = mid + 1;
+    }
     std::vector<PageItem> items;
+    items.reserve(items_of(chunk));
     PageSplit n;
     uint64_t ws = 0;
+    uint32_t i = 0;
     for (const PageSeq& q : p->pass) {
         if (!q.rows) continue;
-        const uint32_t tiles = (uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count;
-        const uint32_t parts = (tiles + chunk - 1) / chunk;
-        for (uint32_t i = 0; i < parts; i++) {
-            items.push_back({q.slot, q.q0, q.rows, q.len, (uint32_t)((uint64_t)tiles * i / parts),
-                             (uint32_t)((uint64_t)tiles * (i + 1) / parts), (uint32_t)ws, parts});
-            if (parts > 1) ws += q.rows;
-        }
-        if (parts > 1) n.split = true;
+        const uint32_t t = tiles[i++], parts = (t + chunk - 1) / chunk;
+        for (uint32_t k = 0; k < parts; k++)
+            items.push_back({q.slot, q.q0, q.rows, q.len, (uint32_t)((uint64_t)t * k / parts),
+                             (uint32_t)((uint64_t)t * (k + 1) / parts), (uint32_t)ws, parts, k, 0});
+        if (parts == 1) continue;
+        ws += (uint64_t)parts * q.rows;
+        n.split = true;
     }
     if (ws * d->n_heads > 0x7FFFFFFFu) return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
     if (items.size() > p->items_cap) return fail(p->ctx, PF_ERR_STATE, "pages: work list exceeded");

@@ -197,7 +197,10 @@ __global__ __launch_bounds__(256) void k_pages_move(MoveArgs a) {
             uint32_t i = threadIdx.x;
             for (; i + 768 < n16; i += 1024) {                // four loads under way
                 const u4v x0 = s[i], x1 = s[i + 256], x2 = s[i + 512], x3 = s[i + 768];
-                d[i] = x0; d[i + 256] = x1; d[i + 512] = x2; d[i + 768] = x3;
+                __builtin_nontemporal_store(x0, d + i);
+                __builtin_nontemporal_store(x1, d + i + 256);
+                __builtin_nontemporal_store(x2, d + i + 512);
+                __builtin_nontemporal_store(x3, d + i + 768);
             }
             for (; i < n16; i += 256) d[i] = s[i];
             if (a.ks) {
@@ -460,7 +463,7 @@ extern "C" pf_status pf_pages_create(pf_ctx* c, const pf_pages_config* g, pf_pag
     p->esize = g->type == PF_TYPE_I8 ? 1 : 2;
     p->scales = (size_t)g->n_pages * g->n_kv_heads * g->page_size;
     p->plane = p->scales * g->head_dim * p->esize;
-    p->items_cap = g->max_seqs + PG_GROUPS;
+    p->items_cap = 2 * g->max_seqs + PG_MOST_ITEMS;
     if (pf_status s = no_throw(c, [&] { return pages_alloc(p); })) {
         const std::string msg = c->err;
         pf_pages_destroy(p);

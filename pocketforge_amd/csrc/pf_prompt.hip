@@ -416,9 +416,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
             for (int g = 0; g < 2; g++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)part[g], 8 * (i / 4) + i % 4, 1);
-                    const uint32_t x = __builtin_bit_cast(uint32_t, (float)s[g][i]);
-                    s[g][i] = __builtin_bit_cast(float, (x & on) | (0xFF800000u & ~on));   // -infinity
+                    s[g][i] = bits_or(s[g][i], -INFINITY, __builtin_amdgcn_sbfe((int)part[g], 8 * (i / 4) + i % 4, 1));
                 }
         }
         float top = s[0][0];
