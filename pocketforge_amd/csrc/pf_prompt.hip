@@ -67,202 +67,265 @@ __device__ __forceinline__ PromptUnit prompt_unit(uint32_t u, uint32_t tiles, ui
 // need one exchange between two lanes, and exp(S)^T is already the operand
 // of O^T = V^T P^T, whose other operand comes from V's rows in LDS through
 // transposing reads.
-template <int ACT, int DP, bool EXACT>
-__global__ __launch_bounds__(256) void k_prompt_attn(PromptArgs a) {
-    constexpr bool BF = op_bf<ACT>;
-    constexpr int NP = op_pieces<ACT>;
-    constexpr int STR = DP + 16;                 // LDS row stride in values
-    constexpr int C = DP / 16, DT = DP / 32;
-    __shared__ __align__(16) short sk[NP][PR_KEYS][STR];
-    __shared__ __align__(16) short sv[NP][PR_KEYS][STR];
-    __shared__ int s_bad;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, row = lane & 31, half = lane >> 5;
 
-    // the sequence of this tile: the last one whose first tile is not past it
+// What a workgroup knows of its tile of 128 query rows.
+struct PromptTile {
+    uint32_t q0, k0, head;
+    int nq, nk, r0, off;          // lengths, first row, position of row 0
+    int p0, p1;                   // positions of the first and the last row
+    int first, sinks, tiles, wa, wb, whole;
+
+    // The key tiles that some row sees, in the order they are taken: those that
+    // all rows see whole (wa .. wb - 1), then the sinks' and the rest from `first`.
+    __device__ __forceinline__ int key_tile(int it) const {
+        if (it < whole) return wa + it;
+        it -= whole;
+        if (it < sinks) return it;
+        it += first - sinks;
+        return it < wa ? it : it + whole;
+    }
+    // rows a .. b of the tile see something of the keys from key0 on
+    __device__ __forceinline__ bool some(const PromptArgs& a, int key0, int wave) const {
+        const int w0 = p0 + wave * 32, w1 = min(w0 + 31, p1);
+        return !((a.causal && key0 > w1) | (a.window && key0 + PR_KEYS <= w0 - a.window + 1 && key0 >= a.sink));
+    }
+};
+__device__ __forceinline__ bool prompt_tile(const PromptArgs& a, PromptTile* t) {
     const PromptUnit unit = prompt_unit(blockIdx.x, a.tiles, a.n_heads / a.group, a.group);
-    if (unit.none) return;
-    const uint32_t tile = unit.tile, head = unit.head;
-    const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= tile);
+    if (unit.none) return false;
+    const int lane = threadIdx.x & 63;
+    const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= unit.tile);
     const int seq = 63 - __builtin_clzll(before);
-    const uint32_t q0 = a.seq[seq].q0, k0 = a.seq[seq].k0;
-    const int nq = (int)a.seq[seq].nq, nk = (int)a.seq[seq].nk;
-    const int off = nk - nq, r0 = (int)(tile - a.tile0[seq]) * 128;
-    const int my = r0 + wave * 32 + row;         // this lane's query
-    const int p = off + my;
+    t->head = unit.head;
+    t->q0 = a.seq[seq].q0; t->k0 = a.seq[seq].k0;
+    t->nq = (int)a.seq[seq].nq; t->nk = (int)a.seq[seq].nk;
+    t->off = t->nk - t->nq;
+    t->r0 = (int)(unit.tile - a.tile0[seq]) * 128;
+    t->p0 = t->off + t->r0;
+    t->p1 = t->off + min(t->r0 + 128, t->nq) - 1;
+    const int end = min(t->nk, a.causal ? t->p1 + 1 : t->nk), last = end <= 0 ? 0 : (end + PR_KEYS - 1) / PR_KEYS;
+    t->first = (a.window ? max(0, t->p0 - a.window + 1) : 0) / PR_KEYS;
+    t->sinks = min(min((a.sink + PR_KEYS - 1) / PR_KEYS, t->first), last);
+    t->tiles = max(0, last - t->first) + t->sinks;
+    t->wa = a.window ? max(t->first, (max(0, t->p1 - a.window + 1) + PR_KEYS - 1) / PR_KEYS) : 0;
+    t->wb = max(t->wa, min(t->nk, a.causal ? max(0, t->p0 + 1) : t->nk) / PR_KEYS);
+    t->whole = t->tiles ? t->wb - t->wa : 0;
+    return true;
+}
+
+// The scores of a tile that a row does not see become -infinity; one bit per
+// key, lanes of the upper half four keys on.
+__device__ __forceinline__ void mask_scores(f16v (&s)[2], const PromptArgs& a, int nk, int hi, int lo, int key0, int half) {
+    const uint64_t see = first_bits(min(hi, nk - 1) + 1 - key0) & (~first_bits(lo - key0) | first_bits(a.sink - key0));
+    const uint32_t part[2] = {(uint32_t)see >> (4 * half), (uint32_t)(see >> 32) >> (4 * half)};
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            s[g][i] = bits_or(s[g][i], -INFINITY, __builtin_amdgcn_sbfe((int)part[g], 8 * (i / 4) + i % 4, 1));
+}
+
+// The running maximum over a tile's scores (scaled to base 2), with the sum and
+// the output corrected where it moves; the value to subtract.
+template <int DT>
+__device__ __forceinline__ float new_maximum(const f16v (&s)[2], float scale, float& m, float& l, f16v (&o)[DT]) {
+    float top = s[0][0];
+#pragma unroll
+    for (int g = 0; g < 2; g++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) top = fmaxf(top, s[g][i]);
+    top *= scale;
+    if (__any(top > m + MAX_SLACK)) {
+        const float to = fmaxf(m, max32(top));
+        const float f = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] *= f;
+    }
+    return m == -INFINITY ? 0.0f : m;
+}
+
+// The rows' results: O^T over the sums.  A row that sees no key is zero; one
+// whose scores are all -infinity is 0 / 0.
+template <int ACT, int DT, bool EXACT>
+__device__ __forceinline__ void put_rows(const PromptArgs& a, const PromptTile& t, int my, int half, float l, const f16v (&o)[DT]) {
+    l = sum32(l);
+    if (my >= t.nq) return;
+    const bool none = !(a.causal ? t.off + my >= 0 : t.nk > 0);
+    const float inv = none ? 0.0f : 1.0f / l;
+    uint8_t* op = (uint8_t*)a.out + ((size_t)(t.q0 + (uint32_t)my) * a.os + (size_t)t.head * a.dim) * act_size<ACT>;
+#pragma unroll
+    for (int n = 0; n < DT; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = n * 32 + 8 * (i / 4) + 4 * half;
+            if (!EXACT && d >= (int)a.dim) continue;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[n][i + j] * inv;
+            store4<ACT>(op + (size_t)d * act_size<ACT>, x);
+        }
+}
+
+// fp32 rows, three bf16 pieces each: six matrix instructions where 16-bit rows
+// take one.  A tile's rows wait in registers while the tile before is worked
+// on, and are cut into pieces on their way to LDS.
+template <int DP, bool EXACT>
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptArgs a) {
+    constexpr int ACT = PF_TYPE_F32, NP = 3;
+    constexpr int KS = DP + 8, VS = DP + 32;     // LDS row strides without bank conflicts for either kind of read
+    constexpr int C = DP / 16, DT = DP / 32, CH = DP / 8, LOADS = PR_KEYS * CH / 256;
+    __shared__ __align__(16) short sk[NP][PR_KEYS][KS];
+    __shared__ __align__(16) short sv[NP][PR_KEYS][VS];
+    __shared__ int s_odd;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, row = lane & 31, half = lane >> 5;
+    PromptTile T;
+    if (!prompt_tile(a, &T)) return;
+    const int nk = T.nk, my = T.r0 + wave * 32 + row, p = T.off + my;
     const int hi = a.causal ? p : nk - 1, lo = a.window ? p - a.window + 1 : 0;
 
-    // Q^T: 16 dims of a row per matrix instruction
-    s8v qf[NP][C];
+    s8v qf[NP][C];                               // Q^T: 16 dims of a row per matrix instruction
     {
-        const uint32_t qr = q0 + (uint32_t)min(my, nq - 1);
-        const uint8_t* qp = (const uint8_t*)a.q + ((size_t)qr * a.qs + (size_t)head * a.dim) * act_size<ACT>;
+        const uint32_t qr = T.q0 + (uint32_t)min(my, T.nq - 1);
+        const float* qp = (const float*)a.q + (size_t)qr * a.qs + (size_t)T.head * a.dim + half * 8;
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            const int d = c * 16 + half * 8;
             float x[8] = {};
-            if (EXACT || d < (int)a.dim) load8<ACT>(qp + (size_t)d * act_size<ACT>, x);
+            if (EXACT || c * 16 + half * 8 < (int)a.dim) load8<ACT>(qp + c * 16, x);
             s8v t[NP];
-            pieces<BF, NP>(x, t);
+            split3(x, t);
 #pragma unroll
             for (int n = 0; n < NP; n++) qf[n][c] = t[n];
         }
     }
 
-    // keys that any row of the workgroup sees
-    const int p0 = off + r0, p1 = off + min(r0 + 128, nq) - 1;
-    const int end = min(nk, a.causal ? p1 + 1 : nk);
-    const int wlo = a.window ? max(0, p0 - a.window + 1) : 0;
-    const int first = wlo / PR_KEYS;
-    const int sinks = min((a.sink + PR_KEYS - 1) / PR_KEYS, first);
-    const int tiles = end <= 0 ? 0 : max(0, (end + PR_KEYS - 1) / PR_KEYS - first) + min(sinks, (end + PR_KEYS - 1) / PR_KEYS);
+    const size_t kv_head = (size_t)(T.head / a.group) * a.dim;
+    const float* kg = (const float*)a.k + (size_t)T.k0 * a.ks + kv_head;
+    const float* vg = (const float*)a.v + (size_t)T.k0 * a.vs + kv_head;
+    float xk[LOADS][8], xv[LOADS][8];
+    auto load = [&](int it) {
+        const int key0 = T.key_tile(it) * PR_KEYS;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int e = i * 256 + tid, d = e % CH * 8;
+            const uint32_t kr = (uint32_t)min(key0 + e / CH, nk - 1);   // (rows past the end: masked)
+            const bool on = EXACT || d < (int)a.dim;
+            const size_t at = on ? d : 0;
+            load8<ACT>(kg + (size_t)kr * a.ks + at, xk[i]);
+            load8<ACT>(vg + (size_t)kr * a.vs + at, xv[i]);
+            if (!EXACT && !on)
+#pragma unroll
+                for (int j = 0; j < 8; j++) xk[i][j] = xv[i][j] = 0.0f;
+        }
+    };
 
     f16v o[DT];
 #pragma unroll
     for (int t = 0; t < DT; t++) o[t] = (f16v)0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    const size_t kv_head = (size_t)(head / a.group) * a.dim;
-    for (int it = 0; it < tiles; it++) {
-        const int key0 = (it < sinks ? it : it - sinks + first) * PR_KEYS;
-        // a tile that every row of the workgroup sees whole needs no mask
-        const bool whole = key0 + PR_KEYS <= nk && (!a.causal || key0 + PR_KEYS - 1 <= p0) &&
-                           (!a.window || key0 >= p1 - a.window + 1 || key0 + PR_KEYS <= a.sink);
-        __syncthreads();
-        if (tid == 0) s_bad = 0;
-        __syncthreads();
-        bool bad = false;
+    auto body = [&](auto masked, int it) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const int key0 = T.key_tile(it) * PR_KEYS;
+        __syncthreads();                         // nobody reads the tile before
+        float z = 0.0f;
 #pragma unroll
-        for (int e = tid; e < PR_KEYS * (DP / 8); e += 256) {
-            const int r = e / (DP / 8), d = e % (DP / 8) * 8, key = key0 + r;
-            float xk[8] = {}, xv[8] = {};
-            if (key < nk && (EXACT || d < (int)a.dim)) {
-                const size_t kr = k0 + (uint32_t)key;
-                load8<ACT>((const uint8_t*)a.k + (kr * a.ks + kv_head + d) * act_size<ACT>, xk);
-                load8<ACT>((const uint8_t*)a.v + (kr * a.vs + kv_head + d) * act_size<ACT>, xv);
-            }
+        for (int i = 0; i < LOADS; i++) {
+            const int e = i * 256 + tid, r = e / CH, d = e % CH * 8;
             s8v tk[NP], tv[NP];
-            pieces<BF, NP>(xk, tk);
-            pieces<BF, NP>(xv, tv);
+            split3(xk[i], tk);
+            split3(xv[i], tv);
 #pragma unroll
             for (int n = 0; n < NP; n++) {
                 *(s8v*)&sk[n][r][d] = tk[n];
                 *(s8v*)&sv[n][r][d] = tv[n];
             }
-            if (!whole) bad |= any_not_finite<BF>(tv[0]);
+            if constexpr (MASKED)
+#pragma unroll
+                for (int j = 0; j < 8; j++) z = __builtin_fmaf(xv[i][j], 0.0f, z);
         }
-        if (bad) s_bad = 1;
+        if (MASKED && z != z) s_odd = it;
         __syncthreads();
-        const bool odd = s_bad != 0;             // values that masked rows must not meet
-
+        if (it + 1 < T.tiles) load(it + 1);
+        if constexpr (MASKED) {
+            // values that are not finite reach the rows that see them, whatever
+            // their weight, and the products find zeros in their places
+            if (s_odd == it) {
+                for (int r = 0; r < PR_KEYS; r++) {
+                    const int key = key0 + r;
+                    if (key >= nk || !key_visible(key, hi, lo, a.sink)) continue;
+#pragma unroll
+                    for (int t = 0; t < DT; t++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int d = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                            if (not_finite<true>(sv[0][r][d])) o[t][i] += to_float<PF_TYPE_BF16>(sv[0][r][d]);
+                        }
+                }
+                __syncthreads();
+                for (int i = 0; i < LOADS; i++) {
+                    const int e = i * 256 + tid, r = e / CH, d = e % CH * 8;
+                    const s8v x = *(const s8v*)&sv[0][r][d];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (not_finite<true>(x[j])) sv[0][r][d + j] = sv[1][r][d + j] = sv[2][r][d + j] = 0;
+                }
+                __syncthreads();
+            }
+            if (!T.some(a, key0, wave)) return;
+        }
         f16v s[2];
+        s[0] = s[1] = (f16v)0.0f;
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            s[g] = (f16v)0.0f;
+        for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int c = 0; c < C; c++) {
+            for (int g = 0; g < 2; g++) {
                 s8v kf[NP];
 #pragma unroll
                 for (int n = 0; n < NP; n++) kf[n] = *(const s8v*)&sk[n][g * 32 + row][c * 16 + half * 8];
 #pragma unroll
                 for (int x = 0; x < NP; x++)
 #pragma unroll
-                    for (int y = 0; y < NP; y++)
-                        if (x + y < 3) s[g] = mfma32<BF>(kf[x], qf[y][c], s[g]);
+                    for (int y = 0; x + y < NP; y++) s[g] = mfma32<true>(kf[x], qf[y][c], s[g]);
             }
-        }
-        float top = -INFINITY;
+        if constexpr (MASKED) mask_scores(s, a, nk, hi, lo, key0, half);
+        const float ms = new_maximum<DT>(s, a.scale_log2, m, l, o);
 #pragma unroll
-        for (int g = 0; g < 2; g++)
+        for (int gh = 0; gh < 4; gh++) {         // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float x = s[g][i] * a.scale_log2;
-                if (!whole) {
-                    const int key = key0 + g * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                    if (key >= nk || !key_visible(key, hi, lo, a.sink)) x = -INFINITY;
+            for (int i = 0; i < 8; i++) {
+                x[i] = exp2_fast(__builtin_fmaf(s[gh / 2][8 * (gh & 1) + i], a.scale_log2, -ms));
+                l += x[i];
+            }
+            s8v pf[NP];
+            split3(x, pf);
+            const int r = gh * 16 + 4 * half + (lane & 15) / 4;
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+                const int d = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+                s8v vf[NP];
+#pragma unroll
+                for (int n = 0; n < NP; n++) {
+                    const s4v x0 = lds_read_tr(&sv[n][r][d]), x1 = lds_read_tr(&sv[n][r + 8][d]);
+                    vf[n] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
                 }
-                s[g][i] = x;
-                top = fmaxf(top, x);
-            }
-        if (__any(top > m + MAX_SLACK)) {
-            const float to = fmaxf(m, max32(top));
-            const float f = to == -INFINITY ? 1.0f : exp2_fast(m - to);
-            m = to;
-            l *= f;
 #pragma unroll
-            for (int t = 0; t < DT; t++)
+                for (int u = 0; u < NP; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[t][i] *= f;
-        }
-        const float ms = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int g = 0; g < 2; g++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                s[g][i] = exp2_fast(s[g][i] - ms);
-                l += s[g][i];
-            }
-#pragma unroll
-        for (int g = 0; g < 2; g++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {        // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = s[g][8 * h + i];
-                s8v pf[NP];
-                pieces<BF, NP>(x, pf);
-                const int kr = g * 32 + h * 16 + 4 * half + (lane & 15) / 4;
-#pragma unroll
-                for (int t = 0; t < DT; t++) {
-                    const int d = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-                    s8v vf[NP];
-#pragma unroll
-                    for (int n = 0; n < NP; n++) {
-                        const s4v x0 = lds_read_tr(&sv[n][kr][d]), x1 = lds_read_tr(&sv[n][kr + 8][d]);
-                        vf[n] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                        if (odd) vf[n] = finite_or_zero<BF>(vf[n]);
-                    }
-#pragma unroll
-                    for (int x = 0; x < NP; x++)
-#pragma unroll
-                        for (int y = 0; y < NP; y++)
-                            if (x + y < 3) o[t] = mfma32<BF>(vf[x], pf[y], o[t]);
-                }
-            }
-        if (odd) {
-            // infinities and NaN reach the rows that see them, whatever their weight
-            for (int r = 0; r < PR_KEYS; r++) {
-                const int key = key0 + r;
-                if (key >= nk || !key_visible(key, hi, lo, a.sink)) continue;
-#pragma unroll
-                for (int t = 0; t < DT; t++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int d = t * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                        if (!not_finite<BF>(sv[0][r][d])) continue;
-#pragma unroll
-                        for (int n = 0; n < NP; n++) o[t][i] += to_float<BF ? PF_TYPE_BF16 : PF_TYPE_F16>(sv[n][r][d]);
-                    }
+                    for (int y = 0; u + y < NP; y++) o[t] = mfma32<true>(vf[u], pf[y], o[t]);
             }
         }
-    }
-
-    l = sum32(l);
-    if (my >= nq) return;
-    // a row that sees no key is zero; one whose scores are all -infinity is 0 / 0
-    const bool none = !(a.causal ? p >= 0 : nk > 0);
-    const float inv = none ? 0.0f : 1.0f / l;
-    uint8_t* op = (uint8_t*)a.out + ((size_t)(q0 + (uint32_t)my) * a.os + (size_t)head * a.dim) * act_size<ACT>;
-#pragma unroll
-    for (int t = 0; t < DT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = t * 32 + 8 * (i / 4) + 4 * half;
-            if (!EXACT && d >= (int)a.dim) continue;
-            float x[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[t][i + j] * inv;
-            store4<ACT>(op + (size_t)d * act_size<ACT>, x);
-        }
+    };
+    if (tid == 0) s_odd = -1;
+    if (T.tiles) load(0);
+    int it = 0;
+    for (; it < T.whole; it++) body(std::false_type{}, it);
+    for (; it < T.tiles; it++) body(std::true_type{}, it);
+    put_rows<ACT, DT, EXACT>(a, T, my, half, l, o);
 }
 
 // fp16 and bf16 rows: K and V tiles go from memory straight to LDS, two tiles
@@ -297,22 +360,15 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     __shared__ int s_odd;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, row = lane & 31, half = lane >> 5;
 
-    const PromptUnit unit = prompt_unit(blockIdx.x, a.tiles, a.n_heads / a.group, a.group);
-    if (unit.none) return;
-    const uint32_t tile = unit.tile, head = unit.head;
-    const uint64_t before = __ballot(lane < (int)a.n_seq && a.tile0[lane] <= tile);
-    const int seq = 63 - __builtin_clzll(before);
-    const uint32_t q0 = a.seq[seq].q0, k0 = a.seq[seq].k0;
-    const int nq = (int)a.seq[seq].nq, nk = (int)a.seq[seq].nk;
-    const int off = nk - nq, r0 = (int)(tile - a.tile0[seq]) * 128;
-    const int my = r0 + wave * 32 + row;
-    const int p = off + my;
+    PromptTile T;
+    if (!prompt_tile(a, &T)) return;
+    const int nk = T.nk, my = T.r0 + wave * 32 + row, p = T.off + my;
     const int hi = a.causal ? p : nk - 1, lo = a.window ? p - a.window + 1 : 0;
 
     s8v qf[C];
     {
-        const uint32_t qr = q0 + (uint32_t)min(my, nq - 1);
-        const short* qp = (const short*)a.q + (size_t)qr * a.qs + (size_t)head * a.dim + half * 8;
+        const uint32_t qr = T.q0 + (uint32_t)min(my, T.nq - 1);
+        const short* qp = (const short*)a.q + (size_t)qr * a.qs + (size_t)T.head * a.dim + half * 8;
 #pragma unroll
         for (int c = 0; c < C; c++) {
             qf[c] = (s8v)(short)0;
@@ -320,28 +376,9 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         }
     }
 
-    // tiles that any row of the workgroup sees: sinks, then first .. last - 1;
-    // of those, all rows see wa .. wb - 1 whole.  These come first.
-    const int p0 = off + r0, p1 = off + min(r0 + 128, nq) - 1;
-    const int end = min(nk, a.causal ? p1 + 1 : nk);
-    const int wlo = a.window ? max(0, p0 - a.window + 1) : 0;
-    const int first = wlo / PR_KEYS, last = end <= 0 ? 0 : (end + PR_KEYS - 1) / PR_KEYS;
-    const int sinks = min(min((a.sink + PR_KEYS - 1) / PR_KEYS, first), last);
-    const int tiles = max(0, last - first) + sinks;
-    const int wa = a.window ? max(first, (max(0, p1 - a.window + 1) + PR_KEYS - 1) / PR_KEYS) : 0;
-    const int wb = max(wa, min(nk, a.causal ? max(0, p0 + 1) : nk) / PR_KEYS);
-    const int whole = tiles ? wb - wa : 0;
-    auto tile_of = [&](int it) {
-        if (it < whole) return wa + it;
-        it -= whole;
-        if (it < sinks) return it;
-        it += first - sinks;
-        return it < wa ? it : it + whole;
-    };
-
-    const size_t kv_head = (size_t)(head / a.group) * a.dim;
-    const short* kg = (const short*)a.k + (size_t)k0 * a.ks + kv_head;
-    const short* vg = (const short*)a.v + (size_t)k0 * a.vs + kv_head;
+    const size_t kv_head = (size_t)(T.head / a.group) * a.dim;
+    const short* kg = (const short*)a.k + (size_t)T.k0 * a.ks + kv_head;
+    const short* vg = (const short*)a.v + (size_t)T.k0 * a.vs + kv_head;
     // a lane's place in a tile's rows as 32-bit offsets from the tile's first row
     const int lr = lane / CH, lc = lane % CH;
     const bool near = (uint64_t)max(a.ks, a.vs) * (PR_KEYS * 2) <= 0xFFFFFFFFull;
@@ -364,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     }
     auto load = [&](auto buf, int it) {
         constexpr bool B = decltype(buf)::value;
-        const int key0 = tile_of(it) * PR_KEYS;
+        const int key0 = T.key_tile(it) * PR_KEYS;
         const uint8_t* kt = (const uint8_t*)(kg + (size_t)(uint32_t)key0 * a.ks);
         const uint8_t* vt = (const uint8_t*)(vg + (size_t)(uint32_t)key0 * a.vs);
         short *sk = B ? sk1 : sk0, *sv = B ? sv1 : sv0;
@@ -407,35 +444,8 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
                 const s8v kf = *(const s8v*)&sk[(g * 32 + row) * DP + k_place<DP>(row, c * 2 + half) * 8];
                 s[g] = mfma32<BF>(kf, qf[c], s[g]);
             }
-        if constexpr (MASKED) {
-            // one bit per key of the tile
-            const uint64_t see = first_bits(min(hi, nk - 1) + 1 - key0) &
-                                 (~first_bits(lo - key0) | first_bits(a.sink - key0));
-            const uint32_t part[2] = {(uint32_t)see >> (4 * half), (uint32_t)(see >> 32) >> (4 * half)};
-#pragma unroll
-            for (int g = 0; g < 2; g++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    s[g][i] = bits_or(s[g][i], -INFINITY, __builtin_amdgcn_sbfe((int)part[g], 8 * (i / 4) + i % 4, 1));
-                }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int g = 0; g < 2; g++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, s[g][i]);
-        top *= a.scale_log2;
-        if (__any(top > m + MAX_SLACK)) {
-            const float to = fmaxf(m, max32(top));
-            const float f = to == -INFINITY ? 1.0f : exp2_fast(m - to);
-            m = to;
-            l *= f;
-#pragma unroll
-            for (int t = 0; t < DT; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[t][i] *= f;
-        }
-        const float ms = m == -INFINITY ? 0.0f : m;
+        if constexpr (MASKED) mask_scores(s, a, nk, hi, lo, key0, half);
+        const float ms = new_maximum<DT>(s, a.scale_log2, m, l, o);
         s8v pf[4];
         float l1 = 0.0f;
 #pragma unroll
@@ -507,55 +517,35 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     };
-    // this wave's rows see something of the tile
-    auto some = [&](int key0) {
-        const int w0 = p0 + wave * 32, w1 = min(w0 + 31, p1);
-        return !((a.causal && key0 > w1) | (a.window && key0 + PR_KEYS <= w0 - a.window + 1 && key0 >= a.sink));
-    };
     constexpr std::false_type no{};
     constexpr std::true_type yes{};
 
     if (tid == 0) s_odd = -1;
-    if (tiles) load(no, 0);
+    if (T.tiles) load(no, 0);
     int it = 0;
-    for (; it + 1 < whole; it += 2) {
+    for (; it + 1 < T.whole; it += 2) {
         turn();
         load(yes, it + 1);
         body(no, no, 0);
         turn();
-        if (it + 2 < tiles) load(no, it + 2);
+        if (it + 2 < T.tiles) load(no, it + 2);
         body(no, yes, 0);
     }
-    for (; it < tiles; it += 2) {                // (at most one whole tile among these)
-        int key0 = tile_of(it) * PR_KEYS;
+    for (; it < T.tiles; it += 2) {                // (at most one whole tile among these)
+        int key0 = T.key_tile(it) * PR_KEYS;
         turn();
-        if (it + 1 < tiles) load(yes, it + 1);
+        if (it + 1 < T.tiles) load(yes, it + 1);
         clean(no, it, key0);
-        if (some(key0)) body(yes, no, key0);
-        if (it + 1 >= tiles) break;
-        key0 = tile_of(it + 1) * PR_KEYS;
+        if (T.some(a, key0, wave)) body(yes, no, key0);
+        if (it + 1 >= T.tiles) break;
+        key0 = T.key_tile(it + 1) * PR_KEYS;
         turn();
-        if (it + 2 < tiles) load(no, it + 2);
+        if (it + 2 < T.tiles) load(no, it + 2);
         clean(yes, it + 1, key0);
-        if (some(key0)) body(yes, yes, key0);
+        if (T.some(a, key0, wave)) body(yes, yes, key0);
     }
 
-    l = sum32(l);
-    if (my >= nq) return;
-    const bool none = !(a.causal ? p >= 0 : nk > 0);
-    const float inv = none ? 0.0f : 1.0f / l;
-    short* op = (short*)a.out + (size_t)(q0 + (uint32_t)my) * a.os + (size_t)head * a.dim;
-#pragma unroll
-    for (int t = 0; t < DT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = t * 32 + 8 * (i / 4) + 4 * half;
-            if (!EXACT && d >= (int)a.dim) continue;
-            float x[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[t][i + j] * inv;
-            store4<ACT>(op + d, x);
-        }
+    put_rows<ACT, DT, EXACT>(a, T, my, half, l, o);
 }
 
 }  // namespace pf
@@ -590,7 +580,7 @@ template <int ACT, int DP, bool EXACT>
 static void prompt_one(hipStream_t st, const PromptArgs& a) {
     const uint32_t units = prompt_units(a.tiles, a.n_heads / a.group, a.group);
     if constexpr (ACT == PF_TYPE_F32)
-        hipLaunchKernelGGL((k_prompt_attn<ACT, DP, EXACT>), dim3(units), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_prompt_attn32<DP, EXACT>), dim3(units), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((k_prompt_attn16<ACT, DP, EXACT>), dim3(units), dim3(256), 0, st, a);
 }
