@@ -6,6 +6,7 @@ the gfx950 kernels; there is no CPU fallback.  If the library is missing the
 import raises.  Device buffers for the kernel-level entry points come from
 the library's own pf_malloc (DeviceArray).
 """
+import array
 import ctypes as C
 import os
 
@@ -285,17 +286,15 @@ def _rows(t, what):
 
 
 def _u32(a, what):
-    """A list of numbers from 0 as a C array."""
-    if type(a) is list or type(a) is tuple:
-        try:
-            if not a or (min(a) >= 0 and max(a) <= 0xFFFFFFFF):
-                return (C.c_uint32 * len(a))(*a)
-        except TypeError:
-            pass
-    x = np.atleast_1d(np.asarray(a))
-    if x.ndim != 1 or (x.size and (x.dtype.kind not in "iu" or x.min() < 0 or x.max() > 0xFFFFFFFF)):
-        raise PFError(f"{what} is a list of numbers from 0")
-    return (C.c_uint32 * x.size)(*x.tolist())
+    """A list of numbers from 0 as an array of 32-bit numbers."""
+    try:
+        return array.array("I", a.tolist() if isinstance(a, np.ndarray) else a)
+    except (TypeError, OverflowError, ValueError):
+        raise PFError(f"{what} is a list of numbers from 0") from None
+
+
+def _at(a):
+    return a.buffer_info()[0]
 
 
 def _vptr(a):
@@ -462,7 +461,7 @@ class Context:
         if (n2, H2, D3) != (nq, H, D) or not t == _type(k) == _type(v) == _type(y):
             raise PFError("q, k, v and out have one type, q and out one shape")
         d = AttnDesc(t, H, G, D, causal, window, sink, scale, qs, ks, vs, os)
-        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), ql, kl,
+        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), _at(ql), _at(kl),
                                              len(ql)), "pf_prompt_attention")
         if out is None:
             self.synchronize()
@@ -609,7 +608,7 @@ class PagedCache:
         s, r = _u32(seqs, "seqs"), _u32(rows, "rows")
         if len(s) != len(r):
             raise PFError("seqs and rows have one length")
-        self.ctx.check(lib().pf_pages_append(self.h, s, r, len(s)), "pf_pages_append")
+        self.ctx.check(lib().pf_pages_append(self.h, _at(s), _at(r), len(s)), "pf_pages_append")
         self.pass_rows = sum(r)
 
     def _kv(self, k, v, rows):
@@ -645,14 +644,14 @@ class PagedCache:
         """The sequences' rows of one layer, packed: (k, v)."""
         s = _u32(seqs, "seqs")
         lens = np.zeros(len(s), np.int64)
-        self.ctx.check(lib().pf_pages_tables(self.h, s, len(s), None, 0, _vptr(lens)), "pf_pages_tables")
+        self.ctx.check(lib().pf_pages_tables(self.h, _at(s), len(s), None, 0, _vptr(lens)), "pf_pages_tables")
         n = int(lens.sum())
         if out is None:
             k, v = (self.ctx.empty((n, self.n_kv_heads, self.head_dim), dtype) for _ in range(2))
         else:
             k, v = out
         t, ks, vs = self._kv(k, v, n)
-        self.ctx.check(lib().pf_pages_gather(self.h, layer, s, len(s), t, _dptr(k), _dptr(v), ks, vs),
+        self.ctx.check(lib().pf_pages_gather(self.h, layer, _at(s), len(s), t, _dptr(k), _dptr(v), ks, vs),
                        "pf_pages_gather")
         if out is None:
             self.ctx.synchronize()
@@ -660,23 +659,23 @@ class PagedCache:
 
     def fork(self, src, dst):
         d = _u32(dst, "dst")
-        self.ctx.check(lib().pf_pages_fork(self.h, src, d, len(d)), "pf_pages_fork")
+        self.ctx.check(lib().pf_pages_fork(self.h, src, _at(d), len(d)), "pf_pages_fork")
 
     def copy(self, src, dst):
         s, d = _u32(src, "src"), _u32(dst, "dst")
         if len(s) != len(d):
             raise PFError("src and dst have one length")
-        self.ctx.check(lib().pf_pages_copy(self.h, s, d, len(d)), "pf_pages_copy")
+        self.ctx.check(lib().pf_pages_copy(self.h, _at(s), _at(d), len(d)), "pf_pages_copy")
 
     def truncate(self, seqs, lengths):
         s, n = _u32(seqs, "seqs"), _u32(lengths, "lengths")
         if len(s) != len(n):
             raise PFError("seqs and lengths have one length")
-        self.ctx.check(lib().pf_pages_truncate(self.h, s, n, len(s)), "pf_pages_truncate")
+        self.ctx.check(lib().pf_pages_truncate(self.h, _at(s), _at(n), len(s)), "pf_pages_truncate")
 
     def free(self, seqs):
         s = _u32(seqs, "seqs")
-        self.ctx.check(lib().pf_pages_free(self.h, s, len(s)), "pf_pages_free")
+        self.ctx.check(lib().pf_pages_free(self.h, _at(s), len(s)), "pf_pages_free")
 
     def compact(self):
         """The number of pages that moved."""
@@ -691,10 +690,10 @@ class PagedCache:
         """Page numbers of the sequences, -1 past their ends, and their lengths."""
         s = _u32(seqs, "seqs")
         lens = np.zeros(len(s), np.int64)
-        self.ctx.check(lib().pf_pages_tables(self.h, s, len(s), None, 0, _vptr(lens)), "pf_pages_tables")
+        self.ctx.check(lib().pf_pages_tables(self.h, _at(s), len(s), None, 0, _vptr(lens)), "pf_pages_tables")
         cap = -(-int(lens.max(initial=0)) // self.page_size)
         pages = np.empty((len(s), cap), np.int64)
-        self.ctx.check(lib().pf_pages_tables(self.h, s, len(s), _vptr(pages), cap, None), "pf_pages_tables")
+        self.ctx.check(lib().pf_pages_tables(self.h, _at(s), len(s), _vptr(pages), cap, None), "pf_pages_tables")
         return pages, lens
 
     def planes(self, layer=None):
