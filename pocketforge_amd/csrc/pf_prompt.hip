@@ -154,53 +154,50 @@ __device__ __forceinline__ float new_maximum(const f16v (&s)[G], float scale, fl
     return m == -INFINITY ? 0.0f : m;
 }
 
-// The rows' results: O^T over the sums.  A row that sees no key is zero; one
-// whose scores are all -infinity is 0 / 0.
-// SPLIT 2: the waves of the upper key halves hand theirs over through LDS.
-template <int ACT, int DT, bool EXACT, int SPLIT>
-__device__ __forceinline__ void put_rows(const PromptArgs& a, const PromptTile<SPLIT>& t, int my, int wave, float m, float l,
-                                         f16v (&o)[DT], float* lds) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
+// SPLIT 2: the waves of the upper key halves hand their results to the others
+// through LDS: DT / 2 pieces of 8 KB in x0 and in x1, 2 KB in x2.
+template <int DT>
+__device__ __forceinline__ void join_halves(int wave, float& m, float& l, f16v (&o)[DT], void* x0, void* x1, void* x2) {
+    const int lane = threadIdx.x & 63, at = (wave & 1) * 256 + lane;
+    f4v* ml = (f4v*)x2 + (wave & 1) * 64 + lane;
     l = sum32(l);
-    if constexpr (SPLIT == 2) {
-        f4v* p = (f4v*)lds + (wave & 1) * (DT * 4 + 1) * 64 + lane;
-        __syncthreads();
-        if (wave >= 2) {
+    __syncthreads();
+    if (wave >= 2) {
 #pragma unroll
-            for (int n = 0; n < DT; n++)
+        for (int n = 0; n < DT; n++) {
+            f4v* p = (f4v*)(n < DT / 2 ? x0 : x1) + n % (DT / 2) * 512 + at;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const f4v x = {o[n][4 * i], o[n][4 * i + 1], o[n][4 * i + 2], o[n][4 * i + 3]};
-                    p[(n * 4 + i) * 64] = x;
-                }
-            const f4v ml = {m, l, 0.0f, 0.0f};
-            p[DT * 4 * 64] = ml;
+            for (int i = 0; i < 4; i++) {
+                const f4v x = {o[n][4 * i], o[n][4 * i + 1], o[n][4 * i + 2], o[n][4 * i + 3]};
+                p[i * 64] = x;
+            }
         }
-        __syncthreads();
-        if (wave >= 2) return;
-        const f4v ml = p[DT * 4 * 64];
-        const float to = fmaxf(m, ml[0]), ms = to == -INFINITY ? 0.0f : to, f0 = exp2_fast(m - ms), f1 = exp2_fast(ml[0] - ms);
-        l = l * f0 + ml[1] * f1;
-#pragma unroll
-        for (int n = 0; n < DT; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[n][i] = o[n][i] * f0 + p[(n * 4 + i / 4) * 64][i % 4] * f1;
+        const f4v x = {m, l, 0.0f, 0.0f};
+        *ml = x;
     }
-    if (my >= t.nq) return;
-    const bool none = !(a.causal ? t.off + my >= 0 : t.nk > 0);
-    const float inv = none ? 0.0f : 1.0f / l;
-    uint8_t* op = (uint8_t*)a.out + ((size_t)(t.q0 + (uint32_t)my) * a.os + (size_t)t.head * a.dim) * act_size<ACT>;
+    __syncthreads();
+    if (wave >= 2) return;
+    const f4v x = *ml;
+    const float to = fmaxf(m, x[0]), ms = to == -INFINITY ? 0.0f : to, f0 = exp2_fast(m - ms), f1 = exp2_fast(x[0] - ms);
+    l = l * f0 + x[1] * f1;
 #pragma unroll
-    for (int n = 0; n < DT; n++)
+    for (int n = 0; n < DT; n++) {
+        const f4v* p = (const f4v*)(n < DT / 2 ? x0 : x1) + n % (DT / 2) * 512 + at;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = n * 32 + 8 * (i / 4) + 4 * half;
-            if (!EXACT && d >= (int)a.dim) continue;
-            float x[4];
+        for (int i = 0; i < 4; i++) {
+            const f4v y = p[i * 64];
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[n][i + j] * inv;
-            store4<ACT>(op + (size_t)d * act_size<ACT>, x);
+            for (int j = 0; j < 4; j++) o[n][4 * i + j] = o[n][4 * i + j] * f0 + y[j] * f1;
         }
+    }
+}
+
+// What a row's output is multiplied by.  A row that sees no key is zero; one
+// whose scores are all -infinity is 0 / 0.
+template <int ROWS>
+__device__ __forceinline__ float row_factor(const PromptArgs& a, const PromptTile<ROWS>& t, int my, float l, bool* none) {
+    *none = !(a.causal ? t.off + my >= 0 : t.nk > 0);
+    return *none ? 0.0f : 1.0f / l;
 }
 
 // fp32 rows, three bf16 pieces each: six matrix instructions where 16-bit rows
@@ -361,7 +358,29 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptA
     int it = 0;
     for (; it < T.whole; it++) body(std::false_type{}, it);
     for (; it < T.tiles; it++) body(std::true_type{}, it);
-    put_rows<ACT, DT, EXACT>(a, T, my, wave, m, l, o, (float*)&sv[0][0][0]);
+    if constexpr (SPLIT == 2) {
+        uint8_t* x = (uint8_t*)&sv[0][0][0];
+        static_assert(DT * 8192 + 2048 <= sizeof(sv), "the halves' exchange fits V's tile");
+        join_halves(wave, m, l, o, x, x + DT / 2 * 8192, x + DT * 8192);
+        if (wave >= 2) return;
+    } else {
+        l = sum32(l);
+    }
+    if (my >= T.nq) return;
+    bool none;
+    const float f = row_factor(a, T, my, l, &none);
+    float* op = (float*)a.out + (size_t)(T.q0 + (uint32_t)my) * a.os + (size_t)T.head * a.dim;
+#pragma unroll
+    for (int n = 0; n < DT; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = n * 32 + 8 * (i / 4) + 4 * half;
+            if (!EXACT && d >= (int)a.dim) continue;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[n][i + j] * f;
+            store4<ACT>(op + d, x);
+        }
 }
 
 // fp16 and bf16 rows: K and V tiles go from memory straight to LDS, two tiles
@@ -584,7 +603,36 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         if (T.some(a, key0, wave)) body(yes, yes, key0);
     }
 
-    put_rows<ACT, DT, EXACT>(a, T, my, wave, m, l, o, (float*)sk0);
+    if constexpr (SPLIT == 2) {
+        static_assert(DT / 2 * 8192 <= sizeof(sk0) && 2048 <= sizeof(sv1), "the halves' exchange fits the tiles");
+        join_halves(wave, m, l, o, sk0, sk1, sv1);
+        if (wave >= 2) return;
+    } else {
+        l = sum32(l);
+        __syncthreads();                         // nobody reads V any more
+    }
+    // rows go out whole, 16 bytes a lane, by way of LDS (8 bytes of 32 rows at a
+    // time take 6 us more of 57 for 24 packed prompts)
+    bool none;
+    const float f = row_factor(a, T, my, l, &none);
+    short* st = (wave < 2 ? sv0 : sv1) + (wave & 1) * 32 * DP;
+#pragma unroll
+    for (int n = 0; n < DT; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = none ? 0.0f : o[n][i + j] * f;
+            store4<ACT>(st + row * DP + k_place<DP>(row, n * 4 + i / 4) * 8 + 4 * half, x);
+        }
+    __builtin_amdgcn_wave_barrier();
+    short* op = (short*)a.out + (size_t)T.head * a.dim + lc * 8;
+#pragma unroll
+    for (int i = 0; i < 32 / RPL; i++) {
+        const int r = i * RPL + lr, at = my - row + r;
+        if (at < T.nq && (EXACT || lc * 8 < (int)a.dim))
+            *(s8v*)(op + (size_t)(T.q0 + (uint32_t)at) * a.os) = *(const s8v*)&st[r * DP + k_place<DP>(r, lc) * 8];
+    }
 }
 
 }  // namespace pf
