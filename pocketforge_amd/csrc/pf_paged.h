@@ -30,6 +30,7 @@ struct PageSplit {
     uint32_t window = 0, sink = 0, heads = 0;
     int32_t type = -1;
     uint32_t n_items = 0, ws_rows = 0, most_rows = 0;
+    uint32_t waves = 4;
     bool split = false;
 };
 

@@ -22,22 +22,22 @@ __host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
     return dp == 64 ? (nt == 1 ? (wide ? 3 : 4) : 2) : nt == 1 ? 2 : wide ? 1 : 2;
 }
 
-// A workgroup: 4 waves, each on 32-key tiles of its own, four tiles apart.
+// A workgroup: W waves (4 or 8), each on 32-key tiles of its own.
 // A lane's matrix operands of K are 16 bytes of a row as the page holds them,
 // straight from memory; V's rows go through LDS, which transposes them.  The
 // rows of all query heads of the kv head are the columns of the score tile
 // S^T = K Q^T, 16 at a time (NT tiles); exp(S)^T is the operand of O^T = V^T P^T
 // without moving a value between lanes.
-template <int ACT, int CT, int DP, int NT, bool EXACT>
-__global__ __launch_bounds__(256, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
+template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
+__global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
     constexpr bool BF = op_bf<ACT>, I8 = CT == PF_TYPE_I8;
     constexpr int NP = op_pieces<ACT>, PP = weight_pieces<ACT>, C = DP / 32, DT = DP / 16;
     constexpr int STR = DP + 16;                 // LDS row stride in values
     constexpr int VCH = I8 ? DP / 16 : DP / 8;   // 16-byte chunks of a V row
     constexpr int VL = 32 * VCH / 64;            // V loads of a lane
     constexpr int KL = I8 ? DP / 64 : C;         // K loads of a lane per 16 keys
-    __shared__ __align__(16) short sv[4][32][STR];
-    __shared__ float s_ml[4][16][2];
+    __shared__ __align__(16) short sv[W][32][STR];
+    __shared__ float s_ml[W][16][2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
 
     const PageItem it = a.items[blockIdx.x];
@@ -51,14 +51,14 @@ __global__ __launch_bounds__(256, paged_waves(ACT, DP, NT)) void k_paged_attn(Pa
     const auto pos_of = [&](int t) { return (t < pt.sinks ? t : t - pt.sinks + pt.first) * 32; };
 
     // The share's tiles in this wave's order: first those that all rows see whole,
-    // wa .. wb - 1, then the others; the four waves take them in turn.
+    // wa .. wb - 1, then the others; the waves take them in turn.
     const int t0 = (int)it.t0, t1 = (int)it.t1;
     const int wa = min(max(pt.sinks + (lo1 + 31) / 32 - pt.first, max(t0, pt.sinks)), t1);
     const int wb = min(max(pt.sinks + (a.causal ? p0 + 1 : len) / 32 - pt.first, wa), t1);
-    const int n_whole = (wb - wa + 3 - wave) >> 2, n_tiles = n_whole + ((t1 - t0 - (wb - wa) + wave) >> 2);
+    const int n_whole = (wb - wa + W - 1 - wave) / W, n_tiles = n_whole + (t1 - t0 - (wb - wa) + wave) / W;
     const auto tile_of = [&](int n) {
-        if (n < n_whole) return wa + wave + 4 * n;
-        const int e = t0 + 3 - wave + 4 * (n - n_whole);      // (the waves in the other order)
+        if (n < n_whole) return wa + wave + W * n;
+        const int e = t0 + W - 1 - wave + W * (n - n_whole);      // (the waves in the other order)
         return e < wa ? e : e + wb - wa;
     };
 
@@ -269,8 +269,8 @@ __global__ __launch_bounds__(256, paged_waves(ACT, DP, NT)) void k_paged_attn(Pa
     for (; n_tile < n_whole; n_tile++) body(std::false_type{}, n_tile);
     for (; n_tile < n_tiles; n_tile++) body(std::true_type{}, n_tile);
 
-    // the four waves' results meet in LDS, 16 rows at a time
-    float* so = (float*)&sv[0][0][0];            // [4][16][DP]
+    // the waves' results meet in LDS, 16 rows at a time
+    float* so = (float*)&sv[0][0][0];            // [W][16][DP]
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const float lw = sum16(l[n]);
@@ -282,20 +282,20 @@ __global__ __launch_bounds__(256, paged_waves(ACT, DP, NT)) void k_paged_attn(Pa
             s_ml[wave][col][1] = lw;
         }
         __syncthreads();
-        constexpr int PER = DP / 16;             // dims of a thread
-        const int r = tid >> 4, d0 = (tid & 15) * PER, row = rt0 + n * 16 + r;
+        constexpr int PER = DP / (4 * W);        // dims of a thread
+        const int r = tid / (4 * W), d0 = tid % (4 * W) * PER, row = rt0 + n * 16 + r;
         float M = -INFINITY, L = 0.0f, acc[PER] = {};
 #pragma unroll
-        for (int w = 0; w < 4; w++) M = fmaxf(M, s_ml[w][r][0]);
+        for (int w = 0; w < W; w++) M = fmaxf(M, s_ml[w][r][0]);
         const float ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
             const float f = exp2_fast(s_ml[w][r][0] - ms);
             L += f * s_ml[w][r][1];
 #pragma unroll
             for (int i = 0; i < PER; i++) acc[i] += f * so[(w * 16 + r) * DP + d0 + i];
         }
-        if (row >= R || (!EXACT && d0 >= (int)a.dim)) continue;
+        if (row >= R || (!EXACT && d0 >= (int)a.dim)) continue;   // (pairs of threads together)
         const int j = row / (int)a.group, h = (int)head0 + row - j * (int)a.group;
         if (it.parts == 1) {
             const float inv = 1.0f / L;
@@ -303,9 +303,18 @@ __global__ __launch_bounds__(256, paged_waves(ACT, DP, NT)) void k_paged_attn(Pa
 #pragma unroll
             for (int i = 0; i < PER; i += 4) {
                 float x[4];
+                if constexpr (PER >= 4) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = acc[i + e] * inv;
-                if (EXACT || d0 + i < (int)a.dim) store4<ACT>(op + i * act_size<ACT>, x);
+                    for (int e = 0; e < 4; e++) x[e] = acc[i + e] * inv;
+                    if (EXACT || d0 + i < (int)a.dim) store4<ACT>(op + i * act_size<ACT>, x);
+                } else {
+                    // two dims a thread (8 waves, 64 dims): pairs of threads meet
+                    static_assert(PER == 2 || PER >= 4, "two dims a thread at least");
+                    const float y0 = acc[0] * inv, y1 = acc[1] * inv;
+                    x[0] = y0; x[1] = y1;
+                    x[2] = __shfl_down(y0, 1); x[3] = __shfl_down(y1, 1);
+                    if ((tid & 1) == 0 && (EXACT || d0 < (int)a.dim)) store4<ACT>(op, x);
+                }
             }
         } else {
             const size_t w = (size_t)(it.ws0 + it.part * it.rows + (uint32_t)j) * a.n_heads + (uint32_t)h;
@@ -381,60 +390,92 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
 
 // ================================================================== host
 
+template <int ACT, int CT, int DP, int NT, bool EXACT>
+static void paged_one(hipStream_t st, const PageSplit& u, uint32_t z, const PagedArgs& a) {
+    const dim3 grid(u.n_items, a.kv_heads, z);
+    if constexpr (paged_waves(ACT, DP, NT) > 1)
+        if (u.waves == 8) {
+            hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, NT, EXACT, 8>), grid, dim3(512), 0, st, a);
+            return;
+        }
+    hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, NT, EXACT, 4>), grid, dim3(256), 0, st, a);
+}
+
 template <int ACT, int CT, int DP, bool EXACT>
-static void paged_rows(hipStream_t st, uint32_t items, uint32_t most, const PagedArgs& a) {
-    const uint32_t R = most * a.group;
+static void paged_rows(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
+    const uint32_t R = u.most_rows * a.group;
     // one tile of 16 rows, or two: the keys are read once for both
-    if (R <= 16)
-        hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, 1, EXACT>), dim3(items, a.kv_heads), dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, 2, EXACT>), dim3(items, a.kv_heads, (R + 31) / 32), dim3(256), 0, st, a);
+    if (R <= 16) paged_one<ACT, CT, DP, 1, EXACT>(st, u, 1, a);
+    else paged_one<ACT, CT, DP, 2, EXACT>(st, u, (R + 31) / 32, a);
 }
 
 template <int ACT, int CT>
-static void paged_dim(hipStream_t st, uint32_t items, uint32_t most, const PagedArgs& a) {
-    if (a.dim == 128) paged_rows<ACT, CT, 128, true>(st, items, most, a);
-    else if (a.dim == 64) paged_rows<ACT, CT, 64, true>(st, items, most, a);
-    else if (a.dim < 64) paged_rows<ACT, CT, 64, false>(st, items, most, a);
-    else paged_rows<ACT, CT, 128, false>(st, items, most, a);
+static void paged_dim(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
+    if (a.dim == 128) paged_rows<ACT, CT, 128, true>(st, u, a);
+    else if (a.dim == 64) paged_rows<ACT, CT, 64, true>(st, u, a);
+    else if (a.dim < 64) paged_rows<ACT, CT, 64, false>(st, u, a);
+    else paged_rows<ACT, CT, 128, false>(st, u, a);
 }
 
-// Cuts the pass's keys: the smallest shares with which one round of workgroups
-// holds them all (two per sequence and head, if that is more: a long sequence
-// beside short ones), but of PG_LEAST tiles, one for each wave.
-constexpr uint32_t PG_LEAST = 4, PG_CUS = 256;
+// Cuts the pass's keys into shares of at most `chunk` tiles, by what they would
+// take: the rounds of workgroups (`per` for each share), each as long as its
+// longest wave's run of tiles and about a tile's time more, and the second
+// kernel, about two tiles', where a sequence is cut.  Looked at: no cut, and the
+// smallest shares that one round of workgroups holds, or two for each sequence
+// (a long one beside short ones), but of a tile for each wave; with workgroups
+// of 4 waves, and of 8 (half as many shares, to join as well).
+constexpr uint32_t PG_CUS = 256, PG_JOIN = 2;
+struct PageShares {
+    uint32_t chunk = 1, waves = 4;
+    uint64_t cost = ~0ull;
+};
+static uint64_t page_shares_of(const std::vector<uint32_t>& tiles, uint32_t chunk) {
+    uint64_t n = 0;
+    for (uint32_t t : tiles) n += (t + chunk - 1) / chunk;
+    return n;
+}
+static void page_shares(const std::vector<uint32_t>& tiles, uint32_t longest, uint64_t per, uint64_t round, uint32_t waves,
+                        PageShares* best) {
+    const auto take = [&](uint32_t chunk) {
+        const uint64_t rounds = (page_shares_of(tiles, chunk) * per + round - 1) / round;
+        const uint64_t cost = rounds * ((chunk + waves - 1) / waves + 1) + (chunk < longest ? PG_JOIN : 0);
+        if (cost < best->cost) *best = {chunk, waves, cost};
+    };
+    const uint32_t least = std::max<uint32_t>(waves, (longest + PG_MOST_PARTS - 1) / PG_MOST_PARTS);
+    take(std::max(longest, 1u));
+    for (const uint64_t budget : {round / per, (uint64_t)2 * tiles.size()}) {
+        uint32_t chunk = least, high = std::max(least, longest);
+        while (chunk < high) {
+            const uint32_t mid = chunk + (high - chunk) / 2;
+            if (page_shares_of(tiles, mid) <= budget) high = mid;
+            else chunk = mid + 1;
+        }
+        if (chunk < longest) take(chunk);
+    }
+}
 static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
     PageSplit& u = p->cut;
     if (u.type == d->type && u.window == s.window && u.sink == s.sink && u.heads == d->n_heads) return PF_OK;
     const uint32_t group = d->n_heads / d->n_kv_heads;
     std::vector<uint32_t> tiles;
     tiles.reserve(p->pass.size());
-    uint64_t all = 0;
     uint32_t most = 0, longest = 0;
     for (const PageSeq& q : p->pass) {
         if (!q.rows) continue;
         tiles.push_back((uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count);
-        all += tiles.back();
         longest = std::max(longest, tiles.back());
         most = std::max(most, q.rows);
     }
     const uint64_t R = (uint64_t)most * group, per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
-    const uint64_t round = (uint64_t)PG_CUS * paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
-    const uint64_t budget = std::max<uint64_t>(round / per, 2 * tiles.size());
-    const auto items_of = [&](uint32_t chunk) {
-        uint64_t n = 0;
-        for (uint32_t t : tiles) n += (t + chunk - 1) / chunk;
-        return n;
-    };
-    uint32_t chunk = std::max<uint32_t>(PG_LEAST, (longest + PG_MOST_PARTS - 1) / PG_MOST_PARTS), high = std::max(chunk, longest);
-    while (chunk < high) {                       // (the fewest tiles that the budget allows)
-        const uint32_t mid = chunk + (high - chunk) / 2;
-        if (items_of(mid) <= budget) high = mid;
-        else chunk = mid + 1;
-    }
-    std::vector<PageItem> items;
-    items.reserve(items_of(chunk));
+    const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
+    PageShares best;
+    page_shares(tiles, longest, per, (uint64_t)PG_CUS * held, 4, &best);
+    if (held > 1) page_shares(tiles, longest, per, (uint64_t)PG_CUS * (held / 2), 8, &best);
+    const uint32_t chunk = best.chunk;
     PageSplit n;
+    n.waves = best.waves;
+    std::vector<PageItem> items;
+    items.reserve(page_shares_of(tiles, chunk));
     uint64_t ws = 0;
     uint32_t i = 0;
     for (const PageSeq& q : p->pass) {
@@ -494,7 +535,7 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
     a.causal = d->causal != 0; a.window = (int32_t)s.window; a.sink = (int32_t)s.sink;
     a.scale_log2 = s.scale_log2;
     hipStream_t st = c->stream;
-#define PF_PAGED(A, T) paged_dim<A, T>(st, u.n_items, u.most_rows, a)
+#define PF_PAGED(A, T) paged_dim<A, T>(st, u, a)
     if (ct == PF_TYPE_I8) {
         if (d->type == PF_TYPE_F32) PF_PAGED(PF_TYPE_F32, PF_TYPE_I8);
         else if (d->type == PF_TYPE_F16) PF_PAGED(PF_TYPE_F16, PF_TYPE_I8);
