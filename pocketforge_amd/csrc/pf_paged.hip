@@ -30,7 +30,9 @@ __host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
 // without moving a value between lanes.
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
 __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
-    constexpr bool BF = op_bf<ACT>, I8 = CT == PF_TYPE_I8;
+    // Weights over int8 rows take the rows' scales, whose range fp16 does not
+    // have, so their products with the codes are in bf16 for fp16 rows too.
+    constexpr bool I8 = CT == PF_TYPE_I8, BF = op_bf<ACT>, VB = I8 || BF;
     constexpr int NP = op_pieces<ACT>, PP = weight_pieces<ACT>, C = DP / 32, DT = DP / 16;
     constexpr int STR = DP + 16;                 // LDS row stride in values
     constexpr int VCH = I8 ? DP / 16 : DP / 8;   // 16-byte chunks of a V row
@@ -178,9 +180,9 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
             if constexpr (I8) {
                 float x[8];
                 codes8(w[0], w[1], x);
-                *(s8v*)place(i) = pack8<BF>(x);
+                *(s8v*)place(i) = pack8<VB>(x);
                 codes8(w[2], w[3], x);
-                *(s8v*)(place(i) + 8) = pack8<BF>(x);
+                *(s8v*)(place(i) + 8) = pack8<VB>(x);
             } else {
                 if constexpr (MASKED) z = sum8<BF>(__builtin_bit_cast(s8v, w), z, 0.0f);
                 *(u4v*)place(i) = w;
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                     if constexpr (MASKED) x[e] = bits_or(x[e], 0.0f, __builtin_amdgcn_sbfe((int)part, 16 * (e / 4) + e % 4, 1));
                 }
             }
-            pieces<BF, PP>(x, pf[n]);
+            pieces<VB, PP>(x, pf[n]);
         }
         __builtin_amdgcn_wave_barrier();
         if constexpr (MASKED && !I8) {
@@ -260,7 +262,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int x = 0; x < PP; x++) o[n][d] = mfma16<BF>(vf[d], pf[n][x], o[n][d]);
+                for (int x = 0; x < PP; x++) o[n][d] = mfma16<VB>(vf[d], pf[n][x], o[n][d]);
         __builtin_amdgcn_wave_barrier();
     };
 
@@ -468,6 +470,7 @@ static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& 
     }
     const uint64_t R = (uint64_t)most * group, per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
     const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
+    if (R > 32 * 65535u) return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
     PageShares best;
     page_shares(tiles, longest, per, (uint64_t)PG_CUS * held, 4, &best);
     if (held > 1) page_shares(tiles, longest, per, (uint64_t)PG_CUS * (held / 2), 8, &best);

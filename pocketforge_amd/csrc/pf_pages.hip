@@ -378,9 +378,14 @@ static void more_pages(pf_pages* p, uint32_t seq, size_t n) {
     if (t.capacity() < n) t.reserve(std::max(n, 2 * t.capacity()));
 }
 // The device's tables learn of changes with the next pass, or the next call that
-// reads them.  (Room for `n` of them before anything changes.)
-static void more_changes(pf_pages* p, size_t n) {
+// reads them, or when there are many.  (Room for `n` more before anything
+// changes.)
+constexpr size_t DIRTY_MOST = 1 << 16;
+static pf_status more_changes(pf_pages* p, size_t n) {
+    if (p->dirty.size() > DIRTY_MOST)
+        if (pf_status st = tables_to_device(p)) return st;
     if (p->dirty.capacity() - p->dirty.size() < n) p->dirty.reserve(std::max(p->dirty.size() + n, 2 * p->dirty.capacity()));
+    return PF_OK;
 }
 static void change(pf_pages* p, uint32_t seq, uint32_t at) { p->dirty.push_back(seq * p->per_seq + at); }
 
@@ -560,7 +565,7 @@ static pf_status pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t*
     DeviceScope on(c);
     // (all host memory that the changes need first)
     std::vector<uint32_t> moves;
-    more_changes(p, need);
+    if (pf_status st = more_changes(p, need)) return st;
     moves.reserve(3 * copies);
     for (uint32_t i = 0; i < n; i++) more_pages(p, seqs[i], pages_for(p, p->len[seqs[i]] + rows[i]));
     p->pass.clear();
@@ -717,7 +722,8 @@ static pf_status pages_fork(pf_pages* p, uint32_t src, const uint32_t* dst, uint
     if (src >= p->cfg.max_seqs) return fail(p->ctx, PF_ERR_ARG, "pages: sequence out of range");
     if (pf_status st = all_empty(p, dst, n)) return st;
     if (!n || !p->len[src]) return PF_OK;
-    more_changes(p, (size_t)n * p->pages[src].size());
+    DeviceScope on(p->ctx);
+    if (pf_status st = more_changes(p, (size_t)n * p->pages[src].size())) return st;
     for (uint32_t i = 0; i < n; i++) more_pages(p, dst[i], p->pages[src].size());
     end_pass(p);
     for (uint32_t i = 0; i < n; i++) {
@@ -746,7 +752,7 @@ static pf_status pages_copy(pf_pages* p, const uint32_t* src, const uint32_t* ds
     if (need > p->heap.size()) return fail(p->ctx, PF_ERR_CAPACITY, "pages: too few free pages");
     DeviceScope on(p->ctx);
     std::vector<uint32_t> moves;
-    more_changes(p, need);
+    if (pf_status st = more_changes(p, need)) return st;
     moves.reserve(3 * need);
     for (uint32_t i = 0; i < n; i++) more_pages(p, dst[i], p->pages[src[i]].size());
     end_pass(p);
@@ -808,8 +814,8 @@ static pf_status pages_compact(pf_pages* p, uint32_t* moved) {
     size_t named = 0;
     for (const std::vector<uint32_t>& t : p->pages)
         for (uint32_t page : t) named += page >= used;
-    more_changes(p, named);
     DeviceScope on(p->ctx);
+    if (pf_status st = more_changes(p, named)) return st;
     end_pass(p);
     if (moves.empty()) return PF_OK;
     for (uint32_t s = 0; s < p->cfg.max_seqs; s++)

@@ -20,6 +20,7 @@ namespace pf {
 constexpr int PR_SEQS = 64;       // sequences of one launch
 constexpr int PR_KEYS = 64;       // keys of a tile
 constexpr uint32_t PR_CUS = 256;  // compute units
+constexpr uint64_t PR_MOST_UNITS = (1u << 24) - 64;   // workgroups of a launch
 
 struct PromptArgs {
     const void *q, *k, *v;
@@ -64,11 +65,11 @@ __device__ __forceinline__ PromptUnit prompt_unit(uint32_t u, uint32_t tiles, ui
 }
 
 // A workgroup: 4 waves of one head, each with 32 query rows; SPLIT 2: two and
-// two waves share 32 rows, and each takes half of every key tile.  Scores are formed as
-// S^T = K Q^T, so that a lane holds 16 keys of one row: its maximum and sum
-// need one exchange between two lanes, and exp(S)^T is already the operand
-// of O^T = V^T P^T, whose other operand comes from V's rows in LDS through
-// transposing reads.
+// two waves share 32 rows, and each takes half of every key tile.  Scores are
+// formed as S^T = K Q^T, so that a lane holds 16 keys of one row: its maximum
+// and sum need one exchange between two lanes, and exp(S)^T is already the
+// operand of O^T = V^T P^T, whose other operand comes from V's rows in LDS
+// through transposing reads.
 
 // What a workgroup knows of its tile of 128 / SPLIT query rows.
 template <int SPLIT>
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptA
     if (!prompt_tile(a, &T)) return;
     const int nk = T.nk, my = T.r0 + wave % (4 / SPLIT) * 32 + row, p = T.off + my;
     const int part = SPLIT == 2 ? wave / 2 * 32 : 0;   // first key of a tile that this wave takes
-    const int hi = a.causal ? p : nk - 1, lo = a.window ? p - a.window + 1 : 0;
+    const int hi = a.causal ? p : nk - 1, lo = a.window ? max(0, p - a.window + 1) : 0;
 
     s8v qf[NP][C];                               // Q^T: 16 dims of a row per matrix instruction
     {
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     if (!prompt_tile(a, &T)) return;
     const int nk = T.nk, my = T.r0 + wave % (4 / SPLIT) * 32 + row, p = T.off + my;
     const int part = SPLIT == 2 ? wave / 2 * 32 : 0;   // first key of a tile that this wave takes
-    const int hi = a.causal ? p : nk - 1, lo = a.window ? p - a.window + 1 : 0;
+    const int hi = a.causal ? p : nk - 1, lo = a.window ? max(0, p - a.window + 1) : 0;
 
     s8v qf[C];
     {
@@ -699,6 +700,8 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
         nk += k_lens[i];
     }
     if (!nq) return PF_OK;
+    // (a grid has fewer than 2^32 threads)
+    if ((nq / 64 + n_seq) * d->n_heads > PR_MOST_UNITS) return fail(c, PF_ERR_UNSUPPORTED, "attention: too many rows at once");
     if (nq > 0x7FFFFFFFu || nk > 0x7FFFFFFFu) return fail(c, PF_ERR_UNSUPPORTED, "attention: over 2^31 rows in all");
     if (!q || !out || (nk && (!k || !v))) return fail(c, PF_ERR_ARG, "attention: a buffer is NULL");
     if (!aligned16(q) || !aligned16(out) || !aligned16(k) || !aligned16(v))

@@ -1,0 +1,99 @@
+"""What the attention and paged-cache entry points answer without a GPU: NULL
+handles, the Python binding's argument checks, and the tests' own float64
+attention against a direct sum."""
+import numpy as np
+import pytest
+
+import attention_ref as R
+import pocketforge_amd as pf
+
+
+def test_null_handles():
+    L = pf.lib()
+    assert L.pf_prompt_attention(None, None, None, None, None, None, None, None, 0) == -1
+    assert L.pf_pages_create(None, None, None) == -1
+    L.pf_pages_destroy(None)
+    assert L.pf_pages_memory_usage(None) == 0 and L.pf_pages_free_count(None) == 0 and L.pf_pages_length(None, 0) == 0
+    assert L.pf_pages_tables(None, None, 0, None, 0, None) == -1
+    assert L.pf_pages_planes(None, None, None, None, None) == -1
+    assert L.pf_pages_append(None, None, None, 0) == -1
+    assert L.pf_pages_store(None, 0, pf.TYPE_F32, None, None, 0, 0) == -1
+    assert L.pf_pages_attention(None, None, 0, None, None) == -1
+    assert L.pf_pages_gather(None, 0, None, 0, pf.TYPE_F32, None, None, 0, 0) == -1
+    assert L.pf_pages_fork(None, 0, None, 0) == -1 and L.pf_pages_copy(None, None, None, 0) == -1
+    assert L.pf_pages_truncate(None, None, None, 0) == -1 and L.pf_pages_free(None, None, 0) == -1
+    assert L.pf_pages_compact(None, None) == -1
+
+
+def test_lists():
+    for a in ([], [1, 2], (3,), range(4), np.arange(3), np.arange(3, dtype=np.uint32), [np.int64(7)]):
+        assert list(pf._u32(a, "a")) == [int(x) for x in a]
+    for a in ([-1], [1.5], [1 << 32], "ab", 5, None, np.array([0.5]), [[1]]):
+        with pytest.raises(pf.PFError):
+            pf._u32(a, "a")
+
+
+class Rows:
+    """What the binding looks at in a device array."""
+
+    def __init__(self, shape, stride, dtype):
+        self.shape, self._stride, self.dtype = shape, stride, dtype
+
+    def stride(self):
+        return self._stride
+
+
+def test_rows():
+    assert pf._rows(Rows((5, 4, 64), (256, 64, 1), "torch.float16"), "q") == (5, 4, 64, 256)
+    assert pf._rows(Rows((5, 4, 64), (768, 64, 1), "torch.float16"), "q") == (5, 4, 64, 768)
+    assert pf._rows(Rows((1, 4, 64), (1, 64, 1), "torch.float16"), "q") == (1, 4, 64, 256)
+    for shape, stride in (((5, 256), (256, 1)), ((5, 4, 64), (256, 1, 4)), ((5, 4, 64), (64, 320, 1))):
+        with pytest.raises(pf.PFError):
+            pf._rows(Rows(shape, stride, "torch.float16"), "q")
+
+
+def test_types():
+    for name, t in (("float32", pf.TYPE_F32), ("float16", pf.TYPE_F16), ("torch.bfloat16", pf.TYPE_BF16),
+                    (np.dtype(np.uint16), pf.TYPE_BF16)):
+        assert pf._type(Rows((), (), name)) == t
+    with pytest.raises(pf.PFError):
+        pf._type(Rows((), (), "torch.int8"))
+
+
+@pytest.mark.parametrize("causal,window,sink", [(True, 0, 0), (False, 0, 0), (True, 3, 1), (False, 2, 0), (True, 1, 9)])
+def test_reference_attention(causal, window, sink):
+    rng = np.random.default_rng(1)
+    nq, nk, H, G, D = 5, 9, 4, 2, 8
+    q, k, v = (rng.standard_normal(s) for s in ((nq, H, D), (nk, G, D), (nk, G, D)))
+    got, tol = R.attend(q, k, v, R.visible(nq, nk, causal, window, sink), 0.3, "f32")
+    for i in range(nq):
+        p = nk - nq + i
+        for h in range(H):
+            num, den = np.zeros(D), 0.0
+            for j in range(nk):
+                if causal and j > p:
+                    continue
+                if window and not (j > p - window or j < sink):
+                    continue
+                w = np.exp(0.3 * float(q[i, h] @ k[j, h // 2]))
+                num += w * v[j, h // 2]
+                den += w
+            np.testing.assert_allclose(got[i, h], num / den, rtol=1e-12, atol=1e-14)
+    assert (tol > 0).all() and (tol < 1e-4).all()
+
+
+def test_reference_empty_rows_and_masked_nan():
+    rng = np.random.default_rng(2)
+    q, k, v = rng.standard_normal((4, 1, 8)), rng.standard_normal((2, 1, 8)), rng.standard_normal((2, 1, 8))
+    v[1] = np.nan
+    got, _ = R.attend(q, k, v, R.visible(4, 2), 1.0, "f32")
+    assert (got[:2] == 0).all() and np.isfinite(got[2]).all() and np.isnan(got[3]).all()
+
+
+def test_reference_types():
+    x = np.array([1.0, 1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8, -0.0, np.inf, np.nan, 3e38], np.float32)
+    b = R.from_bits(R.to_bits(x, "bf16"), "bf16")
+    assert b[0] == 1 and b[1] == 1 and b[2] == 1 + 2.0 ** -6 and b[4] == np.inf and np.isnan(b[5])
+    c, s = R.quantize_rows(np.array([[0.0, 0.0], [1.0, -2.0], [np.inf, 1.0]], np.float32))
+    assert c.tolist() == [[0, 0], [64, -127], [0, 0]] and s[0, 0] == 1 and s[1, 0] == np.float32(2) / np.float32(127)
+    assert np.isnan(s[2, 0])

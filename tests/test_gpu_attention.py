@@ -582,3 +582,74 @@ def test_two_caches_and_a_second_pass_between(gpu):
         b.attention(4, [1, 0], [1, 1])
     a.c.close()
     b.c.close()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("size", [3e-4, 1.2e4])
+def test_paged_int8_value_range(gpu, t, size):
+    """Values far from one, in int8 pages: their row scales are outside what fp16 weights hold."""
+    m = Mirror(gpu, "i8", 2, 64, 32, 20, 1, 600, t=t)
+    k = R.rand(m.rng, (500, 2, 64), t)
+    v = R.to_bits((m.rng.standard_normal((500, 2, 64)) * size).astype(np.float32), t)
+    m.append([0], [500], (k, v))
+    m.append([0], [2], (k[:2], v[:2]))
+    m.attention(4, [0], [2])
+    m.c.close()
+
+
+def test_prompt_window_before_the_first_key(gpu):
+    """Queries before the first key with a window: causal, they see nothing; else every key and the sinks."""
+    for causal in (True, False):
+        prompt_case(gpu, "bf16", 2, 2, 64, [40, 130, 7], [10, 20, 0], causal, 5, 2)
+
+
+def test_prompt_too_many_rows(gpu):
+    b = gpu.empty((64, 64, 64), np.float16)
+    d = pf.AttnDesc(pf.TYPE_F16, 64, 64, 64, 1, 0, 0, 0.0, 0, 0, 0, 0)
+    lens = (C.c_uint32 * 1)(1 << 30)
+    p = C.c_void_p(b.ptr)
+    assert pf.lib().pf_prompt_attention(gpu.h, C.byref(d), p, p, p, p, lens, None, 1) == -4
+
+
+def test_many_forks_without_a_pass(gpu):
+    """Table changes that no pass sends go to the device when there are many."""
+    m = Mirror(gpu, "bf16", 1, 16, 16, 2010, 12, 32000)
+    m.append([0], [31999])
+    for _ in range(6):
+        m.c.fork(0, list(range(1, 12)))
+        m.c.free(list(range(2, 12)))
+        m.c.copy([], [])
+        m.c.free([1])
+    m.c.fork(0, [5])
+    m.rows[5] = list(m.rows[0])
+    m.check([5])
+    m.append([5], [1])
+    m.check([0, 5])
+    m.attention(2, [5], [1])
+    m.c.close()
+
+
+def test_copies_in_one_call(gpu):
+    """More copies on write than go with a step's message, and a step of more sequences than fit one message."""
+    n = 200
+    m = Mirror(gpu, "i8", 2, 32, 16, 900, n + 1, 64)
+    m.append([0], [23])
+    m.c.fork(0, list(range(1, n + 1)))
+    for s in range(1, n + 1):
+        m.rows[s] = list(m.rows[0])
+    m.append(list(range(n, 0, -1)), [1 + s % 3 for s in range(n)])
+    m.check(range(n + 1))
+    m.attention(2, list(range(n, 0, -1)), [1 + s % 3 for s in range(n)])
+    m.c.free(list(range(1, n, 2)))
+    for s in range(1, n, 2):
+        m.rows[s] = [tuple(x[:0] for x in kv) for kv in m.rows[s]]
+    m.c.copy([0] * 100, list(range(1, n, 2)))
+    for s in range(1, n, 2):
+        m.rows[s] = list(m.rows[0])
+    m.check(range(n + 1))
+    m.c.free(list(range(2, n + 1, 2)))
+    for s in range(2, n + 1, 2):
+        m.rows[s] = [tuple(x[:0] for x in kv) for kv in m.rows[s]]
+    m.c.compact()
+    m.check(range(n + 1))
+    m.c.close()
