@@ -10,6 +10,7 @@
 #include "pf_attend.h"
 #include "pf_context.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -22,6 +23,9 @@ constexpr int PR_KEYS = 64;       // keys of a tile
 constexpr uint32_t PR_CUS = 256;  // compute units
 constexpr uint64_t PR_MOST_UNITS = (1u << 24) - 64;   // workgroups of a launch
 
+struct PromptSeq {
+    uint32_t q0, nq, k0, nk;      // first rows and lengths
+};
 struct PromptArgs {
     const void *q, *k, *v;
     void* out;
@@ -31,7 +35,7 @@ struct PromptArgs {
     float scale_log2;
     uint32_t tiles;               // query tiles of all sequences
     uint32_t tile0[PR_SEQS];      // first query tile of each sequence
-    struct { uint32_t q0, nq, k0, nk; } seq[PR_SEQS];   // first rows and lengths
+    PromptSeq seq[PR_SEQS];
 };
 
 // The workgroups of a launch.  Workgroup u runs on XCD u mod 8, each with an L2
@@ -728,16 +732,22 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
     const uint32_t full = PR_CUS * (d->type == PF_TYPE_F32 && d->head_dim > 64 ? 1 : 2), rows = units < full ? 64 : 128;
     uint32_t qa = 0, ka = 0;
     for (uint32_t b = 0; b < n_seq;) {
-        uint32_t tiles = 0;
         a.n_seq = 0;
         for (; b < n_seq && a.n_seq < PR_SEQS; b++) {
-            if (q_lens[b]) {
-                a.tile0[a.n_seq] = tiles;
-                a.seq[a.n_seq++] = {qa, q_lens[b], ka, k_lens[b]};
-                tiles += (q_lens[b] + rows - 1) / rows;
-            }
+            if (q_lens[b]) a.seq[a.n_seq++] = {qa, q_lens[b], ka, k_lens[b]};
             qa += q_lens[b];
             ka += k_lens[b];
+        }
+        // Tiles are taken from the last: the sequences with the most keys go first, so
+        // that short ones fill the end (10 prompts of up to 1000 fp32 rows, 12 heads of
+        // 64: 79 us in the order given, 66 so).  All sequences' last tiles first, then
+        // the ones before, balances more (62) but parts the tiles that share keys in
+        // L2 (64 prompts of up to 2000 bf16 rows, 16 heads of 128: 660 -> 710)
+        std::sort(a.seq, a.seq + a.n_seq, [](const PromptSeq& x, const PromptSeq& y) { return x.nk < y.nk; });
+        uint32_t tiles = 0;
+        for (uint32_t i = 0; i < a.n_seq; i++) {
+            a.tile0[i] = tiles;
+            tiles += (a.seq[i].nq + rows - 1) / rows;
         }
         if (!tiles) continue;
         a.tiles = tiles;
