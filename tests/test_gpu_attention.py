@@ -603,6 +603,12 @@ def test_prompt_window_before_the_first_key(gpu):
         prompt_case(gpu, "bf16", 2, 2, 64, [40, 130, 7], [10, 20, 0], causal, 5, 2)
 
 
+@pytest.mark.parametrize("H,G", [(40, 40), (48, 24), (80, 40), (32, 8), (12, 6)])
+def test_prompt_many_heads(gpu, H, G):
+    """Each head's tiles are taken once, whatever the order that the heads and the sequences go in."""
+    prompt_case(gpu, "bf16", H, G, 32, [33, 300, 1, 130], [40, 300, 400, 135])
+
+
 def test_prompt_too_many_rows(gpu):
     b = gpu.empty((64, 64, 64), np.float16)
     d = pf.AttnDesc(pf.TYPE_F16, 64, 64, 64, 1, 0, 0, 0.0, 0, 0, 0, 0)
