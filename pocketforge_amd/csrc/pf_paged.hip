@@ -406,7 +406,8 @@ static void paged_one(hipStream_t st, const PageSplit& u, uint32_t z, const Page
 template <int ACT, int CT, int DP, bool EXACT>
 static void paged_rows(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
     const uint32_t R = u.most_rows * a.group;
-    // one tile of 16 rows, or two: the keys are read once for both
+    // one tile of 16 rows, or two: the keys are read once for both (64 contexts of
+    // up to 4000 bf16 keys, 20 rows a kv head: 71 us, 128 as two single tiles)
     if (R <= 16) paged_one<ACT, CT, DP, 1, EXACT>(st, u, 1, a);
     else paged_one<ACT, CT, DP, 2, EXACT>(st, u, (R + 31) / 32, a);
 }
@@ -420,13 +421,19 @@ static void paged_dim(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
 }
 
 // Cuts the pass's keys into shares of at most `chunk` tiles, by what they would
-// take: the rounds of workgroups (`per` for each share), each as long as its
-// longest wave's run of tiles and about a tile's time more, and the second
-// kernel, about two tiles', where a sequence is cut.  Looked at: no cut, and the
-// smallest shares that one round of workgroups holds, or two for each sequence
-// (a long one beside short ones), but of a tile for each wave; with workgroups
-// of 4 waves, and of 8 (half as many shares, to join as well).
-constexpr uint32_t PG_CUS = 256, PG_JOIN = 2;
+// take, in half tiles' times: the rounds of workgroups (`per` for each share),
+// each as long as its longest wave's run of tiles and a tile's time more (two
+// with 8 waves, whose results meet in LDS: two bf16 contexts of 221 keys, 12
+// heads, 8.0 us with 8 and 6.8 with 4), and where a sequence is cut the second
+// kernel, PG_JOIN and one for each PG_JOIN_ROWS rows and heads (48 contexts of
+// up to 3000 bf16 keys, 32 heads of 64, five rows: 59 us cut, 31 uncut).  Looked
+// at: no cut, and the smallest shares that one round of workgroups holds, or two
+// for each sequence (a long one beside short ones), but of a tile for each wave;
+// with workgroups of 4 waves, and of 8 (half as many shares, to join as well: 16
+// verify passes of five fp32 rows over 2100 int8 keys of 16 heads, 25 us uncut
+// with 8, 29 cut with 4; one bf16 row over 700 keys, 11.8 and 10.0).  Two
+// contexts of 60000 fp16 keys take 25 us cut, 509 uncut.
+constexpr uint32_t PG_CUS = 256, PG_JOIN = 5, PG_JOIN_ROWS = 512;
 struct PageShares {
     uint32_t chunk = 1, waves = 4;
     uint64_t cost = ~0ull;
@@ -437,10 +444,10 @@ static uint64_t page_shares_of(const std::vector<uint32_t>& tiles, uint32_t chun
     return n;
 }
 static void page_shares(const std::vector<uint32_t>& tiles, uint32_t longest, uint64_t per, uint64_t round, uint32_t waves,
-                        PageShares* best) {
+                        uint64_t join, PageShares* best) {
     const auto take = [&](uint32_t chunk) {
         const uint64_t rounds = (page_shares_of(tiles, chunk) * per + round - 1) / round;
-        const uint64_t cost = rounds * ((chunk + waves - 1) / waves + 1) + (chunk < longest ? PG_JOIN : 0);
+        const uint64_t cost = 2 * rounds * ((chunk + waves - 1) / waves + waves / 4) + (chunk < longest ? join : 0);
         if (cost < best->cost) *best = {chunk, waves, cost};
     };
     const uint32_t least = std::max<uint32_t>(waves, (longest + PG_MOST_PARTS - 1) / PG_MOST_PARTS);
@@ -472,8 +479,9 @@ static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& 
     const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
     if (R > 32 * 65535u) return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
     PageShares best;
-    page_shares(tiles, longest, per, (uint64_t)PG_CUS * held, 4, &best);
-    if (held > 1) page_shares(tiles, longest, per, (uint64_t)PG_CUS * (held / 2), 8, &best);
+    const uint64_t join = PG_JOIN + (uint64_t)p->pass_rows * d->n_heads / PG_JOIN_ROWS;
+    page_shares(tiles, longest, per, (uint64_t)PG_CUS * held, 4, join, &best);
+    if (held > 1) page_shares(tiles, longest, per, (uint64_t)PG_CUS * (held / 2), 8, join, &best);
     const uint32_t chunk = best.chunk;
     PageSplit n;
     n.waves = best.waves;
