@@ -203,10 +203,10 @@ typedef struct {
  * sees no key gets zeros.  Lengths are host arrays and may be 0; q_lens may
  * exceed k_lens.  Buffers and strides are multiples of 16 bytes; out may not
  * overlap the inputs.  Sums are fp32 whatever the type; fp32 rows (values
- * below 3.38e38) are multiplied to fp32 accuracy.  An infinity or a NaN in k or v reaches the
- * queries that see it and no others (fp32 rows: as a NaN).  Asynchronous on
- * the context's stream: what other streams write or read is the caller's to
- * order (pf_synchronize); allocates nothing. */
+ * below 3.38e38) are multiplied to fp32 accuracy.  An infinity or a NaN in k
+ * or v reaches the queries that see it and no others (fp32 rows: as a NaN).
+ * Asynchronous on the context's stream: what other streams write or read is
+ * the caller's to order (pf_synchronize); allocates nothing. */
 pf_status pf_prompt_attention(pf_ctx* ctx, const pf_attn_desc* desc, const void* q_dev, const void* k_dev,
                               const void* v_dev, void* out_dev, const uint32_t* q_lens, const uint32_t* k_lens,
                               uint32_t n_seq);
@@ -219,9 +219,10 @@ pf_status pf_prompt_attention(pf_ctx* ctx, const pf_attn_desc* desc, const void*
  * until one of them grows into a shared one, which it then copies.  A page
  * holds the rows of every layer and kv head.  Pages are handed out lowest
  * number first.  Page tables live on the device and follow the calls in
- * stream order; no call synchronizes, and only create, destroy and
- * pf_pages_attention's first call of a larger size (the context's scratch)
- * allocate.  Every call checks its arguments before it changes anything. */
+ * stream order; no call waits for the device, but for room in its queue of
+ * 32 large messages, and only create, destroy and pf_pages_attention's first
+ * call of a larger size (the context's scratch) allocate there.  Every call
+ * checks its arguments before it changes anything. */
 typedef struct pf_pages pf_pages;
 typedef struct {
     int32_t type;              /* PF_TYPE_F16, BF16 or I8 */
@@ -247,7 +248,8 @@ pf_status pf_pages_tables(const pf_pages* p, const uint32_t* seqs, uint32_t n, i
 pf_status pf_pages_planes(const pf_pages* p, void** k_dev, void** v_dev, float** ks_dev, float** vs_dev);
 /* Begins a pass: sequence seqs[i] (distinct) grows by rows[i] rows (0 is
  * allowed).  pf_pages_store and pf_pages_attention then work on these rows,
- * packed in this order, until the next append; the calls below end the pass.
+ * packed in this order, until the next append; fork, copy, truncate, free
+ * and compact end the pass.
  * PF_ERR_CAPACITY, with nothing changed, if a sequence would exceed
  * max_context or the pool has too few free pages. */
 pf_status pf_pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t* rows, uint32_t n);
