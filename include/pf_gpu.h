@@ -206,7 +206,9 @@ typedef struct {
  * below 3.38e38) are multiplied to fp32 accuracy.  An infinity or a NaN in k
  * or v reaches the queries that see it and no others (fp32 rows: as a NaN).
  * Asynchronous on the context's stream: what other streams write or read is
- * the caller's to order (pf_synchronize); allocates nothing. */
+ * the caller's to order (pf_synchronize).  Few queries over many keys take
+ * workgroups for parts of the keys; only a call that needs more room for
+ * their results than the context's scratch has allocates. */
 pf_status pf_prompt_attention(pf_ctx* ctx, const pf_attn_desc* desc, const void* q_dev, const void* k_dev,
                               const void* v_dev, void* out_dev, const uint32_t* q_lens, const uint32_t* k_lens,
                               uint32_t n_seq);

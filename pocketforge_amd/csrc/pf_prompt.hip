@@ -35,6 +35,9 @@ struct PromptArgs {
     int32_t causal, window, sink;
     float scale_log2;
     uint32_t tiles;               // query tiles of all sequences
+    uint32_t parts, rows;         // parts that the keys are cut in (grid y), rows of a part's results
+    float* ws_o;                  // parts > 1: [parts][rows][n_heads][dim]
+    float* ws_ml;                 // [parts][rows][n_heads][2]
     uint32_t tile0[PR_SEQS];      // first query tile of each sequence
     PromptSeq seq[PR_SEQS];
 };
@@ -86,11 +89,13 @@ struct PromptTile {
     uint32_t q0, k0, head;
     int nq, nk, r0, off;          // lengths, first row, position of row 0
     int p0, p1;                   // positions of the first and the last row
-    int first, sinks, tiles, wa, wb, whole;
+    int first, sinks, wa, wb, whole;
+    int at, tiles, n_whole;       // this part's: first key tile in that order, tiles, whole ones (they are first)
 
     // The key tiles that some row sees, in the order they are taken: those that
     // all rows see whole (wa .. wb - 1), then the sinks' and the rest from `first`.
     __device__ __forceinline__ int key_tile(int it) const {
+        it += at;
         if (it < whole) return wa + it;
         it -= whole;
         if (it < sinks) return it;
@@ -120,10 +125,17 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs& a, PromptTile<SPLI
     const int end = min(t->nk, a.causal ? t->p1 + 1 : t->nk), last = end <= 0 ? 0 : (end + PR_KEYS - 1) / PR_KEYS;
     t->first = (a.window ? max(0, t->p0 - a.window + 1) : 0) / PR_KEYS;
     t->sinks = min(min((a.sink + PR_KEYS - 1) / PR_KEYS, t->first), last);
-    t->tiles = max(0, last - t->first) + t->sinks;
+    const int tiles = max(0, last - t->first) + t->sinks;
     t->wa = a.window ? max(t->first, (max(0, t->p1 - a.window + 1) + PR_KEYS - 1) / PR_KEYS) : 0;
     t->wb = max(t->wa, min(t->nk, a.causal ? max(0, t->p0 + 1) : t->nk) / PR_KEYS);
-    t->whole = t->tiles ? t->wb - t->wa : 0;
+    t->whole = tiles ? t->wb - t->wa : 0;
+    t->at = 0;
+    t->tiles = tiles;
+    if (SPLIT == 2) {
+        t->at = (int)((uint32_t)tiles * blockIdx.y / a.parts);
+        t->tiles = (int)((uint32_t)tiles * (blockIdx.y + 1) / a.parts) - t->at;
+    }
+    t->n_whole = min(max(0, t->whole - t->at), t->tiles);
     return true;
 }
 
@@ -188,6 +200,7 @@ __device__ __forceinline__ void join_halves(int wave, float& m, float& l, f16v (
     if (wave >= 2) return;
     const f4v x = *ml;
     const float to = fmaxf(m, x[0]), ms = to == -INFINITY ? 0.0f : to, f0 = exp2_fast(m - ms), f1 = exp2_fast(x[0] - ms);
+    m = to;
     l = l * f0 + x[1] * f1;
 #pragma unroll
     for (int n = 0; n < DT; n++) {
@@ -207,6 +220,69 @@ template <int ROWS>
 __device__ __forceinline__ float row_factor(const PromptArgs& a, const PromptTile<ROWS>& t, int my, float l, bool* none) {
     *none = !(a.causal ? t.off + my >= 0 : t.nk > 0);
     return *none ? 0.0f : 1.0f / l;
+}
+
+// SPLIT 2: a part's results, where the keys are cut.
+template <bool EXACT, int DT>
+__device__ __forceinline__ void store_part(const PromptArgs& a, const PromptTile<2>& t, int my, int half, float m, float l,
+                                           const f16v (&o)[DT]) {
+    if (my >= t.nq) return;
+    bool none;
+    row_factor(a, t, my, l, &none);
+    const size_t w = ((size_t)blockIdx.y * a.rows + t.q0 + (uint32_t)my) * a.n_heads + t.head;
+    float* op = a.ws_o + w * a.dim;
+#pragma unroll
+    for (int n = 0; n < DT; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = n * 32 + 8 * (i / 4) + 4 * half;
+            if (!EXACT && d >= (int)a.dim) continue;
+            const f4v x = {o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]};
+            *(f4v*)(op + d) = none ? (f4v)0.0f : x;
+        }
+    if (half == 0) {                             // (a row that sees no key: zeros of weight 1)
+        a.ws_ml[2 * w] = none ? 0.0f : m;
+        a.ws_ml[2 * w + 1] = none ? 1.0f : l;
+    }
+}
+
+// Joins the parts (up to 32): 32 threads take a row of a head, 4 dims each.
+// Bound by a launch's latency and the parts' bytes.
+constexpr uint32_t PR_MOST_PARTS = 32;
+template <int ACT>
+__global__ __launch_bounds__(256) void k_prompt_join(PromptArgs a) {
+    const uint32_t lane = threadIdx.x & 31, unit = blockIdx.x * 8 + (threadIdx.x >> 5), d = lane * 4;
+    const size_t step = (size_t)a.rows * a.n_heads;
+    if (unit >= step) return;
+    float m = -INFINITY, l = 0.0f;
+    if (lane < a.parts) {
+        m = a.ws_ml[2 * (unit + lane * step)];
+        l = a.ws_ml[2 * (unit + lane * step) + 1];
+    }
+    float top = m;
+#pragma unroll
+    for (int b = 1; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor(top, b));
+    const float f = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
+    l *= f;
+#pragma unroll
+    for (int b = 1; b < 32; b <<= 1) l += __shfl_xor(l, b);
+    f4v acc = (f4v)0.0f;
+    const float* op = a.ws_o + (size_t)unit * a.dim + d;
+#pragma unroll 4
+    for (uint32_t p = 0; p < a.parts; p++) {
+        const float fp = __shfl(f, (int)p, 32);
+        if (d < a.dim) {
+            const f4v x = *(const f4v*)(op + p * step * a.dim);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] += fp * x[i];
+        }
+    }
+    if (d >= a.dim) return;
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = acc[i] / l;
+    const uint32_t row = unit / a.n_heads, h = unit % a.n_heads;
+    store4<ACT>((uint8_t*)a.out + ((size_t)row * a.os + (size_t)h * a.dim + d) * act_size<ACT>, y);
 }
 
 // fp32 rows, three bf16 pieces each: six matrix instructions where 16-bit rows
@@ -369,13 +445,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptA
     if (tid == 0) s_odd = -1;
     if (T.tiles) load(0);
     int it = 0;
-    for (; it < T.whole; it++) body(std::false_type{}, it);
+    for (; it < T.n_whole; it++) body(std::false_type{}, it);
     for (; it < T.tiles; it++) body(std::true_type{}, it);
     if constexpr (SPLIT == 2) {
         uint8_t* x = (uint8_t*)&sv[0][0][0];
         static_assert(DT * 8192 + 2048 <= sizeof(sv), "the halves' exchange fits V's tile");
         join_halves(wave, m, l, o, x, x + DT / 2 * 8192, x + DT * 8192);
         if (wave >= 2) return;
+        if (a.parts > 1) return store_part<EXACT>(a, T, my, half, m, l, o);
     } else {
         l = sum32(l);
     }
@@ -606,7 +683,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     if (tid == 0) s_odd = -1;
     if (T.tiles) load(no, 0);
     int it = 0;
-    for (; it + 1 < T.whole; it += 2) {
+    for (; it + 1 < T.n_whole; it += 2) {
         turn();
         load(yes, it + 1);
         body(no, no, 0);
@@ -632,6 +709,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         static_assert(DT / 2 * 8192 <= sizeof(sk0) && 2048 <= sizeof(sv1), "the halves' exchange fits the tiles");
         join_halves(wave, m, l, o, sk0, sk1, sv1);
         if (wave >= 2) return;
+        if (a.parts > 1) return store_part<EXACT>(a, T, my, half, m, l, o);
     } else {
         l = sum32(l);
         __syncthreads();                         // nobody reads V any more
@@ -692,9 +770,9 @@ template <int ACT, int DP, bool EXACT, int SPLIT>
 static void prompt_one(hipStream_t st, const PromptArgs& a) {
     const uint32_t units = prompt_units(a.tiles, a.n_heads / a.group, a.group);
     if constexpr (ACT == PF_TYPE_F32)
-        hipLaunchKernelGGL((k_prompt_attn32<DP, EXACT, SPLIT>), dim3(units), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_prompt_attn32<DP, EXACT, SPLIT>), dim3(units, a.parts), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((k_prompt_attn16<ACT, DP, EXACT, SPLIT>), dim3(units), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_prompt_attn16<ACT, DP, EXACT, SPLIT>), dim3(units, a.parts), dim3(256), 0, st, a);
 }
 
 template <int ACT, int DP, bool EXACT>
@@ -709,6 +787,30 @@ static void prompt_dim(hipStream_t st, uint32_t rows, const PromptArgs& a) {
     else if (a.dim == 64) prompt_rows<ACT, 64, true>(st, rows, a);
     else if (a.dim < 64) prompt_rows<ACT, 64, false>(st, rows, a);
     else prompt_rows<ACT, 128, false>(st, rows, a);
+}
+
+// The parts that the keys are cut in, where 64-row workgroups are few and some
+// see many key tiles: as many as fill the compute units with at least four
+// tiles each (two of fp32 rows), where the longest workgroup's tiles are fewer
+// then, with the join: six tiles' time (two) and what its rows add.  64 bf16
+// rows after 2000 cached, 16 heads of 128 over 4: 34 us whole, 18.5 cut; 8000
+// rows of one head of 64: 70 and 32; 1000 of 16 heads: 20.4, and 27.9 cut in
+// two; 1000 fp32 rows of 12 heads of 64: 18.5 and 16.3.
+static uint32_t prompt_parts(const pf_attn_desc* d, const AttnShape& s, const uint32_t* q_lens, const uint32_t* k_lens,
+                             uint32_t n_seq, uint32_t full) {
+    uint64_t units = 0, keys = 0;
+    for (uint32_t i = 0; i < n_seq; i++) {
+        if (!q_lens[i]) continue;
+        units += (uint64_t)((q_lens[i] + 63) / 64) * d->n_heads;
+        uint64_t seen = k_lens[i];
+        if (s.window) seen = std::min<uint64_t>(seen, (uint64_t)s.window + std::min(q_lens[i], 64u) + s.sink);
+        keys = std::max(keys, seen);
+    }
+    const uint64_t tiles = (keys + PR_KEYS - 1) / PR_KEYS;
+    const bool wide = d->type == PF_TYPE_F32;
+    const uint64_t parts = std::min<uint64_t>({full / units, tiles / (wide ? 2 : 4), PR_MOST_PARTS});
+    if (parts < 2 || (tiles + parts - 1) / parts + (wide ? 2 : 6) + parts * units / 128 >= tiles) return 1;
+    return (uint32_t)parts;
 }
 
 extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const void* q, const void* k, const void* v,
@@ -750,6 +852,16 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
     uint64_t units = 0;
     for (uint32_t i = 0; i < n_seq; i++) units += (uint64_t)((q_lens[i] + 127) / 128) * d->n_heads;
     const uint32_t full = PR_CUS * (d->type == PF_TYPE_F32 && d->head_dim > 64 ? 1 : 2), rows = units < full ? 64 : 128;
+    a.parts = 1;
+    a.rows = (uint32_t)nq;
+    if (rows == 64) a.parts = prompt_parts(d, s, q_lens, k_lens, n_seq, full);
+    if (a.parts > 1) {
+        const size_t n = (size_t)a.parts * a.rows * a.n_heads;
+        void* ws = nullptr;
+        if (pf_status st = ctx_scratch(c, n * (a.dim + 2) * 4, &ws)) return st;
+        a.ws_o = (float*)ws;
+        a.ws_ml = a.ws_o + n * a.dim;
+    }
     uint32_t qa = 0, ka = 0;
     for (uint32_t b = 0; b < n_seq;) {
         a.n_seq = 0;
@@ -776,6 +888,13 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
             case PF_TYPE_F16: prompt_dim<PF_TYPE_F16>(c->stream, rows, a); break;
             default: prompt_dim<PF_TYPE_BF16>(c->stream, rows, a); break;
         }
+        PF_LAUNCHED(c);
+    }
+    if (a.parts > 1) {
+        const dim3 grid((uint32_t)((nq * a.n_heads + 7) / 8));
+        if (d->type == PF_TYPE_F32) hipLaunchKernelGGL(k_prompt_join<PF_TYPE_F32>, grid, dim3(256), 0, c->stream, a);
+        else if (d->type == PF_TYPE_F16) hipLaunchKernelGGL(k_prompt_join<PF_TYPE_F16>, grid, dim3(256), 0, c->stream, a);
+        else hipLaunchKernelGGL(k_prompt_join<PF_TYPE_BF16>, grid, dim3(256), 0, c->stream, a);
         PF_LAUNCHED(c);
     }
     return PF_OK;

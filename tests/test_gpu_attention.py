@@ -609,6 +609,45 @@ def test_prompt_many_heads(gpu, H, G):
     prompt_case(gpu, "bf16", H, G, 32, [33, 300, 1, 130], [40, 300, 400, 135])
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("H,G,D,ql,kl,causal,window,sink", [
+    (4, 4, 128, [1], [2049], True, 0, 0), (4, 2, 64, [5, 64, 130], [2000, 700, 131], True, 0, 0),
+    (3, 1, 48, [70], [1500], False, 0, 0), (2, 2, 112, [33, 2, 0, 9], [900, 1, 70, 0], True, 0, 0),
+    (2, 1, 128, [90], [3000], True, 1200, 130), (2, 2, 64, [900, 40], [880, 10], True, 0, 0),
+    (1, 1, 16, [1, 1, 65], [1279, 64, 1300], True, 0, 0),
+])
+def test_prompt_few_rows_many_keys(gpu, t, H, G, D, ql, kl, causal, window, sink):
+    """Keys cut over workgroups, whose parts are joined: parts that a row sees nothing of, rows that see nothing."""
+    prompt_case(gpu, t, H, G, D, ql, kl, causal, window, sink)
+
+
+def test_prompt_parts_of_many_sequences(gpu):
+    """More sequences than a launch takes, each cut; a smaller call between two of them finds its results whole."""
+    lens = [600 + 13 * (i % 40) for i in range(70)]
+    ql = [1 + i % 3 for i in range(70)]
+    prompt_case(gpu, "bf16", 2, 1, 32, ql, lens)
+    prompt_case(gpu, "bf16", 4, 4, 128, [3], [1111])
+    prompt_case(gpu, "f32", 2, 1, 32, ql, lens)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_prompt_parts_not_finite(gpu, t):
+    """A NaN in one part's keys reaches the rows that see it and no others; so does one in a value."""
+    rng = np.random.default_rng(5)
+    nq, nk, H, D = 130, 1500, 1, 64
+    for spot in (3, 1400):
+        q, k, v = (R.rand(rng, (n, H, D), t) for n in (nq, nk, nk))
+        v[spot, 0, 5] = k[1450, 0, 7] = R.to_bits(np.float32(np.nan), t)
+        print(f"parts not finite {t} {spot}", flush=True)
+        y = R.from_bits(gpu.prompt_attention(dev(gpu, q), dev(gpu, k), dev(gpu, v), [nq], [nk]).numpy(), t)
+        q, k, v = (R.from_bits(x, t) for x in (q, k, v))
+        want, tol = R.attend(q, k, v, R.visible(nq, nk), R.default_scale(D), t)
+        R.check(y, want, tol)
+        p = nk - nq + np.arange(nq)
+        assert np.isnan(y[p >= 1450]).all() and np.isfinite(y[p < 1450][:, :, 6:]).all()
+        np.testing.assert_array_equal(np.isnan(y[:, 0, 5]), p >= spot)
+
+
 def test_prompt_too_many_rows(gpu):
     b = gpu.empty((64, 64, 64), np.float16)
     d = pf.AttnDesc(pf.TYPE_F16, 64, 64, 64, 1, 0, 0, 0.0, 0, 0, 0, 0)
