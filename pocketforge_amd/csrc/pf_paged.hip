@@ -281,13 +281,15 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
     for (; n_tile < n_tiles; n_tile++) body(std::true_type{}, n_tile);
 
     // the waves' results meet in LDS, 16 rows at a time
-    float* so = (float*)&sv[0][0][0];            // [W][16][DP]
+    constexpr int OS = DP + 4;                   // (16 rows' chunks of 16 bytes in different banks)
+    float* so = (float*)&sv[0][0][0];            // [W][16][OS]
+    static_assert(W * 16 * OS * 4 <= (int)sizeof(sv), "the waves' results fit V's tiles");
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const float lw = sum16(l[n]);
         __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DT; d++) *(f4v*)&so[(wave * 16 + col) * DP + d * 16 + 4 * g] = o[n][d];
+        for (int d = 0; d < DT; d++) *(f4v*)&so[(wave * 16 + col) * OS + d * 16 + 4 * g] = o[n][d];
         if (g == 0) {
             s_ml[wave][col][0] = m[n];
             s_ml[wave][col][1] = lw;
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
             const float f = exp2_fast(s_ml[w][r][0] - ms);
             L += f * s_ml[w][r][1];
 #pragma unroll
-            for (int i = 0; i < PER; i++) acc[i] += f * so[(w * 16 + r) * DP + d0 + i];
+            for (int i = 0; i < PER; i++) acc[i] += f * so[(w * 16 + r) * OS + d0 + i];
         }
         if (row >= R || (!EXACT && d0 >= (int)a.dim)) continue;   // (pairs of threads together)
         const int j = row / (int)a.group, h = (int)head0 + row - j * (int)a.group;
