@@ -31,12 +31,12 @@ __host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
 //
 // Each key and value row is read once, and with many sequences these bytes bound
 // it: 64 contexts of 2000 to 8000 bf16 keys, 16 heads of 128 over 4, one row:
-// 657 MB in 123 us, 5.3 TB/s (a large copy: 5.1).  Contexts of 60000 and 32000
-// fp16 keys, 16 heads over 2, in 241 shares: 94 MB in 18 us and the join's 6.
+// 657 MB in 122 us, 5.4 TB/s (a large copy: 5.1).  Contexts of 60000 and 32000
+// fp16 keys, 16 heads over 2, in 241 shares: 94 MB in 17 us and the join's 6.
 // 16 verify passes of five fp32 rows over 500 to 2100 int8 keys, 16 heads of
-// 128: 94 MB in 25 us; one round of workgroups with up to 9 tiles a wave, each a memory
+// 128: 94 MB in 23 us; one round of workgroups with up to 9 tiles a wave, each a memory
 // round trip, the codes' way to bf16 and three products per piece of the rows.
-// One context of 700 keys: 6.5 us and the join's 3.6, both latency.
+// One context of 700 keys: 5.8 us and the join's 3.5, both latency.
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
 __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
     // Weights over int8 rows take the rows' scales, whose range fp16 does not
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
 // Joins the parts of the sequences that were cut: one workgroup per (sequence's
 // first item, head), its rows one after another.  8 groups of 32 threads take
 // every eighth part, 4 dims a thread; then the groups meet in LDS, in order.
-// Latency: 3.6 us for one sequence of 6 parts, 6.4 for two of 241.  (The last
+// Latency: 3.5 us for one sequence of 6 parts, 6.4 for two of 241.  (The last
 // workgroup to end joining inside the attention, with a fence of the whole
 // device, took more: 64 contexts 158 us instead of 128.)
 template <int ACT>
@@ -421,7 +421,7 @@ template <int ACT, int CT, int DP, bool EXACT>
 static void paged_rows(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
     const uint32_t R = u.most_rows * a.group;
     // one tile of 16 rows, or two: the keys are read once for both (64 contexts of
-    // up to 4000 bf16 keys, 20 rows a kv head: 71 us, 128 as two single tiles)
+    // up to 4000 bf16 keys, 20 rows a kv head: 65 us, 104 as two single tiles)
     if (R <= 16) paged_one<ACT, CT, DP, 1, EXACT>(st, u, 1, a);
     else paged_one<ACT, CT, DP, 2, EXACT>(st, u, (R + 31) / 32, a);
 }
@@ -437,16 +437,16 @@ static void paged_dim(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
 // Cuts the pass's keys into shares of at most `chunk` tiles, by what they would
 // take, in half tiles' times: the rounds of workgroups (`per` for each share),
 // each as long as its longest wave's run of tiles and a tile's time more (two
-// with 8 waves, whose results meet in LDS: two bf16 contexts of 221 keys, 12
-// heads, 8.0 us with 8 and 6.8 with 4), and where a sequence is cut the second
+// with 8 waves, whose results meet in LDS: one bf16 row over 700 keys, 16 heads,
+// 10.5 us uncut with 8, 9.3 cut with 4), and where a sequence is cut the second
 // kernel, PG_JOIN and one for each PG_JOIN_ROWS rows and heads (48 contexts of
-// up to 3000 bf16 keys, 32 heads of 64, five rows: 59 us cut, 31 uncut).  Looked
+// up to 3000 bf16 keys, 32 heads of 64, five rows: 39 us cut, 31 uncut).  Looked
 // at: no cut, and the smallest shares that one round of workgroups holds, or two
 // for each sequence (a long one beside short ones), but of a tile for each wave;
 // with workgroups of 4 waves, and of 8 (half as many shares, to join as well: 16
-// verify passes of five fp32 rows over up to 2100 int8 keys of 16 heads, 25 us
-// uncut with 8, 29 cut with 4; one bf16 row over 700 keys, 11.8 and 10.0).  Two
-// contexts of 60000 and 32000 fp16 keys take 25 us cut, 509 uncut.
+// verify passes of five fp32 rows over up to 2100 int8 keys of 16 heads, 23 us
+// uncut with 8, 27 cut with 4).  Contexts of 60000 and 32000 fp16 keys take 23
+// us cut, 510 uncut.
 constexpr uint32_t PG_CUS = 256, PG_JOIN = 5, PG_JOIN_ROWS = 512;
 struct PageShares {
     uint32_t chunk = 1, waves = 4;

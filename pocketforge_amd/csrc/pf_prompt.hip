@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptA
 // transposing read lie in different quarters of the banks: no counted conflicts
 // beyond 1% of the LDS cycles.
 //
-// 8192 causal bf16 rows, 16 heads of 128: 283 us, 970 TFLOP/s of the 1210 that a
+// 8192 causal bf16 rows, 16 heads of 128: 288 us, 950 TFLOP/s of the 1210 that a
 // large bf16 product by the library reaches.  What bounds it: the matrix and the
 // exp instructions at the clock that they leave (1.95-2.05 GHz; matrix unit busy
 // 50% of the cycles that a compute unit has work): without loads, LDS reads and
