@@ -164,7 +164,7 @@ __device__ __forceinline__ float new_maximum(const f16v (&s)[G], float scale, fl
     top *= scale;
     if (__any(top > m + MAX_SLACK)) {
         const float to = fmaxf(m, max32(top));
-        const float f = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+        const float f = m == -INFINITY ? 1.0f : exp2_fast(m - to);   // (nothing yet, or infinities that stay)
         m = to;
         l *= f;
 #pragma unroll
@@ -199,7 +199,8 @@ __device__ __forceinline__ void join_halves(int wave, float& m, float& l, f16v (
     __syncthreads();
     if (wave >= 2) return;
     const f4v x = *ml;
-    const float to = fmaxf(m, x[0]), ms = to == -INFINITY ? 0.0f : to, f0 = exp2_fast(m - ms), f1 = exp2_fast(x[0] - ms);
+    const float to = fmaxf(m, x[0]), ms = to == -INFINITY ? 0.0f : to, f1 = exp2_fast(x[0] - ms);
+    const float f0 = m == -INFINITY ? 1.0f : exp2_fast(m - ms);      // (as in new_maximum)
     m = to;
     l = l * f0 + x[1] * f1;
 #pragma unroll

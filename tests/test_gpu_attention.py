@@ -630,6 +630,19 @@ def test_prompt_parts_of_many_sequences(gpu):
     prompt_case(gpu, "f32", 2, 1, 32, ql, lens)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n,window,spot", [(50, 0, 10), (50, 0, 0), (64, 12, 45), (300, 20, 40), (200, 0, 63)])
+def test_prompt_infinity_in_a_first_tile(gpu, t, n, window, spot):
+    """An infinite value in the first tile that a row sees, or in the only half of one, reaches it as that infinity."""
+    rng = np.random.default_rng(9)
+    q, k, v = (R.rand(rng, (n, 1, 64), t) for _ in range(3))
+    v[spot, 0, 3] = R.to_bits(np.float32(np.inf), t)
+    y = R.from_bits(gpu.prompt_attention(dev(gpu, q), dev(gpu, k), dev(gpu, v), [n], window=window).numpy(), t)
+    p = np.arange(n)
+    see = (p >= spot) & (p < spot + window if window else True)
+    assert (y[see, 0, 3] == np.inf).all() and np.isfinite(y[~see]).all() and np.isfinite(y[:, 0, 4:]).all()
+
+
 @pytest.mark.parametrize("t", ["bf16", "f32"])
 def test_prompt_parts_not_finite(gpu, t):
     """A NaN in one part's keys reaches the rows that see it and no others; so does one in a value."""
