@@ -848,8 +848,8 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
     a.scale_log2 = s.scale_log2;
     // 128 query rows a workgroup, or 64 where those would not fill the compute
     // units (two workgroups each; one of fp32 rows of over 64 dims).  One prompt of
-    // 1000 bf16 rows, 16 heads of 128: 19.7 us instead of 25.5; 16 prompts of up to
-    // 300: 23.7 instead of 20.0, where 128 rows make 528 workgroups
+    // 1000 bf16 rows, 16 heads of 128: 21 us instead of 27; 16 prompts of up to 300:
+    // 23.0 instead of 20.2, where 128 rows make 528 workgroups
     uint64_t units = 0;
     for (uint32_t i = 0; i < n_seq; i++) units += (uint64_t)((q_lens[i] + 127) / 128) * d->n_heads;
     const uint32_t full = PR_CUS * (d->type == PF_TYPE_F32 && d->head_dim > 64 ? 1 : 2), rows = units < full ? 64 : 128;
