@@ -282,6 +282,8 @@ def _rows(t, what):
     s, sh, sd = t.stride()
     if (d > 1 and sd != 1) or (h > 1 and sh != d):
         raise PFError(f"{what}: the heads of a row lie one after another")
+    if n > 1 and s < h * d:                     # (0, as expand gives, would be read as packed)
+        raise PFError(f"{what}: rows overlap (stride {s} of {h * d} elements); make it contiguous")
     return n, h, d, (s if n > 1 else h * d)
 
 

@@ -97,3 +97,14 @@ def test_reference_types():
     c, s = R.quantize_rows(np.array([[0.0, 0.0], [1.0, -2.0], [np.inf, 1.0]], np.float32))
     assert c.tolist() == [[0, 0], [64, -127], [0, 0]] and s[0, 0] == 1 and s[1, 0] == np.float32(2) / np.float32(127)
     assert np.isnan(s[2, 0])
+
+
+@pytest.mark.parametrize("stride", [0, 64, 255])
+def test_rows_that_overlap(stride):
+    """Rows that share memory (x.expand(n, heads, head_dim) has a stride of 0, which the C calls read as packed)."""
+    assert pf._rows(Rows((1, 4, 64), (stride, 64, 1), "torch.float16"), "q") == (1, 4, 64, 256)
+    with pytest.raises(pf.PFError):
+        pf._rows(Rows((5, 4, 64), (stride, 64, 1), "torch.float16"), "q")
+    torch = pytest.importorskip("torch")
+    with pytest.raises(pf.PFError):
+        pf._rows(torch.zeros((1, 4, 64)).expand(5, 4, 64), "k")
