@@ -287,6 +287,22 @@ def _rows(t, what):
     return n, h, d, (s if n > 1 else h * d)
 
 
+def _here(ctx, **arrays):
+    """Checks that arrays are device memory of the context's GPU (an address
+    from elsewhere would fault it)."""
+    for what, t in arrays.items():
+        if isinstance(t, DeviceArray):
+            if t.ctx.device != ctx.device or not t.ptr:
+                raise PFError(f"{what} is freed, or on another GPU than the context's {ctx.device}")
+            continue
+        try:
+            at = t.get_device()
+        except AttributeError:
+            raise PFError(f"{what} is a DeviceArray or a tensor on the GPU, not {type(t).__name__}") from None
+        if at != ctx.device:
+            raise PFError(f"{what} is {'in host memory' if at < 0 else f'on GPU {at}'}, not on the context's GPU {ctx.device}")
+
+
 def _u32(a, what):
     """A list of numbers from 0 as an array of 32-bit numbers."""
     try:
@@ -341,6 +357,7 @@ def quantize_matrix(w, fmt):
 
 class Context:
     def __init__(self, device=0):
+        self.device = device
         self.h = vp()
         rc = lib().pf_init(device, C.byref(self.h))
         if rc:
@@ -448,6 +465,7 @@ class Context:
         q_lens[s] positions of each sequence.  With `out` the call is
         asynchronous on the context's stream; without, a new array is
         returned when it is done."""
+        _here(self, q=q, k=k, v=v)
         ql = _u32(q_lens, "q_lens")
         kl = ql if k_lens is None else _u32(k_lens, "k_lens")
         nq, H, D, qs = _rows(q, "q")
@@ -458,7 +476,11 @@ class Context:
         if len(kl) != len(ql) or sum(ql) != nq or sum(kl) != nk:
             raise PFError("q_lens and k_lens name every row of q and of k")
         t = _type(q)
-        y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        if out is None:
+            y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t])
+        else:
+            _here(self, out=out)
+            y = out
         n2, H2, D3, os = _rows(y, "out")
         if (n2, H2, D3) != (nq, H, D) or not t == _type(k) == _type(v) == _type(y):
             raise PFError("q, k, v and out have one type, q and out one shape")
@@ -614,6 +636,7 @@ class PagedCache:
         self.pass_rows = sum(r)
 
     def _kv(self, k, v, rows):
+        _here(self.ctx, k=k, v=v)
         n, h, d, ks = _rows(k, "k")
         n1, h1, d1, vs = _rows(v, "v")
         if (n, h, d) != (n1, h1, d1) or (n, h, d) != (rows, self.n_kv_heads, self.head_dim):
@@ -630,9 +653,14 @@ class PagedCache:
 
     def attention(self, layer, q, causal=True, window=0, sink=0, scale=0.0, out=None):
         """The pass's rows over their sequences.  With `out` asynchronous, as Context.prompt_attention."""
+        _here(self.ctx, q=q)
         n, H, D, qs = _rows(q, "q")
         t = _type(q)
-        y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        if out is None:
+            y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t])
+        else:
+            _here(self.ctx, out=out)
+            y = out
         n1, H1, D1, os = _rows(y, "out")
         if n != self.pass_rows or (n1, H1, D1) != (n, H, D) or _type(y) != t:
             raise PFError(f"q and out are [{self.pass_rows}][heads][{self.head_dim}] of one type")

@@ -108,3 +108,45 @@ def test_rows_that_overlap(stride):
     torch = pytest.importorskip("torch")
     with pytest.raises(pf.PFError):
         pf._rows(torch.zeros((1, 4, 64)).expand(5, 4, 64), "k")
+
+
+class Placed:
+    """A tensor of one GPU, as the binding asks for it."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+def test_rows_elsewhere():
+    """Rows in host memory or on another GPU than the context's are refused before their address goes anywhere."""
+    ctx = pf.Context.__new__(pf.Context)
+    ctx.device, ctx.h = 1, None
+    own = pf.DeviceArray.__new__(pf.DeviceArray)
+    own.ctx, own.ptr = ctx, 256
+    pf._here(ctx, q=own, k=Placed(1))
+    other = pf.Context.__new__(pf.Context)
+    other.device, other.h = 0, None
+    far = pf.DeviceArray.__new__(pf.DeviceArray)
+    far.ctx, far.ptr = other, 256
+    freed = pf.DeviceArray.__new__(pf.DeviceArray)
+    freed.ctx, freed.ptr = ctx, None
+    for x in (far, freed, Placed(0), Placed(-1), np.zeros((2, 4, 64), np.float16), [1.0], None):
+        with pytest.raises(pf.PFError, match="k "):
+            pf._here(ctx, q=own, k=x)
+    torch = pytest.importorskip("torch")
+    with pytest.raises(pf.PFError, match="out "):
+        pf._here(ctx, out=torch.zeros((2, 4, 64)))
+    x = np.zeros((2, 4, 64), np.float16)
+    host = torch.zeros((2, 4, 64), dtype=torch.float16)
+    cache = pf.PagedCache.__new__(pf.PagedCache)
+    cache.ctx, cache.h, cache.pass_rows, cache.n_kv_heads, cache.head_dim = ctx, None, 2, 4, 64
+    for a in (x, host):
+        with pytest.raises(pf.PFError, match="GPU"):
+            ctx.prompt_attention(a, a, a, [2], out=a)
+        with pytest.raises(pf.PFError, match="GPU"):
+            cache.store(0, a, a)
+        with pytest.raises(pf.PFError, match="GPU"):
+            cache.attention(0, a, out=a)
