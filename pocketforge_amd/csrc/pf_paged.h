@@ -81,7 +81,7 @@ struct pf_pages {
     int32_t* table = nullptr;                      // device [max_seqs][per_seq]
     pf::PageSeq* seqs = nullptr;                   // device: the open pass
     pf::PageItem* items = nullptr;                 // device
-    uint32_t items_cap = 0;
+    size_t items_cap = 0;
     uint32_t* pairs = nullptr;                     // device: page copies under way
     PageStaging* staging = nullptr;
 

@@ -483,6 +483,9 @@ extern "C" pf_status pf_pages_create(pf_ctx* c, const pf_pages_config* g, pf_pag
     const uint32_t per_seq = (g->max_context + g->page_size - 1) / g->page_size;
     if ((uint64_t)per_seq * g->max_seqs > 0xFFFFFFFFull)
         return fail(c, PF_ERR_UNSUPPORTED, "pages: max_seqs times the pages of max_context is 2^32 at most");
+    const size_t scales = (size_t)g->n_pages * g->n_kv_heads * g->page_size, esize = g->type == PF_TYPE_I8 ? 1 : 2;
+    const size_t plane = scales * g->head_dim * esize;           // (below 2^63 within the limits above)
+    if (plane > (SIZE_MAX >> 2) / g->n_layers) return fail(c, PF_ERR_UNSUPPORTED, "pages: a pool of over 2^62 bytes");
     DeviceScope on(c);
     pf_pages* p = new (std::nothrow) pf_pages();
     if (!p) return fail(c, PF_ERR_CAPACITY, "out of host memory");
@@ -490,10 +493,10 @@ extern "C" pf_status pf_pages_create(pf_ctx* c, const pf_pages_config* g, pf_pag
     p->cfg = *g;
     p->shift = (uint32_t)__builtin_ctz(g->page_size);
     p->per_seq = per_seq;
-    p->esize = g->type == PF_TYPE_I8 ? 1 : 2;
-    p->scales = (size_t)g->n_pages * g->n_kv_heads * g->page_size;
-    p->plane = p->scales * g->head_dim * p->esize;
-    p->items_cap = 2 * g->max_seqs + PG_MOST_ITEMS;
+    p->esize = esize;
+    p->scales = scales;
+    p->plane = plane;
+    p->items_cap = (size_t)2 * g->max_seqs + PG_MOST_ITEMS;
     if (pf_status s = no_throw(c, [&] { return pages_alloc(p); })) {
         const std::string msg = c->err;
         pf_pages_destroy(p);

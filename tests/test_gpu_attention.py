@@ -711,3 +711,12 @@ def test_copies_in_one_call(gpu):
     m.c.compact()
     m.check(range(n + 1))
     m.c.close()
+
+
+def test_pool_sizes_past_64_bits(gpu):
+    """A pool whose bytes do not fit 64 bits is refused: 2^64 bytes came out as none, and were taken."""
+    h = pf.vp()
+    for ct, layers in ((pf.TYPE_BF16, 1 << 13), (pf.TYPE_BF16, (1 << 13) + 1), (pf.TYPE_I8, 1 << 14), (pf.TYPE_F16, 65535)):
+        cfg = pf.PagesConfig(ct, layers, 1 << 15, 128, 256, 1 << 20, 1, 256)
+        assert pf.lib().pf_pages_create(gpu.h, C.byref(cfg), C.byref(h)) == -4, (ct, layers)
+    assert not h
