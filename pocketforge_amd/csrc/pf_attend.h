@@ -204,11 +204,17 @@ __device__ __forceinline__ float sum16(float x) { x += __shfl_xor(x, 16); return
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Softmax runs in base 2 (scores times log2 e).  The running maximum only
-// moves when a score exceeds it by more than this: weights then reach 2^8,
-// far inside fp32 and fp16, and most tiles need no reduction over lanes and
-// no rescaling of the output.
-constexpr float MAX_SLACK = 8.0f;
+// Softmax runs in base 2 (scores times log2 e).  The running maximum m is held
+// above the scores' own by m_above, and moves only when a score exceeds it by
+// more than m_slack: most tiles need no reduction over lanes and no rescaling of
+// the output, and the weights 2^(s - m), which reach 2^(m_slack - m_above), stay
+// far inside fp32.  fp16's smallest step is 2^-24, so its weights are held up
+// against 2^15: what rounding takes of one is then below 2^-36 of the largest
+// weight (2^-25 of it if they were held against 1, and a thousand keys that
+// weigh that little beside a sink key would vanish).  8192 fp16 rows, 16 heads
+// of 128: 295 us with a slack of 4, 296 with 8 (2^-32), 299 with 2 (2^-38).
+template <bool BF> constexpr float m_slack = BF ? 8.0f : 4.0f;
+template <bool BF> constexpr float m_above = BF ? 0.0f : m_slack<BF> - 15.0f;
 
 // Visibility of a key at position `pos` for a query whose last visible
 // position is hi: the last `window` of the causal range start at lo.

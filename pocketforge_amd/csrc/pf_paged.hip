@@ -214,8 +214,8 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                 if constexpr (MASKED) x[e] = bits_or(x[e], -INFINITY, __builtin_amdgcn_sbfe((int)part, 16 * (e / 4) + e % 4, 1));
                 top = fmaxf(top, x[e]);
             }
-            if (__any(top > m[n] + MAX_SLACK)) {
-                const float to = fmaxf(m[n], max16(top));
+            if (__any(top > m[n] + (m_slack<VB> - m_above<VB>))) {
+                const float to = fmaxf(m[n], max16(top) + m_above<VB>);
                 const float f = to == -INFINITY ? 1.0f : exp2_fast(m[n] - to);
                 m[n] = to;
                 l[n] *= f;

@@ -154,7 +154,7 @@ __device__ __forceinline__ void mask_scores(f16v (&s)[G], const PromptArgs& a, i
 
 // The running maximum over a tile's scores (scaled to base 2), with the sum and
 // the output corrected where it moves; the value to subtract.
-template <int DT, int G>
+template <bool BF, int DT, int G>
 __device__ __forceinline__ float new_maximum(const f16v (&s)[G], float scale, float& m, float& l, f16v (&o)[DT]) {
     float top = s[0][0];
 #pragma unroll
@@ -162,8 +162,8 @@ __device__ __forceinline__ float new_maximum(const f16v (&s)[G], float scale, fl
 #pragma unroll
         for (int i = 0; i < 16; i++) top = fmaxf(top, s[g][i]);
     top *= scale;
-    if (__any(top > m + MAX_SLACK)) {
-        const float to = fmaxf(m, max32(top));
+    if (__any(top > m + (m_slack<BF> - m_above<BF>))) {
+        const float to = fmaxf(m, max32(top) + m_above<BF>);
         const float f = m == -INFINITY ? 1.0f : exp2_fast(m - to);   // (nothing yet, or infinities that stay)
         m = to;
         l *= f;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptA
                     for (int y = 0; x + y < NP; y++) s[g] = mfma32<true>(kf[x], qf[y][c], s[g]);
             }
         if constexpr (MASKED) mask_scores(s, a, nk, hi, lo, key0 + part, half);
-        const float ms = new_maximum(s, a.scale_log2, m, l, o);
+        const float ms = new_maximum<true>(s, a.scale_log2, m, l, o);
 #pragma unroll
         for (int gh = 0; gh < 2 * G; gh++) {     // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
             float x[8];
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
                 s[g] = mfma32<BF>(kf, qf[c], s[g]);
             }
         if constexpr (MASKED) mask_scores(s, a, nk, hi, lo, key0 + part, half);
-        const float ms = new_maximum(s, a.scale_log2, m, l, o);
+        const float ms = new_maximum<BF>(s, a.scale_log2, m, l, o);
         s8v pf[2 * G];
         float l1 = 0.0f;
 #pragma unroll

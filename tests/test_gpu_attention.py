@@ -720,3 +720,45 @@ def test_pool_sizes_past_64_bits(gpu):
         cfg = pf.PagesConfig(ct, layers, 1 << 15, 128, 256, 1 << 20, 1, 256)
         assert pf.lib().pf_pages_create(gpu.h, C.byref(cfg), C.byref(h)) == -4, (ct, layers)
     assert not h
+
+
+def beside_a_sink(t, n, low, first):
+    """One key that outweighs the n - 1 others by exp(low) each, with a value of zero; theirs are about 100."""
+    rng = np.random.default_rng(31)
+    k, v = np.zeros((n, 1, 64), np.float32), (100 + 10 * rng.standard_normal((n, 1, 64))).astype(np.float32)
+    k[:, :, 0] = -low
+    k[0 if first else n - 1, :, 0] = 0
+    v[0 if first else n - 1] = 0
+    return R.to_bits(k, t), R.to_bits(v, t)
+
+
+def fp16_step(v):
+    """What rounding takes of n weights: they are held against 2^11 times the largest at least, and half a step of
+    fp16's smallest values is 2^-25, so 2^-36 of the largest each (fp32 and bf16 reach far below)."""
+    return 2.0 ** -36 * np.abs(v).sum(0)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("low", [14, 16, 18, 20])
+def test_many_keys_beside_a_sink(gpu, t, first, low):
+    """Thousands of keys that weigh 2^-20 to 2^-29 of one: together they are what comes out."""
+    n, nq = 8000, 3
+    k, v = beside_a_sink(t, n, low, first)
+    q = R.to_bits(np.zeros((nq, 2, 64), np.float32), t)
+    q[:, :, 0] = R.to_bits(np.float32(1), t)
+    kf, vf = R.from_bits(k, t), R.from_bits(v, t)
+    want, tol = R.attend(R.from_bits(q, t), kf, vf, R.visible(nq, n, False), 1.0, t)
+    if t == "f16":
+        tol = tol + fp16_step(vf)
+    print(f"beside a sink {t} first {first} low {low}", flush=True)
+    y = gpu.prompt_attention(dev(gpu, q), dev(gpu, k), dev(gpu, v), [nq], [n], causal=False, scale=1.0).numpy()
+    R.check(R.from_bits(y, t), want, tol, "prompt")
+    c = pf.PagedCache(gpu, 1, 1, 64, 130, 1, n, 64, TYPE[t])
+    c.append([0], [n - nq])
+    c.store(0, dev(gpu, k[:-nq]), dev(gpu, v[:-nq]))
+    c.append([0], [nq])
+    c.store(0, dev(gpu, k[-nq:]), dev(gpu, v[-nq:]))
+    y = c.attention(0, dev(gpu, q), causal=False, scale=1.0).numpy()
+    R.check(R.from_bits(y, t), want, tol, "pages")
+    c.close()
