@@ -202,10 +202,12 @@ typedef struct {
  * k_lens[s] - q_lens[s] + i); k_lens NULL: the same as q_lens.  A query that
  * sees no key gets zeros.  Lengths are host arrays and may be 0; q_lens may
  * exceed k_lens.  Buffers and strides are multiples of 16 bytes; out may not
- * overlap the inputs.  Sums are fp32 whatever the type; fp32 rows (values
- * below 3.38e38) are multiplied to fp32 accuracy.  The weights of fp16 and
- * bf16 rows are rounded once to that type (pf_pages_attention: twice as many
- * bits), fp16 ones in steps of at least 2^-35 of the row's largest.  An infinity or a NaN in k
+ * overlap the inputs.  Sums are fp32 whatever the type, and values up to the
+ * type's largest do not overflow them, however many keys there are (fp32 rows:
+ * below 3.38e38; what lies below 2^-110 times the number of keys is lost); fp32
+ * rows are multiplied to fp32 accuracy.  The weights of fp16 and bf16 rows are
+ * rounded once to that type (pf_pages_attention: twice as many bits), fp16 ones
+ * to 2^-36 of the row's largest where they are smaller.  An infinity or a NaN in k
  * or v reaches the queries that see it and no others (fp32 rows: as a NaN).
  * Asynchronous on the context's stream: what other streams write or read is
  * the caller's to order (pf_synchronize).  Few queries over many keys take

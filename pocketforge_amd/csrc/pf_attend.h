@@ -204,17 +204,26 @@ __device__ __forceinline__ float sum16(float x) { x += __shfl_xor(x, 16); return
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Softmax runs in base 2 (scores times log2 e).  The running maximum m is held
-// above the scores' own by m_above, and moves only when a score exceeds it by
-// more than m_slack: most tiles need no reduction over lanes and no rescaling of
-// the output, and the weights 2^(s - m), which reach 2^(m_slack - m_above), stay
-// far inside fp32.  fp16's smallest step is 2^-24, so its weights are held up
-// against 2^15: what rounding takes of one is then below 2^-36 of the largest
-// weight (2^-25 of it if they were held against 1, and a thousand keys that
-// weigh that little beside a sink key would vanish).  8192 fp16 rows, 16 heads
-// of 128: 295 us with a slack of 4, 296 with 8 (2^-32), 299 with 2 (2^-38).
+// Softmax runs in base 2 (scores times log2 e).  The running maximum m moves only
+// when a score exceeds it by more than m_slack, so that most tiles need no
+// reduction over lanes and no rescaling of the output.  Outputs are summed as
+// they come and divided by the sum of the weights at the end, so the weights are
+// held at a distance from one that keeps those sums in fp32's range:
+//  * fp32 rows: weights 2^(s - m), which reach 2^m_slack, times 2^-K with K =
+//    keys_shift of the call's longest sequence.  2^K is over 2^m_slack times the
+//    keys, so values up to the type's largest do not overflow; what is lost below
+//    is less than 2^-126+K for each key.
+//  * bf16 operands of 16-bit rows: m is held K above the scores' own maximum,
+//    which is the same without the product, but rounds s - m at 2^-20.
+//  * fp16 operands cannot overflow, but their smallest step is 2^-24: m is held so
+//    far below that the weights reach 2^15.  What rounding takes of one is then
+//    below 2^-36 of the largest weight (2^-25 of it if they were held against 1,
+//    and a thousand keys that weigh that little beside a sink key would vanish).
+//    8192 fp16 rows, 16 heads of 128: 295 us with a slack of 4, 296 with 8
+//    (2^-32), 299 with 2 (2^-38).
 template <bool BF> constexpr float m_slack = BF ? 8.0f : 4.0f;
-template <bool BF> constexpr float m_above = BF ? 0.0f : m_slack<BF> - 15.0f;
+constexpr float FP16_ABOVE = m_slack<false> - 15.0f;
+inline int keys_shift(uint32_t keys) { return (int)m_slack<true> + 1 + (keys ? 32 - __builtin_clz(keys) : 0); }
 
 // Visibility of a key at position `pos` for a query whose last visible
 // position is hi: the last `window` of the causal range start at lo.

@@ -30,6 +30,7 @@ struct PageSplit {
     uint32_t window = 0, sink = 0, heads = 0;
     int32_t type = -1;
     uint32_t n_items = 0, ws_rows = 0, most_rows = 0;
+    uint32_t longest = 0;         // keys of the longest sequence
     uint32_t waves = 4;
     bool split = false;
 };
@@ -62,6 +63,7 @@ struct PagedArgs {
     uint32_t qs, os, n_heads, kv_heads, group, dim, page_shift;
     int32_t causal, window, sink;
     float scale_log2;
+    float above, down;            // as in pf_prompt.hip
     float* ws_o;                  // [ws_rows][n_heads][dim]
     float* ws_ml;                 // [ws_rows][n_heads][2]
 };

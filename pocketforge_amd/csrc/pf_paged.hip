@@ -9,6 +9,7 @@
 #include "pf_paged.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 using namespace pf;
@@ -106,6 +107,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
         }
     }
 
+    const float above = ACT == PF_TYPE_F32 ? 0.0f : VB ? a.above : FP16_ABOVE;
     f4v o[NT][DT];
     float m[NT], l[NT];
 #pragma unroll
@@ -214,8 +216,8 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                 if constexpr (MASKED) x[e] = bits_or(x[e], -INFINITY, __builtin_amdgcn_sbfe((int)part, 16 * (e / 4) + e % 4, 1));
                 top = fmaxf(top, x[e]);
             }
-            if (__any(top > m[n] + (m_slack<VB> - m_above<VB>))) {
-                const float to = fmaxf(m[n], max16(top) + m_above<VB>);
+            if (__any(top > m[n] + (m_slack<VB> - above))) {
+                const float to = fmaxf(m[n], max16(top) + above);
                 const float f = to == -INFINITY ? 1.0f : exp2_fast(m[n] - to);
                 m[n] = to;
                 l[n] *= f;
@@ -228,6 +230,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 x[e] = exp2_fast(x[e] - ms);
+                if constexpr (ACT == PF_TYPE_F32) x[e] *= a.down;
                 l[n] += x[e];
                 if constexpr (I8) {
                     x[e] *= vscale[e / 4][e % 4];
@@ -482,12 +485,13 @@ static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& 
     const uint32_t group = d->n_heads / d->n_kv_heads;
     std::vector<uint32_t> tiles;
     tiles.reserve(p->pass.size());
-    uint32_t most = 0, longest = 0;
+    uint32_t most = 0, longest = 0, keys = 0;
     for (const PageSeq& q : p->pass) {
         if (!q.rows) continue;
         tiles.push_back((uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count);
         longest = std::max(longest, tiles.back());
         most = std::max(most, q.rows);
+        keys = std::max(keys, q.len);
     }
     const uint64_t R = (uint64_t)most * group, per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
     const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
@@ -517,7 +521,7 @@ static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& 
     if (items.size() > p->items_cap) return fail(p->ctx, PF_ERR_STATE, "pages: work list exceeded");
     if (pf_status st = pages_upload(p, p->items, items.data(), items.size() * sizeof(PageItem))) return st;
     n.window = s.window; n.sink = s.sink; n.heads = d->n_heads; n.type = d->type;
-    n.n_items = (uint32_t)items.size(); n.ws_rows = (uint32_t)ws; n.most_rows = most;
+    n.n_items = (uint32_t)items.size(); n.ws_rows = (uint32_t)ws; n.most_rows = most; n.longest = keys;
     u = n;
     return PF_OK;
 }
@@ -559,6 +563,8 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
     a.page_shift = p->shift;
     a.causal = d->causal != 0; a.window = (int32_t)s.window; a.sink = (int32_t)s.sink;
     a.scale_log2 = s.scale_log2;
+    a.above = (float)keys_shift(u.longest);
+    a.down = std::ldexp(1.0f, -keys_shift(u.longest));
     hipStream_t st = c->stream;
 #define PF_PAGED(A, T) paged_dim<A, T>(st, u, a)
     if (ct == PF_TYPE_I8) {

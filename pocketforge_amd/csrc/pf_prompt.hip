@@ -34,6 +34,7 @@ struct PromptArgs {
     uint32_t qs, ks, vs, os;      // row strides in elements
     int32_t causal, window, sink;
     float scale_log2;
+    float above, down;            // how far m is held above the scores (bf16 rows), what weights are held to (fp32)
     uint32_t tiles;               // query tiles of all sequences
     uint32_t parts, rows;         // parts that the keys are cut in (grid y), rows of a part's results
     float* ws_o;                  // parts > 1: [parts][rows][n_heads][dim]
@@ -155,15 +156,15 @@ __device__ __forceinline__ void mask_scores(f16v (&s)[G], const PromptArgs& a, i
 // The running maximum over a tile's scores (scaled to base 2), with the sum and
 // the output corrected where it moves; the value to subtract.
 template <bool BF, int DT, int G>
-__device__ __forceinline__ float new_maximum(const f16v (&s)[G], float scale, float& m, float& l, f16v (&o)[DT]) {
+__device__ __forceinline__ float new_maximum(const f16v (&s)[G], float scale, float above, float& m, float& l, f16v (&o)[DT]) {
     float top = s[0][0];
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
         for (int i = 0; i < 16; i++) top = fmaxf(top, s[g][i]);
     top *= scale;
-    if (__any(top > m + (m_slack<BF> - m_above<BF>))) {
-        const float to = fmaxf(m, max32(top) + m_above<BF>);
+    if (__any(top > m + (m_slack<BF> - above))) {
+        const float to = fmaxf(m, max32(top) + above);
         const float f = m == -INFINITY ? 1.0f : exp2_fast(m - to);   // (nothing yet, or infinities that stay)
         m = to;
         l *= f;
@@ -415,13 +416,13 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void k_prompt_attn32(PromptA
                     for (int y = 0; x + y < NP; y++) s[g] = mfma32<true>(kf[x], qf[y][c], s[g]);
             }
         if constexpr (MASKED) mask_scores(s, a, nk, hi, lo, key0 + part, half);
-        const float ms = new_maximum<true>(s, a.scale_log2, m, l, o);
+        const float ms = new_maximum<true>(s, a.scale_log2, 0.0f, m, l, o);
 #pragma unroll
         for (int gh = 0; gh < 2 * G; gh++) {     // 16 keys: a lane's 8 are 4 half .. + 3 and 8 + 4 half .. + 3
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[i] = exp2_fast(__builtin_fmaf(s[gh / 2][8 * (gh & 1) + i], a.scale_log2, -ms));
+                x[i] = exp2_fast(__builtin_fmaf(s[gh / 2][8 * (gh & 1) + i], a.scale_log2, -ms)) * a.down;
                 l += x[i];
             }
             s8v pf[NP];
@@ -606,7 +607,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
                 s[g] = mfma32<BF>(kf, qf[c], s[g]);
             }
         if constexpr (MASKED) mask_scores(s, a, nk, hi, lo, key0 + part, half);
-        const float ms = new_maximum<BF>(s, a.scale_log2, m, l, o);
+        const float ms = new_maximum<BF>(s, a.scale_log2, BF ? a.above : FP16_ABOVE, m, l, o);
         s8v pf[2 * G];
         float l1 = 0.0f;
 #pragma unroll
@@ -821,10 +822,12 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
     if (pf_status st = attn_desc_check(c, d, &s)) return st;
     if (!k_lens) k_lens = q_lens;
     uint64_t nq = 0, nk = 0;
+    uint32_t longest = 0;
     for (uint32_t i = 0; i < n_seq; i++) {
         if (q_lens[i] > SEQ_ROWS || k_lens[i] > SEQ_ROWS) return fail(c, PF_ERR_UNSUPPORTED, "attention: a sequence of over 2^30 rows");
         nq += q_lens[i];
         nk += k_lens[i];
+        longest = std::max(longest, k_lens[i]);
     }
     if (!nq) return PF_OK;
     // (a grid has fewer than 2^32 threads)
@@ -846,6 +849,8 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
     a.qs = s.qs; a.ks = s.ks; a.vs = s.vs; a.os = s.os;
     a.causal = d->causal != 0; a.window = (int32_t)s.window; a.sink = (int32_t)s.sink;
     a.scale_log2 = s.scale_log2;
+    a.above = (float)keys_shift(longest);
+    a.down = std::ldexp(1.0f, -keys_shift(longest));
     // 128 query rows a workgroup, or 64 where those would not fill the compute
     // units (two workgroups each; one of fp32 rows of over 64 dims).  One prompt of
     // 1000 bf16 rows, 16 heads of 128: 21 us instead of 27; 16 prompts of up to 300:

@@ -762,3 +762,58 @@ def test_many_keys_beside_a_sink(gpu, t, first, low):
     y = c.attention(0, dev(gpu, q), causal=False, scale=1.0).numpy()
     R.check(R.from_bits(y, t), want, tol, "pages")
     c.close()
+
+
+LARGE = [("f32", 3e38), ("f32", 1e37), ("bf16", 3e38), ("bf16", 1e36), ("f16", 6e4), ("f32", 1e-30), ("bf16", 1e-30)]
+
+
+def far_values(rng, t, n, nq, size, G=1):
+    """Rows whose scores rise by 7.9 (base 2) after the first keys, less than what moves the running maximum:
+    weights of 2^7.9, and values all near `size`."""
+    k = np.zeros((n, G, 64), np.float32)
+    k[70:, :, 0] = 7.9 * np.log(2)
+    v = (size * (1 - 0.02 * rng.random((n, G, 64)))).astype(np.float32)
+    v[:, :, 32:] *= np.where(np.arange(n) % 2, 1, -1)[:, None, None].astype(np.float32)
+    q = np.zeros((nq, 2 * G, 64), np.float32)
+    q[:, :, 0] = 1
+    return (R.to_bits(x, t) for x in (q, k, v))
+
+
+def lost_below(t, n):
+    """What sums lose below fp32's normal range: 2^-126 of each product, weights held to 2^-K, K = 10 + log2 n at
+    most (six products of each key where rows are fp32, and two pieces else)."""
+    return 0.0 if t == "f16" else 6 * n * 2.0 ** (-126 + 10 + np.log2(n))
+
+
+@pytest.mark.parametrize("t,size", LARGE)
+@pytest.mark.parametrize("ql,kl", [([3], [100]), ([2, 1], [3000, 80]), ([5], [700]), ([130], [300])])
+def test_prompt_far_values(gpu, t, size, ql, kl):
+    """Values near the type's largest, or far below one: sums of them stay in range whatever the number of keys."""
+    rng = np.random.default_rng(8)
+    q, k, v = (np.concatenate(x) for x in zip(*(list(far_values(rng, t, n, a, size)) for a, n in zip(ql, kl))))
+    print(f"far values {t} {size} {ql} {kl}", flush=True)
+    y = R.from_bits(gpu.prompt_attention(dev(gpu, q), dev(gpu, k), dev(gpu, v), ql, kl, scale=1.0).numpy(), t)
+    q, k, v = (R.from_bits(x, t) for x in (q, k, v))
+    qa = ka = 0
+    for a, n in zip(ql, kl):
+        want, tol = R.attend(q[qa:qa + a], k[ka:ka + n], v[ka:ka + n], R.visible(a, n), 1.0, t)
+        R.check(y[qa:qa + a], want, tol + lost_below(t, max(kl)), f"{n} keys")
+        qa, ka = qa + a, ka + n
+
+
+@pytest.mark.parametrize("t,ct,size", [("f32", "bf16", 3e38), ("f32", "bf16", 1e-30), ("bf16", "bf16", 3e38),
+                                       ("bf16", "bf16", 1e-30), ("f32", "i8", 3e38), ("f32", "i8", 1e36),
+                                       ("bf16", "i8", 3e38), ("f32", "i8", 1e-25), ("f16", "i8", 6e4), ("f16", "f16", 6e4)])
+@pytest.mark.parametrize("n,nq", [(100, 1), (3000, 2), (700, 5)])
+def test_paged_far_values(gpu, t, ct, size, n, nq):
+    """The same over pages."""
+    m = Mirror(gpu, ct, 1, 64, 64, 50, 1, 3200, t=t)
+    q, k, v = far_values(m.rng, t, n, nq, size)
+    m.append([0], [n - nq], (k[:-nq], v[:-nq]))
+    m.append([0], [nq], (k[-nq:], v[-nq:]))
+    print(f"far values {t} over {ct} {size} {n}", flush=True)
+    y = R.from_bits(m.c.attention(0, dev(gpu, q), scale=1.0).numpy(), t)
+    kf, vf = m.rows[0][0]
+    want, tol = R.attend(R.from_bits(q, t), kf, vf, R.visible(nq, n), 1.0, t, ct == "i8")
+    R.check(y, want, tol + lost_below(t, n))
+    m.c.close()
