@@ -204,11 +204,12 @@ typedef struct {
  * exceed k_lens.  Buffers and strides are multiples of 16 bytes; out may not
  * overlap the inputs.  Sums are fp32 whatever the type, and values up to the
  * type's largest do not overflow them, however many keys there are (fp32 rows:
- * below 3.38e38; what lies below 2^-110 times the number of keys is lost); fp32
- * rows are multiplied to fp32 accuracy.  The weights of fp16 and bf16 rows are
+ * below 3.38e38; what lies below 2^-113 times the square of their number may be
+ * lost); fp32 rows are multiplied to fp32 accuracy.  The weights of fp16 and bf16 rows are
  * rounded once to that type (pf_pages_attention: twice as many bits), fp16 ones
  * to 2^-36 of the row's largest where they are smaller.  An infinity or a NaN in k
- * or v reaches the queries that see it and no others (fp32 rows: as a NaN).
+ * or v reaches the queries that see it and no others; one in v as itself or, where
+ * its weight vanishes or rows are fp32, as a NaN.
  * Asynchronous on the context's stream: what other streams write or read is
  * the caller's to order (pf_synchronize).  Few queries over many keys take
  * workgroups for parts of the keys; only a call that needs more room for
@@ -268,7 +269,9 @@ pf_status pf_pages_store(pf_pages* p, uint32_t layer, int32_t type, const void* 
 /* Attention of the pass's rows over their sequences' rows in one layer (store
  * them first): q and out [sum rows][n_heads][head_dim] of desc->type.  A
  * 16-bit cache takes rows of its own type, a bf16 or int8 cache fp32 rows
- * too, an int8 cache all three.  The k and v strides are not used. */
+ * too, an int8 cache all three.  Sums, and values that are not finite, as in
+ * pf_prompt_attention, for fp32 rows as for the others.  The k and v strides are
+ * not used. */
 pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* desc, uint32_t layer, const void* q_dev, void* out_dev);
 /* Reads n sequences' rows of one layer back, packed in this order, as `type`
  * (F32, F16 or BF16): with pf_prompt_attention, a long pass over a cached

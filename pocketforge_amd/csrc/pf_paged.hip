@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                 codes8(w[2], w[3], x);
                 *(s8v*)(place(i) + 8) = pack8<VB>(x);
             } else {
-                if constexpr (MASKED) z = sum8<BF>(__builtin_bit_cast(s8v, w), z, 0.0f);
+                z = sum8<BF>(__builtin_bit_cast(s8v, w), z, 0.0f);
                 *(u4v*)place(i) = w;
             }
         }
@@ -240,14 +240,16 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
             pieces<VB, PP>(x, pf[n]);
         }
         __builtin_amdgcn_wave_barrier();
-        if constexpr (MASKED && !I8) {
+        if constexpr (!I8) {
             if (__any(z != z)) {
                 // infinities and NaN reach the rows that see them, whatever their weight,
-                // and the products find zeros in their places
+                // and the products find zeros in their places (a weight's second piece is
+                // zero or negative as often as not, which would make a NaN of an infinity;
+                // looking every tile through takes 0.3 us of 24 where two contexts are cut)
                 for (int r = 0; r < 32; r++)
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        if (pos0 + r >= len || !key_visible(pos0 + r, hi[n], lo[n], a.sink)) continue;
+                        if (MASKED && (pos0 + r >= len || !key_visible(pos0 + r, hi[n], lo[n], a.sink))) continue;
 #pragma unroll
                         for (int d = 0; d < DT; d++)
 #pragma unroll

@@ -817,3 +817,30 @@ def test_paged_far_values(gpu, t, ct, size, n, nq):
     want, tol = R.attend(R.from_bits(q, t), kf, vf, R.visible(nq, n), 1.0, t, ct == "i8")
     R.check(y, want, tol + lost_below(t, n))
     m.c.close()
+
+
+@pytest.mark.parametrize("t,ct", [("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("n,window", [(36, 0), (700, 0), (700, 300), (5000, 0)])
+@pytest.mark.parametrize("D,H", [(64, 2), (128, 20), (48, 2)])
+def test_paged_infinity_as_the_context_grows(gpu, t, ct, n, window, D, H):
+    """An infinite value reaches the rows that see it as that infinity wherever its key lies; two that differ as a
+    NaN; the rest of the row as ever."""
+    spot = n - 30
+    for bad in (np.inf, -np.inf):
+        m = Mirror(gpu, ct, 1, D, 32, 160, 1, 5100, t=t)
+        k, v = (R.rand(m.rng, (n, 1, D), t) for _ in range(2))
+        v[spot, 0, 5] = v[spot - 1, 0, 5] = v[spot - 3, 0, 6] = R.to_bits(np.float32(bad), t)
+        v[spot - 4, 0, 6] = R.to_bits(np.float32(-bad), t)
+        m.append([0], [n - 2], (k[:-2], v[:-2]))
+        m.append([0], [2], (k[-2:], v[-2:]))
+        print(f"infinity {t} over {ct} n {n} window {window} D {D} {bad}", flush=True)
+        for grown in (0, 1, 64):             # the key moves into tiles that every row sees whole
+            if grown:
+                new = [R.rand(m.rng, (grown, 1, D), t) for _ in range(2)]
+                m.append([0], [grown], new)
+            rows = grown or 2
+            q = R.rand(m.rng, (rows, H, D), t)
+            y = R.from_bits(m.c.attention(0, dev(gpu, q), window=window).numpy(), t)
+            assert (y[:, :, 5] == bad).all() and np.isnan(y[:, :, 6]).all()
+            assert np.isfinite(y[:, :, :5]).all() and np.isfinite(y[:, :, 7:]).all()
+        m.c.close()
