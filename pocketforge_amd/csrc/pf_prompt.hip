@@ -547,7 +547,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
     auto chunks = [&](int r, int* ck, int* cv) {
         *ck = k_place<DP>(r, lc);
         *cv = v_place<DP>(r, lc);
-        if (!EXACT) {                            // (past head_dim: q's zeros, unused outputs)
+        if (!EXACT) {                            // (past head_dim: unused)
             *ck = min(*ck, (int)a.dim / 8 - 1);
             *cv = min(*cv, (int)a.dim / 8 - 1);
         }
@@ -603,6 +603,7 @@ __global__ __launch_bounds__(256, 2) void k_prompt_attn16(PromptArgs a) {
         for (int c = 0; c < C; c++)
 #pragma unroll
             for (int g = 0; g < G; g++) {
+                if (!EXACT && c * 16 >= (int)a.dim) break;   // (no dims: zeros would meet another chunk's infinities)
                 const s8v kf = *(const s8v*)&sk[(part + g * 32 + row) * DP + k_place<DP>(row, c * 2 + half) * 8];
                 s[g] = mfma32<BF>(kf, qf[c], s[g]);
             }

@@ -844,3 +844,25 @@ def test_paged_infinity_as_the_context_grows(gpu, t, ct, n, window, D, H):
             assert (y[:, :, 5] == bad).all() and np.isnan(y[:, :, 6]).all()
             assert np.isfinite(y[:, :, :5]).all() and np.isfinite(y[:, :, 7:]).all()
         m.c.close()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [16, 48, 64, 80, 112, 128])
+def test_minus_infinity_in_a_key(gpu, t, D):
+    """A key of minus infinity where the queries are positive has a score of minus infinity: it weighs nothing."""
+    rng = np.random.default_rng(6)
+    n, at = 150, 20
+    q, k, v = (R.rand(rng, (n, 2, D), t) for _ in range(3))
+    q[:, :, D - 2] = R.to_bits(np.float32(0.5), t)
+    k[at, :, D - 2] = R.to_bits(np.float32(-np.inf), t)
+    print(f"minus infinity {t} {D}", flush=True)
+    qf, kf, vf = (R.from_bits(x, t) for x in (q, k, v))
+    want, tol = R.attend(qf, np.where(np.isinf(kf), 0, kf), vf, R.visible(n, n) & (np.arange(n) != at)[None],
+                         R.default_scale(D), t)
+    y = R.from_bits(gpu.prompt_attention(dev(gpu, q), dev(gpu, k), dev(gpu, v), [n]).numpy(), t)
+    R.check(y, want, tol, "prompt")
+    c = pf.PagedCache(gpu, 1, 2, D, 10, 1, 160, 16, TYPE[t])
+    c.append([0], [n])
+    c.store(0, dev(gpu, k), dev(gpu, v))
+    R.check(R.from_bits(c.attention(0, dev(gpu, q)).numpy(), t), want, tol, "pages")
+    c.close()
