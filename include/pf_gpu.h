@@ -191,7 +191,7 @@ typedef struct {
     int32_t causal;            /* 1: a query sees keys up to its own position */
     uint32_t window, sink;     /* window > 0: of the keys up to its own position a query sees the last
                                   `window` and the first `sink` */
-    float scale;               /* of the scores; 0: 1 / sqrt(head_dim); not negative */
+    float scale;               /* of the scores; 0: 1 / sqrt(head_dim); not negative, below 2^127 */
     uint32_t q_stride, k_stride, v_stride, o_stride;   /* elements from one token's heads to the next
                                   token's; 0: heads * head_dim */
 } pf_attn_desc;

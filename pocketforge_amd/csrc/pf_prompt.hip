@@ -766,6 +766,7 @@ pf_status attn_desc_check(pf_ctx* c, const pf_attn_desc* d, AttnShape* s) {
         *out[i] = (uint32_t)st;
     }
     s->scale_log2 = (d->scale == 0.0f ? 1.0f / std::sqrt((float)d->head_dim) : d->scale) * LOG2E;
+    if (!std::isfinite(s->scale_log2)) return fail(c, PF_ERR_ARG, "attention: scale is below 2^127");
     return PF_OK;
 }
 

@@ -866,3 +866,21 @@ def test_minus_infinity_in_a_key(gpu, t, D):
     c.store(0, dev(gpu, k), dev(gpu, v))
     R.check(R.from_bits(c.attention(0, dev(gpu, q)).numpy(), t), want, tol, "pages")
     c.close()
+
+
+def test_scale_out_of_range(gpu):
+    """A scale that is not finite in base 2 would make a NaN of scores of zero: it is refused."""
+    q, k, v, o = (gpu.empty((4, 2, 64), np.float16) for _ in range(4))
+    c = pf.PagedCache(gpu, 1, 2, 64, 1, 1, 16, 16, pf.TYPE_F16)
+    c.append([0], [4])
+    c.store(0, k, v)
+    for scale in (2.4e38, 3e38, float("inf")):
+        with pytest.raises(pf.PFError, match=r"\(-1\)"):
+            gpu.prompt_attention(q, k, v, [4], scale=scale, out=o)
+        with pytest.raises(pf.PFError, match=r"\(-1\)"):
+            c.attention(0, q, scale=scale, out=o)
+    z = dev(gpu, np.zeros((4, 2, 64), np.float16))
+    x = np.arange(512, dtype=np.float16).reshape(4, 2, 64)
+    y = gpu.prompt_attention(z, z, dev(gpu, x), [4], causal=False, scale=1.6e38).numpy()
+    np.testing.assert_array_equal(y, np.broadcast_to(x.astype(np.float64).mean(0).astype(np.float16), y.shape))
+    c.close()
