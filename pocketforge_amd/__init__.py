@@ -8,6 +8,7 @@ the library's own pf_malloc (DeviceArray).
 """
 import array
 import ctypes as C
+import operator
 import os
 
 import numpy as np
@@ -284,7 +285,7 @@ def _rows(t, what):
         raise PFError(f"{what}: the heads of a row lie one after another")
     if n > 1 and s < h * d:                     # (0, as expand gives, would be read as packed)
         raise PFError(f"{what}: rows overlap (stride {s} of {h * d} elements); make it contiguous")
-    return n, h, d, (s if n > 1 else h * d)
+    return n, h, d, _num(s if n > 1 else h * d, f"{what}'s stride")
 
 
 def _here(ctx, **arrays):
@@ -309,6 +310,16 @@ def _u32(a, what):
         return array.array("I", a.tolist() if isinstance(a, np.ndarray) else a)
     except (TypeError, OverflowError, ValueError):
         raise PFError(f"{what} is a list of numbers from 0") from None
+
+
+def _num(x, what):
+    """A number from 0 that fits 32 bits (ctypes would take it modulo 2^32)."""
+    try:
+        if 0 <= (i := operator.index(x)) < 1 << 32:
+            return i
+    except TypeError:
+        pass
+    raise PFError(f"{what} is a number from 0 below 2^32, not {x!r}")
 
 
 def _at(a):
@@ -484,7 +495,7 @@ class Context:
         n2, H2, D3, os = _rows(y, "out")
         if (n2, H2, D3) != (nq, H, D) or not t == _type(k) == _type(v) == _type(y):
             raise PFError("q, k, v and out have one type, q and out one shape")
-        d = AttnDesc(t, H, G, D, causal, window, sink, scale, qs, ks, vs, os)
+        d = AttnDesc(t, H, G, D, bool(causal), _num(window, "window"), _num(sink, "sink"), scale, qs, ks, vs, os)
         self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), _at(ql), _at(kl),
                                              len(ql)), "pf_prompt_attention")
         if out is None:
@@ -622,7 +633,9 @@ class PagedCache:
         self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv_heads, head_dim
         self.page_size, self.n_pages, self.max_seqs, self.type = page_size, n_pages, max_seqs, type
         self.pass_rows = 0
-        cfg = PagesConfig(type, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_context)
+        sizes = dict(n_layers=n_layers, n_kv_heads=n_kv_heads, head_dim=head_dim, page_size=page_size, n_pages=n_pages,
+                     max_seqs=max_seqs, max_context=max_context)
+        cfg = PagesConfig(type, **{k: _num(v, k) for k, v in sizes.items()})
         h = vp()
         ctx.check(lib().pf_pages_create(ctx.h, C.byref(cfg), C.byref(h)), "pf_pages_create")
         self.h = h
@@ -649,7 +662,7 @@ class PagedCache:
     def store(self, layer, k, v):
         """The pass's new rows of one layer."""
         t, ks, vs = self._kv(k, v, self.pass_rows)
-        self.ctx.check(lib().pf_pages_store(self.h, layer, t, _dptr(k), _dptr(v), ks, vs), "pf_pages_store")
+        self.ctx.check(lib().pf_pages_store(self.h, _num(layer, "layer"), t, _dptr(k), _dptr(v), ks, vs), "pf_pages_store")
 
     def attention(self, layer, q, causal=True, window=0, sink=0, scale=0.0, out=None):
         """The pass's rows over their sequences.  With `out` asynchronous, as Context.prompt_attention."""
@@ -664,14 +677,16 @@ class PagedCache:
         n1, H1, D1, os = _rows(y, "out")
         if n != self.pass_rows or (n1, H1, D1) != (n, H, D) or _type(y) != t:
             raise PFError(f"q and out are [{self.pass_rows}][heads][{self.head_dim}] of one type")
-        d = AttnDesc(t, H, self.n_kv_heads, D, causal, window, sink, scale, qs, 0, 0, os)
-        self.ctx.check(lib().pf_pages_attention(self.h, C.byref(d), layer, _dptr(q), _dptr(y)), "pf_pages_attention")
+        d = AttnDesc(t, H, self.n_kv_heads, D, bool(causal), _num(window, "window"), _num(sink, "sink"), scale, qs, 0, 0, os)
+        self.ctx.check(lib().pf_pages_attention(self.h, C.byref(d), _num(layer, "layer"), _dptr(q), _dptr(y)),
+                       "pf_pages_attention")
         if out is None:
             self.ctx.synchronize()
         return y
 
     def gather(self, layer, seqs, out=None, dtype=np.float32):
         """The sequences' rows of one layer, packed: (k, v)."""
+        _num(layer, "layer")
         s = _u32(seqs, "seqs")
         lens = np.zeros(len(s), np.int64)
         self.ctx.check(lib().pf_pages_tables(self.h, _at(s), len(s), None, 0, _vptr(lens)), "pf_pages_tables")
@@ -689,7 +704,7 @@ class PagedCache:
 
     def fork(self, src, dst):
         d = _u32(dst, "dst")
-        self.ctx.check(lib().pf_pages_fork(self.h, src, _at(d), len(d)), "pf_pages_fork")
+        self.ctx.check(lib().pf_pages_fork(self.h, _num(src, "src"), _at(d), len(d)), "pf_pages_fork")
 
     def copy(self, src, dst):
         s, d = _u32(src, "src"), _u32(dst, "dst")
@@ -714,7 +729,7 @@ class PagedCache:
         return n.value
 
     def length(self, seq):
-        return lib().pf_pages_length(self.h, int(seq))
+        return lib().pf_pages_length(self.h, _num(seq, "seq"))
 
     def tables(self, seqs):
         """Page numbers of the sequences, -1 past their ends, and their lengths."""
@@ -730,6 +745,8 @@ class PagedCache:
         """The pool in device memory: k and v [layers][pages][kv heads][page
         size][head_dim] and, for int8, their row scales [layers][pages][kv
         heads][page size][1]; of one layer, without the first dimension."""
+        if layer is not None and _num(layer, "layer") >= self.n_layers:
+            raise PFError(f"layer {layer} of {self.n_layers}")
         p = [vp() for _ in range(4)]
         self.ctx.check(lib().pf_pages_planes(self.h, C.byref(p[0]), C.byref(p[1]), C.byref(p[2]), C.byref(p[3])),
                        "pf_pages_planes")

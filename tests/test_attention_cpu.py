@@ -150,3 +150,42 @@ def test_rows_elsewhere():
             cache.store(0, a, a)
         with pytest.raises(pf.PFError, match="GPU"):
             cache.attention(0, a, out=a)
+
+
+def test_numbers():
+    """Numbers that do not fit 32 bits are refused, not taken modulo 2^32."""
+    assert [pf._num(x, "n") for x in (0, 7, np.int64(9), 0xFFFFFFFF)] == [0, 7, 9, 0xFFFFFFFF]
+    for x in (-1, 1 << 32, 1.5, "1", None, [1]):
+        with pytest.raises(pf.PFError, match="n is"):
+            pf._num(x, "n")
+    ctx = pf.Context.__new__(pf.Context)
+    ctx.device, ctx.h = 0, None
+    x = pf.DeviceArray.__new__(pf.DeviceArray)
+    x.ctx, x.ptr, x.shape, x.dtype = ctx, 256, (2, 4, 64), np.dtype(np.float16)
+    y = pf.DeviceArray.__new__(pf.DeviceArray)
+    y.ctx, y.ptr, y.shape, y.dtype = ctx, 4096, (2, 4, 64), np.dtype(np.float16)
+    c = pf.PagedCache.__new__(pf.PagedCache)
+    c.ctx, c.h, c.pass_rows, c.n_kv_heads, c.head_dim, c.max_seqs, c.n_layers = ctx, None, 2, 4, 64, 3, 2
+    for bad in (-1, 1 << 32):
+        for kw in (dict(window=bad), dict(sink=bad)):
+            with pytest.raises(pf.PFError, match=next(iter(kw))):
+                ctx.prompt_attention(x, x, x, [2], out=y, **kw)
+            with pytest.raises(pf.PFError, match=next(iter(kw))):
+                c.attention(0, x, out=y, **kw)
+        for f in (lambda: c.attention(bad, x, out=y), lambda: c.store(bad, x, x), lambda: c.gather(bad, []),
+                  lambda: c.planes(bad)):
+            with pytest.raises(pf.PFError, match="layer"):
+                f()
+        with pytest.raises(pf.PFError, match="src"):
+            c.fork(bad, [1])
+        with pytest.raises(pf.PFError, match="seq"):
+            c.length(bad)
+        for name in ("n_layers", "n_kv_heads", "head_dim", "n_pages", "max_seqs", "max_context", "page_size"):
+            f = dict(n_layers=1, n_kv_heads=1, head_dim=64, n_pages=1, max_seqs=1, max_context=64, page_size=64)
+            f[name] = bad
+            with pytest.raises(pf.PFError, match=name):
+                pf.PagedCache(ctx, **f)
+    with pytest.raises(pf.PFError, match="layer"):
+        c.planes(2)
+    with pytest.raises(pf.PFError, match="stride"):
+        pf._rows(Rows((2, 4, 64), ((1 << 32) + 256, 64, 1), "torch.float16"), "q")
