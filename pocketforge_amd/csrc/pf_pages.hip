@@ -727,7 +727,6 @@ extern "C" pf_status pf_pages_gather(pf_pages* p, uint32_t layer, const uint32_t
 static pf_status pages_fork(pf_pages* p, uint32_t src, const uint32_t* dst, uint32_t n) {
     if (src >= p->cfg.max_seqs) return fail(p->ctx, PF_ERR_ARG, "pages: sequence out of range");
     if (pf_status st = all_empty(p, dst, n)) return st;
-    if (!n || !p->len[src]) return PF_OK;
     DeviceScope on(p->ctx);
     if (pf_status st = more_changes(p, (size_t)n * p->pages[src].size())) return st;
     for (uint32_t i = 0; i < n; i++) more_pages(p, dst[i], p->pages[src].size());

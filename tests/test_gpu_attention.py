@@ -884,3 +884,19 @@ def test_scale_out_of_range(gpu):
     y = gpu.prompt_attention(z, z, dev(gpu, x), [4], causal=False, scale=1.6e38).numpy()
     np.testing.assert_array_equal(y, np.broadcast_to(x.astype(np.float64).mean(0).astype(np.float16), y.shape))
     c.close()
+
+
+def test_calls_that_change_nothing_end_the_pass(gpu):
+    """fork, copy, truncate, free and compact end the pass, whatever there is for them to do."""
+    c = pf.PagedCache(gpu, 1, 2, 64, 4, 3, 64, 16, pf.TYPE_BF16)
+    k = gpu.empty((2, 2, 64), np.uint16)
+    for f in (lambda: c.fork(1, [2]), lambda: c.fork(0, []), lambda: c.copy([], []), lambda: c.truncate([], []),
+              lambda: c.free([]), c.compact):
+        c.free([0])
+        c.append([0], [2])
+        c.store(0, k, k)
+        f()
+        with pytest.raises(pf.PFError, match=r"\(-5\)"):
+            c.store(0, k, k)
+        assert c.length(0) == 2 and c.length(2) == 0 and c.free_pages == 3
+    c.close()
