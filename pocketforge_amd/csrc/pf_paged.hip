@@ -481,37 +481,62 @@ static void page_shares(const std::vector<uint32_t>& tiles, uint32_t longest, ui
         if (chunk < longest) take(chunk);
     }
 }
+// What a pass's attention takes: its sequences' tiles (of those with rows), and
+// how they are cut.
+struct PagePlan {
+    std::vector<uint32_t> tiles;
+    uint32_t most = 0, longest = 0, keys = 0;   // rows, tiles and keys of a sequence at most
+    PageShares shares;
+};
+static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc* d, const AttnShape& s) {
+    PagePlan n;
+    n.tiles.reserve(pass.size());
+    uint64_t rows = 0;
+    for (const PageSeq& q : pass) {
+        if (!q.rows) continue;
+        n.tiles.push_back((uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count);
+        n.longest = std::max(n.longest, n.tiles.back());
+        n.most = std::max(n.most, q.rows);
+        n.keys = std::max(n.keys, q.len);
+        rows += q.rows;
+    }
+    const uint64_t R = (uint64_t)n.most * (d->n_heads / d->n_kv_heads), per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
+    const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
+    const uint64_t join = PG_JOIN + rows * d->n_heads / PG_JOIN_ROWS;
+    page_shares(n.tiles, n.longest, per, (uint64_t)PG_CUS * held, 4, join, &n.shares);
+    if (held > 1) page_shares(n.tiles, n.longest, per, (uint64_t)PG_CUS * (held / 2), 8, join, &n.shares);
+    return n;
+}
+extern "C" pf_status pf_test_pages_plan(const pf_attn_desc* d, const uint32_t* rows, const uint32_t* lens, uint32_t n,
+                                        uint32_t* waves, uint32_t* chunk, uint32_t* longest) {
+    AttnShape s;
+    if (pf_status st = attn_desc_check(nullptr, d, &s)) return st;
+    return no_throw(nullptr, [&] {
+        std::vector<PageSeq> pass;
+        for (uint32_t i = 0; i < n; i++) pass.push_back({i, 0, rows[i], lens[i]});
+        const PagePlan plan = paged_plan(pass, d, s);
+        *waves = plan.shares.waves;
+        *chunk = plan.shares.chunk;
+        *longest = plan.longest;
+        return (pf_status)PF_OK;
+    });
+}
 static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
     PageSplit& u = p->cut;
     if (u.type == d->type && u.window == s.window && u.sink == s.sink && u.heads == d->n_heads) return PF_OK;
-    const uint32_t group = d->n_heads / d->n_kv_heads;
-    std::vector<uint32_t> tiles;
-    tiles.reserve(p->pass.size());
-    uint32_t most = 0, longest = 0, keys = 0;
-    for (const PageSeq& q : p->pass) {
-        if (!q.rows) continue;
-        tiles.push_back((uint32_t)page_tiles(q.rows, q.len, s.window, s.sink).count);
-        longest = std::max(longest, tiles.back());
-        most = std::max(most, q.rows);
-        keys = std::max(keys, q.len);
-    }
-    const uint64_t R = (uint64_t)most * group, per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
-    const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
-    if (R > 32 * 65535u) return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
-    PageShares best;
-    const uint64_t join = PG_JOIN + (uint64_t)p->pass_rows * d->n_heads / PG_JOIN_ROWS;
-    page_shares(tiles, longest, per, (uint64_t)PG_CUS * held, 4, join, &best);
-    if (held > 1) page_shares(tiles, longest, per, (uint64_t)PG_CUS * (held / 2), 8, join, &best);
-    const uint32_t chunk = best.chunk;
+    const PagePlan plan = paged_plan(p->pass, d, s);
+    if ((uint64_t)plan.most * (d->n_heads / d->n_kv_heads) > 32 * 65535u)
+        return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
+    const uint32_t chunk = plan.shares.chunk;
     PageSplit n;
-    n.waves = best.waves;
+    n.waves = plan.shares.waves;
     std::vector<PageItem> items;
-    items.reserve(page_shares_of(tiles, chunk));
+    items.reserve(page_shares_of(plan.tiles, chunk));
     uint64_t ws = 0;
     uint32_t i = 0;
     for (const PageSeq& q : p->pass) {
         if (!q.rows) continue;
-        const uint32_t t = tiles[i++], parts = (t + chunk - 1) / chunk;
+        const uint32_t t = plan.tiles[i++], parts = (t + chunk - 1) / chunk;
         for (uint32_t k = 0; k < parts; k++)
             items.push_back({q.slot, q.q0, q.rows, q.len, (uint32_t)((uint64_t)t * k / parts),
                              (uint32_t)((uint64_t)t * (k + 1) / parts), (uint32_t)ws, parts, k, 0});
@@ -523,7 +548,7 @@ static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& 
     if (items.size() > p->items_cap) return fail(p->ctx, PF_ERR_STATE, "pages: work list exceeded");
     if (pf_status st = pages_upload(p, p->items, items.data(), items.size() * sizeof(PageItem))) return st;
     n.window = s.window; n.sink = s.sink; n.heads = d->n_heads; n.type = d->type;
-    n.n_items = (uint32_t)items.size(); n.ws_rows = (uint32_t)ws; n.most_rows = most; n.longest = keys;
+    n.n_items = (uint32_t)items.size(); n.ws_rows = (uint32_t)ws; n.most_rows = plan.most; n.longest = plan.keys;
     u = n;
     return PF_OK;
 }

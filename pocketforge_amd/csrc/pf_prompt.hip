@@ -817,6 +817,31 @@ static uint32_t prompt_parts(const pf_attn_desc* d, const AttnShape& s, const ui
     return (uint32_t)parts;
 }
 
+// 128 query rows a workgroup, or 64 where those would not fill the compute
+// units (two workgroups each; one of fp32 rows of over 64 dims).  One prompt of
+// 1000 bf16 rows, 16 heads of 128: 21 us instead of 27; 16 prompts of up to 300:
+// 23.0 instead of 20.2, where 128 rows make 528 workgroups
+struct PromptPlan {
+    uint32_t rows, parts;
+};
+static PromptPlan prompt_plan(const pf_attn_desc* d, const AttnShape& s, const uint32_t* q_lens, const uint32_t* k_lens,
+                              uint32_t n_seq) {
+    uint64_t units = 0;
+    for (uint32_t i = 0; i < n_seq; i++) units += (uint64_t)((q_lens[i] + 127) / 128) * d->n_heads;
+    const uint32_t full = PR_CUS * (d->type == PF_TYPE_F32 && d->head_dim > 64 ? 1 : 2);
+    if (units >= full) return {128, 1};
+    return {64, prompt_parts(d, s, q_lens, k_lens, n_seq, full)};
+}
+extern "C" pf_status pf_test_prompt_plan(const pf_attn_desc* d, const uint32_t* q_lens, const uint32_t* k_lens,
+                                         uint32_t n_seq, uint32_t* rows, uint32_t* parts) {
+    AttnShape s;
+    if (pf_status st = attn_desc_check(nullptr, d, &s)) return st;
+    const PromptPlan plan = prompt_plan(d, s, q_lens, k_lens, n_seq);
+    *rows = plan.rows;
+    *parts = plan.parts;
+    return PF_OK;
+}
+
 extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const void* q, const void* k, const void* v,
                                          void* out, const uint32_t* q_lens, const uint32_t* k_lens, uint32_t n_seq) {
     if (!c || !d || (n_seq && !q_lens)) return PF_ERR_ARG;
@@ -853,16 +878,10 @@ extern "C" pf_status pf_prompt_attention(pf_ctx* c, const pf_attn_desc* d, const
     a.scale_log2 = s.scale_log2;
     a.above = (float)keys_shift(longest);
     a.down = std::ldexp(1.0f, -keys_shift(longest));
-    // 128 query rows a workgroup, or 64 where those would not fill the compute
-    // units (two workgroups each; one of fp32 rows of over 64 dims).  One prompt of
-    // 1000 bf16 rows, 16 heads of 128: 21 us instead of 27; 16 prompts of up to 300:
-    // 23.0 instead of 20.2, where 128 rows make 528 workgroups
-    uint64_t units = 0;
-    for (uint32_t i = 0; i < n_seq; i++) units += (uint64_t)((q_lens[i] + 127) / 128) * d->n_heads;
-    const uint32_t full = PR_CUS * (d->type == PF_TYPE_F32 && d->head_dim > 64 ? 1 : 2), rows = units < full ? 64 : 128;
-    a.parts = 1;
     a.rows = (uint32_t)nq;
-    if (rows == 64) a.parts = prompt_parts(d, s, q_lens, k_lens, n_seq, full);
+    const PromptPlan plan = prompt_plan(d, s, q_lens, k_lens, n_seq);
+    const uint32_t rows = plan.rows;
+    a.parts = plan.parts;
     if (a.parts > 1) {
         const size_t n = (size_t)a.parts * a.rows * a.n_heads;
         void* ws = nullptr;

@@ -900,3 +900,104 @@ def test_calls_that_change_nothing_end_the_pass(gpu):
             c.store(0, k, k)
         assert c.length(0) == 2 and c.length(2) == 0 and c.free_pages == 3
     c.close()
+
+
+# ------------------------------------------- each kernel of the dispatch rules
+
+def prompt_plan(t, H, G, D, ql, kl):
+    """(query rows of a workgroup, parts of the keys) that a call takes."""
+    d = pf.AttnDesc(TYPE[t], H, G, D, 1, 0, 0, 0.0, 0, 0, 0, 0)
+    rows, parts = C.c_uint32(), C.c_uint32()
+    a, b = ((C.c_uint32 * len(x))(*x) for x in (ql, kl))
+    assert pf.lib().pf_test_prompt_plan(C.byref(d), a, b, len(ql), C.byref(rows), C.byref(parts)) == 0
+    return rows.value, parts.value
+
+
+def pages_plan(t, H, G, D, rows, lens, window=0, sink=0):
+    """(waves of a workgroup, whether the keys are cut) of a pass."""
+    d = pf.AttnDesc(TYPE[t], H, G, D, 1, window, sink, 0.0, 0, 0, 0, 0)
+    x = [C.c_uint32() for _ in range(3)]
+    a, b = ((C.c_uint32 * len(y))(*y) for y in (rows, lens))
+    assert pf.lib().pf_test_pages_plan(C.byref(d), a, b, len(lens), *map(C.byref, x)) == 0
+    return x[0].value, x[1].value < x[2].value
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [48, 64, 80, 128])
+@pytest.mark.parametrize("ql,prefix,causal,window,sink", [
+    ([1, 130, 2, 0, 3, 129, 1, 9], 0, True, 0, 0), ([64, 129, 5, 33, 1, 2, 7], 300, True, 0, 0),
+    ([64, 129, 5, 33, 1, 2, 7], 200, True, 70, 5), ([1, 200, 2, 0, 3, 129, 1, 9], 20, False, 0, 0),
+    ([140, 129, 40, 1, 5, 2], -40, True, 30, 2),
+])
+def test_prompt_tiles_of_128_rows(gpu, t, D, ql, prefix, causal, window, sink):
+    """Enough heads and sequences that a workgroup takes 128 query rows, a wave 32 of them over whole key tiles."""
+    kl = [max(0, n + prefix) for n in ql]
+    assert prompt_plan(t, 64, 16, D, ql, kl) == (128, 1)
+    prompt_case(gpu, t, 64, 16, D, ql, kl, causal, window, sink)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [64, 112])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_prompt_tiles_of_128_rows_not_finite(gpu, t, D, bad):
+    """An infinity or a NaN in a value reaches the rows that see it and no others, over whole tiles and others."""
+    rng = np.random.default_rng(12)
+    n, H, spots = 150, 64, (3, 70, 149)
+    lens = [n] * 4
+    assert prompt_plan(t, H, H, D, lens, lens) == (128, 1)
+    q, k, v = (R.rand(rng, (4 * n, H, D), t) for _ in range(3))
+    for s, at in enumerate(spots):
+        v[s * n + at, :, 9] = R.to_bits(np.float32(bad), t)
+    print(f"128 rows not finite {t} {D} {bad}", flush=True)
+    y = R.from_bits(gpu.prompt_attention(dev(gpu, q), dev(gpu, k), dev(gpu, v), lens).numpy(), t)
+    for s, at in enumerate(spots + (n,)):
+        got = y[s * n:(s + 1) * n]
+        assert np.isfinite(got[:at]).all() and np.isfinite(got[:, :, :9]).all() and np.isfinite(got[:, :, 10:]).all()
+        if t == "f32" or np.isnan(bad):
+            assert not np.isfinite(got[at:, :, 9]).any()
+        else:
+            assert (got[at:, :, 9] == bad).all()
+
+
+@pytest.mark.parametrize("t,ct", COMBOS)
+@pytest.mark.parametrize("D", [48, 64, 112, 128])
+@pytest.mark.parametrize("H,G,lens,new,window,sink,causal", [
+    (4, 2, [500, 405, 9, 430], 1, 0, 0, True), (16, 2, [402, 33, 512], 1, 0, 0, True),
+    (8, 2, [390, 461], 5, 0, 0, True), (6, 1, [480, 7], 7, 0, 0, True), (4, 2, [900, 500, 30], 3, 420, 5, True),
+    (8, 1, [700, 460], 4, 410, 0, True), (6, 2, [449, 403], 6, 0, 0, False),
+])
+def test_paged_workgroups_of_8_waves(gpu, t, ct, D, H, G, lens, new, window, sink, causal):
+    """Contexts that workgroups of 8 waves take uncut (fp32 rows of over 64 dims and 16 score columns: 4 waves)."""
+    waves, _ = pages_plan(t, H, G, D, [new] * len(lens), lens, window, sink)
+    assert waves == (4 if t == "f32" and D > 64 and new * H // G > 16 else 8)
+    m = Mirror(gpu, ct, G, D, 32, sum(-(-n // 32) for n in lens), len(lens), max(lens), t=t)
+    seqs = list(range(len(lens)))
+    print(f"8 waves {t} over {ct} D {D} H {H} G {G} lens {lens} new {new} window {window}", flush=True)
+    m.append(seqs, [n - new for n in lens])
+    m.append(seqs, [new] * len(lens))
+    m.attention(H, seqs, [new] * len(lens), causal=causal, window=window, sink=sink)
+    m.c.close()
+
+
+@pytest.mark.parametrize("t,ct", [("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("D,H", [(48, 2), (64, 10), (128, 2)])
+def test_paged_workgroups_of_8_waves_not_finite(gpu, t, ct, D, H):
+    """Infinities and NaN in values reach the rows that see them as themselves, and no others."""
+    n, new = 450, 4
+    assert pages_plan(t, H, 1, D, [new], [n])[0] == 8
+    m = Mirror(gpu, ct, 1, D, 16, 29, 1, n, t=t)
+    k, v = (R.rand(m.rng, (n, 1, D), t) for _ in range(2))
+    for at, d, bad in ((7, 1, np.inf), (300, 2, -np.inf), (n - 2, 3, np.inf), (n - 1, 4, np.nan)):
+        v[at, 0, d] = R.to_bits(np.float32(bad), t)
+    m.append([0], [n - new], (k[:-new], v[:-new]))
+    m.append([0], [new], (k[-new:], v[-new:]))
+    q = R.rand(m.rng, (new, H, D), t)
+    print(f"8 waves not finite {t} over {ct} D {D} H {H}", flush=True)
+    y = R.from_bits(m.c.attention(0, dev(gpu, q)).numpy(), t)
+    kf, vf = m.rows[0][0]
+    want, tol = R.attend(R.from_bits(q, t), kf, vf, R.visible(new, n), R.default_scale(D), t)
+    with np.errstate(invalid="ignore"):
+        R.check(y, want, tol)
+    assert (y[:, :, 1] == np.inf).all() and (y[:, :, 2] == -np.inf).all() and np.isfinite(y[:2, :, 3:]).all()
+    assert (y[2:, :, 3] == np.inf).all() and np.isfinite(y[2, :, 4:]).all() and np.isnan(y[3, :, 4]).all()
+    m.c.close()
