@@ -154,13 +154,6 @@ __device__ __forceinline__ bool not_finite(short v) {
     return ((uint16_t)v & mask) == mask;
 }
 template <bool BF>
-__device__ __forceinline__ bool any_not_finite(s8v v) {
-    bool r = false;
-#pragma unroll
-    for (int i = 0; i < 8; i++) r |= not_finite<BF>(v[i]);
-    return r;
-}
-template <bool BF>
 __device__ __forceinline__ s8v finite_or_zero(s8v v) {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = not_finite<BF>(v[i]) ? (short)0 : v[i];

@@ -19,7 +19,7 @@ struct PageSeq {
 // ws0 + part * rows .. of the partial results, or, where parts == 1, to the
 // output.
 struct PageItem {
-    uint32_t slot, q0, rows, len, t0, t1, ws0, parts, part, unused;
+    uint32_t slot, q0, rows, len, t0, t1, ws0, parts, part;
 };
 constexpr uint32_t PG_KEYS = 32;
 constexpr uint32_t PG_MOST_PARTS = 1024;   // of one sequence
@@ -53,9 +53,8 @@ __host__ __device__ __forceinline__ PageTiles page_tiles(uint32_t rows, uint32_t
 
 struct PagedArgs {
     const PageItem* items;
-    const PageSeq* seqs;
     const int32_t* table;
-    uint32_t table_stride, n_seq;
+    uint32_t table_stride;
     const void *k, *v;            // this layer's planes
     const float *ks, *vs;
     const void* q;

@@ -539,7 +539,7 @@ static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& 
         const uint32_t t = plan.tiles[i++], parts = (t + chunk - 1) / chunk;
         for (uint32_t k = 0; k < parts; k++)
             items.push_back({q.slot, q.q0, q.rows, q.len, (uint32_t)((uint64_t)t * k / parts),
-                             (uint32_t)((uint64_t)t * (k + 1) / parts), (uint32_t)ws, parts, k, 0});
+                             (uint32_t)((uint64_t)t * (k + 1) / parts), (uint32_t)ws, parts, k});
         if (parts == 1) continue;
         ws += (uint64_t)parts * q.rows;
         n.split = true;
@@ -582,7 +582,7 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
         a.ws_o = (float*)ws;
         a.ws_ml = a.ws_o + rows * d->head_dim;
     }
-    a.items = p->items; a.seqs = p->seqs; a.table = p->table; a.table_stride = p->per_seq; a.n_seq = (uint32_t)p->pass.size();
+    a.items = p->items; a.table = p->table; a.table_stride = p->per_seq;
     a.k = (const uint8_t*)p->k + layer * p->plane; a.v = (const uint8_t*)p->v + layer * p->plane;
     if (p->ks) { a.ks = p->ks + layer * p->scales; a.vs = p->vs + layer * p->scales; }
     a.q = q; a.out = out; a.qs = s.qs; a.os = s.os;
