@@ -271,37 +271,44 @@ def _type(t):
         return _TYPE_OF.setdefault(t.dtype, _TYPES[name])
 
 
-def _rows(t, what):
+def _rows(t, what, ctx=None):
     """(rows, heads, head_dim, elements from one row to the next) of a
-    [rows][heads][head_dim] device array; a torch tensor may be a view whose
-    rows lie apart, as the parts of a fused QKV product do."""
-    if len(t.shape) != 3:
-        raise PFError(f"{what} is [rows][heads][head_dim], not {tuple(t.shape)}")
-    n, h, d = t.shape
-    if isinstance(t, DeviceArray):
+    [rows][heads][head_dim] device array (of the context's GPU, where it is
+    given); a torch tensor may be a view whose rows lie apart, as the parts of a
+    fused QKV product do."""
+    own = isinstance(t, DeviceArray)
+    # (dict: what is no tensor is on no GPU)
+    if ctx is not None and (own or getattr(t, "get_device", dict)() != ctx.device):
+        _here(ctx, t, what)
+    try:
+        n, h, d = t.shape
+    except ValueError:
+        raise PFError(f"{what} is [rows][heads][head_dim], not {tuple(t.shape)}") from None
+    if own:
         return int(n), int(h), int(d), int(h * d)
     s, sh, sd = t.stride()
     if (d > 1 and sd != 1) or (h > 1 and sh != d):
         raise PFError(f"{what}: the heads of a row lie one after another")
-    if n > 1 and s < h * d:                     # (0, as expand gives, would be read as packed)
-        raise PFError(f"{what}: rows overlap (stride {s} of {h * d} elements); make it contiguous")
-    return n, h, d, _num(s if n > 1 else h * d, f"{what}'s stride")
+    if n <= 1:
+        return n, h, d, h * d
+    if not h * d <= s < 1 << 32:                # (0, as expand gives, would be read as packed)
+        raise PFError(f"{what}: rows of {h * d} elements overlap, or lie too far apart, at a stride of {s}")
+    return n, h, d, s
 
 
-def _here(ctx, **arrays):
-    """Checks that arrays are device memory of the context's GPU (an address
+def _here(ctx, t, what):
+    """Checks that an array is device memory of the context's GPU (an address
     from elsewhere would fault it)."""
-    for what, t in arrays.items():
-        if isinstance(t, DeviceArray):
-            if t.ctx.device != ctx.device or not t.ptr:
-                raise PFError(f"{what} is freed, or on another GPU than the context's {ctx.device}")
-            continue
-        try:
-            at = t.get_device()
-        except AttributeError:
-            raise PFError(f"{what} is a DeviceArray or a tensor on the GPU, not {type(t).__name__}") from None
-        if at != ctx.device:
-            raise PFError(f"{what} is {'in host memory' if at < 0 else f'on GPU {at}'}, not on the context's GPU {ctx.device}")
+    if isinstance(t, DeviceArray):
+        if t.ctx.device != ctx.device or not t.ptr:
+            raise PFError(f"{what} is freed, or on another GPU than the context's {ctx.device}")
+        return
+    try:
+        at = t.get_device()
+    except AttributeError:
+        raise PFError(f"{what} is a DeviceArray or a tensor on the GPU, not {type(t).__name__}") from None
+    if at != ctx.device:
+        raise PFError(f"{what} is {'in host memory' if at < 0 else f'on GPU {at}'}, not on the context's GPU {ctx.device}")
 
 
 def _u32(a, what):
@@ -315,8 +322,10 @@ def _u32(a, what):
 def _num(x, what):
     """A number from 0 that fits 32 bits (ctypes would take it modulo 2^32)."""
     try:
-        if 0 <= (i := operator.index(x)) < 1 << 32:
-            return i
+        if type(x) is not int:
+            x = operator.index(x)
+        if 0 <= x < 1 << 32:
+            return x
     except TypeError:
         pass
     raise PFError(f"{what} is a number from 0 below 2^32, not {x!r}")
@@ -324,6 +333,10 @@ def _num(x, what):
 
 def _at(a):
     return a.buffer_info()[0]
+
+
+def _addr(t):
+    return t.ptr if isinstance(t, DeviceArray) else t.data_ptr()
 
 
 def _vptr(a):
@@ -476,27 +489,22 @@ class Context:
         q_lens[s] positions of each sequence.  With `out` the call is
         asynchronous on the context's stream; without, a new array is
         returned when it is done."""
-        _here(self, q=q, k=k, v=v)
         ql = _u32(q_lens, "q_lens")
         kl = ql if k_lens is None else _u32(k_lens, "k_lens")
-        nq, H, D, qs = _rows(q, "q")
-        nk, G, D1, ks = _rows(k, "k")
-        n1, G1, D2, vs = _rows(v, "v")
+        nq, H, D, qs = _rows(q, "q", self)
+        nk, G, D1, ks = _rows(k, "k", self)
+        n1, G1, D2, vs = _rows(v, "v", self)
         if (n1, G1) != (nk, G) or D1 != D or D2 != D:
             raise PFError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are alike, with q's head_dim {D}")
         if len(kl) != len(ql) or sum(ql) != nq or sum(kl) != nk:
             raise PFError("q_lens and k_lens name every row of q and of k")
         t = _type(q)
-        if out is None:
-            y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t])
-        else:
-            _here(self, out=out)
-            y = out
-        n2, H2, D3, os = _rows(y, "out")
+        y = self.empty((nq, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        n2, H2, D3, os = _rows(y, "out", self)
         if (n2, H2, D3) != (nq, H, D) or not t == _type(k) == _type(v) == _type(y):
             raise PFError("q, k, v and out have one type, q and out one shape")
         d = AttnDesc(t, H, G, D, bool(causal), _num(window, "window"), _num(sink, "sink"), scale, qs, ks, vs, os)
-        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _dptr(q), _dptr(k), _dptr(v), _dptr(y), _at(ql), _at(kl),
+        self.check(lib().pf_prompt_attention(self.h, C.byref(d), _addr(q), _addr(k), _addr(v), _addr(y), _at(ql), _at(kl),
                                              len(ql)), "pf_prompt_attention")
         if out is None:
             self.synchronize()
@@ -649,9 +657,8 @@ class PagedCache:
         self.pass_rows = sum(r)
 
     def _kv(self, k, v, rows):
-        _here(self.ctx, k=k, v=v)
-        n, h, d, ks = _rows(k, "k")
-        n1, h1, d1, vs = _rows(v, "v")
+        n, h, d, ks = _rows(k, "k", self.ctx)
+        n1, h1, d1, vs = _rows(v, "v", self.ctx)
         if (n, h, d) != (n1, h1, d1) or (n, h, d) != (rows, self.n_kv_heads, self.head_dim):
             raise PFError(f"k and v are [{rows}][{self.n_kv_heads}][{self.head_dim}], not {tuple(k.shape)}, {tuple(v.shape)}")
         t = _type(k)
@@ -662,23 +669,18 @@ class PagedCache:
     def store(self, layer, k, v):
         """The pass's new rows of one layer."""
         t, ks, vs = self._kv(k, v, self.pass_rows)
-        self.ctx.check(lib().pf_pages_store(self.h, _num(layer, "layer"), t, _dptr(k), _dptr(v), ks, vs), "pf_pages_store")
+        self.ctx.check(lib().pf_pages_store(self.h, _num(layer, "layer"), t, _addr(k), _addr(v), ks, vs), "pf_pages_store")
 
     def attention(self, layer, q, causal=True, window=0, sink=0, scale=0.0, out=None):
         """The pass's rows over their sequences.  With `out` asynchronous, as Context.prompt_attention."""
-        _here(self.ctx, q=q)
-        n, H, D, qs = _rows(q, "q")
+        n, H, D, qs = _rows(q, "q", self.ctx)
         t = _type(q)
-        if out is None:
-            y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t])
-        else:
-            _here(self.ctx, out=out)
-            y = out
-        n1, H1, D1, os = _rows(y, "out")
+        y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        n1, H1, D1, os = _rows(y, "out", self.ctx)
         if n != self.pass_rows or (n1, H1, D1) != (n, H, D) or _type(y) != t:
             raise PFError(f"q and out are [{self.pass_rows}][heads][{self.head_dim}] of one type")
         d = AttnDesc(t, H, self.n_kv_heads, D, bool(causal), _num(window, "window"), _num(sink, "sink"), scale, qs, 0, 0, os)
-        self.ctx.check(lib().pf_pages_attention(self.h, C.byref(d), _num(layer, "layer"), _dptr(q), _dptr(y)),
+        self.ctx.check(lib().pf_pages_attention(self.h, C.byref(d), _num(layer, "layer"), _addr(q), _addr(y)),
                        "pf_pages_attention")
         if out is None:
             self.ctx.synchronize()
@@ -696,7 +698,7 @@ class PagedCache:
         else:
             k, v = out
         t, ks, vs = self._kv(k, v, n)
-        self.ctx.check(lib().pf_pages_gather(self.h, layer, _at(s), len(s), t, _dptr(k), _dptr(v), ks, vs),
+        self.ctx.check(lib().pf_pages_gather(self.h, layer, _at(s), len(s), t, _addr(k), _addr(v), ks, vs),
                        "pf_pages_gather")
         if out is None:
             self.ctx.synchronize()

@@ -126,7 +126,8 @@ def test_rows_elsewhere():
     ctx.device, ctx.h = 1, None
     own = pf.DeviceArray.__new__(pf.DeviceArray)
     own.ctx, own.ptr = ctx, 256
-    pf._here(ctx, q=own, k=Placed(1))
+    pf._here(ctx, own, "q")
+    pf._here(ctx, Placed(1), "k")
     other = pf.Context.__new__(pf.Context)
     other.device, other.h = 0, None
     far = pf.DeviceArray.__new__(pf.DeviceArray)
@@ -135,15 +136,15 @@ def test_rows_elsewhere():
     freed.ctx, freed.ptr = ctx, None
     for x in (far, freed, Placed(0), Placed(-1), np.zeros((2, 4, 64), np.float16), [1.0], None):
         with pytest.raises(pf.PFError, match="k "):
-            pf._here(ctx, q=own, k=x)
+            pf._here(ctx, x, "k")
     torch = pytest.importorskip("torch")
     with pytest.raises(pf.PFError, match="out "):
-        pf._here(ctx, out=torch.zeros((2, 4, 64)))
+        pf._here(ctx, torch.zeros((2, 4, 64)), "out")
     x = np.zeros((2, 4, 64), np.float16)
     host = torch.zeros((2, 4, 64), dtype=torch.float16)
     cache = pf.PagedCache.__new__(pf.PagedCache)
     cache.ctx, cache.h, cache.pass_rows, cache.n_kv_heads, cache.head_dim = ctx, None, 2, 4, 64
-    for a in (x, host):
+    for a, ctx.device in ((x, 1), (host, 1), (x, 0), (host, 0)):
         with pytest.raises(pf.PFError, match="GPU"):
             ctx.prompt_attention(a, a, a, [2], out=a)
         with pytest.raises(pf.PFError, match="GPU"):
