@@ -207,7 +207,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 //    keys, so values up to the type's largest do not overflow; what is lost below
 //    is less than 2^-126+K for each key.
 //  * bf16 operands of 16-bit rows: m is held K above the scores' own maximum,
-//    which is the same without the product, but rounds s - m at 2^-20.
+//    which is the same without the product, but rounds s - m to 2^-19.
 //  * fp16 operands cannot overflow, but their smallest step is 2^-24: m is held so
 //    far below that the weights reach 2^15.  What rounding takes of one is then
 //    below 2^-36 of the largest weight (2^-25 of it if they were held against 1,
