@@ -33,9 +33,9 @@ __host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
 // Each key and value row is read once, and with many sequences these bytes bound
 // it: 64 contexts of 2000 to 8000 bf16 keys, 16 heads of 128 over 4, one row:
 // 657 MB in 122 us, 5.4 TB/s (a large copy: 5.1).  Contexts of 60000 and 32000
-// fp16 keys, 16 heads over 2, in 241 shares: 94 MB in 17 us and the join's 6.
+// fp16 keys, 16 heads over 2, in 241 shares: 94 MB in 18 us and the join's 6.
 // 16 verify passes of five fp32 rows over 500 to 2100 int8 keys, 16 heads of
-// 128: 94 MB in 23 us; one round of workgroups with up to 9 tiles a wave, each a memory
+// 128: 94 MB in 24 us; one round of workgroups with up to 9 tiles a wave, each a memory
 // round trip, the codes' way to bf16 and three products per piece of the rows.
 // One context of 700 keys: 5.8 us and the join's 3.5, both latency.
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>

@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptArgs a) {
 // take one, which bound it (a bf16 instruction does 16 times the fp32 one's
 // work).  A tile's rows wait in registers while the tile before is worked on,
 // and are cut into pieces on their way to LDS.  3 prompts of up to 1100 rows
-// after 333 cached, 12 heads of 64, window 1024: 61 us, or 98 TFLOP/s of fp32
+// after 333 cached, 12 heads of 64, window 1024: 62 us, or 96 TFLOP/s of fp32
 // products (a large one by the library reaches 137); 516 workgroups of 64 rows
 // are one round, whose longest ends last.
 template <int DP, bool EXACT, int SPLIT>
