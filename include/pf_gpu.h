@@ -204,12 +204,12 @@ typedef struct {
  * exceed k_lens.  Buffers and strides are multiples of 16 bytes; out may not
  * overlap the inputs.  Sums are fp32 whatever the type, and values up to the
  * type's largest do not overflow them, however many keys there are (fp32 rows:
- * below 3.38e38; what lies below 2^-113 times the square of their number may be
- * lost); fp32 rows are multiplied to fp32 accuracy.  The weights of fp16 and bf16 rows are
- * rounded once to that type (pf_pages_attention: twice as many bits), fp16 ones
- * to 2^-36 of the row's largest where they are smaller.  An infinity or a NaN in k
- * or v reaches the queries that see it and no others; one in v as itself or, where
- * its weight vanishes or rows are fp32, as a NaN.
+ * below 3.38e38; what lies below 2^-108 times the square of their number may be
+ * lost); fp32 rows are multiplied to fp32 accuracy.  The weights of fp16 and
+ * bf16 rows are rounded once to that type (pf_pages_attention: twice as many
+ * bits), fp16 ones to 2^-36 of the row's largest where they are smaller.  An
+ * infinity or a NaN in k or v reaches the queries that see it and no others;
+ * one in v as itself or, where its weight vanishes or rows are fp32, as a NaN.
  * Asynchronous on the context's stream: what other streams write or read is
  * the caller's to order (pf_synchronize).  Few queries over many keys take
  * workgroups for parts of the keys; only a call that needs more room for
