@@ -1001,3 +1001,56 @@ def test_paged_workgroups_of_8_waves_not_finite(gpu, t, ct, D, H):
     assert (y[:, :, 1] == np.inf).all() and (y[:, :, 2] == -np.inf).all() and np.isfinite(y[:2, :, 3:]).all()
     assert (y[2:, :, 3] == np.inf).all() and np.isfinite(y[2, :, 4:]).all() and np.isnan(y[3, :, 4]).all()
     m.c.close()
+
+
+@pytest.mark.parametrize("t,ct", [("bf16", "bf16"), ("f32", "i8")])
+def test_pool_past_32_bits(gpu, t, ct):
+    """A sequence whose pages lie more than 2^32 bytes (and values) into a layer, in the second layer."""
+    G, D, page, pages = 8, 128, 256, 17000
+    m = Mirror(gpu, ct, G, D, page, pages, 4, 16996 * page, layers=2, t=t)
+    assert pages * G * page * D > 1 << 32
+    m.c.append([0], [16995 * page])              # (its rows are never read)
+    m.append([1], [300])
+    assert m.c.tables([1])[0].tolist() == [[16995, 16996]]
+    m.c.copy([1], [2])
+    m.c.fork(1, [3])
+    m.rows[2], m.rows[3] = list(m.rows[1]), list(m.rows[1])
+    assert m.c.free_pages == 1
+    m.c.truncate([2], [256])
+    m.rows[2] = [tuple(x[:256] for x in kv) for kv in m.rows[2]]
+    m.append([3, 1], [2, 1])                     # 3 copies the last page
+    print(f"past 32 bits {t} over {ct}", flush=True)
+    for layer in (0, 1):
+        m.attention(16, [3, 1], [2, 1], layer=layer)
+    m.check([1, 2, 3])
+    m.c.free([0])
+    m.c.compact()
+    m.check([1, 2, 3])
+    m.append([2], [1])
+    m.attention(16, [2], [1], layer=1)
+    m.c.close()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f32"])
+def test_prompt_rows_past_32_bits(gpu, t):
+    """Key and value rows so far apart that a tile of them spans more than 2^32 bytes."""
+    H, G, D, n, nq = 4, 2, 64, 70, 3
+    es = np.dtype(R.DTYPE[t]).itemsize
+    stride = (1 << 27) // es                     # 2^27 bytes: 64 rows are 2^33
+    rng = np.random.default_rng(2)
+    q, k, v = R.rand(rng, (nq, H, D), t), R.rand(rng, (n, G, D), t), R.rand(rng, (n, G, D), t)
+    buf = gpu.empty(((n - 1) * (stride * es) + 2 * G * D * es,), np.uint8)
+    L = pf.lib()
+    for i in range(n):
+        row = np.concatenate([k[i].ravel(), v[i].ravel()])
+        gpu.check(L.pf_memcpy(gpu.h, C.c_void_p(buf.ptr + i * stride * es), row.ctypes.data_as(pf.vp), row.nbytes, 0), "row")
+    qd, o = dev(gpu, q), gpu.empty((nq, H, D), R.DTYPE[t])
+    d = pf.AttnDesc(TYPE[t], H, G, D, 1, 0, 0, 0.0, 0, stride, stride, 0)
+    a, b = (C.c_uint32 * 1)(nq), (C.c_uint32 * 1)(n)
+    print(f"rows past 32 bits {t}", flush=True)
+    gpu.check(L.pf_prompt_attention(gpu.h, C.byref(d), C.c_void_p(qd.ptr), C.c_void_p(buf.ptr),
+                                    C.c_void_p(buf.ptr + G * D * es), C.c_void_p(o.ptr), a, b, 1), "prompt")
+    y = R.from_bits(o.numpy(), t)
+    want, tol = R.attend(*(R.from_bits(x, t) for x in (q, k, v)), R.visible(nq, n), R.default_scale(D), t)
+    R.check(y, want, tol)
+    buf.free()
