@@ -299,7 +299,7 @@ def _fill(cache, k, v, lens, counts):
 
 def _rotary(case):
     import pocketforge_amd as pf
-    return pf.Rotary(case["dim"], turn=case["turn"], interleaved=case["pairs"], base=case["base"],
+    return pf.Rotary(_context(), case["dim"], turn=case["turn"], interleaved=case["pairs"], base=case["base"],
                      factor=case["factor"], low=case["low"], high=case["high"], original=case["original"],
                      magnitude=case["magnitude"])
 
@@ -315,7 +315,7 @@ def prepare(case, seed):
             at = torch.tensor(_far(case, seed), dtype=torch.int32)
         state["at"] = at.cuda()
         if own:
-            state["ctx"], state["rotary"] = _context(), _rotary(case)
+            state["rotary"] = _rotary(case)
     elif kind == "sample":
         state["logits"] = _logits(case, seed)
         state["u"] = torch.rand(case["rows"], generator=torch.Generator(device="cuda").manual_seed(seed + 2),
@@ -529,7 +529,7 @@ def run(s):
             return _write(s, s["k"], s["v"])
         return {"decode": _plain_decode, "turned": _plain_turned, "sample": _plain_sample}[kind](s)
     if kind == "rotary":
-        return s["ctx"].rotary(s["rotary"], s["x"], s["at"], out=s["out"])
+        return s["rotary"].apply(s["x"], s["at"], out=s["out"])
     if kind == "sample":
         tokens, probs = s["ctx"].sample_rows(s["logits"], s["u"], temperature=s["temperature"], top_k=s["top_k"],
                                              top_p=s["top_p"], min_p=s["min_p"], out=(s["tokens"], s["probs"]))
