@@ -183,6 +183,7 @@ size_t pf_kv_memory_usage(const pf_kv* kv);
 #define PF_TYPE_F16 1
 #define PF_TYPE_BF16 2
 #define PF_TYPE_I8 3           /* cache pages: int8 codes and an fp32 scale per row */
+#define PF_TYPE_FP4 4          /* cache pages: 4-bit floats and a power of two per 32 dims of a row */
 
 typedef struct {
     int32_t type;              /* PF_TYPE_F32, F16 or BF16: q, k, v and out */
@@ -232,7 +233,7 @@ pf_status pf_prompt_attention(pf_ctx* ctx, const pf_attn_desc* desc, const void*
  * checks its arguments before it changes anything. */
 typedef struct pf_pages pf_pages;
 typedef struct {
-    int32_t type;              /* PF_TYPE_F16, BF16 or I8 */
+    int32_t type;              /* PF_TYPE_F16, BF16, I8 or FP4 */
     uint32_t n_layers, n_kv_heads, head_dim;   /* head_dim: a multiple of 16, 16 .. 128 */
     uint32_t page_size;        /* rows of a page: 16, 32, 64, 128 or 256 */
     uint32_t n_pages, max_seqs;
@@ -251,7 +252,12 @@ pf_status pf_pages_tables(const pf_pages* p, const uint32_t* seqs, uint32_t n, i
                           int64_t* lengths);
 /* Device addresses of the pool: k and v [n_layers][n_pages][n_kv_heads]
  * [page_size][head_dim] of the cache's type; ks, vs the row scales
- * [n_layers][n_pages][n_kv_heads][page_size] of PF_TYPE_I8, else NULL. */
+ * [n_layers][n_pages][n_kv_heads][page_size] of PF_TYPE_I8, else NULL.
+ * PF_TYPE_FP4, with b = ceil(head_dim / 32) blocks of 32 dims (the last one's
+ * dims past head_dim are 0): k and v [..][page_size][b][16] bytes, a dim of an
+ * even number in a byte's low half, a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6
+ * (codes 0 .. 7; 8 .. 15 negative); ks and vs are bytes too, [..][page_size][b]:
+ * a block's values are those times 2^(byte - 127), NaN for 255. */
 pf_status pf_pages_planes(const pf_pages* p, void** k_dev, void** v_dev, float** ks_dev, float** vs_dev);
 /* Begins a pass: sequence seqs[i] (distinct) grows by rows[i] rows (0 is
  * allowed).  pf_pages_store and pf_pages_attention then work on these rows,
@@ -263,13 +269,19 @@ pf_status pf_pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t* row
 /* Writes the pass's key and value rows of one layer: [sum rows][n_kv_heads]
  * [head_dim] of `type` (F32, F16 or BF16), rounded to the cache's type, or
  * quantized by KVCache::quantize_row (a row with an infinity or a NaN reads
- * back as NaN).  Strides as in pf_attn_desc; buffers of 16 bytes. */
+ * back as NaN).  PF_TYPE_FP4: each block of 32 dims takes the smallest power of
+ * two, 2^-125 .. 2^125, that brings its largest value to 7 or less, and its
+ * values go to the nearest code (ties to even codes; over 6 to 6), which is up
+ * to a sixth more than what it was: values over 57344 stand for 65536, an
+ * infinity where fp16 rows come out of it.  A block with an infinity or a NaN
+ * reads back as NaN.  Strides as in pf_attn_desc; buffers
+ * of 16 bytes. */
 pf_status pf_pages_store(pf_pages* p, uint32_t layer, int32_t type, const void* k_dev, const void* v_dev,
                          uint32_t k_stride, uint32_t v_stride);
 /* Attention of the pass's rows over their sequences' rows in one layer (store
  * them first): q and out [sum rows][n_heads][head_dim] of desc->type.  A
  * 16-bit cache takes rows of its own type, a bf16 or int8 cache fp32 rows
- * too, an int8 cache all three.  Sums, and values that are not finite, as in
+ * too, an int8 or 4-bit cache all three.  Sums, and values that are not finite, as in
  * pf_prompt_attention, for fp32 rows as for the others.  The k and v strides are
  * not used. */
 pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* desc, uint32_t layer, const void* q_dev, void* out_dev);

@@ -22,7 +22,7 @@ FMT_Q4, FMT_Q2, FMT_Q15, FMT_Q8 = 0, 1, 2, 3
 def block_bytes(fmt):
     """Code bytes of one 32-element block in the interchange layout."""
     return {FMT_Q4: 16, FMT_Q8: 32}.get(fmt, 8)
-TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8, TYPE_FP4 = 0, 1, 2, 3, 4
 MAT_Q, MAT_K, MAT_V, MAT_O, MAT_GATE, MAT_UP, MAT_DOWN = range(7)
 
 f32p = C.POINTER(C.c_float)
@@ -746,16 +746,20 @@ class PagedCache:
     def planes(self, layer=None):
         """The pool in device memory: k and v [layers][pages][kv heads][page
         size][head_dim] and, for int8, their row scales [layers][pages][kv
-        heads][page size][1]; of one layer, without the first dimension."""
+        heads][page size][1]; for 4 bits, b = ceil(head_dim / 32) blocks a row:
+        codes [..][page size][16 b] and exponents [..][page size][b], in bytes.
+        Of one layer, without the first dimension."""
         if layer is not None and _num(layer, "layer") >= self.n_layers:
             raise PFError(f"layer {layer} of {self.n_layers}")
         p = [vp() for _ in range(4)]
         self.ctx.check(lib().pf_pages_planes(self.h, C.byref(p[0]), C.byref(p[1]), C.byref(p[2]), C.byref(p[3])),
                        "pf_pages_planes")
         rows = (self.n_pages, self.n_kv_heads, self.page_size)
+        blocks = -(-self.head_dim // 32)
+        row, scale = {TYPE_I8: ((self.head_dim, 1, "|i1"), (1, 4, "<f4")),
+                      TYPE_FP4: ((16 * blocks, 1, "|u1"), (blocks, 1, "|u1"))}.get(self.type, ((self.head_dim, 2, "<i2"), (0, 0, "")))
         out = []
-        for i, (ptr, last, size, kind) in enumerate(zip(p, 2 * [self.head_dim] + 2 * [1], 2 * [1 if self.type == TYPE_I8 else 2] + [4, 4],
-                                                        2 * ["|i1" if self.type == TYPE_I8 else "<i2"] + 2 * ["<f4"])):
+        for ptr, (last, size, kind) in zip(p, (row, row, scale, scale)):
             if ptr.value is None:
                 continue
             shape = rows + (last,)

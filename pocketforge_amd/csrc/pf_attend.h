@@ -114,6 +114,51 @@ __device__ __forceinline__ void codes8(uint32_t w0, uint32_t w1, float (&x)[8]) 
     }
 }
 
+// 4-bit pages: rows of ceil(head_dim / 32) blocks of 32 values, 16 bytes each (an
+// even dim in a byte's low half; what lies past head_dim is 0), and an exponent
+// byte e for each block, worth 2^(e - 127).  A code is a sign and 0 .5 1 1.5 2 3
+// 4 6, so a value has two significant bits and bf16 holds it exactly; gfx950
+// converts two codes an instruction, with their power of two.
+constexpr uint32_t FP4_BLOCK = 32;
+__host__ __device__ constexpr uint32_t fp4_blocks(uint32_t dim) { return (dim + FP4_BLOCK - 1) / FP4_BLOCK; }
+__device__ __forceinline__ float fp4_scale(uint32_t e) { return __builtin_bit_cast(float, e << 23); }   // (255: NaN values)
+
+// The exponent of a block whose largest value is `top` (finite): the smallest
+// power of two X that takes it to 7 or less.  What 6 holds of (6, 7] is then off
+// by no more than X, as is what the step of 2 X between 4 and 6 rounds; a limit
+// of 6 would double X, and every step, for a sixth of all blocks.  Held to 2 .. 252, where
+// every code is a normal number: blocks below 2^-126 become zeros, values above
+// 6 * 2^125 that.
+__device__ __forceinline__ uint32_t fp4_exponent(float top) {
+    const int e = (int)((__builtin_bit_cast(uint32_t, top) + 0x1FFFFFu) >> 23) - 2;
+    return (uint32_t)min(max(e, 2), 252);
+}
+// Eight floats as codes of a block of scale s (nearest, ties to even codes).
+__device__ __forceinline__ uint32_t fp4_pack(const float (&x)[8], float s) {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+    return w;
+}
+// Eight codes as floats, and as a bf16 operand; both exact.
+__device__ __forceinline__ void fp4_floats(uint32_t w, float s, float (&x)[8]) {
+    typedef float f2v __attribute__((ext_vector_type(2)));
+    const f2v r[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1),
+                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3)};
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = r[i / 2][i % 2];
+}
+__device__ __forceinline__ s8v fp4_bf16(uint32_t w, float s) {
+    u4v r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+    return __builtin_bit_cast(s8v, r);
+}
+
 // Eight values of a row of type T at p (16-byte aligned).
 template <int T>
 __device__ __forceinline__ void load8(const void* p, float (&x)[8]) {

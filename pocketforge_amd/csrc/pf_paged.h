@@ -56,7 +56,7 @@ struct PagedArgs {
     const int32_t* table;
     uint32_t table_stride;
     const void *k, *v;            // this layer's planes
-    const float *ks, *vs;
+    const void *ks, *vs;          // int8: fp32 scales; 4 bits: exponent bytes
     const void* q;
     void* out;
     uint32_t qs, os, n_heads, kv_heads, group, dim, page_shift;
@@ -67,6 +67,55 @@ struct PagedArgs {
     float* ws_ml;                 // [ws_rows][n_heads][2]
 };
 
+// Eight values of a row of one head (dims d .. d + 7, one of 16 lanes that hold
+// it; zeros past the last dim) into the row's place in a layer's plane.  Lanes of
+// a head that is not there (`live` false) take part.  int8:
+// KVCache::quantize_row's arithmetic (code = round(x * (127 / max|x|)), scale =
+// max|x| / 127).
+template <int CT>
+__device__ __forceinline__ void page_put8(const float (&x)[8], bool live, void* plane, void* scales, size_t place, uint32_t d,
+                                          uint32_t dim) {
+    const bool on = live && d < dim;
+    if constexpr (CT == PF_TYPE_I8 || CT == PF_TYPE_FP4) {
+        float amax = 0.0f;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            amax = fmaxf(amax, fabsf(x[i]));
+            odd |= !(fabsf(x[i]) < INFINITY);
+        }
+        uint32_t bad = odd;
+        // (4 lanes hold a block of 32)
+#pragma unroll
+        for (int b = 1; b < (CT == PF_TYPE_FP4 ? 4 : 16); b <<= 1) {
+            amax = fmaxf(amax, __shfl_xor(amax, b));
+            bad |= (uint32_t)__shfl_xor((int)bad, b);
+        }
+        if constexpr (CT == PF_TYPE_FP4) {
+            const uint32_t blocks = fp4_blocks(dim), e = fp4_exponent(amax);
+            if (!live || d >= blocks * FP4_BLOCK) return;
+            *(uint32_t*)((uint8_t*)plane + place * blocks * 16 + d / 2) = bad ? 0u : fp4_pack(x, fp4_scale(e));
+            if (d % FP4_BLOCK == 0) ((uint8_t*)scales)[place * blocks + d / FP4_BLOCK] = (uint8_t)(bad ? 255u : e);
+        } else {
+            // (rows below 2^-121 have an infinite 127 / max|x|: the largest float keeps their codes finite)
+            const float inv = amax == 0.0f ? 1.0f : fminf(127.0f / amax, 3.4028234663852886e38f);
+            uint32_t c[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int code = bad ? 0 : (int)__builtin_roundf(x[i] * inv);
+                c[i / 4] |= (uint32_t)(uint8_t)(int8_t)code << (8 * (i % 4));
+            }
+            if (on) {
+                u2v r = {c[0], c[1]};
+                *(u2v*)((uint8_t*)plane + place * dim + d) = r;
+                if (d == 0) ((float*)scales)[place] = bad ? NAN : amax == 0.0f ? 1.0f : amax / 127.0f;
+            }
+        }
+    } else if (on) {
+        *(s8v*)((uint8_t*)plane + (place * dim + d) * 2) = pack8<CT == PF_TYPE_BF16>(x);
+    }
+}
+
 }  // namespace pf
 
 struct PageStaging;
@@ -75,10 +124,11 @@ struct pf_pages {
     pf_ctx* ctx = nullptr;
     pf_pages_config cfg{};
     uint32_t shift = 0, per_seq = 0;               // log2(page_size), table entries of a sequence
-    size_t plane = 0, esize = 0, scales = 0;       // bytes of a plane, of a value; scales of a plane
+    uint32_t row_bytes = 0, scale_bytes = 0;       // of a row of one head, of its scales (0: none)
+    size_t plane = 0, scales = 0;                  // bytes of a layer's rows, of their scales
     size_t bytes = 0;
     void *k = nullptr, *v = nullptr;
-    float *ks = nullptr, *vs = nullptr;
+    void *ks = nullptr, *vs = nullptr;
     int32_t* table = nullptr;                      // device [max_seqs][per_seq]
     pf::PageSeq* seqs = nullptr;                   // device: the open pass
     pf::PageItem* items = nullptr;                 // device

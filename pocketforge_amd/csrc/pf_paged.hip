@@ -41,13 +41,17 @@ __host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
 __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
     // Weights over int8 rows take the rows' scales, whose range fp16 does not
-    // have, so their products with the codes are in bf16 for fp16 rows too.
-    constexpr bool I8 = CT == PF_TYPE_I8, BF = op_bf<ACT>, VB = I8 || BF;
-    constexpr int NP = op_pieces<ACT>, PP = weight_pieces<ACT>, C = DP / 32, DT = DP / 16;
+    // have, so their products with the codes are in bf16 for fp16 rows too.  4-bit
+    // values are bf16 (with their scales: fp16 has not their range either), and
+    // fp16 query rows two bf16 pieces beside them, which hold all of a value.
+    constexpr bool I8 = CT == PF_TYPE_I8, F4 = CT == PF_TYPE_FP4, BF = F4 || op_bf<ACT>, VB = I8 || BF;
+    constexpr int NP = F4 && ACT == PF_TYPE_F16 ? 2 : op_pieces<ACT>, PP = weight_pieces<ACT>, C = DP / 32, DT = DP / 16;
     constexpr int STR = DP + 16;                 // LDS row stride in values
-    constexpr int VCH = I8 ? DP / 16 : DP / 8;   // 16-byte chunks of a V row
+    constexpr int CB = F4 && DP == 64 ? 8 : 16;  // bytes of a chunk: 4 bits, a quarter of a row
+    constexpr int VCH = F4 ? 4 : I8 ? DP / 16 : DP / 8;   // chunks of a V row
     constexpr int VL = 32 * VCH / 64;            // V loads of a lane
-    constexpr int KL = I8 ? DP / 64 : C;         // K loads of a lane per 16 keys
+    constexpr int KL = F4 ? 1 : I8 ? DP / 64 : C;         // K loads of a lane per 16 keys
+    typedef std::conditional_t<CB == 8, u2v, u4v> chunk;
     __shared__ __align__(16) short sv[W][32][STR];
     __shared__ float s_ml[W][16][2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
@@ -96,8 +100,8 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                             ((size_t)(it.q0 + (uint32_t)j) * a.qs + (size_t)(head0 + (uint32_t)h) * a.dim) * act_size<ACT>;
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            // the dims of K's operand: int8 rows give a lane 16 codes at a time
-            const int d = I8 ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
+            // the dims of K's operand: int8 rows give a lane 16 codes at a time, 4 bits a quarter of a row
+            const int d = F4 ? g * (DP / 4) + c * 8 : I8 ? (c >> 1) * 64 + g * 16 + (c & 1) * 8 : c * 32 + g * 8;
             float x[8] = {};
             if (EXACT || d < (int)a.dim) load8<ACT>(qp + (size_t)d * act_size<ACT>, x);
             s8v t[NP];
@@ -118,13 +122,16 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
         for (int t = 0; t < DT; t++) o[n][t] = (f4v)0.0f;
     }
 
-    const uint32_t row_bytes = (EXACT ? DP : a.dim) * (I8 ? 1 : 2);
-    const uint32_t k_off = (uint32_t)col * row_bytes + (uint32_t)g * 16;
-    const uint32_t v_row = (uint32_t)lane / VCH, v_off = v_row * row_bytes + (uint32_t)lane % VCH * 16;
+    const uint32_t blocks = fp4_blocks(EXACT ? DP : a.dim);
+    const uint32_t row_bytes = F4 ? blocks * 16 : (EXACT ? DP : a.dim) * (I8 ? 1 : 2);
+    const uint32_t k_off = (uint32_t)col * row_bytes + (uint32_t)g * CB;
+    const uint32_t v_row = (uint32_t)lane / VCH, v_off = v_row * row_bytes + (uint32_t)lane % VCH * CB;
     constexpr int VR = 64 / VCH;                 // V rows of one load of the wave
+    const uint32_t k_block = (uint32_t)g * CB / 16, v_block = (uint32_t)lane % VCH * CB / 16;
 
-    u4v kr[2][KL], vr[VL];
-    f4v ksc[2], vsc[2];
+    chunk kr[2][KL], vr[VL];
+    f4v ksc[2], vsc[2];                          // int8
+    uint32_t kex[2], vex[VL];                    // 4 bits: exponents
     auto load = [&](int n) {                     // this wave's n-th tile
         const int pos0 = pos_of(tile_of(n));
 #pragma unroll
@@ -134,13 +141,17 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
             const uint8_t *kp = (const uint8_t*)a.k + row0 * row_bytes, *vp = (const uint8_t*)a.v + row0 * row_bytes;
 #pragma unroll
             for (int c = 0; c < KL; c++)
-                kr[s][c] = (EXACT || c * 64 + g * 16 < (int)row_bytes) ? *(const u4v*)(kp + k_off + c * 64) : (u4v)0u;
+                kr[s][c] = (EXACT || c * 64 + g * CB < (int)row_bytes) ? *(const chunk*)(kp + k_off + c * 64) : (chunk)0u;
 #pragma unroll
             for (int i = 0; i < VL / 2; i++)
-                vr[s * (VL / 2) + i] = (EXACT || lane % VCH * 16 < (int)row_bytes) ? *(const u4v*)(vp + v_off + i * VR * row_bytes) : (u4v)0u;
+                vr[s * (VL / 2) + i] = (EXACT || lane % VCH * CB < (int)row_bytes) ? *(const chunk*)(vp + v_off + i * VR * row_bytes) : (chunk)0u;
             if constexpr (I8) {
-                ksc[s] = *(const f4v*)((const uint8_t*)(a.ks + row0) + 16 * g);
-                vsc[s] = *(const f4v*)((const uint8_t*)(a.vs + row0) + 16 * g);
+                ksc[s] = *(const f4v*)((const uint8_t*)((const float*)a.ks + row0) + 16 * g);
+                vsc[s] = *(const f4v*)((const uint8_t*)((const float*)a.vs + row0) + 16 * g);
+            }
+            if constexpr (F4) {
+                kex[s] = EXACT || k_block < blocks ? ((const uint8_t*)a.ks)[(row0 + (uint32_t)col) * blocks + k_block] : 0u;
+                vex[s] = EXACT || v_block < blocks ? ((const uint8_t*)a.vs)[(row0 + v_row) * blocks + v_block] : 0u;
             }
         }
     };
@@ -151,7 +162,7 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
         const int pos0 = pos_of(tile_of(n_tile));
         constexpr bool MASKED = decltype(masked)::value;
         short* sw = &sv[wave][0][0];
-        auto place = [&](int i) { return sw + (i * VR + v_row) * STR + (lane % VCH) * (I8 ? 16 : 8); };
+        auto place = [&](int i) { return sw + (i * VR + v_row) * STR + (lane % VCH) * (F4 ? 2 * CB : I8 ? 16 : 8); };
         f4v kscale[2], vscale[2];
         s8v kf[2][C];
 #pragma unroll
@@ -165,6 +176,9 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                     codes8(kr[s][c >> 1][(c & 1) * 2], kr[s][c >> 1][(c & 1) * 2 + 1], x);
                     kf[s][c] = pack8<BF>(x);
                 }
+            } else if constexpr (F4) {
+#pragma unroll
+                for (int c = 0; c < C; c++) kf[s][c] = fp4_bf16(kr[s][0][c], fp4_scale(kex[s]));
             } else {
 #pragma unroll
                 for (int c = 0; c < C; c++) kf[s][c] = __builtin_bit_cast(s8v, kr[s][c]);
@@ -186,14 +200,20 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
         float z = 0.0f;
 #pragma unroll
         for (int i = 0; i < VL; i++) {
-            u4v w = vr[i];
-            if constexpr (MASKED) w &= (uint32_t)-(int)((any >> (i * VR + v_row)) & 1u);
+            chunk w = vr[i];
+            const uint32_t on = MASKED ? (uint32_t)-(int)((any >> (i * VR + v_row)) & 1u) : ~0u;
+            if constexpr (MASKED) w &= on;
             if constexpr (I8) {
                 float x[8];
                 codes8(w[0], w[1], x);
                 *(s8v*)place(i) = pack8<VB>(x);
                 codes8(w[2], w[3], x);
                 *(s8v*)(place(i) + 8) = pack8<VB>(x);
+            } else if constexpr (F4) {
+                const uint32_t e = MASKED ? vex[i] & on : vex[i];
+                if (e == 255) z = NAN;
+#pragma unroll
+                for (int c = 0; c < CB / 4; c++) *(s8v*)(place(i) + 8 * c) = fp4_bf16(w[c], fp4_scale(e));
             } else {
                 z = sum8<BF>(__builtin_bit_cast(s8v, w), z, 0.0f);
                 *(u4v*)place(i) = w;
@@ -259,7 +279,9 @@ __global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn
                             }
                     }
                 __builtin_amdgcn_wave_barrier();
-                for (int i = 0; i < VL; i++) *(s8v*)place(i) = finite_or_zero<BF>(*(const s8v*)place(i));
+                for (int i = 0; i < VL; i++)
+                    for (int c = 0; c < (F4 ? CB / 4 : 1); c++)
+                        *(s8v*)(place(i) + 8 * c) = finite_or_zero<BF>(*(const s8v*)(place(i) + 8 * c));
                 __builtin_amdgcn_wave_barrier();
             }
         }
@@ -562,7 +584,7 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
     if (d->n_kv_heads != p->cfg.n_kv_heads || d->head_dim != p->cfg.head_dim)
         return fail(c, PF_ERR_ARG, "pages: n_kv_heads and head_dim are the cache's");
     const int32_t ct = p->cfg.type;
-    if (ct != PF_TYPE_I8 && ct != d->type && !(ct == PF_TYPE_BF16 && d->type == PF_TYPE_F32))
+    if (ct != PF_TYPE_I8 && ct != PF_TYPE_FP4 && ct != d->type && !(ct == PF_TYPE_BF16 && d->type == PF_TYPE_F32))
         return fail(c, PF_ERR_UNSUPPORTED, "pages: rows of this type over a cache of that type");
     if (!p->open) return fail(c, PF_ERR_STATE, "pages: no open pass (pf_pages_append begins one)");
     if (!p->pass_rows) return PF_OK;
@@ -584,7 +606,7 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
     }
     a.items = p->items; a.table = p->table; a.table_stride = p->per_seq;
     a.k = (const uint8_t*)p->k + layer * p->plane; a.v = (const uint8_t*)p->v + layer * p->plane;
-    if (p->ks) { a.ks = p->ks + layer * p->scales; a.vs = p->vs + layer * p->scales; }
+    a.ks = (const uint8_t*)p->ks + layer * p->scales; a.vs = (const uint8_t*)p->vs + layer * p->scales;
     a.q = q; a.out = out; a.qs = s.qs; a.os = s.os;
     a.n_heads = d->n_heads; a.kv_heads = d->n_kv_heads; a.group = d->n_heads / d->n_kv_heads; a.dim = d->head_dim;
     a.page_shift = p->shift;
@@ -598,6 +620,10 @@ extern "C" pf_status pf_pages_attention(pf_pages* p, const pf_attn_desc* d, uint
         if (d->type == PF_TYPE_F32) PF_PAGED(PF_TYPE_F32, PF_TYPE_I8);
         else if (d->type == PF_TYPE_F16) PF_PAGED(PF_TYPE_F16, PF_TYPE_I8);
         else PF_PAGED(PF_TYPE_BF16, PF_TYPE_I8);
+    } else if (ct == PF_TYPE_FP4) {
+        if (d->type == PF_TYPE_F32) PF_PAGED(PF_TYPE_F32, PF_TYPE_FP4);
+        else if (d->type == PF_TYPE_F16) PF_PAGED(PF_TYPE_F16, PF_TYPE_FP4);
+        else PF_PAGED(PF_TYPE_BF16, PF_TYPE_FP4);
     } else if (ct == PF_TYPE_F16) PF_PAGED(PF_TYPE_F16, PF_TYPE_F16);
     else if (d->type == PF_TYPE_F32) PF_PAGED(PF_TYPE_F32, PF_TYPE_BF16);
     else PF_PAGED(PF_TYPE_BF16, PF_TYPE_BF16);

@@ -59,14 +59,12 @@ struct StoreArgs {
     const PageSeq* seqs;
     const int32_t* table;
     const void *k, *v;
-    void *pk, *pv;
-    float *ks, *vs;
+    void *pk, *pv, *ks, *vs;
     uint32_t n_seq, rows, uniform, per_seq, shift, kv_heads, dim, kstride, vstride;
 };
 
 // New rows into their pages.  16 lanes hold a row of one head, 8 values each; a
-// wave has 4 heads of a token, K and V in turn.  int8: KVCache::quantize_row's
-// arithmetic (code = round(x * (127 / max|x|)), scale = max|x| / 127).  Bound by
+// wave has 4 heads of a token, K and V in turn.  Bound by
 // its bytes where there are many: 4717 fp32 rows of 16 heads of 128 to int8, 97
 // MB in 19 us, 5.1 TB/s; a decode step's 64 bf16 rows 3 us, a launch's latency.
 template <int T, int CT>
@@ -80,7 +78,7 @@ __global__ __launch_bounds__(256) void k_pages_store(StoreArgs a) {
     const PageSeq q = a.seqs[s];
     const uint32_t pos = q.len - q.rows + (row - q.q0);
     const uint32_t page = (uint32_t)a.table[(size_t)q.slot * a.per_seq + (pos >> a.shift)];
-    const bool on = head < a.kv_heads && d < a.dim;
+    const bool live = head < a.kv_heads, on = live && d < a.dim;
     const size_t place = (((size_t)page * a.kv_heads + head) << a.shift) + (pos & ((1u << a.shift) - 1));
 #pragma unroll
     for (int w = 0; w < 2; w++) {
@@ -88,45 +86,14 @@ __global__ __launch_bounds__(256) void k_pages_store(StoreArgs a) {
         const uint32_t stride = w ? a.vstride : a.kstride;
         float x[8] = {};
         if (on) load8<T>((const uint8_t*)src + ((size_t)row * stride + (size_t)head * a.dim + d) * act_size<T>, x);
-        uint8_t* dst = (uint8_t*)(w ? a.pv : a.pk);
-        if constexpr (CT == PF_TYPE_I8) {
-            float amax = 0.0f;
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                amax = fmaxf(amax, fabsf(x[i]));
-                odd |= !(fabsf(x[i]) < INFINITY);
-            }
-            uint32_t bad = odd;
-#pragma unroll
-            for (int b = 1; b < 16; b <<= 1) {
-                amax = fmaxf(amax, __shfl_xor(amax, b));
-                bad |= (uint32_t)__shfl_xor((int)bad, b);
-            }
-            // (rows below 2^-121 have an infinite 127 / max|x|: the largest float keeps their codes finite)
-            const float inv = amax == 0.0f ? 1.0f : fminf(127.0f / amax, 3.4028234663852886e38f);
-            uint32_t c[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int code = bad ? 0 : (int)__builtin_roundf(x[i] * inv);
-                c[i / 4] |= (uint32_t)(uint8_t)(int8_t)code << (8 * (i % 4));
-            }
-            if (on) {
-                u2v r = {c[0], c[1]};
-                *(u2v*)(dst + place * a.dim + d) = r;
-                if (d == 0) (w ? a.vs : a.ks)[place] = bad ? NAN : amax == 0.0f ? 1.0f : amax / 127.0f;
-            }
-        } else if (on) {
-            *(s8v*)(dst + (place * a.dim + d) * 2) = pack8<CT == PF_TYPE_BF16>(x);
-        }
+        page_put8<CT>(x, live, w ? a.pv : a.pk, w ? a.vs : a.ks, place, d, a.dim);
     }
 }
 
 constexpr int GATHER_SEQS = 64;
 struct GatherArgs {
     const int32_t* table;
-    const void *pk, *pv;
-    const float *ks, *vs;
+    const void *pk, *pv, *ks, *vs;
     void *k, *v;
     uint32_t n_seq, rows, per_seq, shift, kv_heads, dim, kstride, vstride, row0;
     uint32_t first[GATHER_SEQS], slot[GATHER_SEQS];   // first packed row, sequence
@@ -152,10 +119,14 @@ __global__ __launch_bounds__(256) void k_pages_gather(GatherArgs a) {
         float x[8];
         if constexpr (CT == PF_TYPE_I8) {
             const u2v c = *(const u2v*)(src + place * a.dim + d);
-            const float sc = (w ? a.vs : a.ks)[place];
+            const float sc = ((const float*)(w ? a.vs : a.ks))[place];
             codes8(c[0], c[1], x);
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] *= sc;
+        } else if constexpr (CT == PF_TYPE_FP4) {
+            const uint32_t blocks = fp4_blocks(a.dim);
+            const uint32_t c = *(const uint32_t*)(src + place * blocks * 16 + d / 2);
+            fp4_floats(c, fp4_scale(((const uint8_t*)(w ? a.vs : a.ks))[place * blocks + d / FP4_BLOCK]), x);
         } else {
             load8<CT>(src + (place * a.dim + d) * 2, x);
         }
@@ -171,15 +142,14 @@ __global__ __launch_bounds__(256) void k_pages_gather(GatherArgs a) {
     }
 }
 
-// Copies pages: (from, to, rows) of every layer and head, K and V and the int8
+// Copies pages: (from, to, rows) of every layer and head, K and V and their
 // scales.  One workgroup takes one (copy, layer) and a share of its heads.
 // Outputs pass the caches: 12 sequences of 24 pages, 24 layers, write 905 MB in
 // 176 us, 5.1 TB/s (their one source stays in the caches), 227 us otherwise.
 struct MoveArgs {
-    uint8_t *k, *v;
-    float *ks, *vs;
-    uint32_t kv_heads, page_size, row_bytes;
-    size_t plane, scales;         // of one layer
+    uint8_t *k, *v, *ks, *vs;
+    uint32_t kv_heads, page_size, row_bytes, scale_bytes;
+    size_t plane, scales;         // bytes of one layer's
 };
 __device__ __forceinline__ void move_page(const MoveArgs& a, uint32_t src, uint32_t dst, uint32_t rows, uint32_t layer,
                                           uint32_t h0, uint32_t dh) {
@@ -202,9 +172,12 @@ __device__ __forceinline__ void move_page(const MoveArgs& a, uint32_t src, uint3
             }
             for (; i < n16; i += 256) d[i] = s[i];
             if (a.ks) {
-                float* sc = (w ? a.vs : a.ks) + layer * a.scales + (size_t)h * a.page_size;
-                const size_t per = (size_t)a.kv_heads * a.page_size;
-                for (uint32_t r = threadIdx.x; r < rows; r += 256) sc[dst * per + r] = sc[src * per + r];
+                // whole words (a head's scales in a page are words, whatever the rows' are)
+                const size_t head_scales = (size_t)a.page_size * a.scale_bytes, per = head_scales * a.kv_heads;
+                uint8_t* sc = (w ? a.vs : a.ks) + layer * a.scales + h * head_scales;
+                const uint32_t* s = (const uint32_t*)(sc + src * per);
+                uint32_t* d = (uint32_t*)(sc + dst * per);
+                for (uint32_t r = threadIdx.x; r < (rows * a.scale_bytes + 3) / 4; r += 256) d[r] = s[r];
             }
         }
     }
@@ -265,8 +238,8 @@ static pf_status stage_send(pf_pages* p, const uint32_t* msg, uint32_t words, vo
 static MoveArgs move_args(const pf_pages* p) {
     const pf_pages_config& g = p->cfg;
     MoveArgs a{};
-    a.k = (uint8_t*)p->k; a.v = (uint8_t*)p->v; a.ks = p->ks; a.vs = p->vs;
-    a.kv_heads = g.n_kv_heads; a.page_size = g.page_size; a.row_bytes = (uint32_t)(g.head_dim * p->esize);
+    a.k = (uint8_t*)p->k; a.v = (uint8_t*)p->v; a.ks = (uint8_t*)p->ks; a.vs = (uint8_t*)p->vs;
+    a.kv_heads = g.n_kv_heads; a.page_size = g.page_size; a.row_bytes = p->row_bytes; a.scale_bytes = p->scale_bytes;
     a.plane = p->plane; a.scales = p->scales;
     return a;
 }
@@ -414,7 +387,9 @@ static pf_status all_empty(pf_pages* p, const uint32_t* seqs, uint32_t n) {
 }
 static void end_pass(pf_pages* p) { p->open = false; }
 
-static bool cache_type(int32_t t) { return t == PF_TYPE_F16 || t == PF_TYPE_BF16 || t == PF_TYPE_I8; }
+static bool cache_type(int32_t t) {
+    return t == PF_TYPE_F16 || t == PF_TYPE_BF16 || t == PF_TYPE_I8 || t == PF_TYPE_FP4;
+}
 
 static pf_status pages_alloc(pf_pages* p) {
     pf_ctx* c = p->ctx;
@@ -430,14 +405,14 @@ static pf_status pages_alloc(pf_pages* p) {
     const size_t pool = p->plane * g.n_layers, sc = p->scales * g.n_layers;
     pf_status s = dalloc(c, &p->k, pool);
     if (!s) s = dalloc(c, &p->v, pool);
-    if (!s && g.type == PF_TYPE_I8) s = dalloc_t(c, &p->ks, sc);
-    if (!s && g.type == PF_TYPE_I8) s = dalloc_t(c, &p->vs, sc);
+    if (!s && sc) s = dalloc(c, &p->ks, sc);
+    if (!s && sc) s = dalloc(c, &p->vs, sc);
     if (!s) s = dalloc_t(c, &p->table, (size_t)g.max_seqs * p->per_seq);
     if (!s) s = dalloc_t(c, &p->seqs, g.max_seqs);
     if (!s) s = dalloc_t(c, &p->items, p->items_cap);
     if (!s) s = dalloc_t(c, &p->pairs, 3 * MOVE_MOST);
     if (s) return s;
-    p->bytes = 2 * pool + (g.type == PF_TYPE_I8 ? 8 * sc : 0) + (size_t)g.max_seqs * p->per_seq * 4;
+    p->bytes = 2 * pool + 2 * sc + (size_t)g.max_seqs * p->per_seq * 4;
     PF_HIP(c, hipHostMalloc((void**)&p->staging->mem, STAGE_BYTES * STAGE_SLOTS, hipHostMallocDefault));
     for (hipEvent_t& e : p->staging->done) PF_HIP(c, hipEventCreateWithFlags(&e, hipEventDisableTiming));
     return PF_OK;
@@ -452,8 +427,8 @@ extern "C" void pf_pages_destroy(pf_pages* p) {
     const size_t pool = p->plane * g.n_layers, sc = p->scales * g.n_layers;
     dfree(c, p->k, pool);
     dfree(c, p->v, pool);
-    dfree(c, p->ks, sc * 4);
-    dfree(c, p->vs, sc * 4);
+    dfree(c, p->ks, sc);
+    dfree(c, p->vs, sc);
     dfree(c, p->table, (size_t)g.max_seqs * p->per_seq * 4);
     dfree(c, p->seqs, g.max_seqs * sizeof(PageSeq));
     dfree(c, p->items, p->items_cap * sizeof(PageItem));
@@ -470,7 +445,7 @@ extern "C" void pf_pages_destroy(pf_pages* p) {
 extern "C" pf_status pf_pages_create(pf_ctx* c, const pf_pages_config* g, pf_pages** out) {
     if (!c || !g || !out) return PF_ERR_ARG;
     *out = nullptr;
-    if (!cache_type(g->type)) return fail(c, PF_ERR_ARG, "pages: type is PF_TYPE_F16, BF16 or I8");
+    if (!cache_type(g->type)) return fail(c, PF_ERR_ARG, "pages: type is PF_TYPE_F16, BF16, I8 or FP4");
     if (!g->n_layers || !g->n_kv_heads || !g->n_pages || !g->max_seqs || !g->max_context)
         return fail(c, PF_ERR_ARG, "pages: a size is 0");
     if (g->n_layers > 65535 || g->n_kv_heads > 65535) return fail(c, PF_ERR_UNSUPPORTED, "pages: over 65535 layers or heads");
@@ -483,8 +458,10 @@ extern "C" pf_status pf_pages_create(pf_ctx* c, const pf_pages_config* g, pf_pag
     const uint32_t per_seq = (g->max_context + g->page_size - 1) / g->page_size;
     if ((uint64_t)per_seq * g->max_seqs > 0xFFFFFFFFull)
         return fail(c, PF_ERR_UNSUPPORTED, "pages: max_seqs times the pages of max_context is 2^32 at most");
-    const size_t scales = (size_t)g->n_pages * g->n_kv_heads * g->page_size, esize = g->type == PF_TYPE_I8 ? 1 : 2;
-    const size_t plane = scales * g->head_dim * esize;           // (below 2^63 within the limits above)
+    const bool fp4 = g->type == PF_TYPE_FP4, i8 = g->type == PF_TYPE_I8;
+    const uint32_t row_bytes = fp4 ? 16 * fp4_blocks(g->head_dim) : g->head_dim * (i8 ? 1 : 2);
+    const size_t rows = (size_t)g->n_pages * g->n_kv_heads * g->page_size;
+    const size_t plane = rows * row_bytes;                       // (below 2^63 within the limits above)
     if (plane > (SIZE_MAX >> 2) / g->n_layers) return fail(c, PF_ERR_UNSUPPORTED, "pages: a pool of over 2^62 bytes");
     DeviceScope on(c);
     pf_pages* p = new (std::nothrow) pf_pages();
@@ -493,8 +470,9 @@ extern "C" pf_status pf_pages_create(pf_ctx* c, const pf_pages_config* g, pf_pag
     p->cfg = *g;
     p->shift = (uint32_t)__builtin_ctz(g->page_size);
     p->per_seq = per_seq;
-    p->esize = esize;
-    p->scales = scales;
+    p->row_bytes = row_bytes;
+    p->scale_bytes = fp4 ? fp4_blocks(g->head_dim) : i8 ? 4 : 0;
+    p->scales = rows * p->scale_bytes;
     p->plane = plane;
     p->items_cap = (size_t)2 * g->max_seqs + PG_MOST_ITEMS;
     if (pf_status s = no_throw(c, [&] { return pages_alloc(p); })) {
@@ -530,7 +508,7 @@ extern "C" pf_status pf_pages_tables(const pf_pages* p, const uint32_t* seqs, ui
 
 extern "C" pf_status pf_pages_planes(const pf_pages* p, void** k, void** v, float** ks, float** vs) {
     if (!p || !k || !v || !ks || !vs) return PF_ERR_ARG;
-    *k = p->k; *v = p->v; *ks = p->ks; *vs = p->vs;
+    *k = p->k; *v = p->v; *ks = (float*)p->ks; *vs = (float*)p->vs;
     return PF_OK;
 }
 
@@ -660,11 +638,12 @@ extern "C" pf_status pf_pages_store(pf_pages* p, uint32_t layer, int32_t type, c
     StoreArgs a{};
     a.seqs = p->seqs; a.table = p->table; a.k = k; a.v = v;
     a.pk = (uint8_t*)p->k + layer * p->plane; a.pv = (uint8_t*)p->v + layer * p->plane;
-    if (p->ks) { a.ks = p->ks + layer * p->scales; a.vs = p->vs + layer * p->scales; }
+    a.ks = (uint8_t*)p->ks + layer * p->scales; a.vs = (uint8_t*)p->vs + layer * p->scales;
     a.n_seq = (uint32_t)p->pass.size(); a.rows = p->pass_rows; a.uniform = p->uniform; a.per_seq = p->per_seq;
     a.shift = p->shift; a.kv_heads = p->cfg.n_kv_heads; a.dim = p->cfg.head_dim; a.kstride = kst; a.vstride = vst;
     const uint32_t blocks = (uint32_t)((waves + 3) / 4);
-    if (p->cfg.type == PF_TYPE_I8) store_type<PF_TYPE_I8>(c->stream, type, blocks, a);
+    if (p->cfg.type == PF_TYPE_FP4) store_type<PF_TYPE_FP4>(c->stream, type, blocks, a);
+    else if (p->cfg.type == PF_TYPE_I8) store_type<PF_TYPE_I8>(c->stream, type, blocks, a);
     else if (p->cfg.type == PF_TYPE_F16) store_type<PF_TYPE_F16>(c->stream, type, blocks, a);
     else store_type<PF_TYPE_BF16>(c->stream, type, blocks, a);
     PF_LAUNCHED(c);
@@ -698,7 +677,7 @@ extern "C" pf_status pf_pages_gather(pf_pages* p, uint32_t layer, const uint32_t
     GatherArgs a{};
     a.table = p->table; a.k = k; a.v = v;
     a.pk = (const uint8_t*)p->k + layer * p->plane; a.pv = (const uint8_t*)p->v + layer * p->plane;
-    if (p->ks) { a.ks = p->ks + layer * p->scales; a.vs = p->vs + layer * p->scales; }
+    a.ks = (const uint8_t*)p->ks + layer * p->scales; a.vs = (const uint8_t*)p->vs + layer * p->scales;
     a.per_seq = p->per_seq; a.shift = p->shift; a.kv_heads = p->cfg.n_kv_heads; a.dim = p->cfg.head_dim;
     a.kstride = kst; a.vstride = vst;
     uint32_t row0 = 0;
@@ -714,7 +693,8 @@ extern "C" pf_status pf_pages_gather(pf_pages* p, uint32_t layer, const uint32_t
         if (!a.rows) break;
         row0 += a.rows;
         const uint32_t blocks = (uint32_t)(((uint64_t)a.rows * heads4 + 3) / 4);
-        if (p->cfg.type == PF_TYPE_I8) gather_type<PF_TYPE_I8>(c->stream, type, blocks, a);
+        if (p->cfg.type == PF_TYPE_FP4) gather_type<PF_TYPE_FP4>(c->stream, type, blocks, a);
+        else if (p->cfg.type == PF_TYPE_I8) gather_type<PF_TYPE_I8>(c->stream, type, blocks, a);
         else if (p->cfg.type == PF_TYPE_F16) gather_type<PF_TYPE_F16>(c->stream, type, blocks, a);
         else gather_type<PF_TYPE_BF16>(c->stream, type, blocks, a);
         PF_LAUNCHED(c);
