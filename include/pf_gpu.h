@@ -219,6 +219,40 @@ pf_status pf_prompt_attention(pf_ctx* ctx, const pf_attn_desc* desc, const void*
                               const void* v_dev, void* out_dev, const uint32_t* q_lens, const uint32_t* k_lens,
                               uint32_t n_seq);
 
+/* ---------------------------------------------------- rotary positions
+ * (new) The engine turns q and k inside its QKV product (src/engine.cpp:
+ * 656-682, 728-750); these turn rows that the caller holds.  Pair i of a head,
+ * i < turn / 2, is dims 2i, 2i + 1 (interleaved, as the engine's) or i, i +
+ * turn / 2; at position p it becomes (a c - b s, a s + b c) with c, s =
+ * magnitude * cos, sin of p f_i and f_i = base^(-2i / turn).  Dims past `turn`
+ * stay.  Longer contexts than a model's own:
+ *   low = high = 0: f_i / factor (every position divided by factor);
+ *   low < high: with t = original f_i / (2 pi) turns over the original context
+ *     and g = (t - low) / (high - low) held to 0 .. 1, f_i (g + (1 - g) /
+ *     factor): fast pairs stay, slow ones are stretched.
+ * Angles are formed in 64 bits (more where positions are far), products in
+ * fp32. */
+typedef struct pf_rotary pf_rotary;
+typedef struct {
+    uint32_t head_dim;         /* a multiple of 16, 16 .. 128 */
+    uint32_t turn;             /* a multiple of 8 up to head_dim; 0: head_dim */
+    int32_t interleaved;
+    float base;                /* 0: 5e6, the engine's; above 1 */
+    float factor;              /* 0: 1; positive */
+    float low, high;
+    uint32_t original;         /* rows of the original context, where low < high */
+    float magnitude;           /* 0: 1; positive */
+} pf_rotary_desc;
+
+pf_status pf_rotary_create(pf_ctx* ctx, const pf_rotary_desc* desc, pf_rotary** out);
+void pf_rotary_destroy(pf_rotary* r);
+/* x and out [rows][n_heads][head_dim] of `type` (F32, F16 or BF16), row i at
+ * positions_dev[i] (any 32-bit number).  Strides as in pf_attn_desc; buffers
+ * of 16 bytes.  out may be x, with its stride, or columns of the same rows
+ * beside it.  q and k that lie side by side are one call. */
+pf_status pf_rotary_apply(const pf_rotary* r, int32_t type, uint32_t n_heads, const void* x_dev, void* out_dev,
+                          const int32_t* positions_dev, uint32_t rows, uint32_t x_stride, uint32_t o_stride);
+
 /* ----------------------------------------------------- paged KV cache
  * (new) No counterpart in the reference, whose KVCache holds one sequence
  * (include/forge/kv_cache.hpp:33-56).  A pool of pages of page_size rows,
@@ -278,6 +312,15 @@ pf_status pf_pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t* row
  * of 16 bytes. */
 pf_status pf_pages_store(pf_pages* p, uint32_t layer, int32_t type, const void* k_dev, const void* v_dev,
                          uint32_t k_stride, uint32_t v_stride);
+/* pf_pages_store of a pass before its rotary positions: the key rows turned at
+ * their positions in their sequences (0 for a sequence's first) and stored, the
+ * values stored as they are, and the query rows q [sum rows][n_heads][head_dim]
+ * turned into q_out, in one launch.  A turned row is rounded once to the
+ * cache's type; for int8 and 4-bit pages its fp32 value is quantized.  r's
+ * head_dim is the cache's; q_out may be q. */
+pf_status pf_pages_store_rotary(pf_pages* p, uint32_t layer, const pf_rotary* r, int32_t type, uint32_t n_heads,
+                                const void* q_dev, const void* k_dev, const void* v_dev, void* q_out_dev,
+                                uint32_t q_stride, uint32_t k_stride, uint32_t v_stride, uint32_t o_stride);
 /* Attention of the pass's rows over their sequences' rows in one layer (store
  * them first): q and out [sum rows][n_heads][head_dim] of desc->type.  A
  * 16-bit cache takes rows of its own type, a bf16 or int8 cache fp32 rows
@@ -302,6 +345,41 @@ pf_status pf_pages_free(pf_pages* p, const uint32_t* seqs, uint32_t n);
 /* Moves used pages so that they are numbers 0 .. used - 1; *moved (may be
  * NULL) is how many moved. */
 pf_status pf_pages_compact(pf_pages* p, uint32_t* moved);
+
+/* ---------------------------------------------- tokens from rows of logits
+ * (new) Engine::sample (src/engine.cpp:881-1003) takes one row, and of top-p
+ * and top-k one; this takes a batch's rows where the unembedding left them,
+ * each with settings of its own, and random numbers that the caller draws.
+ * With the tokens of a row in order of their logits l (equal ones by number)
+ * and w = exp((l - l_max) / temperature): the first top_k stay; of these, as
+ * many of the first as it takes to reach top_p of their weight; of these,
+ * those with w >= min_p.  The token is the first whose cumulative weight
+ * exceeds u times that of all that stay, u in [0, 1).
+ * temperature 0 or below (or NaN): the largest logit's first token.  top_k
+ * below 1 or n_vocab and above, top_p 1 and above (or NaN), min_p 0 and below
+ * (or NaN): off; top_p 0 and below: the first token alone; min_p above 1: 1.
+ * A logit of -infinity or NaN is masked; of infinities the infinities alone
+ * weigh.  A row without any other gives -1.
+ * Weights are held in steps of 2^-43, and their sums are exact: the same
+ * inputs give the same tokens. */
+typedef struct {
+    int32_t type;              /* logits: PF_TYPE_F32, F16 or BF16 */
+    uint32_t n_vocab;          /* 1 .. 2^20 */
+    uint32_t stride;           /* logits from one row to the next; 0: n_vocab */
+    float temperature;         /* of every row, where the pointers below are NULL */
+    uint32_t top_k;
+    float top_p, min_p;
+    const float* temperature_dev;   /* [rows], or NULL */
+    const int32_t* top_k_dev;
+    const float* top_p_dev;
+    const float* min_p_dev;
+} pf_sample_desc;
+
+/* tokens [rows]; probs [rows] (may be NULL): the token's share of what stayed
+ * (1 where the temperature is 0, 0 for a row without tokens).  Rows may start
+ * anywhere that is a multiple of their type's size. */
+pf_status pf_sample_rows(pf_ctx* ctx, const pf_sample_desc* desc, const void* logits_dev, const float* u_dev,
+                         uint32_t rows, int32_t* tokens_dev, float* probs_dev);
 
 /* --------------------------------------------------------------- model */
 typedef struct {

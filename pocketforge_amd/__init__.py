@@ -73,6 +73,18 @@ class AttnDesc(C.Structure):
                 ("o_stride", C.c_uint32)]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [("head_dim", C.c_uint32), ("turn", C.c_uint32), ("interleaved", C.c_int32), ("base", C.c_float),
+                ("factor", C.c_float), ("low", C.c_float), ("high", C.c_float), ("original", C.c_uint32),
+                ("magnitude", C.c_float)]
+
+
+class SampleDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_vocab", C.c_uint32), ("stride", C.c_uint32), ("temperature", C.c_float),
+                ("top_k", C.c_uint32), ("top_p", C.c_float), ("min_p", C.c_float), ("temperature_dev", vp),
+                ("top_k_dev", vp), ("top_p_dev", vp), ("min_p_dev", vp)]
+
+
 class PagesConfig(C.Structure):
     _fields_ = [("type", C.c_int32)] + [(n, C.c_uint32) for n in (
         "n_layers", "n_kv_heads", "head_dim", "page_size", "n_pages", "max_seqs", "max_context")]
@@ -158,6 +170,10 @@ SYMBOLS = {
     "pf_engine_gemv_by_size": (C.c_int32, [vp, C.c_uint32, C.POINTER(C.c_double), u32p, C.POINTER(C.c_double),
                                            u32p]),
     "pf_prompt_attention": (C.c_int32, [vp, C.POINTER(AttnDesc), vp, vp, vp, vp, vp, vp, C.c_uint32]),
+    "pf_rotary_create": (C.c_int32, [vp, C.POINTER(RotaryDesc), C.POINTER(vp)]),
+    "pf_rotary_destroy": (None, [vp]),
+    "pf_rotary_apply": (C.c_int32, [vp, C.c_int32, C.c_uint32, vp, vp, vp, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "pf_sample_rows": (C.c_int32, [vp, C.POINTER(SampleDesc), vp, vp, C.c_uint32, vp, vp]),
     "pf_pages_create": (C.c_int32, [vp, C.POINTER(PagesConfig), C.POINTER(vp)]),
     "pf_pages_destroy": (None, [vp]),
     "pf_pages_memory_usage": (C.c_size_t, [vp]),
@@ -167,6 +183,7 @@ SYMBOLS = {
     "pf_pages_planes": (C.c_int32, [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp)]),
     "pf_pages_append": (C.c_int32, [vp, vp, vp, C.c_uint32]),
     "pf_pages_store": (C.c_int32, [vp, C.c_uint32, C.c_int32, vp, vp, C.c_uint32, C.c_uint32]),
+    "pf_pages_store_rotary": (C.c_int32, [vp, C.c_uint32, vp, C.c_int32, C.c_uint32, vp, vp, vp, vp] + 4 * [C.c_uint32]),
     "pf_pages_attention": (C.c_int32, [vp, C.POINTER(AttnDesc), C.c_uint32, vp, vp]),
     "pf_pages_gather": (C.c_int32, [vp, C.c_uint32, vp, C.c_uint32, C.c_int32, vp, vp, C.c_uint32, C.c_uint32]),
     "pf_pages_fork": (C.c_int32, [vp, C.c_uint32, vp, C.c_uint32]),
@@ -309,6 +326,36 @@ def _here(ctx, t, what):
         raise PFError(f"{what} is a DeviceArray or a tensor on the GPU, not {type(t).__name__}") from None
     if at != ctx.device:
         raise PFError(f"{what} is {'in host memory' if at < 0 else f'on GPU {at}'}, not on the context's GPU {ctx.device}")
+
+
+def _matrix(t, what, ctx):
+    """(rows, columns, elements from one row to the next) of a 2-d device array."""
+    _here(ctx, t, what)
+    if len(t.shape) != 2:
+        raise PFError(f"{what} is [rows][columns], not {tuple(t.shape)}")
+    n, w = t.shape
+    if isinstance(t, DeviceArray) or n <= 1 and (w <= 1 or t.stride(1) == 1):
+        return int(n), int(w), int(w)
+    s, one = t.stride()
+    if w > 1 and one != 1:
+        raise PFError(f"{what}: the values of a row lie one after another")
+    if not w <= s < 1 << 32:
+        raise PFError(f"{what}: rows of {w} values overlap, or lie too far apart, at a stride of {s}")
+    return n, w, s
+
+
+_WORDS = {}
+
+
+def _column(t, what, n, kind, ctx):
+    """Address of a device array of n packed 32-bit values, a row's each."""
+    own = isinstance(t, DeviceArray)
+    if own or getattr(t, "get_device", dict)() != ctx.device:
+        _here(ctx, t, what)
+    name = _WORDS.get(t.dtype) or _WORDS.setdefault(t.dtype, str(t.dtype).replace("torch.", ""))
+    if tuple(t.shape) != (n,) or name != kind or not (own or n <= 1 or t.stride(0) == 1):
+        raise PFError(f"{what} is {kind} [{n}], packed, not {name} {tuple(t.shape)}")
+    return _addr(t)
 
 
 def _u32(a, what):
@@ -510,6 +557,35 @@ class Context:
             self.synchronize()
         return y
 
+    def sample_rows(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+        """A token from each row of logits [rows][n_vocab], by u [rows] (float32 in
+        [0, 1)): (tokens int32, their probabilities float32).  Each setting is a
+        number, or a device array of the rows' own (int32 for top_k, float32 for
+        the others).  With `out`, two arrays (the second may be None), the call is
+        asynchronous on the context's stream."""
+        rows, V, stride = _matrix(logits, "logits", self)
+        d = SampleDesc(_type(logits), V, stride, 1.0, 0, 1.0, 0.0)
+        for name, value in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
+            if isinstance(value, (int, float, np.floating)):
+                setattr(d, name, value)
+            else:
+                setattr(d, name + "_dev", _column(value, name, rows, "float32", self))
+        if isinstance(top_k, (int, np.integer)):
+            d.top_k = _num(top_k, "top_k")
+        else:
+            d.top_k_dev = _column(top_k, "top_k", rows, "int32", self)
+        if out is None:
+            tokens, probs = self.empty((rows,), np.int32), self.empty((rows,), np.float32)
+        else:
+            tokens, probs = out
+        self.check(lib().pf_sample_rows(self.h, C.byref(d), _addr(logits), _column(u, "u", rows, "float32", self), rows,
+                                        _column(tokens, "tokens", rows, "int32", self),
+                                        None if probs is None else _column(probs, "probs", rows, "float32", self)),
+                   "pf_sample_rows")
+        if out is None:
+            self.synchronize()
+        return tokens, probs
+
     def gemv_f32(self, W, x):
         M = x.shape[0]
         y = self.empty((M, W.rows), np.float32)
@@ -671,6 +747,21 @@ class PagedCache:
         t, ks, vs = self._kv(k, v, self.pass_rows)
         self.ctx.check(lib().pf_pages_store(self.h, _num(layer, "layer"), t, _addr(k), _addr(v), ks, vs), "pf_pages_store")
 
+    def store_rotary(self, layer, rotary, q, k, v, out=None):
+        """store() with the keys turned by their positions, and the pass's queries
+        turned into `out` (may be q; asynchronous then) or a new array."""
+        n, H, D, qs = _rows(q, "q", self.ctx)
+        t, ks, vs = self._kv(k, v, self.pass_rows)
+        y = self.ctx.empty((n, H, D), q.dtype if isinstance(q, DeviceArray) else _NUMPY[t]) if out is None else out
+        n1, H1, D1, os = _rows(y, "out", self.ctx)
+        if n != self.pass_rows or (n1, H1, D1) != (n, H, D) or D != self.head_dim or not t == _type(q) == _type(y):
+            raise PFError(f"q and out are [{self.pass_rows}][heads][{self.head_dim}] of k's type")
+        self.ctx.check(lib().pf_pages_store_rotary(self.h, _num(layer, "layer"), rotary.h, t, H, _addr(q), _addr(k), _addr(v),
+                                                   _addr(y), qs, ks, vs, os), "pf_pages_store_rotary")
+        if out is None:
+            self.ctx.synchronize()
+        return y
+
     def attention(self, layer, q, causal=True, window=0, sink=0, scale=0.0, out=None):
         """The pass's rows over their sequences.  With `out` asynchronous, as Context.prompt_attention."""
         n, H, D, qs = _rows(q, "q", self.ctx)
@@ -777,6 +868,44 @@ class PagedCache:
     def close(self):
         if self.h:
             lib().pf_pages_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        self.close()
+
+
+class Rotary:
+    """Rotary positions of heads of head_dim (pf_rotary_desc): the first `turn`
+    dims in pairs, 2i with 2i + 1 (interleaved) or i with i + turn / 2."""
+
+    def __init__(self, ctx, head_dim, turn=0, interleaved=True, base=5e6, factor=1.0, low=0.0, high=0.0, original=0,
+                 magnitude=1.0):
+        self.ctx, self.head_dim = ctx, head_dim
+        self.h = None
+        d = RotaryDesc(_num(head_dim, "head_dim"), _num(turn, "turn"), bool(interleaved), base, factor, low, high,
+                       _num(original, "original"), magnitude)
+        h = vp()
+        ctx.check(lib().pf_rotary_create(ctx.h, C.byref(d), C.byref(h)), "pf_rotary_create")
+        self.h = h
+
+    def apply(self, x, positions, out=None):
+        """x [rows][heads][head_dim] turned, row i by positions[i] (int32 device array).
+        With `out` (may be x) asynchronous on the context's stream."""
+        n, H, D, xs = _rows(x, "x", self.ctx)
+        t = _type(x)
+        y = self.ctx.empty((n, H, D), x.dtype if isinstance(x, DeviceArray) else _NUMPY[t]) if out is None else out
+        n1, H1, D1, os = _rows(y, "out", self.ctx)
+        if D != self.head_dim or (n1, H1, D1) != (n, H, D) or _type(y) != t:
+            raise PFError(f"x and out are [rows][heads][{self.head_dim}] of one type")
+        self.ctx.check(lib().pf_rotary_apply(self.h, t, H, _addr(x), _addr(y), _column(positions, "positions", n, "int32", self.ctx),
+                                             n, xs, os), "pf_rotary_apply")
+        if out is None:
+            self.ctx.synchronize()
+        return y
+
+    def close(self):
+        if self.h:
+            lib().pf_rotary_destroy(self.h)
             self.h = None
 
     def __del__(self):

@@ -36,6 +36,8 @@ UNITS = [
     ("pf_prompt.hip", "hip"),
     ("pf_paged.hip", "hip"),
     ("pf_pages.hip", "hip"),
+    ("pf_rotary.hip", "hip"),
+    ("pf_sample.hip", "hip"),
     ("pf_host.cpp", "cxx"),
     ("pf_squeeze.cpp", "cxx"),
 ]

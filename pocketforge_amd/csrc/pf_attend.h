@@ -173,6 +173,20 @@ __device__ __forceinline__ void load8(const void* p, float (&x)[8]) {
     }
 }
 
+// Four values of a row of type T.
+template <int T>
+__device__ __forceinline__ void load4(const void* p, float (&x)[4]) {
+    if constexpr (T == PF_TYPE_F32) {
+        const f4v a = *(const f4v*)p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = a[i];
+    } else {
+        const s4v a = *(const s4v*)p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = to_float<T>(a[i]);
+    }
+}
+
 // Four values to a row of type T.
 template <int T>
 __device__ __forceinline__ void store4(void* p, const float (&x)[4]) {

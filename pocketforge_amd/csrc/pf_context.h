@@ -106,6 +106,16 @@ struct DeviceScope {
     return x < y + nb && y < x + na;
 }
 
+// Whether rows of `width` bytes, `n` of them `sa` and `sb` bytes apart, share memory
+// (columns of one buffer's rows do not).
+[[maybe_unused]] static bool rows_overlap(const void* a, size_t sa, const void* b, size_t sb, size_t wa, size_t wb, size_t n) {
+    if (!n || !overlaps(a, (n - 1) * sa + wa, b, (n - 1) * sb + wb)) return false;
+    if (sa != sb || n == 1) return true;
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    const size_t off = x < y ? (y - x) % sa : (sa - (x - y) % sa) % sa;   // of b's columns behind a's
+    return off < wa || off + wb > sa;
+}
+
 // A pf_attn_desc's checked values (pf_prompt.hip).
 constexpr uint32_t SEQ_ROWS = 1u << 30;   // of one sequence
 struct AttnShape {

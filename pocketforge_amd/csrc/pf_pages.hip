@@ -38,23 +38,6 @@ struct SmallMessage {
     uint32_t msg[SMALL_WORDS];
 };
 
-// The sequence of a packed row: the last one whose first row is not past it
-// (sequences without rows share their first row with the next one's, and come
-// before it).  A wave looks at 64 of them at a time.
-__device__ __forceinline__ uint32_t seq_of_row(const PageSeq* seqs, uint32_t n, uint32_t row) {
-    uint32_t lo = 0, count = n;
-    while (count > 64) {
-        const uint32_t step = (count + 63) / 64, i = (threadIdx.x & 63) * step;
-        const uint64_t b = __ballot(i < count && seqs[lo + i].q0 <= row);
-        const uint32_t k = 63 - (uint32_t)__builtin_clzll(b);
-        lo += k * step;
-        count = min(step, count - k * step);
-    }
-    const uint32_t i = threadIdx.x & 63;
-    const uint64_t b = __ballot(i < count && seqs[lo + i].q0 <= row);
-    return lo + 63 - (uint32_t)__builtin_clzll(b);
-}
-
 struct StoreArgs {
     const PageSeq* seqs;
     const int32_t* table;

@@ -42,3 +42,54 @@ def fp4_held(x):
 
 def fp4_bytes(code):
     return code[..., 0::2] | code[..., 1::2] << 4
+
+
+def frequencies(turn, base=5e6, factor=1.0, low=0.0, high=0.0, original=0):
+    """Radians a position, of each pair, in extended precision."""
+    i = np.arange(turn // 2).astype(np.longdouble)
+    f = np.longdouble(np.float32(base)) ** (-2 * i / turn)
+    g = np.zeros_like(f)
+    if low or high:
+        t = original * f / (2 * np.pi)
+        g = np.clip((t - np.float32(low)) / (np.longdouble(np.float32(high)) - np.float32(low)), 0, 1)
+    return f * (g + (1 - g) / np.longdouble(np.float32(factor)))
+
+
+def turned(x, positions, turn, interleaved, magnitude=1.0, **kw):
+    """x [rows][heads][D] (float64) turned, and |a| + |b| of each value's pair (0 past `turn`)."""
+    a = np.asarray(positions).astype(np.longdouble)[:, None, None] * frequencies(turn, **kw)
+    m = np.longdouble(np.float32(magnitude))
+    c, s = np.cos(a) * m, np.sin(a) * m
+    first, second = (np.s_[..., :turn:2], np.s_[..., 1:turn:2]) if interleaved else (np.s_[..., :turn // 2], np.s_[..., turn // 2:turn])
+    u, w = x[first].astype(np.longdouble), x[second].astype(np.longdouble)
+    out, size = x.astype(np.longdouble), np.zeros(x.shape)
+    out[first], out[second] = u * c - w * s, u * s + w * c
+    size[first] = size[second] = (np.abs(u) + np.abs(w)).astype(np.float64) * float(m)
+    return out, size
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, probability) of one row: logits in float64, settings as float32; weights in whole steps of 2^-43."""
+    l = np.where(np.isnan(logits), -np.inf, logits)
+    order = np.lexsort((np.arange(len(l)), -l))
+    order = order[l[order] > -np.inf]
+    if not len(order):
+        return -1, 0.0
+    temperature, top_p, min_p, u = (float(np.float32(v)) for v in (temperature, top_p, min_p, u))
+    if not temperature > 0:
+        return int(order[0]), 1.0
+    l = l[order]
+    with np.errstate(all="ignore"):
+        w = np.exp(np.where(l == l[0], 0.0, -np.inf if np.isinf(l[0]) else (l - l[0]) / temperature))
+    w = np.rint(w * 2.0 ** 43).astype(np.int64)
+    upto = np.cumsum(w)
+    n = top_k if 0 < top_k < len(l) else len(l)
+    mass = int(upto[n - 1])
+    kept = mass
+    if top_p < 1:
+        kept = int(upto[np.searchsorted(upto, max(1.0, np.ceil(top_p * float(mass))))])
+    if min_p > 0:
+        weighs = np.flatnonzero(w.astype(np.float64) >= min(min_p, 1.0) * 2.0 ** 43)
+        kept = min(kept, int(upto[weighs[-1]]))
+    i = np.searchsorted(upto, min(int(max(u, 0.0) * float(kept)), kept - 1), side="right")
+    return int(order[i]), int(w[i]) / kept
