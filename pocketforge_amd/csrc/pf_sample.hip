@@ -4,13 +4,20 @@
 // With the tokens in order of their logits (equal ones by number) each filter
 // keeps a beginning of that order, so the kept set is a mass S = min(M_k, M_p,
 // M_m): of the first k, of the first that reach p M_k, of those that weigh min_p.
-// The token is the first whose cumulative weight exceeds u S.  Nothing has to be
-// sorted but what lies next to those three borders and the token: a histogram
-// over the distance from the largest logit finds their bins, and only these bins'
-// tokens are sorted, or all up to the last where they are few.
+// The token is the first whose cumulative weight exceeds u S.
 //
-// Weights are whole numbers, exp((l - max) / T) in steps of 2^-43, so that every
-// sum is exact, whatever the order in which threads add to it: up to 2^20 tokens
+// Two launches.  Workgroups of a slice of a row each read it once, into
+// registers: its largest logit, the sum of its weights, and its largest few
+// tokens, those above a bound that the threads' own maxima give.  What lies above
+// the largest of these bounds, over all slices, is the beginning of the order: a
+// thousand tokens or the top-k and some more.  A workgroup for each row finds the
+// borders and the token among them, by a histogram and a sort of the bins that the
+// borders are in.  Where one lies further on, as in flat rows, it does the same
+// over the whole row, and where that has more equal logits than it can sort,
+// digit by digit.
+//
+// Weights are whole numbers, exp((l - max) / T) in steps of 2^-43, so that sums
+// are exact, whatever the order in which threads add to them: up to 2^20 tokens
 // of up to 2^43 fit 64 bits, and what a step leaves of 2^20 sums is 2^-24 of the
 // largest weight, what sums of fp32 would lose of the first few.
 #include "pf_attend.h"
@@ -23,7 +30,7 @@ constexpr float BIN_OCTAVES = 44.0f;   // of the weights, that the bins cover (t
 constexpr uint32_t LIST = 2048;        // tokens that are sorted at once
 constexpr uint32_t FEW_K = 1024;       // top-k up to here needs no sums over the row
 constexpr double STEPS = 8796093022208.0;   // 2^43
-constexpr uint64_t ONE = 1ull << 43;
+constexpr double WHOLE = 6755399441055744.0;   // 2^52 + 2^51: what is added to it is whole, in its low bits
 
 struct SampleArgs {
     const void* logits;
@@ -31,13 +38,22 @@ struct SampleArgs {
     const int32_t* top_k;
     float temperature1, top_p1, min_p1;
     uint32_t top_k1;
-    uint32_t rows, vocab, stride, slices, per;      // per: chunks of a slice
+    uint32_t rows, vocab, stride, slices, room;   // room: listed tokens of a slice at most
     int32_t* tokens;
     float* probs;
-    float2* ws_max;               // [rows][slices]: value, token
-    uint64_t* ws_mass;            // [rows][slices][BINS]
-    uint32_t* ws_count;           // [rows][slices][BINS]
-    uint64_t* ws_least;           // [rows][slices]: mass of those that weigh min_p
+    struct Slice* ws_slice;       // [rows][slices]
+    uint64_t* ws_list;            // [rows][slices][room]
+};
+
+// What a slice's workgroup found: the largest logit and its first token, the sum
+// of the weights beside that logit's, the bound above which tokens are listed, and
+// their number (more than the room: not all of them are).
+struct Slice {
+    uint64_t mass;
+    float max;
+    int32_t first;
+    float bound;
+    uint32_t listed;
 };
 
 // A row in chunks of 16 bytes from the last multiple of 16 on; what lies before its
@@ -101,13 +117,15 @@ struct Setting {
         const float d = l == max ? 0.0f : max - l;
         return (int)fminf(d * to_bin, (float)(BINS - 1));      // (rounded alike for all: the order stays)
     }
-    // 2^43 e^((l - max) / T) to the nearest whole number: 2^x = 2^n e^(f ln 2) with
-    // |f| <= 1/2, the series up to z^11 (z^12 / 12! = 6e-15, 2^-47)
-    __device__ __forceinline__ uint64_t weight(float l) const {
-        const double x = ((double)l - (double)max) * scale;
-        if (l == max) return ONE;
-        if (!(x > -44.5)) return 0;
-        const double n = rint(x), z = (x - n) * 0.69314718055994530942;
+    // (l - max) / T in octaves, as far as weights reach
+    __device__ __forceinline__ double octaves(float l) const {
+        return l == max ? 0.0 : fmax(((double)l - (double)max) * scale, -60.0);
+    }
+    // 2^43 2^x to the nearest whole number: 2^x = 2^n e^(f ln 2) with |f| <= 1/2, the
+    // series up to z^11 (z^12 / 12! = 6e-15, 2^-47)
+    static __device__ __forceinline__ uint64_t weight_of(double x) {
+        const double t = x + WHOLE;
+        const double z = (x - (t - WHOLE)) * 0.69314718055994530942;
         double y = 1.0 / 39916800.0;
         y = fma(y, z, 1.0 / 3628800.0);
         y = fma(y, z, 1.0 / 362880.0);
@@ -120,10 +138,12 @@ struct Setting {
         y = fma(y, z, 0.5);
         y = fma(y, z, 1.0);
         y = fma(y, z, 1.0);
-        // (added to 2^52, a number is whole in the last place)
-        const double w = __builtin_ldexp(y, (int)n + 43) + 4503599627370496.0;
+        // times 2^(n + 43), by its exponent; added to 2^52 a number is whole in the last place
+        const uint64_t n = __builtin_bit_cast(uint64_t, t) + 43;
+        const double w = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, y) + (n << 52)) + 4503599627370496.0;
         return __builtin_bit_cast(uint64_t, w) - 0x4330000000000000ull;
     }
+    __device__ __forceinline__ uint64_t weight(float l) const { return weight_of(octaves(l)); }
 };
 
 // Larger logits first: the value as an integer that falls with it.
@@ -135,115 +155,160 @@ __device__ __forceinline__ float falling_value(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k : ~k & 0x7FFFFFFFu);
 }
 
-struct Best {
-    float v;
-    int32_t i;
-};
-__device__ __forceinline__ Best better(Best a, Best b) { return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a; }
-__device__ __forceinline__ Best wave_best(Best b) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) b = better(b, Best{__shfl_xor(b.v, o), __shfl_xor(b.i, o)});
-    return b;
-}
 constexpr int32_t NO_TOKEN = 0x7FFFFFFF;
 
-// The largest logit of a slice and its first token.
-template <int T>
-__global__ __launch_bounds__(256) void k_sample_max(SampleArgs a) {
-    __shared__ Best s_best[4];
-    const Row<T> r(a, blockIdx.y);
-    const uint32_t c0 = blockIdx.x * a.per, c1 = min(c0 + a.per, r.chunks);
-    Best b{-INFINITY, NO_TOKEN};
-#pragma unroll 4
-    for (uint32_t c = c0 + threadIdx.x; c < c1; c += 256) {
-        float x[Row<T>::E];
-        r.load(c, x);
+// Over a wave, by the adders' own lane shifts: rows of 16 lanes, then row to row.
+// Lanes that a shift does not reach take `none`.
+template <class F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, uint32_t none, F&& f) {
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x111, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x112, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x114, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x118, 0xf, 0xf, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x142, 0xa, 0xf, false));
+    return f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, 0x143, 0xc, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {   // with its own
+    return wave_fold(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t wave_least(uint32_t v) {
+    v = wave_fold(v, ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ float wave_max(float v) {
+    const uint32_t m = wave_fold(__builtin_bit_cast(uint32_t, v), 0xFF800000u, [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    });
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane((int)m, 63));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
+    v += dpp64<0x111, 0xf>(v);
+    v += dpp64<0x112, 0xf>(v);
+    v += dpp64<0x114, 0xf>(v);
+    v += dpp64<0x118, 0xf>(v);
+    v += dpp64<0x142, 0xa>(v);
+    return v + dpp64<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return lane64(wave_scan64(v), 63); }
+
+// A wave's c-th largest of its lanes' values, to 16 bits (the next lower such
+// value), as an integer that rises with it; 0 where fewer than c are above -infinity.
+__device__ __forceinline__ uint32_t nth_of_wave(float v, uint32_t c) {
+    const uint32_t key = v == -INFINITY ? 0u : ~falling(v);
+    uint32_t found = 0;
 #pragma unroll
-        for (int i = 0; i < Row<T>::E; i++)
-            if (x[i] > b.v) b = Best{x[i], (int32_t)(c * Row<T>::E) - r.skip + i};
+    for (int b = 31; b >= 16; b--) {
+        const uint32_t to = found | 1u << b;
+        if ((uint32_t)__popcll(__ballot(key >= to)) >= c) found = to;
     }
-    b = wave_best(b);
-    if ((threadIdx.x & 63) == 0) s_best[threadIdx.x >> 6] = b;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        b = better(better(s_best[0], s_best[1]), better(s_best[2], s_best[3]));
-        a.ws_max[(size_t)blockIdx.y * a.slices + blockIdx.x] = float2{b.v, __builtin_bit_cast(float, b.i)};
-    }
+    return found;
 }
 
-// The row's largest logit, of its slices'.
-__device__ __forceinline__ void row_max(const SampleArgs& a, uint32_t row, Setting& s) {
-    Best b{-INFINITY, NO_TOKEN};
-    const uint32_t lane = threadIdx.x & 63;
-    if (lane < a.slices) {
-        const float2 m = a.ws_max[(size_t)row * a.slices + lane];
-        b = Best{m.x, __builtin_bit_cast(int32_t, m.y)};
+// A slice: N chunks a thread.  The bound is the mean of the four waves' c-th
+// largest lanes: of n listed tokens over 256 threads a thread has one with the
+// probability 1 - e^(-n / 256), so c = 64 of that gives about n.
+template <int T, int N>
+__global__ __launch_bounds__(256) void k_sample_slice(SampleArgs a) {
+    constexpr int E = Row<T>::E;
+    __shared__ float s_max[4];
+    __shared__ uint32_t s_bound[4], s_listed, s_first;
+    __shared__ uint64_t s_mass[4];
+    const uint32_t row = blockIdx.y, t = threadIdx.x, wave = t >> 6;
+    if (t == 0) {
+        s_listed = 0;
+        s_first = NO_TOKEN;
     }
-    b = wave_best(b);
-    s.max = b.v;
-    s.first = b.i == NO_TOKEN ? -1 : b.i;
-}
-
-// The tokens of a chunk into the bins.
-template <int E>
-__device__ __forceinline__ void count_chunk(const Setting& s, const float (&x)[E], bool sums, uint32_t* count, uint64_t* mass,
-                                            uint64_t& least) {
+    const Row<T> r(a, row);
+    // (chunks in turn: every slice has its share of each part of the vocabulary)
+    float x[N][E], top = -INFINITY;
+    const auto chunk = [&](int n) { return (blockIdx.x + a.slices * n) * 256 + t; };
+    const auto token = [&](int n, int i) { return (int32_t)(chunk(n) * E) - r.skip + i; };
 #pragma unroll
-    for (int i = 0; i < E; i++) {
-        if (x[i] == -INFINITY) continue;
-        const int b = s.bin(x[i]);
-        atomicAdd(&count[b], 1u);
-        if (sums) {
-            const uint64_t w = s.weight(x[i]);
-            if (w) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w);
-            if ((double)w >= s.least) least += w;
-        }
-    }
-}
-
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
-    return (uint64_t)(uint32_t)__shfl_up((int)(uint32_t)v, o) | (uint64_t)(uint32_t)__shfl_up((int)(v >> 32), o) << 32;
-}
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-    return (uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)v, o) | (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32;
-}
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+    for (int n = 0; n < N; n++) {
+        if (chunk(n) < r.chunks) r.load(chunk(n), x[n]);
+        else
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v += shfl_xor64(v, o);
-    return v;
-}
-
-// A slice's histogram.
-template <int T>
-__global__ __launch_bounds__(256) void k_sample_count(SampleArgs a) {
-    __shared__ uint32_t s_count[BINS];
-    __shared__ uint64_t s_mass[BINS], s_least[4];
-    const uint32_t row = blockIdx.y;
+            for (int i = 0; i < E; i++) x[n][i] = -INFINITY;
+    }
     Setting s;
     s.of(a, row);
-    row_max(a, row, s);
-    if (s.greedy || s.first < 0) return;
-    const bool sums = !s.few;
-    for (int i = threadIdx.x; i < BINS; i += 256) s_count[i] = 0, s_mass[i] = 0;
-    __syncthreads();
-    const Row<T> r(a, row);
-    const uint32_t c0 = blockIdx.x * a.per, c1 = min(c0 + a.per, r.chunks);
-    uint64_t least = 0;
-#pragma unroll 2
-    for (uint32_t c = c0 + threadIdx.x; c < c1; c += 256) {
-        float x[Row<T>::E];
-        r.load(c, x);
-        count_chunk(s, x, sums, s_count, s_mass, least);
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < E; i++) top = fmaxf(top, x[n][i]);
+    // how many tokens are wanted of the row: top-k's and some more, or a thousand
+    const float want = s.greedy ? 0.0f : fminf((s.few ? 1.5f * (float)s.k : 1024.0f) + 16.0f * (float)a.slices, 1700.0f);
+    const uint32_t c = (uint32_t)(64.0f * (1.0f - __builtin_amdgcn_exp2f(want / (float)a.slices * (-1.4426950f / 256.0f)))) + 1;
+    const uint32_t nth = nth_of_wave(top, min(c, 60u));
+    const float wave_top = wave_max(top);
+    if ((t & 63) == 0) {
+        s_max[wave] = wave_top;
+        s_bound[wave] = nth;
     }
-    least = wave_sum64(least);
-    if ((threadIdx.x & 63) == 0) s_least[threadIdx.x >> 6] = least;
     __syncthreads();
-    const size_t at = (size_t)row * a.slices + blockIdx.x;
-    for (int i = threadIdx.x; i < BINS; i += 256) {
-        a.ws_count[at * BINS + i] = s_count[i];
-        if (sums) a.ws_mass[at * BINS + i] = s_mass[i];
+    s.max = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    if (s.max > -INFINITY && wave_top == s.max) {
+        uint32_t first = NO_TOKEN;
+#pragma unroll
+        for (int n = N - 1; n >= 0; n--)
+#pragma unroll
+            for (int i = E - 1; i >= 0; i--)
+                if (x[n][i] == s.max) first = (uint32_t)token(n, i);
+        first = wave_least(first);
+        if ((t & 63) == 0) atomicMin(&s_first, first);
     }
-    if (threadIdx.x == 0) a.ws_least[at] = s_least[0] + s_least[1] + s_least[2] + s_least[3];
+    float bound = -INFINITY;
+    uint64_t mass = 0;
+    if (!s.greedy && s.max > -INFINITY) {
+        uint64_t sum = 0;
+        uint32_t some = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            sum += s_bound[w];
+            some += s_bound[w] != 0;
+        }
+        if (some) bound = falling_value(~(uint32_t)(sum / some));
+        uint32_t hits = 0;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < E; i++) hits += (x[n][i] >= bound) & (x[n][i] > -INFINITY);
+        const uint32_t upto = wave_scan(hits);
+        uint32_t at = 0;
+        if ((t & 63) == 63) at = atomicAdd(&s_listed, upto);
+        at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - hits;
+        uint64_t* list = a.ws_list + ((size_t)row * a.slices + blockIdx.x) * a.room;
+        if (!s.few) {
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int i = 0; i < E; i++) mass += s.weight(x[n][i]);
+            mass = wave_sum64(mass);
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                if (x[n][i] >= bound && x[n][i] > -INFINITY) {
+                    if (at < a.room) list[at] = (uint64_t)falling(x[n][i]) << 32 | (uint32_t)token(n, i);
+                    at++;
+                }
+    }
+    if ((t & 63) == 0) s_mass[wave] = mass;
+    __syncthreads();
+    if (t == 0)
+        a.ws_slice[(size_t)row * a.slices + blockIdx.x] =
+            Slice{s_mass[0] + s_mass[1] + s_mass[2] + s_mass[3], s.max, (int32_t)s_first, bound, s_listed};
 }
 
 // ------------------------------------------------------ one row, 1024 threads
@@ -258,37 +323,24 @@ struct Found {
 };
 
 struct PickLds {
-    uint32_t count[BINS];         // then: tokens before a bin
-    uint64_t mass[BINS];          // then: weight before a bin
+    uint32_t count[BINS];         // tokens of a bin; then before it
+    uint64_t mass[BINS];          // weight of a bin; then before it
     uint64_t list[LIST];          // falling(logit) << 32 | token; or a digit's histogram
     uint64_t upto[LIST];          // cumulative weights of the sorted list
-    uint64_t part[PICK / 64];
-    uint64_t found[4];
-    uint32_t n;
-    Best best[PICK / 64];
+    uint64_t part[PICK / 64], found[4];
+    uint32_t part32[PICK / 64], n, bin;
 };
 
 // Sum over the threads before this one; the sum of all in *total.
 __device__ __forceinline__ uint64_t scan64(PickLds& m, uint64_t v, uint64_t* total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t x = shfl_up64(s, o);
-        if (lane >= (uint32_t)o) s += x;
-    }
+    const uint64_t s = wave_scan64(v);
     __syncthreads();
     if (lane == 63) m.part[wave] = s;
     __syncthreads();
-    uint64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < PICK / 64; w++) {
-        const uint64_t x = m.part[w];
-        if (w < (int)wave) before += x;
-        all += x;
-    }
-    *total = all;
-    return before + s - v;
+    const uint64_t p = lane < PICK / 64 ? m.part[lane] : 0, q = wave_scan64(p);
+    *total = lane64(q, PICK / 64 - 1);
+    return lane64(q - p, (int)__builtin_amdgcn_readfirstlane(wave)) + s - v;
 }
 
 // m.list's first n entries in rising order, as many threads as half of them.
@@ -311,157 +363,88 @@ __device__ __forceinline__ void sort_list(PickLds& m, uint32_t n) {
         }
 }
 
+// A whole row.
 template <int T>
 struct Pick {
     static constexpr int E = Row<T>::E;
-    const SampleArgs& a;
     const Row<T> r;
-    Setting s;
+    const Setting& s;
     PickLds& m;
-    uint32_t row, valid;          // tokens that are not masked
+    uint32_t valid;               // tokens that are not masked
     uint64_t all, least;          // their weight; of those that weigh min_p
-    uint32_t from = 0, upto = 0;  // bins whose tokens the sorted list has, and how many these are
-    uint32_t listed = 0;
-
-    __device__ __forceinline__ Pick(const SampleArgs& args, PickLds& lds, uint32_t row) : a(args), r(args, row), m(lds), row(row) {}
+    uint32_t from, sorted = 0;    // the bin whose tokens the sorted list has, and how many these are
 
     template <class F>
-    __device__ __forceinline__ void each_chunk(F&& f) const {
+    __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll 2
         for (uint32_t c = threadIdx.x; c < r.chunks; c += PICK) {
             float x[E];
             r.load(c, x);
-            f(x, (int32_t)(c * E) - r.skip);
-        }
-    }
-
-    __device__ __forceinline__ void largest() {
-        Best b{-INFINITY, NO_TOKEN};
-        each_chunk([&](const float (&x)[E], int32_t t0) {
 #pragma unroll
             for (int i = 0; i < E; i++)
-                if (x[i] > b.v) b = Best{x[i], t0 + i};
-        });
-        b = wave_best(b);
-        if ((threadIdx.x & 63) == 0) m.best[threadIdx.x >> 6] = b;
-        __syncthreads();
-        b = m.best[0];
-#pragma unroll
-        for (int w = 1; w < PICK / 64; w++) b = better(b, m.best[w]);
-        s.max = b.v;
-        s.first = b.i == NO_TOKEN ? -1 : b.i;
+                if (x[i] != -INFINITY) f(x[i], (int32_t)(c * E) - r.skip + i);
+        }
     }
 
-    // the histogram, of the slices' or of the row; then what lies before each bin
-    __device__ __forceinline__ void count(bool slices, bool sums) {
+    // the histogram, then what lies before each bin
+    __device__ __forceinline__ Pick(const SampleArgs& a, const Setting& s, PickLds& m, uint32_t row) : r(a, row), s(s), m(m) {
         const uint32_t t = threadIdx.x;
         least = 0;
-        uint32_t n = 0;
-        uint64_t w = 0;
-        if (slices) {
-            for (uint32_t i = 0; i < a.slices; i++) {
-                const size_t at = (size_t)row * a.slices + i;
-                n += a.ws_count[at * BINS + t];
-                if (sums) {
-                    w += a.ws_mass[at * BINS + t];
-                    least += a.ws_least[at];
-                }
-            }
-        } else {
-            __syncthreads();
-            m.count[t] = 0;
-            m.mass[t] = 0;
-            __syncthreads();
-            each_chunk([&](const float (&x)[E], int32_t) { count_chunk(s, x, sums, m.count, m.mass, least); });
-            scan64(m, least, &least);
-            n = m.count[t];
-            w = m.mass[t];
-        }
+        __syncthreads();
+        m.count[t] = 0;
+        m.mass[t] = 0;
+        __syncthreads();
+        each([&](float x, int32_t) {
+            const int b = s.bin(x);
+            const uint64_t w = s.weight(x);
+            atomicAdd(&m.count[b], 1u);
+            if (w) atomicAdd((unsigned long long*)&m.mass[b], (unsigned long long)w);
+            if ((double)w >= s.least) least += w;
+        });
+        if (s.least > 0.0) scan64(m, least, &least);
+        __syncthreads();
         uint64_t total;
-        const uint64_t before = scan64(m, n, &total);
+        const uint64_t n = scan64(m, m.count[t], &total);
         valid = (uint32_t)total;
-        m.count[t] = (uint32_t)before;
-        all = 0;
-        if (sums) m.mass[t] = scan64(m, w, &all);
+        const uint64_t w = scan64(m, m.mass[t], &all);
+        m.count[t] = (uint32_t)n;
+        m.mass[t] = w;
         __syncthreads();
     }
     __device__ __forceinline__ uint32_t count_after(uint32_t b) const { return b + 1 < BINS ? m.count[b + 1] : valid; }
     __device__ __forceinline__ uint64_t mass_after(uint32_t b) const { return b + 1 < BINS ? m.mass[b + 1] : all; }
-    // the bin with the n-th token (from 1), with the weight `t` (from 1)
-    __device__ __forceinline__ uint32_t bin_of_count(uint32_t n) {
-        const uint32_t t = threadIdx.x;
-        if (m.count[t] < n && n <= count_after(t)) m.n = t;
-        __syncthreads();
-        const uint32_t b = m.n;
-        __syncthreads();
-        return b;
-    }
-    __device__ __forceinline__ uint32_t bin_of_mass(uint64_t w) {
-        const uint32_t t = threadIdx.x;
-        if (m.mass[t] < w && w <= mass_after(t)) m.n = t;
-        __syncthreads();
-        const uint32_t b = m.n;
-        __syncthreads();
-        return b;
-    }
 
-    // the tokens of bins b0 .. b1 (at most LIST), sorted, with their cumulative weights behind `before`
-    __device__ __forceinline__ void gather(uint32_t b0, uint32_t b1, uint64_t before) {
+    // the tokens of a bin (at most LIST), sorted, with the cumulative weights
+    __device__ __forceinline__ void gather(uint32_t bin) {
         __syncthreads();
         if (threadIdx.x == 0) m.n = 0;
         __syncthreads();
-        each_chunk([&](const float (&x)[E], int32_t t0) {
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                if (x[i] == -INFINITY) continue;
-                const uint32_t b = (uint32_t)s.bin(x[i]);
-                if (b >= b0 && b <= b1) {
-                    const uint32_t at = atomicAdd(&m.n, 1u);
-                    if (at < LIST) m.list[at] = (uint64_t)falling(x[i]) << 32 | (uint32_t)(t0 + i);
-                }
-            }
+        each([&](float x, int32_t token) {
+            if ((uint32_t)s.bin(x) != bin) return;
+            m.list[atomicAdd(&m.n, 1u)] = (uint64_t)falling(x) << 32 | (uint32_t)token;
         });
         __syncthreads();
-        listed = min(m.n, LIST);
-        from = b0;
-        upto = b1;
-        sort_list(m, listed);
+        sorted = m.n;
+        from = bin;
+        sort_list(m, sorted);
         const uint32_t t = threadIdx.x;
         uint64_t w[2], total;
 #pragma unroll
-        for (int i = 0; i < 2; i++) w[i] = 2 * t + i < listed ? s.weight(falling_value((uint32_t)(m.list[2 * t + i] >> 32))) : 0;
-        const uint64_t at = before + scan64(m, w[0] + w[1], &total);
+        for (int i = 0; i < 2; i++) w[i] = 2 * t + i < sorted ? s.weight(falling_value((uint32_t)(m.list[2 * t + i] >> 32))) : 0;
+        const uint64_t at = m.mass[bin] + scan64(m, w[0] + w[1], &total);
         m.upto[2 * t] = at + w[0];
         m.upto[2 * t + 1] = at + w[0] + w[1];
         __syncthreads();
     }
-    // the first place of the list whose cumulative weight reaches w
-    __device__ __forceinline__ Found find(uint64_t w, uint64_t before) {
-        const uint32_t t = threadIdx.x;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t at = 2 * t + i;
-            const uint64_t last = at ? m.upto[at - 1] : before;
-            if (at < listed && last < w && w <= m.upto[at]) {
-                m.found[0] = m.upto[at];
-                m.found[1] = m.upto[at] - last;
-                m.found[2] = (uint32_t)m.list[at];
-            }
-        }
-        __syncthreads();
-        const Found f{m.found[0], m.found[1], (int32_t)m.found[2]};
-        __syncthreads();
-        return f;
-    }
 
-    // The same in a bin of more tokens than the list holds: three digits of the
+    // A place in a bin of more tokens than the list holds: three digits of the
     // falling value, each a histogram of the row, then the number among equals.
     // `counted`: w counts tokens, not weight.
-    __device__ Found search(uint32_t b, uint64_t w, uint64_t before, uint64_t tokens_before, bool counted, bool want_token) {
+    __device__ Found search(uint32_t b, uint64_t w, bool counted, bool want_token) {
         uint64_t* hist = m.list;                  // [2048]
-        listed = 0;
+        sorted = 0;
         uint32_t prefix = 0, known = 0;           // digits found, and their mask
-        uint64_t left = w - (counted ? tokens_before : before), mass_before = before;
+        uint64_t left = w - (counted ? (uint64_t)m.count[b] : m.mass[b]), mass_before = m.mass[b];
         const uint32_t t = threadIdx.x;
         for (int digit = 0; digit < 3; digit++) {
             const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
@@ -470,17 +453,13 @@ struct Pick {
             hist[2 * t] = hist[2 * t + 1] = 0;
             m.upto[2 * t] = m.upto[2 * t + 1] = 0;
             __syncthreads();
-            each_chunk([&](const float (&x)[E], int32_t) {
-#pragma unroll
-                for (int i = 0; i < E; i++) {
-                    if (x[i] == -INFINITY || (uint32_t)s.bin(x[i]) != b) continue;
-                    const uint32_t k = falling(x[i]);
-                    if ((k & known) != prefix) continue;
-                    const uint64_t wt = s.weight(x[i]);
-                    const uint32_t at = (k >> shift) & (size - 1);
-                    atomicAdd((unsigned long long*)&hist[at], (unsigned long long)(counted ? 1 : wt));
-                    if (counted) atomicAdd((unsigned long long*)&m.upto[at], (unsigned long long)wt);
-                }
+            each([&](float x, int32_t) {
+                const uint32_t k = falling(x);
+                if ((uint32_t)s.bin(x) != b || (k & known) != prefix) return;
+                const uint64_t wt = s.weight(x);
+                const uint32_t at = (k >> shift) & (size - 1);
+                atomicAdd((unsigned long long*)&hist[at], (unsigned long long)(counted ? 1 : wt));
+                if (counted) atomicAdd((unsigned long long*)&m.upto[at], (unsigned long long)wt);
             });
             __syncthreads();
             uint64_t total, n0 = hist[2 * t], n1 = hist[2 * t + 1];
@@ -531,35 +510,257 @@ struct Pick {
         __syncthreads();
         return f;
     }
-
-    // the first place whose cumulative weight reaches w, or the w-th (`counted`)
+    // The first place whose cumulative weight reaches w (from 1, to `all`), or the w-th (`counted`, from 1 to `valid`).
     __device__ __forceinline__ Found place(uint64_t w, bool counted, bool want_token) {
-        const uint32_t b = counted ? bin_of_count((uint32_t)w) : bin_of_mass(w);
+        const uint32_t t = threadIdx.x;
+        __syncthreads();
+        if (counted ? m.count[t] < w && w <= count_after(t) : m.mass[t] < w && w <= mass_after(t)) m.bin = t;
+        __syncthreads();
+        const uint32_t b = m.bin;
+        if (count_after(b) - m.count[b] > LIST) return search(b, w, counted, want_token);
+        if (!sorted || b != from) gather(b);
         const uint64_t before = m.mass[b];
-        const uint32_t tokens = m.count[b];
-        if (count_after(b) - tokens > LIST) return search(b, w, before, tokens, counted, want_token);
-        if (!listed || b < from || b > upto) gather(b, b, before);
-        if (counted) {
-            Found f{m.upto[(uint32_t)w - 1 - m.count[from]], 0, -1};
-            __syncthreads();
-            return f;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t at = 2 * t + i;
+            const uint64_t last = at ? m.upto[at - 1] : before;
+            if (at < sorted && (counted ? at + 1 == w - m.count[b] : last < w && w <= m.upto[at])) {
+                m.found[0] = m.upto[at];
+                m.found[1] = m.upto[at] - last;
+                m.found[2] = (uint32_t)m.list[at];
+            }
         }
-        return find(w, m.mass[from]);
+        __syncthreads();
+        return {m.found[0], m.found[1], (int32_t)m.found[2]};
     }
 };
 
-// The row's token.  SLICES: the largest logits and histograms of its slices are in
-// the workspace.
+// The listed tokens of a row: four waves have them in registers, the others take
+// part where all are needed.
+constexpr uint32_t FAST = 256;
+constexpr uint32_t AT_ONCE = 256;      // tokens of one bin that are put in order by comparing each with each
+struct Listed {
+    static constexpr int N = LIST / FAST, B = BINS / FAST;
+    Setting& s;
+    PickLds& m;
+    float x[N];                   // -infinity: none
+    int32_t token[N];
+    uint64_t w[N];
+    uint64_t mass[B + 1];         // before each of the thread's bins, and behind the last
+    uint32_t count[B + 1];
+    uint32_t n;                   // tokens
+    uint64_t all;                 // their weight
+    float bound;                  // what is not listed is below it
+    uint64_t row_mass;            // of the whole row, where top-k does not end it
+
+    __device__ __forceinline__ Listed(Setting& s, PickLds& m) : s(s), m(m) {}
+
+    // The row's largest logit, where the listed tokens end, and these tokens.  False: more than fit, or not all.
+    __device__ __forceinline__ bool load(const SampleArgs& a, uint32_t row) {
+        const uint32_t t = threadIdx.x, lane = t & 63;
+        const Slice* slices = a.ws_slice + (size_t)row * a.slices;
+        const uint64_t* list = a.ws_list + (size_t)row * a.slices * a.room;
+        m.count[t] = 0;
+        m.mass[t] = 0;
+        if (t == 0) m.n = 0;
+        // (a wave a slice, asked for before its bound is known)
+        constexpr uint32_t W = PICK / 64;
+        const uint32_t first = __builtin_amdgcn_readfirstlane(t >> 6);
+        uint64_t e[4];
+        if (first < a.slices)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) e[j] = lane + 64 * j < a.room ? list[first * a.room + lane + 64 * j] : 0;
+        float top = -INFINITY;
+        uint32_t none = NO_TOKEN, most = 0;
+        bound = -INFINITY;
+        for (uint32_t i = lane; i < a.slices; i += 64) {
+            const Slice q = slices[i];
+            bound = fmaxf(bound, q.bound);
+            most = max(most, q.listed);
+            if (q.max > top || (q.max == top && (uint32_t)q.first < none)) {
+                top = q.max;
+                none = (uint32_t)q.first;
+            }
+        }
+        s.max = wave_max(top);
+        bound = wave_max(bound);
+        none = wave_least(top == s.max ? none : (uint32_t)NO_TOKEN);
+        s.first = none == NO_TOKEN ? -1 : (int32_t)none;
+        if (s.greedy || s.first < 0) return true;
+        if (__any(most > a.room)) return false;
+        // the slices' weights beside the row's largest logit
+        row_mass = 0;
+        for (uint32_t i = lane; i < a.slices && !s.few; i += 64) {
+            const Slice q = slices[i];
+            if (q.max == s.max) row_mass += q.mass;
+            else if (q.mass) row_mass += (uint64_t)rint((double)q.mass * exp2(s.octaves(q.max)));
+        }
+        row_mass = wave_sum64(row_mass);
+        __syncthreads();
+        for (uint32_t i = first; i < a.slices; i += W) {
+            const uint32_t listed = slices[i].listed;
+            uint32_t keep = 0, on = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                if (i != first) e[j] = lane + 64 * j < listed ? list[i * a.room + lane + 64 * j] : 0;
+                if (lane + 64 * j < listed && falling_value((uint32_t)(e[j] >> 32)) >= bound) on |= 1u << j;
+                keep += (uint32_t)__popcll(__ballot(on >> j & 1));
+            }
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(&m.n, keep);
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint64_t who = __ballot(on >> j & 1);
+                const uint32_t to = at + (uint32_t)__popcll(who & ((1ull << lane) - 1));
+                if ((on >> j & 1) && to < LIST) m.list[to] = e[j];
+                at += (uint32_t)__popcll(who);
+            }
+        }
+        __syncthreads();
+        n = m.n;
+        return n <= LIST;
+    }
+
+    // the histogram, then what lies before each bin
+    __device__ __forceinline__ void count_all(bool counts) {
+        const uint32_t t = threadIdx.x;
+        if (t < FAST)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                x[i] = -INFINITY;
+                w[i] = 0;
+                if (i * FAST >= n) continue;
+                const uint64_t e = t + i * FAST < n ? m.list[t + i * FAST] : 0xFF800000ull << 32;
+                x[i] = falling_value((uint32_t)(e >> 32));
+                token[i] = (int32_t)(uint32_t)e;
+                w[i] = s.weight(x[i]);
+                if (x[i] == -INFINITY) continue;
+                const int b = s.bin(x[i]);
+                if (counts) atomicAdd(&m.count[b], 1u);
+                atomicAdd((unsigned long long*)&m.mass[b], (unsigned long long)w[i]);
+            }
+        __syncthreads();
+        uint64_t sum = 0;
+        uint32_t cnt = 0;
+        if (t < FAST) {
+            for (int i = 0; i < B; i++) {
+                mass[i] = sum;
+                count[i] = cnt;
+                sum += m.mass[B * t + i];
+                cnt += m.count[B * t + i];
+            }
+            mass[B] = sum;
+            count[B] = cnt;
+            sum = wave_scan64(sum);
+            cnt = wave_scan(cnt);
+            if ((t & 63) == 63) {
+                m.part[t >> 6] = sum;
+                m.part32[t >> 6] = cnt;
+            }
+        }
+        __syncthreads();
+        all = 0;
+        uint64_t before = 0;
+        uint32_t cbefore = 0;
+#pragma unroll
+        for (int i = 0; i < (int)FAST / 64; i++) {
+            if (i < (int)(t >> 6)) {
+                before += m.part[i];
+                cbefore += m.part32[i];
+            }
+            all += m.part[i];
+        }
+        if (t < FAST) {
+            before += sum - mass[B];
+            cbefore += cnt - count[B];
+#pragma unroll
+            for (int i = 0; i <= B; i++) {
+                mass[i] += before;
+                count[i] += cbefore;
+            }
+        }
+    }
+    // of those that weigh min_p
+    __device__ __forceinline__ uint64_t weighing() {
+        const uint32_t t = threadIdx.x;
+        uint64_t v = 0;
+        if (t < FAST)
+#pragma unroll
+            for (int i = 0; i < N; i++) v += (double)w[i] >= s.least ? w[i] : 0;
+        __syncthreads();
+        if (t < FAST) {
+            v = wave_sum64(v);
+            if ((t & 63) == 0) m.part[t >> 6] = v;
+        }
+        __syncthreads();
+        return m.part[0] + m.part[1] + m.part[2] + m.part[3];
+    }
+    // The place whose cumulative weight reaches v, or the v-th (`counted`).  False: too many tokens in its bin.
+    __device__ __forceinline__ bool place(uint64_t v, bool counted, Found& f) {
+        const uint32_t t = threadIdx.x, lane = t & 63;
+        if (t < FAST)
+#pragma unroll
+            for (int i = 0; i < B; i++)
+                if (counted ? count[i] < v && v <= count[i + 1] : mass[i] < v && v <= mass[i + 1]) {
+                    m.bin = B * t + i;
+                    m.found[0] = mass[i];
+                    m.found[1] = count[i];
+                    m.n = 0;
+                }
+        __syncthreads();
+        const uint32_t b = m.bin;
+        const uint64_t before = m.found[0];
+        const uint32_t tokens = (uint32_t)m.found[1];
+        if (t < FAST)
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i * FAST < n && x[i] != -INFINITY && (uint32_t)s.bin(x[i]) == b) {
+                    const uint32_t at = atomicAdd(&m.n, 1u);
+                    m.list[at] = (uint64_t)falling(x[i]) << 32 | (uint32_t)token[i];
+                    m.upto[at] = w[i];
+                }
+        __syncthreads();
+        const uint32_t k = m.n;
+        if (k > AT_ONCE) return false;
+        // each with each (every wave for itself)
+        for (uint32_t i0 = 0; i0 < k; i0 += 64) {
+            const uint32_t i = i0 + lane;
+            const uint64_t e = i < k ? m.list[i] : 0, own = i < k ? m.upto[i] : 0;
+            uint64_t upto = before;
+            uint32_t nth = tokens;
+            for (uint32_t j = 0; j < k; j++) {
+                const bool le = m.list[j] <= e;
+                upto += le ? m.upto[j] : 0;
+                nth += le;
+            }
+            const uint64_t who = __ballot(i < k && (counted ? nth == v : upto - own < v && v <= upto));
+            if (who) {
+                const int l = (int)__builtin_ctzll(who);
+                f = Found{lane64(upto, l), lane64(own, l), (int32_t)__builtin_amdgcn_readlane((int)(uint32_t)e, l)};
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+};
+
+// The row's token, of what its slices' workgroups listed where that is enough, of
+// the whole row otherwise.
 template <int T>
 __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
     __shared__ PickLds m;
     const uint32_t row = blockIdx.x, t = threadIdx.x;
-    Pick<T> p(a, m, row);
-    Setting& s = p.s;
+    Setting s;
     s.of(a, row);
-    const bool slices = a.slices > 0;
-    if (slices) row_max(a, row, s);
-    else p.largest();
+    const float uu = a.u[row];
+    Found f{};
+    uint64_t kept = 0;
+    const double u = uu > 0.0f ? (double)uu : 0.0;
+    const auto reach = [&](uint64_t mass) { return (uint64_t)fmax(1.0, ceil(s.p * (double)mass)); };
+    const auto drawn = [&](uint64_t mass) { return min((uint64_t)(u * (double)mass), mass - 1) + 1; };
+    Listed p(s, m);
+    bool done = p.load(a, row);
     if (s.greedy || s.first < 0) {
         if (t == 0) {
             a.tokens[row] = s.first;
@@ -567,60 +768,46 @@ __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
         }
         return;
     }
-    bool sums = !s.few;
-    p.count(slices, sums);
-    const uint32_t k = s.k < p.valid ? s.k : 0;
-    const double u = a.u[row] > 0.0f ? (double)a.u[row] : 0.0;
-    const auto reach = [&](uint64_t mass) { return (uint64_t)fmax(1.0, ceil(s.p * (double)mass)); };
-    const auto drawn = [&](uint64_t mass) { return min((uint64_t)(u * (double)mass), mass - 1) + 1; };
-    // the bins that the kept set can reach: up to the k-th token; without top-k up to
-    // top-p's border or min_p's (two bins more than where the weight falls below it),
-    // whichever comes first
-    uint32_t end = BINS - 1;
-    bool by_p = s.p < 1.0;
-    if (k) {
-        end = p.bin_of_count(k);
-    } else if (sums) {
-        if (by_p) end = p.bin_of_mass(reach(p.all));
-        if (s.least > 0.0) {
-            const float d = -__builtin_amdgcn_logf((float)(s.least / STEPS)) * (BINS / BIN_OCTAVES) + 2.0f;
-            const uint32_t b = (uint32_t)fminf(d, (float)(BINS - 1));
-            by_p &= end <= b;
-            end = min(end, b);
+    if (done) {
+        p.count_all(s.k != 0);
+        const bool whole = p.bound == -INFINITY;
+        const uint32_t k = whole && s.k >= p.n ? 0 : s.k;
+        kept = whole ? p.all : p.row_mass;
+        done = k <= p.n && (k || !s.few || whole);
+        bool inside = false;                      // some border is among the listed tokens
+        if (done && k) {
+            done = p.place(k, true, f);
+            kept = f.upto;
+            inside = true;
+        }
+        bool beyond = false;                      // top-p's is not
+        if (done && s.p < 1.0) {
+            const uint64_t w = reach(kept);
+            beyond = w > p.all;
+            if (!beyond) {
+                done = p.place(w, false, f);
+                kept = min(kept, f.upto);
+                inside = true;
+            }
+        }
+        if (done && s.least > 0.0 && (whole || (double)s.weight(p.bound) < s.least)) {
+            kept = min(kept, p.weighing());
+            inside = true;
+        } else if (done && (beyond || (s.least > 0.0 && !inside))) {
+            done = false;
+        }
+        if (done) {
+            const uint64_t w = drawn(kept);
+            done = w <= p.all && p.place(w, false, f);
         }
     }
-    Found f;
-    uint64_t kept;
-    if (p.count_after(end) <= LIST) {
-        p.gather(0, end, 0);
-        const uint32_t n = p.listed;
-        kept = sums ? p.all : m.upto[n - 1];
-        if (k) kept = m.upto[k - 1];
-        uint64_t mine = kept;
-        if (by_p) mine = min(mine, p.find(reach(kept), 0).upto);
-        if (s.least > 0.0) {
-            // the weights fall: the last that weighs min_p
-            __syncthreads();
-            if (t == 0) m.found[3] = 0;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t at = 2 * t + i;
-                const auto weighs = [&](uint32_t j) { return (double)(m.upto[j] - (j ? m.upto[j - 1] : 0)) >= s.least; };
-                if (at < n && weighs(at) && (at + 1 == n || !weighs(at + 1))) m.found[3] = m.upto[at];
-            }
-            __syncthreads();
-            mine = min(mine, m.found[3]);
-        }
-        kept = mine;
-        __syncthreads();
-        f = p.find(drawn(kept), 0);
-    } else {
-        if (!sums) p.count(false, sums = true);
-        kept = k ? p.place(k, true, false).upto : p.all;
-        if (s.p < 1.0) kept = min(kept, p.place(reach(kept), false, false).upto);
-        if (s.least > 0.0) kept = min(kept, p.least);
-        f = p.place(drawn(kept), false, true);
+    if (!done) {
+        Pick<T> q(a, s, m, row);
+        const uint32_t k = s.k < q.valid ? s.k : 0;
+        kept = k ? q.place(k, true, false).upto : q.all;
+        if (s.p < 1.0) kept = min(kept, q.place(reach(kept), false, false).upto);
+        if (s.least > 0.0) kept = min(kept, q.least);
+        f = q.place(drawn(kept), false, true);
     }
     if (t == 0) {
         a.tokens[row] = f.token;
@@ -635,14 +822,14 @@ using namespace pf;
 // ================================================================== host
 
 constexpr uint32_t SAMPLE_VOCAB = 1u << 20;
-constexpr uint32_t MOST_SLICES = 16;
 
 template <int T>
-static void sample_type(hipStream_t st, const SampleArgs& a) {
-    if (a.slices) {
-        hipLaunchKernelGGL((k_sample_max<T>), dim3(a.slices, a.rows), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((k_sample_count<T>), dim3(a.slices, a.rows), dim3(256), 0, st, a);
-    }
+static void sample_type(hipStream_t st, uint32_t tokens, const SampleArgs& a) {
+    constexpr int E = Row<T>::E;
+    const dim3 grid(a.slices, a.rows);
+    if (tokens == 8) hipLaunchKernelGGL((k_sample_slice<T, 8 / E>), grid, dim3(256), 0, st, a);
+    else if (tokens == 16) hipLaunchKernelGGL((k_sample_slice<T, 16 / E>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_sample_slice<T, 32 / E>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL((k_sample_pick<T>), dim3(a.rows), dim3(PICK), 0, st, a);
 }
 
@@ -676,21 +863,23 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     a.logits = logits; a.u = u; a.temperature = d->temperature_dev; a.top_k = d->top_k_dev; a.top_p = d->top_p_dev; a.min_p = d->min_p_dev;
     a.temperature1 = d->temperature; a.top_k1 = d->top_k; a.top_p1 = d->top_p; a.min_p1 = d->min_p;
     a.rows = rows; a.vocab = d->n_vocab; a.stride = stride; a.tokens = tokens; a.probs = probs;
-    if (d->n_vocab > 16384 && rows < 512) {
-        const uint32_t chunks = (uint32_t)(d->n_vocab * es + 15 + 15) / 16;      // (the first and the last not whole)
-        a.slices = std::min(MOST_SLICES, (1024 + rows - 1) / rows);
-        a.per = (chunks + a.slices - 1) / a.slices;
-        const size_t parts = (size_t)rows * a.slices;
-        void* ws = nullptr;
-        if (pf_status st = ctx_scratch(c, parts * (BINS * 12 + 16), &ws)) return st;
-        a.ws_mass = (uint64_t*)ws;
-        a.ws_least = a.ws_mass + parts * BINS;
-        a.ws_max = (float2*)(a.ws_least + parts);
-        a.ws_count = (uint32_t*)(a.ws_max + parts);
-    }
-    if (d->type == PF_TYPE_F32) sample_type<PF_TYPE_F32>(c->stream, a);
-    else if (d->type == PF_TYPE_F16) sample_type<PF_TYPE_F16>(c->stream, a);
-    else sample_type<PF_TYPE_BF16>(c->stream, a);
+    // tokens of a thread of the slices' workgroups: the most that leave two of them for
+    // each compute unit, of up to 64 slices (each lists its own share of a row's largest)
+    const uint32_t chunk = 16 / (uint32_t)es, off = aligned16(logits) && stride % chunk == 0 ? 0 : chunk - 1;
+    const uint32_t chunks = (off + d->n_vocab + chunk - 1) / chunk;
+    uint32_t per = 32;
+    const auto slices = [&] { return (chunks + 256 * (per / chunk) - 1) / (256 * (per / chunk)); };
+    while (per > 8 && slices() <= 32 && (uint64_t)rows * slices() < 512) per /= 2;
+    a.slices = slices();
+    a.room = a.slices > 16 ? 128 : 256;
+    const size_t parts = (size_t)rows * a.slices;
+    void* ws = nullptr;
+    if (pf_status st = ctx_scratch(c, parts * (sizeof(Slice) + a.room * 8), &ws)) return st;
+    a.ws_list = (uint64_t*)ws;
+    a.ws_slice = (Slice*)(a.ws_list + parts * a.room);
+    if (d->type == PF_TYPE_F32) sample_type<PF_TYPE_F32>(c->stream, per, a);
+    else if (d->type == PF_TYPE_F16) sample_type<PF_TYPE_F16>(c->stream, per, a);
+    else sample_type<PF_TYPE_BF16>(c->stream, per, a);
     PF_LAUNCHED(c);
     return PF_OK;
 }
