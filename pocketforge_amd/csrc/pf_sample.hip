@@ -45,11 +45,11 @@ struct SampleArgs {
     uint64_t* ws_list;            // [rows][slices][room]
 };
 
-// What a slice's workgroup found: the largest logit and its first token, the sum
-// of the weights beside that logit's, the bound above which tokens are listed, and
-// their number (more than the room: not all of them are).
+// What a slice's workgroup found: the largest logit and its first token, the bound
+// from which on tokens are listed, their number (more than the room: not all of
+// them are), and the weight of the others beside the largest logit's.
 struct Slice {
-    uint64_t mass;
+    uint64_t rest;
     float max;
     int32_t first;
     float bound;
@@ -57,7 +57,8 @@ struct Slice {
 };
 
 // A row in chunks of 16 bytes from the last multiple of 16 on; what lies before its
-// first or behind its last token reads as -infinity, and so does a NaN.
+// first or behind its last token reads as -infinity.  (Masked tokens are those that
+// do not compare above -infinity, so NaN too.)
 template <int T>
 struct Row {
     static constexpr int E = T == PF_TYPE_F32 ? 4 : 8;
@@ -72,23 +73,62 @@ struct Row {
         chunks = (uint32_t)(skip + n + E - 1) / E;
     }
     // tokens E c - skip ..
-    __device__ __forceinline__ void load(uint32_t c, float (&x)[E]) const {
+    __device__ __forceinline__ u4v raw(uint32_t c) const {
         const int t0 = (int)(c * E) - skip;
-        if (t0 >= 0 && t0 + E <= n) {
-            if constexpr (T == PF_TYPE_F32) load4<T>(at + (size_t)c * 16, x);
-            else load8<T>(at + (size_t)c * 16, x);
-        } else {
+        if (t0 >= 0 && t0 + E <= n) return *(const u4v*)(at + (size_t)c * 16);
+        u4v w;
 #pragma unroll
-            for (int i = 0; i < E; i++) {
-                x[i] = -INFINITY;
-                if (t0 + i >= 0 && t0 + i < n) {
-                    if constexpr (T == PF_TYPE_F32) x[i] = ((const float*)at)[t0 + i + skip];
-                    else x[i] = to_float<T>(((const short*)at)[t0 + i + skip]);
-                }
+        for (int i = 0; i < E; i++) {
+            const bool in = t0 + i >= 0 && t0 + i < n;
+            if constexpr (T == PF_TYPE_F32) {
+                w[i] = in ? ((const uint32_t*)at)[t0 + i + skip] : 0xFF800000u;
+            } else {
+                const uint32_t v = in ? ((const uint16_t*)at)[t0 + i + skip] : T == PF_TYPE_BF16 ? 0xFF80u : 0xFC00u;
+                w[i / 2] = i % 2 ? w[i / 2] | v << 16 : v;
             }
         }
+        return w;
+    }
+    static __device__ __forceinline__ float value(u4v w, int i) {
+        if constexpr (T == PF_TYPE_F32) return __builtin_bit_cast(float, (uint32_t)w[i]);
+        else if constexpr (T == PF_TYPE_BF16) return __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+        else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i / 2] >> (i % 2 * 16)));
+    }
+    __device__ __forceinline__ float one(int32_t token) const {
+        if constexpr (T == PF_TYPE_F32) return ((const float*)at)[skip + token];
+        else return to_float<T>(((const short*)at)[skip + token]);
+    }
+    // A workgroup of THREADS goes through the row, with many loads under way: f(chunks,
+    // the first one's first token, a bit for each token that is in range); a thread's
+    // chunks lie THREADS apart.
+    template <int THREADS, class F>
+    __device__ __forceinline__ void batches(F&& f) const {
+        constexpr int U = 8;
+        for (uint32_t c0 = threadIdx.x; c0 - threadIdx.x < chunks; c0 += U * THREADS) {
+            u4v w[U];
+            uint64_t in = 0;
 #pragma unroll
-        for (int i = 0; i < E; i++) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
+            for (int u = 0; u < U; u++) {
+                w[u] = (u4v)0u;
+                if (c0 + u * THREADS < chunks) {
+                    w[u] = raw(c0 + u * THREADS);
+                    in |= ((1ull << E) - 1) << (u * E);
+                }
+            }
+            f(w, (int32_t)(c0 * E) - skip, in);
+        }
+    }
+    // f(value, token) of each
+    template <int THREADS, class F>
+    __device__ __forceinline__ void each(F&& f) const {
+        batches<THREADS>([&](const auto& w, int32_t t0, uint64_t in) {
+            constexpr int U = sizeof(w) / sizeof(u4v);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (in >> (u * E) & 1)
+#pragma unroll
+                    for (int i = 0; i < E; i++) f(value(w[u], i), t0 + u * THREADS * E + i);
+        });
     }
 };
 
@@ -99,7 +139,8 @@ struct Setting {
     bool greedy;
     uint32_t k;                   // 0: off
     double scale, p, least;       // log2(e) / T; p >= 1: off; min_p in steps, 0: off
-    float to_bin;
+    float to_bin, hi, lo;
+    bool plain;
     bool few;                     // top-k alone decides how far to look: no sums over the row
     __device__ __forceinline__ void of(const SampleArgs& a, uint32_t row) {
         const float t = a.temperature ? a.temperature[row] : a.temperature1;
@@ -120,6 +161,16 @@ struct Setting {
     // (l - max) / T in octaves, as far as weights reach
     __device__ __forceinline__ double octaves(float l) const {
         return l == max ? 0.0 : fmax(((double)l - (double)max) * scale, -60.0);
+    }
+    // the same in fp32, where `plain`: off by 2^-19 at most where weights reach, to either side
+    __device__ __forceinline__ void fp32() {
+        hi = (float)scale;
+        lo = (float)(scale - (double)hi);
+        plain = max < INFINITY && hi > 1e-30f && hi < 1e30f;
+    }
+    __device__ __forceinline__ float octaves32(float l) const {
+        const float d = fmaxf(l - max, -3.4028234663852886e38f);       // (masked: no weight)
+        return fmaf(d, hi, d * lo);
     }
     // 2^43 2^x to the nearest whole number: 2^x = 2^n e^(f ln 2) with |f| <= 1/2, the
     // series up to z^11 (z^12 / 12! = 6e-15, 2^-47)
@@ -223,6 +274,7 @@ __global__ __launch_bounds__(256) void k_sample_slice(SampleArgs a) {
     __shared__ float s_max[4];
     __shared__ uint32_t s_bound[4], s_listed, s_first;
     __shared__ uint64_t s_mass[4];
+    __shared__ float s_x[N * E][256];
     const uint32_t row = blockIdx.y, t = threadIdx.x, wave = t >> 6;
     if (t == 0) {
         s_listed = 0;
@@ -235,10 +287,11 @@ __global__ __launch_bounds__(256) void k_sample_slice(SampleArgs a) {
     const auto token = [&](int n, int i) { return (int32_t)(chunk(n) * E) - r.skip + i; };
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        if (chunk(n) < r.chunks) r.load(chunk(n), x[n]);
-        else
+        u4v w = {};
+        const bool in = chunk(n) < r.chunks;
+        if (in) w = r.raw(chunk(n));
 #pragma unroll
-            for (int i = 0; i < E; i++) x[n][i] = -INFINITY;
+        for (int i = 0; i < E; i++) x[n][i] = in ? Row<T>::value(w, i) : -INFINITY;
     }
     Setting s;
     s.of(a, row);
@@ -278,31 +331,41 @@ __global__ __launch_bounds__(256) void k_sample_slice(SampleArgs a) {
             some += s_bound[w] != 0;
         }
         if (some) bound = falling_value(~(uint32_t)(sum / some));
+        // a bit for each of the thread's tokens that are listed; the values to LDS, where
+        // a number picks one
+        const float above = fmaxf(bound, -3.4028234663852886e38f);
         uint32_t hits = 0;
+        // The weights of the others in fp32, exponents too: the sum of a thousand different
+        // ones is off by some 2^-24 of itself, and it is a small part of the row's where that
+        // sum is used.
+        s.fp32();
+        float rest = 0.0f;
 #pragma unroll
         for (int n = 0; n < N; n++)
 #pragma unroll
-            for (int i = 0; i < E; i++) hits += (x[n][i] >= bound) & (x[n][i] > -INFINITY);
-        const uint32_t upto = wave_scan(hits);
+            for (int i = 0; i < E; i++) {
+                const bool hit = x[n][i] >= above;
+                hits |= (hit ? 1u : 0u) << (n * E + i);
+                s_x[n * E + i][t] = x[n][i];
+                if (!s.few) rest += __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
+            }
+        const uint32_t upto = wave_scan((uint32_t)__popc(hits));
         uint32_t at = 0;
         if ((t & 63) == 63) at = atomicAdd(&s_listed, upto);
-        at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - hits;
-        uint64_t* list = a.ws_list + ((size_t)row * a.slices + blockIdx.x) * a.room;
         if (!s.few) {
-#pragma unroll
-            for (int n = 0; n < N; n++)
-#pragma unroll
-                for (int i = 0; i < E; i++) mass += s.weight(x[n][i]);
+            mass = (uint64_t)((double)rest * STEPS);
+            if (!s.plain) {
+                mass = 0;
+                for (uint32_t b = ~hits & (~0u >> (32 - N * E)); b; b &= b - 1) mass += s.weight(s_x[__builtin_ctz(b)][t]);
+            }
             mass = wave_sum64(mass);
         }
-#pragma unroll
-        for (int n = 0; n < N; n++)
-#pragma unroll
-            for (int i = 0; i < E; i++)
-                if (x[n][i] >= bound && x[n][i] > -INFINITY) {
-                    if (at < a.room) list[at] = (uint64_t)falling(x[n][i]) << 32 | (uint32_t)token(n, i);
-                    at++;
-                }
+        at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - (uint32_t)__popc(hits);
+        uint64_t* list = a.ws_list + ((size_t)row * a.slices + blockIdx.x) * a.room;
+        for (; hits; hits &= hits - 1, at++) {
+            const int b = __builtin_ctz(hits);
+            if (at < a.room) list[at] = (uint64_t)falling(s_x[b][t]) << 32 | (uint32_t)token(b / E, b % E);
+        }
     }
     if ((t & 63) == 0) s_mass[wave] = mass;
     __syncthreads();
@@ -322,11 +385,14 @@ struct Found {
     int32_t token;
 };
 
+constexpr int TAIL_BINS = 256, TAIL_COPIES = 32;
+constexpr float TAIL_OCTAVES = 32.0f;  // of weights below the listed tokens', that these bins cover
 struct PickLds {
     uint32_t count[BINS];         // tokens of a bin; then before it
     uint64_t mass[BINS];          // weight of a bin; then before it
     uint64_t list[LIST];          // falling(logit) << 32 | token; or a digit's histogram
     uint64_t upto[LIST];          // cumulative weights of the sorted list
+    uint64_t wide[TAIL_BINS * TAIL_COPIES];
     uint64_t part[PICK / 64], found[4];
     uint32_t part32[PICK / 64], n, bin;
 };
@@ -376,14 +442,9 @@ struct Pick {
 
     template <class F>
     __device__ __forceinline__ void each(F&& f) const {
-#pragma unroll 2
-        for (uint32_t c = threadIdx.x; c < r.chunks; c += PICK) {
-            float x[E];
-            r.load(c, x);
-#pragma unroll
-            for (int i = 0; i < E; i++)
-                if (x[i] != -INFINITY) f(x[i], (int32_t)(c * E) - r.skip + i);
-        }
+        r.template each<PICK>([&](float x, int32_t token) {
+            if (x > -INFINITY) f(x, token);
+        });
     }
 
     // the histogram, then what lies before each bin
@@ -491,15 +552,17 @@ struct Pick {
             uint64_t n = 0, total;
             const bool in = c0 + t < r.chunks;
             if (in) {
-                r.load(c0 + t, x);
+                const u4v w4 = r.raw(c0 + t);
 #pragma unroll
-                for (int i = 0; i < E; i++) n += x[i] != -INFINITY && falling(x[i]) == prefix;
+                for (int i = 0; i < E; i++) x[i] = Row<T>::value(w4, i);
+#pragma unroll
+                for (int i = 0; i < E; i++) n += x[i] > -INFINITY && falling(x[i]) == prefix;
             }
             uint64_t at = seen + scan64(m, n, &total);
             if (in && at <= nth && nth < at + n)
 #pragma unroll
                 for (int i = 0; i < E; i++)
-                    if (x[i] != -INFINITY && falling(x[i]) == prefix && at++ == nth) m.found[3] = (uint64_t)((int64_t)((c0 + t) * E) - r.skip + i);
+                    if (x[i] > -INFINITY && falling(x[i]) == prefix && at++ == nth) m.found[3] = (uint64_t)((int64_t)((c0 + t) * E) - r.skip + i);
             seen += total;
             __syncthreads();
             if (nth < seen) {
@@ -535,10 +598,37 @@ struct Pick {
     }
 };
 
+constexpr uint32_t AT_ONCE = 256;      // tokens of one bin that are put in order by comparing each with each
+
+// Of k entries of m.list, weights in m.upto: the one at which the weight behind
+// `before` reaches v, or the number behind `tokens` (every wave for itself).
+__device__ __forceinline__ bool in_order(const PickLds& m, uint32_t k, uint64_t before, uint32_t tokens, uint64_t v, bool counted,
+                                         Found& f) {
+    const uint32_t lane = threadIdx.x & 63;
+    bool found = false;
+    for (uint32_t i0 = 0; i0 < k; i0 += 64) {
+        const uint32_t i = i0 + lane;
+        const uint64_t e = i < k ? m.list[i] : 0, own = i < k ? m.upto[i] : 0;
+        uint64_t upto = before;
+        uint32_t nth = tokens;
+        for (uint32_t j = 0; j < k; j++) {
+            const bool le = m.list[j] <= e;
+            upto += le ? m.upto[j] : 0;
+            nth += le;
+        }
+        const uint64_t who = __ballot(i < k && (counted ? nth == v : upto - own < v && v <= upto));
+        if (who) {
+            const int l = (int)__builtin_ctzll(who);
+            f = Found{lane64(upto, l), lane64(own, l), (int32_t)__builtin_amdgcn_readlane((int)(uint32_t)e, l)};
+            found = true;
+        }
+    }
+    return found;
+}
+
 // The listed tokens of a row: four waves have them in registers, the others take
 // part where all are needed.
 constexpr uint32_t FAST = 256;
-constexpr uint32_t AT_ONCE = 256;      // tokens of one bin that are put in order by comparing each with each
 struct Listed {
     static constexpr int N = LIST / FAST, B = BINS / FAST;
     Setting& s;
@@ -551,7 +641,7 @@ struct Listed {
     uint32_t n;                   // tokens
     uint64_t all;                 // their weight
     float bound;                  // what is not listed is below it
-    uint64_t row_mass;            // of the whole row, where top-k does not end it
+    uint64_t row_mass;            // of what is below it, where top-k does not end the row
 
     __device__ __forceinline__ Listed(Setting& s, PickLds& m) : s(s), m(m) {}
 
@@ -563,13 +653,13 @@ struct Listed {
         m.count[t] = 0;
         m.mass[t] = 0;
         if (t == 0) m.n = 0;
-        // (a wave a slice, asked for before its bound is known)
+        // (a wave 256 tokens of a slice, asked for before its bound is known)
         constexpr uint32_t W = PICK / 64;
-        const uint32_t first = __builtin_amdgcn_readfirstlane(t >> 6);
+        const uint32_t first = __builtin_amdgcn_readfirstlane(t >> 6), parts = (a.room + 255) / 256;
         uint64_t e[4];
-        if (first < a.slices)
+        if (first < a.slices * parts)
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++) e[j] = lane + 64 * j < a.room ? list[first * a.room + lane + 64 * j] : 0;
+            for (uint32_t j = 0; j < 4; j++) e[j] = lane + 64 * j < a.room ? list[first * min(a.room, 256u) + lane + 64 * j] : 0;
         float top = -INFINITY;
         uint32_t none = NO_TOKEN, most = 0;
         bound = -INFINITY;
@@ -592,18 +682,23 @@ struct Listed {
         row_mass = 0;
         for (uint32_t i = lane; i < a.slices && !s.few; i += 64) {
             const Slice q = slices[i];
-            if (q.max == s.max) row_mass += q.mass;
-            else if (q.mass) row_mass += (uint64_t)rint((double)q.mass * exp2(s.octaves(q.max)));
+            if (q.max == s.max) row_mass += q.rest;
+            else if (q.rest) row_mass += (uint64_t)rint((double)q.rest * exp2(s.octaves(q.max)));
         }
         row_mass = wave_sum64(row_mass);
+        uint64_t below = 0;                       // of listed tokens that others may come before
         __syncthreads();
-        for (uint32_t i = first; i < a.slices; i += W) {
-            const uint32_t listed = slices[i].listed;
+        for (uint32_t i = first; i < a.slices * parts; i += W) {
+            const uint32_t from = (i & (parts - 1)) * 256, some = slices[i >> __builtin_ctz(parts)].listed, listed = some - min(from, some);
             uint32_t keep = 0, on = 0;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {
-                if (i != first) e[j] = lane + 64 * j < listed ? list[i * a.room + lane + 64 * j] : 0;
-                if (lane + 64 * j < listed && falling_value((uint32_t)(e[j] >> 32)) >= bound) on |= 1u << j;
+                if (i != first) e[j] = lane + 64 * j < listed ? list[i * min(a.room, 256u) + lane + 64 * j] : 0;
+                const float x = falling_value((uint32_t)(e[j] >> 32));
+                if (lane + 64 * j < listed) {
+                    if (x >= bound) on |= 1u << j;
+                    else if (!s.few) below += s.weight(x);
+                }
                 keep += (uint32_t)__popcll(__ballot(on >> j & 1));
             }
             uint32_t at = 0;
@@ -617,8 +712,13 @@ struct Listed {
                 at += (uint32_t)__popcll(who);
             }
         }
+        if (!s.few) {
+            below = wave_sum64(below);
+            if (lane == 0) m.part[first] = below;
+        }
         __syncthreads();
         n = m.n;
+        if (!s.few) row_mass += wave_sum64(lane < W ? m.part[lane] : 0);
         return n <= LIST;
     }
 
@@ -698,7 +798,7 @@ struct Listed {
     }
     // The place whose cumulative weight reaches v, or the v-th (`counted`).  False: too many tokens in its bin.
     __device__ __forceinline__ bool place(uint64_t v, bool counted, Found& f) {
-        const uint32_t t = threadIdx.x, lane = t & 63;
+        const uint32_t t = threadIdx.x;
         if (t < FAST)
 #pragma unroll
             for (int i = 0; i < B; i++)
@@ -723,30 +823,188 @@ struct Listed {
         __syncthreads();
         const uint32_t k = m.n;
         if (k > AT_ONCE) return false;
-        // each with each (every wave for itself)
-        for (uint32_t i0 = 0; i0 < k; i0 += 64) {
-            const uint32_t i = i0 + lane;
-            const uint64_t e = i < k ? m.list[i] : 0, own = i < k ? m.upto[i] : 0;
-            uint64_t upto = before;
-            uint32_t nth = tokens;
-            for (uint32_t j = 0; j < k; j++) {
-                const bool le = m.list[j] <= e;
-                upto += le ? m.upto[j] : 0;
-                nth += le;
-            }
-            const uint64_t who = __ballot(i < k && (counted ? nth == v : upto - own < v && v <= upto));
-            if (who) {
-                const int l = (int)__builtin_ctzll(who);
-                f = Found{lane64(upto, l), lane64(own, l), (int32_t)__builtin_amdgcn_readlane((int)(uint32_t)e, l)};
-            }
+        in_order(m, k, before, tokens, v, counted, f);
+        __syncthreads();
+        return true;
+    }
+};
+
+// What a row has below its listed tokens, in weights beside `bound`'s in steps of
+// 2^-30 or finer: a border or a token in flat rows.  One compute unit goes through the row:
+// once for a histogram by value, kept 32 times so that a pair of lanes has one in
+// LDS banks of its own, and once for the tokens of the bin; these again by a finer
+// histogram, so that only a few have to be put in order.
+template <int T>
+struct Tail {
+    const Row<T> r;
+    const Setting& s;
+    PickLds& m;
+    const float bound;
+    float unit, per_bin;          // weights to steps; values to bins
+    double by;                    // steps of 2^43 to these
+    uint64_t all, least = 0;      // of all; of those that weigh min_p
+
+    // (the exponent's product in two pieces: 16-bit logits have few values, whose
+    // roundings would add up)
+    __device__ __forceinline__ uint32_t weight(float x) const {
+        const float d = x - s.max, o = d * s.hi, more = fmaf(d, s.lo, fmaf(d, s.hi, -o));
+        const float w = __builtin_amdgcn_exp2f(o);
+        return (uint32_t)(fmaf(w, more * 0.693147181f, w) * unit);
+    }
+    // 0 .. TAIL_BINS - 1 (and what is left behind the point, up to the last); never falls as x falls
+    __device__ __forceinline__ float place_of(float x) const { return fminf(((s.max - x) - (s.max - bound)) * per_bin, TAIL_BINS - 0.001f); }
+    __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)place_of(x); }
+
+    __device__ __forceinline__ Tail(const SampleArgs& a, const Setting& s, PickLds& m, uint32_t row, float bound)
+        : r(a, row), s(s), m(m), bound(bound) {
+        const uint32_t t = threadIdx.x;
+        const float o = floorf(s.octaves32(bound));
+        unit = __builtin_amdgcn_ldexpf(1.0f, 30 - (int)o);
+        by = exp2(-13.0 - (double)o);
+        per_bin = s.hi * (TAIL_BINS / TAIL_OCTAVES);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TAIL_BINS * TAIL_COPIES / PICK; i++) m.wide[t + i * PICK] = 0;
+        __syncthreads();
+        const uint32_t some = s.least > 0.0 ? (uint32_t)fmin(s.least * by, 4294967295.0) : ~0u;
+        uint64_t* own = m.wide + t % TAIL_COPIES;
+        r.template each<PICK>([&](float x, int32_t) {
+            if (!(x < bound && x > -INFINITY)) return;
+            const uint32_t w = weight(x);
+            atomicAdd((unsigned long long*)&own[bin(x) * TAIL_COPIES], (unsigned long long)w);
+            if (some != ~0u) least += w >= some ? w : 0;
+        });
+        __syncthreads();
+        uint64_t w = 0;
+        if (t < TAIL_BINS)
+            for (int i = 0; i < TAIL_COPIES; i++) w += m.wide[t * TAIL_COPIES + (t + i) % TAIL_COPIES];
+        const uint64_t before = scan64(m, w, &all);
+        m.mass[t] = before;
+        if (s.least > 0.0) scan64(m, least, &least);
+        __syncthreads();
+    }
+    // The place whose cumulative weight reaches v (from 1, to `all`): f.upto in these
+    // weights, f.weight of 2^43.  False: more tokens in its bin than are kept.
+    __device__ __forceinline__ bool place(uint64_t v, Found& f) {
+        const uint32_t t = threadIdx.x, lane = t & 63;
+        __syncthreads();
+        if (t < TAIL_BINS && m.mass[t] < v && v <= m.mass[t + 1]) m.bin = t;      // (behind the last: all)
+        if (t == 0) m.n = 0;
+        m.wide[t] = 0;
+        __syncthreads();
+        const uint32_t b = m.bin;
+        uint64_t before = m.mass[b];
+        // the largest values of the bin and of the next one, digit by digit (the bins never fall as values fall)
+        uint32_t key = 0;
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+            const float x = falling_value(~(key | bit));
+            if (x <= bound && bin(x) >= b + (lane & 1)) key |= bit;
         }
+        const float top = falling_value(~(uint32_t)__builtin_amdgcn_readlane((int)key, 0));
+        const float under = b + 1 < TAIL_BINS ? falling_value(~(uint32_t)__builtin_amdgcn_readlane((int)key, 1)) : -INFINITY;
+        uint32_t* tokens = (uint32_t*)m.upto;
+        r.template batches<PICK>([&](const auto& w, int32_t t0, uint64_t in) {
+            typedef std::remove_reference_t<decltype(w)> W;
+            constexpr int U = sizeof(W) / sizeof(u4v), E = Row<T>::E;
+            uint64_t hits = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < E; i++) {
+                    const float x = Row<T>::value(w[u], i);
+                    hits |= (x <= top && x > under && x < bound ? 1ull : 0ull) << (u * E + i);
+                }
+            hits &= in;
+            const uint32_t n = (uint32_t)__popcll(hits), upto = wave_scan(n);
+            uint32_t at = 0;
+            if (lane == 63 && upto) at = atomicAdd(&m.n, upto);
+            at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - n;
+            for (; hits; hits &= hits - 1, at++) {
+                const int h = __builtin_ctzll(hits);
+                if (at < LIST) tokens[at] = (uint32_t)(t0 + h / E * (int)(PICK * E) + h % E);
+            }
+        });
+        __syncthreads();
+        const uint32_t n = m.n;
+        if (n > LIST) return false;
+        // finer: two of them a thread
+        float x[2];
+        int32_t token[2];
+        uint32_t w[2], fine[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t at = t + i * PICK;
+            x[i] = -INFINITY;
+            fine[i] = ~0u;
+            if (at >= n) continue;
+            token[i] = (int32_t)tokens[at];
+            x[i] = r.one(token[i]);
+            w[i] = weight(x[i]);
+            fine[i] = min((uint32_t)((place_of(x[i]) - (float)b) * (float)BINS), (uint32_t)BINS - 1);
+            if (w[i]) atomicAdd((unsigned long long*)&m.wide[fine[i]], (unsigned long long)w[i]);
+        }
+        __syncthreads();
+        uint64_t total;
+        const uint64_t own = m.wide[t];
+        uint64_t at = before + scan64(m, own, &total);
+        if (at < v && v <= at + own) {
+            m.bin = t;
+            m.found[0] = at;
+        }
+        if (t == 0) m.n = 0;
+        __syncthreads();
+        before = m.found[0];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (fine[i] == m.bin) {
+                const uint32_t to = atomicAdd(&m.n, 1u);
+                m.list[to] = (uint64_t)falling(x[i]) << 32 | (uint32_t)token[i];
+                m.upto[to] = w[i];
+            }
+        __syncthreads();
+        const uint32_t k = m.n;
+        if (k <= AT_ONCE) {
+            if (!in_order(m, k, before, 0, v, false, f)) return false;
+        } else {
+            // many: all of one value, in the order of their numbers; or digit by digit over the row
+            const uint64_t e = m.list[0];
+            bool same = true;
+            for (uint32_t i = t; i < k; i += PICK) same &= m.list[i] >> 32 == e >> 32;
+            if (!__syncthreads_and(same)) return false;
+            const uint64_t each = m.upto[0];
+            uint32_t nth = (uint32_t)((v - before - 1) / each);
+            f.upto = before + (nth + 1) * each;
+            int32_t found = 0;
+#pragma unroll
+            for (int shift = 10; shift >= 0; shift -= 10) {
+                __syncthreads();
+                m.wide[t] = 0;
+                __syncthreads();
+                for (uint32_t i = t; i < k; i += PICK) {
+                    const uint32_t number = (uint32_t)m.list[i];
+                    if (shift || number >> 10 == (uint32_t)found) atomicAdd((unsigned long long*)&m.wide[number >> shift & 1023], 1ull);
+                }
+                __syncthreads();
+                const uint64_t c = m.wide[t], to = scan64(m, c, &total);
+                if (to <= nth && nth < to + c) {
+                    m.found[0] = t;
+                    m.found[1] = to;
+                }
+                __syncthreads();
+                nth -= (uint32_t)m.found[1];
+                found = found << 10 | (int32_t)m.found[0];
+            }
+            f.token = found;
+        }
+        f.weight = s.weight(r.one(f.token));
         __syncthreads();
         return true;
     }
 };
 
 // The row's token, of what its slices' workgroups listed where that is enough, of
-// the whole row otherwise.
+// the rest of the row where a border or the token lies there, of the whole row
+// where listed tokens do not fit or top-k goes beyond them.
 template <int T>
 __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
     __shared__ PickLds m;
@@ -770,35 +1028,64 @@ __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
     }
     if (done) {
         p.count_all(s.k != 0);
+        s.fp32();
         const bool whole = p.bound == -INFINITY;
         const uint32_t k = whole && s.k >= p.n ? 0 : s.k;
-        kept = whole ? p.all : p.row_mass;
+        uint64_t rest = whole ? 0 : p.row_mass;
         done = k <= p.n && (k || !s.few || whole);
-        bool inside = false;                      // some border is among the listed tokens
         if (done && k) {
             done = p.place(k, true, f);
             kept = f.upto;
-            inside = true;
+            rest = 0;
+        } else {
+            kept = p.all + rest;
         }
-        bool beyond = false;                      // top-p's is not
-        if (done && s.p < 1.0) {
+        // borders among the listed tokens
+        bool p_below = s.p < 1.0, m_below = s.least > 0.0 && !whole && !((double)s.weight(p.bound) < s.least);
+        if (done && p_below) {
             const uint64_t w = reach(kept);
-            beyond = w > p.all;
-            if (!beyond) {
+            p_below = w > p.all;
+            if (!p_below) {
                 done = p.place(w, false, f);
                 kept = min(kept, f.upto);
-                inside = true;
+                rest = 0;
             }
         }
-        if (done && s.least > 0.0 && (whole || (double)s.weight(p.bound) < s.least)) {
+        if (done && s.least > 0.0 && !m_below) {
             kept = min(kept, p.weighing());
-            inside = true;
-        } else if (done && (beyond || (s.least > 0.0 && !inside))) {
-            done = false;
+            rest = 0;
         }
-        if (done) {
+        // (borders further on matter if none was found)
+        if (done && (rest == 0 || !(p_below || m_below))) {
             const uint64_t w = drawn(kept);
-            done = w <= p.all && p.place(w, false, f);
+            if (w <= p.all) {
+                done = p.place(w, false, f);
+                rest = 0;
+            }
+        }
+        if (done && rest) {
+            done = s.plain;
+            if (done) {
+                Tail<T> q(a, s, m, row, p.bound);
+                // weights of 2^43 to those beside the bound's and back
+                const double by = q.by;
+                const auto to = [&](uint64_t v) { return min(max((uint64_t)ceil((double)(v - p.all) * by), (uint64_t)1), q.all); };
+                const auto back = [&](uint64_t v) { return p.all + (uint64_t)rint((double)v / by); };
+                done = q.all > 0;
+                kept = back(q.all);
+                if (done && p_below) {
+                    const uint64_t w = reach(kept);
+                    if (w > p.all) {
+                        done = q.place(to(w), f);
+                        kept = min(kept, back(f.upto));
+                    }
+                }
+                if (done && m_below) kept = min(kept, back(q.least));
+                if (done) {
+                    const uint64_t w = drawn(kept);
+                    done = w > p.all && q.place(to(w), f);
+                }
+            }
         }
     }
     if (!done) {
@@ -871,7 +1158,7 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     const auto slices = [&] { return (chunks + 256 * (per / chunk) - 1) / (256 * (per / chunk)); };
     while (per > 8 && slices() <= 32 && (uint64_t)rows * slices() < 512) per /= 2;
     a.slices = slices();
-    a.room = a.slices > 16 ? 128 : 256;
+    a.room = a.slices <= 2 ? 2048 : a.slices <= 4 ? 1024 : a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
     const size_t parts = (size_t)rows * a.slices;
     void* ws = nullptr;
     if (pf_status st = ctx_scratch(c, parts * (sizeof(Slice) + a.room * 8), &ws)) return st;
