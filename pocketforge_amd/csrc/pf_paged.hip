@@ -18,8 +18,9 @@ namespace pf {
 
 // Waves of a SIMD (workgroups of a compute unit) that the registers allow: the
 // next tile's rows wait in registers, and fp32 rows take three operands each.
-__host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
+__host__ __device__ constexpr int paged_waves(int act, int ct, int dp, int nt) {
     const bool wide = act == PF_TYPE_F32;
+    if (ct == PF_TYPE_FP4 && dp == 128 && nt == 1) return 3;
     return dp == 64 ? (nt == 1 ? (wide ? 3 : 4) : 2) : nt == 1 ? 2 : wide ? 1 : 2;
 }
 
@@ -39,7 +40,7 @@ __host__ __device__ constexpr int paged_waves(int act, int dp, int nt) {
 // round trip, the codes' way to bf16 and three products per piece of the rows.
 // One context of 700 keys: 5.8 us and the join's 3.5, both latency.
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
-__global__ __launch_bounds__(64 * W, paged_waves(ACT, DP, NT)) void k_paged_attn(PagedArgs a) {
+__global__ __launch_bounds__(64 * W, paged_waves(ACT, CT, DP, NT)) void k_paged_attn(PagedArgs a) {
     // Weights over int8 rows take the rows' scales, whose range fp16 does not
     // have, so their products with the codes are in bf16 for fp16 rows too.  4-bit
     // values are bf16 (with their scales: fp16 has not their range either), and
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedArgs a) {
 template <int ACT, int CT, int DP, int NT, bool EXACT>
 static void paged_one(hipStream_t st, const PageSplit& u, uint32_t z, const PagedArgs& a) {
     const dim3 grid(u.n_items, a.kv_heads, z);
-    if constexpr (paged_waves(ACT, DP, NT) > 1)
+    if constexpr (paged_waves(ACT, CT, DP, NT) > 1)
         if (u.waves == 8) {
             hipLaunchKernelGGL((k_paged_attn<ACT, CT, DP, NT, EXACT, 8>), grid, dim3(512), 0, st, a);
             return;
@@ -474,7 +475,13 @@ static void paged_dim(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
 // verify passes of five fp32 rows over up to 2100 int8 keys of 16 heads, 23 us
 // uncut with 8, 27 cut with 4).  Contexts of 60000 and 32000 fp16 keys take 23
 // us cut, 510 uncut.
-constexpr uint32_t PG_CUS = 256, PG_JOIN = 5, PG_JOIN_ROWS = 512;
+//
+// Tiles of 4-bit rows take a third of the time, so joining counts twice as much
+// (PG_JOIN4; one context of 700, 16 heads: 9.5 us cut, 7.5 uncut), and a third
+// workgroup on each compute unit, which the registers allow, keeps more bytes
+// under way where a wave has many of them (PG_LONG or more; 64 contexts of up to
+// 16000: 72 us with three, 78.5 with two; two of 120000, 6 a wave: 21 and 19).
+constexpr uint32_t PG_CUS = 256, PG_JOIN = 5, PG_JOIN4 = 10, PG_JOIN_ROWS = 512, PG_LONG = 24;
 struct PageShares {
     uint32_t chunk = 1, waves = 4;
     uint64_t cost = ~0ull;
@@ -510,7 +517,7 @@ struct PagePlan {
     uint32_t most = 0, longest = 0, keys = 0;   // rows, tiles and keys of a sequence at most
     PageShares shares;
 };
-static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc* d, const AttnShape& s) {
+static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc* d, int32_t ct, const AttnShape& s) {
     PagePlan n;
     n.tiles.reserve(pass.size());
     uint64_t rows = 0;
@@ -523,8 +530,14 @@ static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc*
         rows += q.rows;
     }
     const uint64_t R = (uint64_t)n.most * (d->n_heads / d->n_kv_heads), per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
-    const uint32_t held = (uint32_t)paged_waves(d->type, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
-    const uint64_t join = PG_JOIN + rows * d->n_heads / PG_JOIN_ROWS;
+    uint32_t held = (uint32_t)paged_waves(d->type, ct, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
+    const bool fp4 = ct == PF_TYPE_FP4;
+    if (fp4 && held == 3) {
+        uint64_t all = 0;
+        for (uint32_t t : n.tiles) all += t;
+        if (all * per < PG_LONG * 4 * 2 * PG_CUS) held = 2;
+    }
+    const uint64_t join = (fp4 ? PG_JOIN4 : PG_JOIN) + rows * d->n_heads / PG_JOIN_ROWS;
     page_shares(n.tiles, n.longest, per, (uint64_t)PG_CUS * held, 4, join, &n.shares);
     if (held > 1) page_shares(n.tiles, n.longest, per, (uint64_t)PG_CUS * (held / 2), 8, join, &n.shares);
     return n;
@@ -536,7 +549,7 @@ extern "C" pf_status pf_test_pages_plan(const pf_attn_desc* d, const uint32_t* r
     return no_throw(nullptr, [&] {
         std::vector<PageSeq> pass;
         for (uint32_t i = 0; i < n; i++) pass.push_back({i, 0, rows[i], lens[i]});
-        const PagePlan plan = paged_plan(pass, d, s);
+        const PagePlan plan = paged_plan(pass, d, d->type, s);
         *waves = plan.shares.waves;
         *chunk = plan.shares.chunk;
         *longest = plan.longest;
@@ -546,7 +559,7 @@ extern "C" pf_status pf_test_pages_plan(const pf_attn_desc* d, const uint32_t* r
 static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
     PageSplit& u = p->cut;
     if (u.type == d->type && u.window == s.window && u.sink == s.sink && u.heads == d->n_heads) return PF_OK;
-    const PagePlan plan = paged_plan(p->pass, d, s);
+    const PagePlan plan = paged_plan(p->pass, d, p->cfg.type, s);
     if ((uint64_t)plan.most * (d->n_heads / d->n_kv_heads) > 32 * 65535u)
         return fail(p->ctx, PF_ERR_UNSUPPORTED, "pages: too many rows in one pass; cut it");
     const uint32_t chunk = plan.shares.chunk;
