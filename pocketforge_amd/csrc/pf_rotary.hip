@@ -83,27 +83,34 @@ __device__ __forceinline__ void turn_of(const double* table, uint32_t pair, doub
 // A lane's part of a turn: dims d .. d + 7 of a head.  Pairs 2i, 2i + 1 lie in the
 // lane; of pairs i, i + turn / 2 the lane holds one half and reads the other from
 // where the row came from (turn is a multiple of 8, so four dims are in one half).
+// A wave has a pair for each lane at most, and forms each pair's angle once: its
+// lanes then read theirs from LDS (24 prompts of up to 700 rows into 4-bit pages:
+// 31 us with every lane forming its own, 24 so).
 template <int T, bool INTER, class F>
 struct Turn {
     static constexpr int N = INTER ? 4 : 8;
+    typedef F cs __attribute__((ext_vector_type(2)));
     F c[N], s[N];
-    __device__ __forceinline__ Turn(const RotaryArgs& a, uint32_t d, int32_t position) {
-        if (INTER) {
+    // lds: [64], of the wave
+    __device__ __forceinline__ Turn(const RotaryArgs& a, uint32_t d, int32_t position, cs* lds) {
+        const uint32_t lane = threadIdx.x & 63, half = a.turn / 2;
+        F cosine = 1, sine = 0;
+        if (lane < half) turn_of<F>(a.table, lane, position, a.magnitude, cosine, sine);
+        lds[lane] = cs{cosine, sine};
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < 4; i++) turn_of<F>(a.table, d < a.turn ? d / 2 + i : 0, position, a.magnitude, c[i], s[i]);
-        } else {
-            const uint32_t half = a.turn / 2;
+        for (int e = 0; e < N / 4; e++) {
+            const uint32_t g = INTER ? d : d + 4 * e;
+            const bool first = INTER || g < half;
+            const uint32_t pair = g < a.turn ? (INTER ? g / 2 : first ? g : g - half) : 0;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint32_t g = d + 4 * e;
-                const bool first = g < half;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    turn_of<F>(a.table, g < a.turn ? (first ? g : g - half) + i : 0, position, a.magnitude, c[4 * e + i], s[4 * e + i]);
-                    if (first) s[4 * e + i] = -s[4 * e + i];
-                }
+            for (int i = 0; i < 4; i++) {
+                const cs v = lds[pair + i];
+                c[4 * e + i] = v.x;
+                s[4 * e + i] = !INTER && first ? -v.y : v.y;
             }
         }
+        __builtin_amdgcn_wave_barrier();
     }
     // x: the values at `head` + d
     __device__ __forceinline__ void operator()(const RotaryArgs& a, const uint8_t* head, uint32_t d, float (&x)[8]) const {
@@ -141,20 +148,26 @@ __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
     }
 }
 
-// Heads h0, h0 + 4, .. before h1 of a row, four at a time (16 lanes, 8 dims each).
+// Heads h0, h0 + 4, .. before h1 of a row, four at a time (16 lanes, 8 dims each),
+// the next four's rows under way.
 template <int T, bool INTER>
 __device__ __forceinline__ void turn_heads(const RotaryArgs& r, const uint8_t* in, uint8_t* out, uint32_t h0, uint32_t h1,
-                                           int32_t position) {
+                                           int32_t position, void* lds) {
+    typedef Turn<T, INTER, float> turn_t;
     const uint32_t lane = threadIdx.x & 63, d = (lane & 15) * 8;
-    const Turn<T, INTER, float> turn(r, d, position);
+    const auto at = [&](uint32_t h) { return (size_t)h * r.dim * act_size<T>; };
+    uint32_t h = h0 + (lane >> 4);
+    float next[8] = {};
+    if (d < r.dim && h < h1) load8<T>(in + at(h) + d * act_size<T>, next);
+    const turn_t turn(r, d, position, (typename turn_t::cs*)lds);
     if (d >= r.dim) return;
-    for (uint32_t h = h0 + (lane >> 4); h < h1; h += 4) {
-        const size_t at = (size_t)h * r.dim;
-        const uint8_t* head = in + at * act_size<T>;
+    for (; h < h1; h += 4) {
         float x[8];
-        load8<T>(head + d * act_size<T>, x);
-        turn(r, head, d, x);
-        store8<T>(out + (at + d) * act_size<T>, x);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = next[i];
+        if (h + 4 < h1) load8<T>(in + at(h + 4) + d * act_size<T>, next);
+        turn(r, in + at(h), d, x);
+        store8<T>(out + at(h) + d * act_size<T>, x);
     }
 }
 
@@ -169,12 +182,14 @@ struct ApplyArgs {
 // Rows turned where they lie, or into other rows.
 template <int T, bool INTER>
 __global__ __launch_bounds__(256) void k_rotary(ApplyArgs a) {
+    __shared__ __align__(16) float s_turn[4][128];
     const uint32_t parts = (a.heads + a.per - 1) / a.per;
     const uint64_t unit = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row = (uint32_t)(unit / parts), h0 = (uint32_t)(unit % parts) * a.per;
     if (row >= a.rows) return;
     turn_heads<T, INTER>(a.r, (const uint8_t*)a.x + (size_t)row * a.xstride * act_size<T>,
-                         (uint8_t*)a.out + (size_t)row * a.ostride * act_size<T>, h0, min(h0 + a.per, a.heads), a.positions[row]);
+                         (uint8_t*)a.out + (size_t)row * a.ostride * act_size<T>, h0, min(h0 + a.per, a.heads), a.positions[row],
+                         s_turn[threadIdx.x >> 6]);
 }
 
 struct TurnedArgs {
@@ -193,6 +208,7 @@ struct TurnedArgs {
 // moves over a code's border would be a whole step.
 template <int T, int CT, bool INTER>
 __global__ __launch_bounds__(256) void k_pages_turned(TurnedArgs a) {
+    __shared__ __align__(16) double s_turn[4][128];
     const uint32_t kv4 = (a.kv_heads + 3) / 4, parts = kv4 + (a.heads + a.per - 1) / a.per;
     const uint64_t unit = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row = (uint32_t)(unit / parts), part = (uint32_t)(unit % parts);
@@ -203,7 +219,8 @@ __global__ __launch_bounds__(256) void k_pages_turned(TurnedArgs a) {
     if (part >= kv4) {
         const uint32_t h0 = (part - kv4) * a.per;
         turn_heads<T, INTER>(a.r, (const uint8_t*)a.q + (size_t)row * a.qstride * act_size<T>,
-                             (uint8_t*)a.out + (size_t)row * a.ostride * act_size<T>, h0, min(h0 + a.per, a.heads), (int32_t)pos);
+                             (uint8_t*)a.out + (size_t)row * a.ostride * act_size<T>, h0, min(h0 + a.per, a.heads), (int32_t)pos,
+                             s_turn[threadIdx.x >> 6]);
         return;
     }
     const uint32_t lane = threadIdx.x & 63, d = (lane & 15) * 8, head = part * 4 + (lane >> 4);
@@ -218,7 +235,8 @@ __global__ __launch_bounds__(256) void k_pages_turned(TurnedArgs a) {
         load8<T>(vh + d * act_size<T>, y);
     }
     typedef std::conditional_t<CT == PF_TYPE_I8 || CT == PF_TYPE_FP4, double, float> F;
-    const Turn<T, INTER, F> turn(a.r, d, (int32_t)pos);
+    typedef Turn<T, INTER, F> turn_t;
+    const turn_t turn(a.r, d, (int32_t)pos, (typename turn_t::cs*)s_turn[threadIdx.x >> 6]);
     if (on) turn(a.r, kh, d, x);
     page_put8<CT>(x, live, a.pk, a.ks, place, d, a.r.dim);
     page_put8<CT>(y, live, a.pv, a.vs, place, d, a.r.dim);
