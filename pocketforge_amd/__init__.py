@@ -353,9 +353,9 @@ def _column(t, what, n, kind, ctx):
     if own or getattr(t, "get_device", dict)() != ctx.device:
         _here(ctx, t, what)
     name = _WORDS.get(t.dtype) or _WORDS.setdefault(t.dtype, str(t.dtype).replace("torch.", ""))
-    if tuple(t.shape) != (n,) or name != kind or not (own or n <= 1 or t.stride(0) == 1):
+    if name != kind or t.shape != (n,) or not (own or n <= 1 or t.is_contiguous()):
         raise PFError(f"{what} is {kind} [{n}], packed, not {name} {tuple(t.shape)}")
-    return _addr(t)
+    return t.ptr if own else t.data_ptr()
 
 
 def _u32(a, what):
@@ -781,9 +781,9 @@ class PagedCache:
         """The sequences' rows of one layer, packed: (k, v)."""
         _num(layer, "layer")
         s = _u32(seqs, "seqs")
-        lens = np.zeros(len(s), np.int64)
-        self.ctx.check(lib().pf_pages_tables(self.h, _at(s), len(s), None, 0, _vptr(lens)), "pf_pages_tables")
-        n = int(lens.sum())
+        lens = array.array("q", bytes(8 * len(s)))
+        self.ctx.check(lib().pf_pages_tables(self.h, _at(s), len(s), None, 0, _at(lens)), "pf_pages_tables")
+        n = sum(lens)
         if out is None:
             k, v = (self.ctx.empty((n, self.n_kv_heads, self.head_dim), dtype) for _ in range(2))
         else:

@@ -394,7 +394,7 @@ struct PickLds {
     uint64_t upto[LIST];          // cumulative weights of the sorted list
     uint64_t wide[TAIL_BINS * TAIL_COPIES];
     uint64_t part[PICK / 64], found[4];
-    uint32_t part32[PICK / 64], n, bin;
+    uint32_t part32[PICK / 64], n, bin, turn[2];
 };
 
 // Sum over the threads before this one; the sum of all in *total.
@@ -636,6 +636,8 @@ struct Listed {
     float x[N];                   // -infinity: none
     int32_t token[N];
     uint64_t w[N];
+    uint32_t bin[N];
+    uint32_t turns = 0;           // calls of place, by which m.turn is taken in turn
     uint64_t mass[B + 1];         // before each of the thread's bins, and behind the last
     uint32_t count[B + 1];
     uint32_t n;                   // tokens
@@ -683,7 +685,7 @@ struct Listed {
         for (uint32_t i = lane; i < a.slices && !s.few; i += 64) {
             const Slice q = slices[i];
             if (q.max == s.max) row_mass += q.rest;
-            else if (q.rest) row_mass += (uint64_t)rint((double)q.rest * exp2(s.octaves(q.max)));
+            else if (q.rest) row_mass += (uint64_t)rint((double)q.rest * ((double)s.weight(q.max) / STEPS));
         }
         row_mass = wave_sum64(row_mass);
         uint64_t below = 0;                       // of listed tokens that others may come before
@@ -730,15 +732,16 @@ struct Listed {
             for (int i = 0; i < N; i++) {
                 x[i] = -INFINITY;
                 w[i] = 0;
+                bin[i] = ~0u;
                 if (i * FAST >= n) continue;
                 const uint64_t e = t + i * FAST < n ? m.list[t + i * FAST] : 0xFF800000ull << 32;
                 x[i] = falling_value((uint32_t)(e >> 32));
                 token[i] = (int32_t)(uint32_t)e;
                 w[i] = s.weight(x[i]);
                 if (x[i] == -INFINITY) continue;
-                const int b = s.bin(x[i]);
-                if (counts) atomicAdd(&m.count[b], 1u);
-                atomicAdd((unsigned long long*)&m.mass[b], (unsigned long long)w[i]);
+                bin[i] = (uint32_t)s.bin(x[i]);
+                if (counts) atomicAdd(&m.count[bin[i]], 1u);
+                atomicAdd((unsigned long long*)&m.mass[bin[i]], (unsigned long long)w[i]);
             }
         __syncthreads();
         uint64_t sum = 0;
@@ -796,9 +799,12 @@ struct Listed {
         __syncthreads();
         return m.part[0] + m.part[1] + m.part[2] + m.part[3];
     }
-    // The place whose cumulative weight reaches v, or the v-th (`counted`).  False: too many tokens in its bin.
+    // The place whose cumulative weight reaches v, or the v-th (`counted`).  False: too
+    // many tokens in its bin.  (What one call's slower waves still read, the next call
+    // leaves alone until all have come to its first barrier.)
     __device__ __forceinline__ bool place(uint64_t v, bool counted, Found& f) {
         const uint32_t t = threadIdx.x;
+        uint32_t* number = &m.turn[turns++ & 1];
         if (t < FAST)
 #pragma unroll
             for (int i = 0; i < B; i++)
@@ -806,7 +812,7 @@ struct Listed {
                     m.bin = B * t + i;
                     m.found[0] = mass[i];
                     m.found[1] = count[i];
-                    m.n = 0;
+                    *number = 0;
                 }
         __syncthreads();
         const uint32_t b = m.bin;
@@ -815,16 +821,15 @@ struct Listed {
         if (t < FAST)
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (i * FAST < n && x[i] != -INFINITY && (uint32_t)s.bin(x[i]) == b) {
-                    const uint32_t at = atomicAdd(&m.n, 1u);
+                if (i * FAST < n && bin[i] == b) {
+                    const uint32_t at = atomicAdd(number, 1u);
                     m.list[at] = (uint64_t)falling(x[i]) << 32 | (uint32_t)token[i];
                     m.upto[at] = w[i];
                 }
         __syncthreads();
-        const uint32_t k = m.n;
+        const uint32_t k = *number;
         if (k > AT_ONCE) return false;
         in_order(m, k, before, tokens, v, counted, f);
-        __syncthreads();
         return true;
     }
 };

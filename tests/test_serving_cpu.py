@@ -54,6 +54,9 @@ def test_matrices_and_columns():
         def get_device(self):
             return 0
 
+        def is_contiguous(self):
+            return self.t.is_contiguous()
+
         def stride(self, *d):
             return self.t.stride(*d)
 
