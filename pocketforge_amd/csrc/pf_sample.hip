@@ -1114,6 +1114,7 @@ using namespace pf;
 // ================================================================== host
 
 constexpr uint32_t SAMPLE_VOCAB = 1u << 20;
+constexpr size_t SAMPLE_SCRATCH = 64u << 20;
 
 template <int T>
 static void sample_type(hipStream_t st, uint32_t tokens, const SampleArgs& a) {
@@ -1164,14 +1165,29 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     while (per > 8 && slices() <= 32 && (uint64_t)rows * slices() < 512) per /= 2;
     a.slices = slices();
     a.room = a.slices <= 2 ? 2048 : a.slices <= 4 ? 1024 : a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
-    const size_t parts = (size_t)rows * a.slices;
+    while (a.room > 128 && a.room / 2 >= d->n_vocab) a.room /= 2;
+    // as many rows at a time as keep their lists in SAMPLE_SCRATCH
+    const size_t row_bytes = a.slices * (sizeof(Slice) + (size_t)a.room * 8);
+    const uint32_t most = (uint32_t)std::min<size_t>(rows, std::max<size_t>(1, SAMPLE_SCRATCH / row_bytes));
     void* ws = nullptr;
-    if (pf_status st = ctx_scratch(c, parts * (sizeof(Slice) + a.room * 8), &ws)) return st;
+    if (pf_status st = ctx_scratch(c, most * row_bytes, &ws)) return st;
     a.ws_list = (uint64_t*)ws;
-    a.ws_slice = (Slice*)(a.ws_list + parts * a.room);
-    if (d->type == PF_TYPE_F32) sample_type<PF_TYPE_F32>(c->stream, per, a);
-    else if (d->type == PF_TYPE_F16) sample_type<PF_TYPE_F16>(c->stream, per, a);
-    else sample_type<PF_TYPE_BF16>(c->stream, per, a);
+    a.ws_slice = (Slice*)(a.ws_list + (size_t)most * a.slices * a.room);
+    for (uint32_t at = 0; at < rows; at += most) {
+        SampleArgs b = a;
+        b.rows = std::min(most, rows - at);
+        b.logits = (const uint8_t*)logits + (size_t)at * stride * es;
+        b.u += at;
+        b.tokens += at;
+        if (probs) b.probs += at;
+        if (b.temperature) b.temperature += at;
+        if (b.top_k) b.top_k += at;
+        if (b.top_p) b.top_p += at;
+        if (b.min_p) b.min_p += at;
+        if (d->type == PF_TYPE_F32) sample_type<PF_TYPE_F32>(c->stream, per, b);
+        else if (d->type == PF_TYPE_F16) sample_type<PF_TYPE_F16>(c->stream, per, b);
+        else sample_type<PF_TYPE_BF16>(c->stream, per, b);
+    }
     PF_LAUNCHED(c);
     return PF_OK;
 }

@@ -218,6 +218,24 @@ def test_contexts_of_hundreds(gpu, t, D, H, G, lens, new, window, sink, causal):
     m.c.close()
 
 
+def test_many_tiles_a_wave(gpu):
+    """Forks of one context, enough of them for a third workgroup on each compute unit (49152 tiles of 32 keys and a head)."""
+    G, n = 24, 64
+    m = Mirror(gpu, G, 128, 256, 4 + n, n, 1100, t="bf16")
+    m.append([0], [1024])
+    m.c.fork(0, list(range(1, n)))
+    for s in range(1, n):
+        m.rows[s] = list(m.rows[0])
+    seqs = list(range(n))
+    m.append(seqs, [1] * n)
+    q = R.rand(m.rng, (n, G, 128), "bf16")
+    y = R.from_bits(m.c.attention(0, dev(gpu, q)).numpy(), "bf16")
+    for s in range(0, n, 9):
+        want, tol = R.attend(R.from_bits(q[s:s + 1], "bf16"), *m.rows[s][0], R.visible(1, 1025), R.default_scale(128), "bf16")
+        R.check(y[s:s + 1], want, tol, f"sequence {s}")
+    m.c.close()
+
+
 def test_many_sequences(gpu):
     n = 300
     m = Mirror(gpu, 1, 64, 16, 3000, n, 200, t="bf16")

@@ -247,7 +247,7 @@ def test_store_rotary_in_place_and_refusals(gpu):
 SETTINGS = [dict(temperature=0.0), dict(temperature=0.8, top_p=0.95), dict(top_k=50), dict(temperature=0.7, top_k=40, top_p=0.9, min_p=0.05),
             dict(min_p=0.02), dict(temperature=1.3, top_k=200, top_p=0.98), dict(), dict(temperature=2.0, top_p=0.999),
             dict(temperature=3.0, top_k=1500), dict(temperature=1.5, top_k=1100, top_p=0.6, min_p=1e-4), dict(top_k=1), dict(top_p=0.0),
-            dict(min_p=1.0), dict(temperature=1e-3), dict(temperature=float("inf")), dict(temperature=50.0, top_p=0.5)]
+            dict(min_p=1.0), dict(temperature=1e-3), dict(temperature=1e-45), dict(temperature=1e30), dict(temperature=float("inf")), dict(temperature=50.0, top_p=0.5)]
 U = [0.0, 0.1, 0.5, 0.9, 0.999, 1 - 2.0 ** -24]
 
 
@@ -372,6 +372,28 @@ def test_sample_settings_of_all_rows(gpu):
     a, _ = gpu.sample_rows(dev(gpu, x), dev(gpu, np.full(7, 0.8, np.float32)), temperature=1.1, top_k=dev(gpu, k), out=(gpu.empty((7,), np.int32), None))
     gpu.synchronize()
     assert a.numpy().tolist() == [S.sample(x[i].astype(np.float64), 0.8, temperature=1.1, top_k=max(0, int(k[i])))[0] for i in range(7)]
+
+
+def test_sample_many_rows(gpu):
+    """More rows than are taken at a time, with settings of their own."""
+    rng = np.random.default_rng(12)
+    rows, V = 65535, 7
+    x = logits_of(rng, rows, V, "f16", "flat")
+    u = rng.random(rows).astype(np.float32)
+    k = rng.integers(0, 9, rows).astype(np.int32)
+    temp = rng.choice(np.array([0, 0.5, 2], np.float32), rows)
+    tokens, probs = (a.numpy() for a in gpu.sample_rows(dev(gpu, x), dev(gpu, u), temperature=dev(gpu, temp), top_k=dev(gpu, k)))
+    f = R.from_bits(x, "f16")
+    for i in list(range(0, rows, 97)) + [rows - 1, 60000, 60001]:
+        token, prob = S.sample(f[i], u[i], temp[i], int(k[i]))
+        assert tokens[i] == token and abs(probs[i] - prob) <= 2.0 ** -23 * prob + 2.0 ** -44, i
+
+
+@pytest.mark.parametrize("kind", ["zipf", "flat"])
+def test_sample_largest_vocabulary(gpu, kind):
+    x = logits_of(np.random.default_rng(20), 1, 1 << 20, "f32", kind)
+    for s in (dict(temperature=0.0), dict(top_k=50), dict(temperature=0.8, top_p=0.9), dict(), dict(top_k=5000, min_p=1e-3)):
+        sample_case(gpu, x, "f32", [0.2, 0.8, 0.9999], [s])
 
 
 def test_sample_refusals(gpu):
