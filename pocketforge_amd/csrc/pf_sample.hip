@@ -857,7 +857,7 @@ struct Tail {
         return (uint32_t)(fmaf(w, more * 0.693147181f, w) * unit);
     }
     // 0 .. TAIL_BINS - 1 (and what is left behind the point, up to the last); never falls as x falls
-    __device__ __forceinline__ float place_of(float x) const { return fminf(((s.max - x) - (s.max - bound)) * per_bin, TAIL_BINS - 0.001f); }
+    __device__ __forceinline__ float place_of(float x) const { return fminf((bound - x) * per_bin, TAIL_BINS - 0.001f); }
     __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)place_of(x); }
 
     __device__ __forceinline__ Tail(const SampleArgs& a, const Setting& s, PickLds& m, uint32_t row, float bound)
@@ -873,12 +873,18 @@ struct Tail {
         __syncthreads();
         const uint32_t some = s.least > 0.0 ? (uint32_t)fmin(s.least * by, 4294967295.0) : ~0u;
         uint64_t* own = m.wide + t % TAIL_COPIES;
-        r.template each<PICK>([&](float x, int32_t) {
-            if (!(x < bound && x > -INFINITY)) return;
-            const uint32_t w = weight(x);
+        // (no branch: a masked token weighs nothing, nor does a listed one here)
+        const auto add = [&](float x) {
+            const uint32_t w = x < bound ? weight(x) : 0;
             atomicAdd((unsigned long long*)&own[bin(x) * TAIL_COPIES], (unsigned long long)w);
-            if (some != ~0u) least += w >= some ? w : 0;
-        });
+            return w;
+        };
+        if (some == ~0u) r.template each<PICK>([&](float x, int32_t) { add(x); });
+        else
+            r.template each<PICK>([&](float x, int32_t) {
+                const uint32_t w = add(x);
+                least += w >= some ? w : 0;
+            });
         __syncthreads();
         uint64_t w = 0;
         if (t < TAIL_BINS)
