@@ -360,8 +360,11 @@ pf_status pf_pages_compact(pf_pages* p, uint32_t* moved);
  * (or NaN): off; top_p 0 and below: the first token alone; min_p above 1: 1.
  * A logit of -infinity or NaN is masked; of infinities the infinities alone
  * weigh.  A row without any other gives -1.
- * Weights are held in steps of 2^-43, and their sums are exact: the same
- * inputs give the same tokens. */
+ * The largest few weights of a row, a thousand or those of its top-k, are held
+ * in steps of 2^-43 and their sums are exact; the others' are of fp32, off by
+ * 2^-20 of what stays at most (of many equal ones; 2^-24 of different ones).
+ * The same call gives the same tokens.  Of the same row among more or fewer
+ * others these last sums may differ by their rounding. */
 typedef struct {
     int32_t type;              /* logits: PF_TYPE_F32, F16 or BF16 */
     uint32_t n_vocab;          /* 1 .. 2^20 */

@@ -7,19 +7,26 @@
 // The token is the first whose cumulative weight exceeds u S.
 //
 // Two launches.  Workgroups of a slice of a row each read it once, into
-// registers: its largest logit, the sum of its weights, and its largest few
-// tokens, those above a bound that the threads' own maxima give.  What lies above
-// the largest of these bounds, over all slices, is the beginning of the order: a
-// thousand tokens or the top-k and some more.  A workgroup for each row finds the
-// borders and the token among them, by a histogram and a sort of the bins that the
-// borders are in.  Where one lies further on, as in flat rows, it does the same
-// over the whole row, and where that has more equal logits than it can sort,
-// digit by digit.
+// registers: its largest logit, its largest few tokens, those above a bound that
+// the threads' own maxima give, and the sum of the others' weights.  What lies
+// above the largest of these bounds, over all slices, is the beginning of the
+// order: a thousand tokens or the top-k and some more.  A workgroup for each row
+// finds the borders and the token among them, by a histogram and the order of the
+// bins that the borders are in.  Where one lies further on, as in flat rows, it
+// does the same over what is below the listed tokens, and where these do not fit
+// or that has more equal logits than it can sort, over the whole row, digit by
+// digit.  A row that one workgroup's registers hold takes one launch.
 //
-// Weights are whole numbers, exp((l - max) / T) in steps of 2^-43, so that sums
-// are exact, whatever the order in which threads add to them: up to 2^20 tokens
-// of up to 2^43 fit 64 bits, and what a step leaves of 2^20 sums is 2^-24 of the
-// largest weight, what sums of fp32 would lose of the first few.
+// Weights of listed tokens are whole numbers, exp((l - max) / T) in steps of 2^-43,
+// so that sums are exact, whatever the order in which threads add to them: up to
+// 2^20 tokens of up to 2^43 fit 64 bits, and what a step leaves of 2^20 sums is
+// 2^-24 of the largest weight, what sums of fp32 would lose of the first few.
+// The others', each below a thousandth of the row's or so, are fp32's: in fp64 they
+// would be most of a slice's time.  A thread adds its own 8 to 32 of them, and these
+// sums are added as whole numbers.  An exponent o is off by half a step, 2^-21 for
+// o in 8 .. 16, a weight by ln 2 times that and by exp2's 2^-23: of 2^20 equal
+// ones 2^-o of the largest's this is 2^-20 of all at most, of different ones it
+// averages out.
 #include "pf_attend.h"
 #include "pf_context.h"
 
@@ -857,7 +864,7 @@ struct Tail {
         return (uint32_t)(fmaf(w, more * 0.693147181f, w) * unit);
     }
     // 0 .. TAIL_BINS - 1 (and what is left behind the point, up to the last); never falls as x falls
-    __device__ __forceinline__ float place_of(float x) const { return fminf((bound - x) * per_bin, TAIL_BINS - 0.001f); }
+    __device__ __forceinline__ float place_of(float x) const { return __builtin_amdgcn_fmed3f((bound - x) * per_bin, 0.0f, TAIL_BINS - 0.001f); }
     __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)place_of(x); }
 
     __device__ __forceinline__ Tail(const SampleArgs& a, const Setting& s, PickLds& m, uint32_t row, float bound)
@@ -1017,19 +1024,13 @@ struct Tail {
 // the rest of the row where a border or the token lies there, of the whole row
 // where listed tokens do not fit or top-k goes beyond them.
 template <int T>
-__global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
-    __shared__ PickLds m;
-    const uint32_t row = blockIdx.x, t = threadIdx.x;
-    Setting s;
-    s.of(a, row);
-    const float uu = a.u[row];
+__device__ __forceinline__ void pick_token(const SampleArgs& a, PickLds& m, uint32_t row, Setting& s, Listed& p, bool done, float uu) {
+    const uint32_t t = threadIdx.x;
     Found f{};
     uint64_t kept = 0;
     const double u = uu > 0.0f ? (double)uu : 0.0;
     const auto reach = [&](uint64_t mass) { return (uint64_t)fmax(1.0, ceil(s.p * (double)mass)); };
     const auto drawn = [&](uint64_t mass) { return min((uint64_t)(u * (double)mass), mass - 1) + 1; };
-    Listed p(s, m);
-    bool done = p.load(a, row);
     if (s.greedy || s.first < 0) {
         if (t == 0) {
             a.tokens[row] = s.first;
@@ -1094,7 +1095,7 @@ __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
                 if (done && m_below) kept = min(kept, back(q.least));
                 if (done) {
                     const uint64_t w = drawn(kept);
-                    done = w > p.all && q.place(to(w), f);
+                    done = w > p.all ? q.place(to(w), f) : p.place(w, false, f);
                 }
             }
         }
@@ -1111,6 +1112,128 @@ __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
         a.tokens[row] = f.token;
         if (a.probs) a.probs[row] = (float)((double)f.weight / (double)kept);
     }
+}
+
+template <int T>
+__global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
+    __shared__ PickLds m;
+    Setting s;
+    s.of(a, blockIdx.x);
+    const float u = a.u[blockIdx.x];
+    Listed p(s, m);
+    const bool done = p.load(a, blockIdx.x);
+    pick_token<T>(a, m, blockIdx.x, s, p, done, u);
+}
+
+// A row of up to 16 tokens a thread, listed and picked by one workgroup, in one launch
+// (5 rows of 16384 fp32 logits, top-p: 11.8 us, 14.6 in two; 512 rows: 22.6 and 32).
+// With 32 tokens a thread (5 rows of 32000 bf16 logits: 14.7, 13.9 in two) they
+// no longer fit the registers.
+constexpr uint32_t ROW_TOKENS = 16 * PICK;
+template <int T>
+__global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
+    constexpr int E = Row<T>::E, N = 16 / E;
+    constexpr uint32_t W = PICK / 64;
+    __shared__ PickLds m;
+    __shared__ float s_max[W];
+    __shared__ uint32_t s_bound[W], s_first;
+    const uint32_t row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    m.count[t] = 0;
+    m.mass[t] = 0;
+    if (t == 0) {
+        m.n = 0;
+        s_first = NO_TOKEN;
+    }
+    const Row<T> r(a, row);
+    float x[N][E], top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const bool in = t + n * PICK < r.chunks;
+        u4v w = {};
+        if (in) w = r.raw(t + n * PICK);
+#pragma unroll
+        for (int i = 0; i < E; i++) x[n][i] = in ? Row<T>::value(w, i) : -INFINITY;
+    }
+    Setting s;
+    s.of(a, row);
+    const float u = a.u[row];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < E; i++) top = fmaxf(top, x[n][i]);
+    // (as in k_sample_slice, of the threads that have tokens; of fewer than c lanes all are listed)
+    const float want = s.few ? fminf(1.5f * (float)s.k + 16.0f, 1700.0f) : 1040.0f;
+    const float each = want / (float)min((r.chunks + 63) & ~63u, (uint32_t)PICK);
+    const uint32_t nth = nth_of_wave(top, (uint32_t)(64.0f * (1.0f - __builtin_amdgcn_exp2f(each * -1.4426950f))) + 1);
+    const float wave_top = wave_max(top);
+    if (lane == 0) {
+        s_max[wave] = wave_top;
+        s_bound[wave] = nth;
+    }
+    __syncthreads();
+    s.max = wave_max(lane < W ? s_max[lane] : -INFINITY);
+    if (s.max > -INFINITY && wave_top == s.max) {
+        uint32_t first = NO_TOKEN;
+#pragma unroll
+        for (int n = N - 1; n >= 0; n--)
+#pragma unroll
+            for (int i = E - 1; i >= 0; i--)
+                if (x[n][i] == s.max) first = (uint32_t)((int32_t)((t + n * PICK) * E) - r.skip + i);
+        first = wave_least(first);
+        if (lane == 0) atomicMin(&s_first, first);
+    }
+    Listed p(s, m);
+    p.bound = -INFINITY;
+    p.n = 0;
+    uint64_t rest = 0;
+    if (!s.greedy && s.max > -INFINITY) {
+        const uint64_t sum = wave_sum64(lane < W ? s_bound[lane] : 0);
+        const uint32_t some = (uint32_t)__popcll(__ballot(lane < W && s_bound[lane] != 0));
+        if (some) p.bound = falling_value(~(uint32_t)(sum / some));
+        const float above = fmaxf(p.bound, -3.4028234663852886e38f);
+        s.fp32();
+        uint32_t hits = 0;
+        float others = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const bool hit = x[n][i] >= above;
+                hits += hit;
+                if (!s.few) others += __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
+            }
+        if (!s.few) {
+            rest = (uint64_t)((double)others * STEPS);
+            if (!s.plain) {
+                rest = 0;
+#pragma unroll
+                for (int n = 0; n < N; n++)
+#pragma unroll
+                    for (int i = 0; i < E; i++)
+                        if (!(x[n][i] >= above)) rest += s.weight(x[n][i]);
+            }
+            rest = wave_sum64(rest);
+        }
+        const uint32_t upto = wave_scan(hits);
+        uint32_t at = 0;
+        if (lane == 63) at = atomicAdd(&m.n, upto);
+        at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - hits;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                if (x[n][i] >= above) {
+                    if (at < LIST) m.list[at] = (uint64_t)falling(x[n][i]) << 32 | (uint32_t)((int32_t)((t + n * PICK) * E) - r.skip + i);
+                    at++;
+                }
+    }
+    if (lane == 0) m.part[wave] = rest;
+    __syncthreads();
+    s.first = s_first == NO_TOKEN ? -1 : (int32_t)s_first;
+    p.n = m.n;
+    p.row_mass = wave_sum64(lane < W ? m.part[lane] : 0);
+    __syncthreads();
+    pick_token<T>(a, m, row, s, p, p.n <= LIST, u);
 }
 
 }  // namespace pf
@@ -1166,12 +1289,18 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     // each compute unit, of up to 64 slices (each lists its own share of a row's largest)
     const uint32_t chunk = 16 / (uint32_t)es, off = aligned16(logits) && stride % chunk == 0 ? 0 : chunk - 1;
     const uint32_t chunks = (off + d->n_vocab + chunk - 1) / chunk;
+    if (chunks * chunk <= ROW_TOKENS) {
+        if (d->type == PF_TYPE_F32) hipLaunchKernelGGL(k_sample_row<PF_TYPE_F32>, dim3(rows), dim3(PICK), 0, c->stream, a);
+        else if (d->type == PF_TYPE_F16) hipLaunchKernelGGL(k_sample_row<PF_TYPE_F16>, dim3(rows), dim3(PICK), 0, c->stream, a);
+        else hipLaunchKernelGGL(k_sample_row<PF_TYPE_BF16>, dim3(rows), dim3(PICK), 0, c->stream, a);
+        PF_LAUNCHED(c);
+        return PF_OK;
+    }
     uint32_t per = 32;
     const auto slices = [&] { return (chunks + 256 * (per / chunk) - 1) / (256 * (per / chunk)); };
     while (per > 8 && slices() <= 32 && (uint64_t)rows * slices() < 512) per /= 2;
     a.slices = slices();
-    a.room = a.slices <= 2 ? 2048 : a.slices <= 4 ? 1024 : a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
-    while (a.room > 128 && a.room / 2 >= d->n_vocab) a.room /= 2;
+    a.room = a.slices <= 4 ? 1024 : a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
     // as many rows at a time as keep their lists in SAMPLE_SCRATCH
     const size_t row_bytes = a.slices * (sizeof(Slice) + (size_t)a.room * 8);
     const uint32_t most = (uint32_t)std::min<size_t>(rows, std::max<size_t>(1, SAMPLE_SCRATCH / row_bytes));

@@ -389,6 +389,62 @@ def test_sample_many_rows(gpu):
         assert tokens[i] == token and abs(probs[i] - prob) <= 2.0 ** -23 * prob + 2.0 ** -44, i
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [63, 64, 65, 513, 2048, 2049, 4096, 8200, 16383])
+def test_sample_one_workgroup(gpu, t, V):
+    """Rows of one launch, of few threads and of all, and top-k around what they list."""
+    ks = [dict(top_k=k, top_p=p) for k in (2, 20, 300, 1024, 1025) for p in (1.0, 0.9)]
+    for kind in ("zipf", "flat"):
+        sample_case(gpu, logits_of(np.random.default_rng(V), 1, V, t, kind), t, U, SETTINGS[:8] + ks)
+
+
+def test_sample_masked_slices(gpu):
+    """Masks, infinities and NaN in rows of several workgroups."""
+    V = 20003
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((8, V)).astype(np.float32)
+    x[0, rng.permutation(V)[:V - 3]] = -np.inf
+    x[1] = -np.inf
+    x[2] = -np.inf
+    x[2, V - 1] = -3e38
+    x[3, ::2] = np.nan
+    x[4, [7, 12000]] = np.inf
+    x[5] = np.nan
+    x[6] = np.where(np.arange(V) % 2, 3e38, -3e38)
+    x[7, 5:] = np.finfo(np.float32).min
+    sample_case(gpu, x, "f32", [0.0, 0.3, 0.7, 1 - 2.0 ** -24], SETTINGS)
+
+
+def test_sample_many_sliced_rows(gpu):
+    """More rows of several workgroups than have room for their lists at a time, with settings of their own."""
+    rng = np.random.default_rng(13)
+    rows, V = 2500, 16401
+    x = np.tile(logits_of(rng, 50, V, "f16"), (50, 1))
+    u = rng.random(rows).astype(np.float32)
+    k = rng.integers(0, 60, rows).astype(np.int32)
+    temp = rng.choice(np.array([0, 0.5, 1], np.float32), rows)
+    tokens, probs = (a.numpy() for a in gpu.sample_rows(dev(gpu, x), dev(gpu, u), temperature=dev(gpu, temp), top_k=dev(gpu, k)))
+    f = R.from_bits(x[:50], "f16")
+    for i in list(range(0, rows, 61)) + list(range(rows - 520, rows, 13)):
+        token, prob = S.sample(f[i % 50], u[i], temp[i], int(k[i]))
+        assert tokens[i] == token and abs(probs[i] - prob) <= 2.0 ** -23 * prob + 2.0 ** -44, i
+
+
+def test_sample_equal_tails(gpu):
+    """Far below the largest logit a row's weight lies in equal ones, which fp32 rounds alike: a weight 2^-o of the largest's,
+    o up to 32, is off by half a step of o, ln 2 2^-20, and by what exp2 is, 2^-23."""
+    for t, V, d in (("f32", 16000, 9.7), ("bf16", 16000, 7.3125), ("bf16", 100000, 11.125), ("f32", 1 << 18, 17.3)):
+        x = np.full((1, V), 1.0 - d, np.float32)
+        x[0, V // 3] = 1.0
+        b = R.to_bits(x, t)
+        f = R.from_bits(b, t)
+        u = np.array([0.0, 2.0 ** -24], np.float32)
+        tokens, probs = (a.numpy() for a in gpu.sample_rows(dev(gpu, np.tile(b, (2, 1))), dev(gpu, u)))
+        for i in range(2):
+            token, prob = S.sample(f[0], u[i])
+            assert tokens[i] == token and abs(probs[i] - prob) <= 2.0 ** -19.9 * prob, (t, V, d, probs[i], prob)
+
+
 @pytest.mark.parametrize("kind", ["zipf", "flat"])
 def test_sample_largest_vocabulary(gpu, kind):
     x = logits_of(np.random.default_rng(20), 1, 1 << 20, "f32", kind)
