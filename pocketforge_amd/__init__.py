@@ -909,7 +909,8 @@ class Rotary:
             self.h = None
 
     def __del__(self):
-        self.close()
+        if lib is not None and self.ctx.h:      # (not where the program ends, or the context has)
+            self.close()
 
 
 class Squeeze:

@@ -138,8 +138,9 @@ struct Turn {
 };
 
 // Past the caches: what a prompt's rows would leave in them costs the kernels that
-// follow their own (24 prompts of up to 700 rows turned into 4-bit pages, and these
-// read back: 32 us, 42 otherwise; attention over the turned rows takes the same).
+// follow their own (two batches in turn of 24 prompts of up to 700 rows turned into
+// 4-bit pages, and these read back: 32 us, 42 otherwise; with three batches, past
+// the 256 MB cache either way, 44 and 45; attention over the turned rows takes the same).
 template <int T>
 __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
     if constexpr (T == PF_TYPE_F32) {
@@ -309,7 +310,9 @@ extern "C" pf_status pf_rotary_create(pf_ctx* c, const pf_rotary_desc* d, pf_rot
 static RotaryArgs rotary_args(const pf_rotary* r) { return {r->table, (double)r->desc.magnitude, r->turn, r->desc.head_dim}; }
 
 // Heads of a wave: all of a row's, as few waves as fill the card (8 on each of its
-// 1024 SIMDs), since a wave forms its angles once.
+// 1024 SIMDs), since a wave forms its angles once (8192 bf16 rows of 16 heads of 128:
+// 11.3 us, 14.1 with four heads a wave); fewer of them otherwise, which a wave
+// has one after another (64 rows of 128 heads: 5.8 us, 11.7 with all in a wave).
 static uint32_t heads_of_wave(uint32_t rows, uint32_t heads) {
     uint32_t per = (heads + 3) / 4 * 4;
     while (per > 4 && (uint64_t)rows * ((heads + per - 1) / per) < 8192) per = (per / 2 + 3) / 4 * 4;

@@ -1285,8 +1285,11 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     a.logits = logits; a.u = u; a.temperature = d->temperature_dev; a.top_k = d->top_k_dev; a.top_p = d->top_p_dev; a.min_p = d->min_p_dev;
     a.temperature1 = d->temperature; a.top_k1 = d->top_k; a.top_p1 = d->top_p; a.min_p1 = d->min_p;
     a.rows = rows; a.vocab = d->n_vocab; a.stride = stride; a.tokens = tokens; a.probs = probs;
-    // tokens of a thread of the slices' workgroups: the most that leave two of them for
-    // each compute unit, of up to 64 slices (each lists its own share of a row's largest)
+    // tokens of a thread of the slices' workgroups: the most that leave two of these for
+    // each compute unit, where a row has up to 16 (5 rows of 32000 bf16 logits: 13.9 us in
+    // 16 slices each, 16.2 in 4).  More of them cost the row's workgroup, that takes their
+    // lists together, more than they save (one row of 130560: 15.3 us in 16, 16.9 in 64;
+    // 64 rows: 19.5 and 26).
     const uint32_t chunk = 16 / (uint32_t)es, off = aligned16(logits) && stride % chunk == 0 ? 0 : chunk - 1;
     const uint32_t chunks = (off + d->n_vocab + chunk - 1) / chunk;
     if (chunks * chunk <= ROW_TOKENS) {
@@ -1298,7 +1301,7 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     }
     uint32_t per = 32;
     const auto slices = [&] { return (chunks + 256 * (per / chunk) - 1) / (256 * (per / chunk)); };
-    while (per > 8 && slices() <= 32 && (uint64_t)rows * slices() < 512) per /= 2;
+    while (per > 8 && slices() <= 8 && (uint64_t)rows * slices() < 512) per /= 2;
     a.slices = slices();
     a.room = a.slices <= 4 ? 1024 : a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
     // as many rows at a time as keep their lists in SAMPLE_SCRATCH
