@@ -849,9 +849,14 @@ struct Listed {
 // 2^-30 or finer: a border or a token in flat rows.  One compute unit goes through the row:
 // once for a histogram by value, kept 32 times so that a pair of lanes has one in
 // LDS banks of its own, and once for the tokens of the bin; these again by a finer
-// histogram, so that only a few have to be put in order.
+// histogram, so that only a few have to be put in order, or all are equal.  Bound by
+// that one compute unit: 25 us for each border or token in a row of 130560 bf16 logits
+// (drawn from a normal distribution, one row: 14 us without a tail, 50 at temperature
+// 1, 70 with top-p; the whole row instead, `Pick`, takes 133 and 160).
 template <int T>
 struct Tail {
+    static constexpr uint32_t MOST = 8192;   // tokens of a bin
+    static_assert(offsetof(PickLds, upto) == offsetof(PickLds, list) + sizeof(PickLds::list) && MOST * 4 <= 2 * sizeof(PickLds::list), "list and upto");
     const Row<T> r;
     const Setting& s;
     PickLds& m;
@@ -924,7 +929,7 @@ struct Tail {
         }
         const float top = falling_value(~(uint32_t)__builtin_amdgcn_readlane((int)key, 0));
         const float under = b + 1 < TAIL_BINS ? falling_value(~(uint32_t)__builtin_amdgcn_readlane((int)key, 1)) : -INFINITY;
-        uint32_t* tokens = (uint32_t*)m.upto;
+        uint32_t* tokens = (uint32_t*)m.list;
         r.template batches<PICK>([&](const auto& w, int32_t t0, uint64_t in) {
             typedef std::remove_reference_t<decltype(w)> W;
             constexpr int U = sizeof(W) / sizeof(u4v), E = Row<T>::E;
@@ -943,27 +948,30 @@ struct Tail {
             at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - n;
             for (; hits; hits &= hits - 1, at++) {
                 const int h = __builtin_ctzll(hits);
-                if (at < LIST) tokens[at] = (uint32_t)(t0 + h / E * (int)(PICK * E) + h % E);
+                if (at < MOST) tokens[at] = (uint32_t)(t0 + h / E * (int)(PICK * E) + h % E);
             }
         });
         __syncthreads();
         const uint32_t n = m.n;
-        if (n > LIST) return false;
-        // finer: two of them a thread
-        float x[2];
-        int32_t token[2];
-        uint32_t w[2], fine[2];
+        if (n > MOST) return false;
+        // finer: each thread some of them
+        float x[MOST / PICK];
+        int32_t token[MOST / PICK];
+        uint32_t fine[MOST / PICK];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < (int)(MOST / PICK); i++) {
             const uint32_t at = t + i * PICK;
-            x[i] = -INFINITY;
             fine[i] = ~0u;
             if (at >= n) continue;
             token[i] = (int32_t)tokens[at];
             x[i] = r.one(token[i]);
-            w[i] = weight(x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < (int)(MOST / PICK); i++) {
+            if (t + i * PICK >= n) continue;
+            const uint32_t w = weight(x[i]);
             fine[i] = min((uint32_t)((place_of(x[i]) - (float)b) * (float)BINS), (uint32_t)BINS - 1);
-            if (w[i]) atomicAdd((unsigned long long*)&m.wide[fine[i]], (unsigned long long)w[i]);
+            if (w) atomicAdd((unsigned long long*)&m.wide[fine[i]], (unsigned long long)w);
         }
         __syncthreads();
         uint64_t total;
@@ -977,22 +985,26 @@ struct Tail {
         __syncthreads();
         before = m.found[0];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < (int)(MOST / PICK); i++)
             if (fine[i] == m.bin) {
                 const uint32_t to = atomicAdd(&m.n, 1u);
+                if (to >= LIST) continue;
                 m.list[to] = (uint64_t)falling(x[i]) << 32 | (uint32_t)token[i];
-                m.upto[to] = w[i];
+                m.upto[to] = weight(x[i]);
             }
         __syncthreads();
         const uint32_t k = m.n;
-        if (k <= AT_ONCE) {
-            if (!in_order(m, k, before, 0, v, false, f)) return false;
-        } else {
-            // many: all of one value, in the order of their numbers; or digit by digit over the row
+        if (k > LIST) return false;
+        // more than a few are mostly all of one value, in the order of their numbers
+        bool same = k > 32;
+        if (same) {
             const uint64_t e = m.list[0];
-            bool same = true;
             for (uint32_t i = t; i < k; i += PICK) same &= m.list[i] >> 32 == e >> 32;
-            if (!__syncthreads_and(same)) return false;
+            same = __syncthreads_and(same);
+        }
+        if (!same) {
+            if (k > AT_ONCE || !in_order(m, k, before, 0, v, false, f)) return false;
+        } else {
             const uint64_t each = m.upto[0];
             uint32_t nth = (uint32_t)((v - before - 1) / each);
             f.upto = before + (nth + 1) * each;

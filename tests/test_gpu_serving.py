@@ -398,6 +398,14 @@ def test_sample_one_workgroup(gpu, t, V):
         sample_case(gpu, logits_of(np.random.default_rng(V), 1, V, t, kind), t, U, SETTINGS[:8] + ks)
 
 
+@pytest.mark.parametrize("t,V", [("bf16", 130560), ("f32", 130560), ("f16", 90001), ("bf16", 1 << 19)])
+def test_sample_flat(gpu, t, V):
+    """Borders and tokens among thousands of tokens of one bin, equal ones and different ones."""
+    x = logits_of(np.random.default_rng(V + 1), 1, V, t, "flat")
+    sample_case(gpu, x, t, [0.05, 0.3, 0.55, 0.8, 0.97, 1 - 2.0 ** -24],
+                [dict(), dict(temperature=0.8, top_p=0.95), dict(top_p=0.4), dict(temperature=0.5), dict(min_p=0.03), dict(temperature=4.0, top_p=0.9)])
+
+
 def test_sample_masked_slices(gpu):
     """Masks, infinities and NaN in rows of several workgroups."""
     V = 20003
