@@ -1141,14 +1141,13 @@ __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
     pick_token<T>(a, m, blockIdx.x, s, p, done, u);
 }
 
-// A row of up to 16 tokens a thread, listed and picked by one workgroup, in one launch
-// (5 rows of 16384 fp32 logits, top-p: 11.8 us, 14.6 in two; 512 rows: 22.6 and 32).
-// With 32 tokens a thread (5 rows of 32000 bf16 logits: 14.7, 13.9 in two) they
-// no longer fit the registers.
-constexpr uint32_t ROW_TOKENS = 16 * PICK;
-template <int T>
+// A row of up to 32 tokens a thread, listed and picked by one workgroup, in one launch
+// (5 rows of 16384 fp32 logits, top-p: 10.3 us, 13.5 in two; 5 of 32000 bf16: 12.2 and
+// 13.3; 300 of 27000 fp32: 24.8 and 34).  Bound by one compute unit's instructions for
+// each token, then by a few barriers and LDS round trips a border, 1 us each.
+template <int T, int TOKENS>
 __global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
-    constexpr int E = Row<T>::E, N = 16 / E;
+    constexpr int E = Row<T>::E, N = TOKENS / E;
     constexpr uint32_t W = PICK / 64;
     __shared__ PickLds m;
     __shared__ float s_max[W];
@@ -1209,7 +1208,7 @@ __global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
         const float above = fmaxf(p.bound, -3.4028234663852886e38f);
         s.fp32();
         // (as there: a bit for each listed token, the values to LDS)
-        static_assert(sizeof(m.wide) >= 4 * ROW_TOKENS, "the row");
+        static_assert(sizeof(m.wide) >= 4 * 16 * PICK, "16 tokens of each thread");
         float* values = (float*)m.wide + t;
         uint32_t hits = 0;
         float others = 0.0f;
@@ -1219,14 +1218,16 @@ __global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
             for (int i = 0; i < E; i++) {
                 const bool hit = x[n][i] >= above;
                 hits |= (hit ? 1u : 0u) << (n * E + i);
-                values[(n * E + i) * PICK] = x[n][i];
                 if (!s.few) others += __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
             }
         if (!s.few) {
             rest = (uint64_t)((double)others * STEPS);
             if (!s.plain) {
                 rest = 0;
-                for (uint32_t b = ~hits & 0xFFFFu; b; b &= b - 1) rest += s.weight(values[__builtin_ctz(b) * PICK]);
+#pragma unroll
+                for (int n = 0; n < N; n++)
+#pragma unroll 1
+                    for (int i = 0; i < E; i++) rest += hits >> (n * E + i) & 1 ? 0 : s.weight(x[n][i]);
             }
             rest = wave_sum64(rest);
         }
@@ -1234,10 +1235,16 @@ __global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
         uint32_t at = 0;
         if (lane == 63) at = atomicAdd(&m.n, upto);
         at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - (uint32_t)__popc(hits);
-        for (; hits; hits &= hits - 1, at++) {
-            const int b = __builtin_ctz(hits);
-            if (at < LIST)
-                m.list[at] = (uint64_t)falling(values[b * PICK]) << 32 | (uint32_t)((int32_t)((t + b / E * PICK) * E) - r.skip + b % E);
+#pragma unroll
+        for (int n0 = 0; n0 < N; n0 += 16 / E) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) values[j * PICK] = x[n0 + j / E][j % E];
+            for (uint32_t some = hits >> (n0 * E) & 0xFFFFu; some; some &= some - 1, at++) {
+                const int b = __builtin_ctz(some);
+                if (at < LIST)
+                    m.list[at] = (uint64_t)falling(values[b * PICK]) << 32 |
+                                 (uint32_t)((int32_t)((t + (n0 + b / E) * PICK) * E) - r.skip + b % E);
+            }
         }
     }
     if (lane == 0) m.part[wave] = rest;
@@ -1262,10 +1269,15 @@ template <int T>
 static void sample_type(hipStream_t st, uint32_t tokens, const SampleArgs& a) {
     constexpr int E = Row<T>::E;
     const dim3 grid(a.slices, a.rows);
-    if (tokens == 8) hipLaunchKernelGGL((k_sample_slice<T, 8 / E>), grid, dim3(256), 0, st, a);
-    else if (tokens == 16) hipLaunchKernelGGL((k_sample_slice<T, 16 / E>), grid, dim3(256), 0, st, a);
+    if (tokens == 16) hipLaunchKernelGGL((k_sample_slice<T, 16 / E>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_sample_slice<T, 32 / E>), grid, dim3(256), 0, st, a);
     hipLaunchKernelGGL((k_sample_pick<T>), dim3(a.rows), dim3(PICK), 0, st, a);
+}
+
+template <int T>
+static void sample_row(hipStream_t st, uint32_t tokens, const SampleArgs& a) {
+    if (tokens == 16) hipLaunchKernelGGL((k_sample_row<T, 16>), dim3(a.rows), dim3(PICK), 0, st, a);
+    else hipLaunchKernelGGL((k_sample_row<T, 32>), dim3(a.rows), dim3(PICK), 0, st, a);
 }
 
 extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const void* logits, const float* u, uint32_t rows,
@@ -1298,25 +1310,25 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
     a.logits = logits; a.u = u; a.temperature = d->temperature_dev; a.top_k = d->top_k_dev; a.top_p = d->top_p_dev; a.min_p = d->min_p_dev;
     a.temperature1 = d->temperature; a.top_k1 = d->top_k; a.top_p1 = d->top_p; a.min_p1 = d->min_p;
     a.rows = rows; a.vocab = d->n_vocab; a.stride = stride; a.tokens = tokens; a.probs = probs;
-    // tokens of a thread of the slices' workgroups: the most that leave two of these for
-    // each compute unit, where a row has up to 16 (5 rows of 32000 bf16 logits: 13.9 us in
-    // 16 slices each, 16.2 in 4).  More of them cost the row's workgroup, that takes their
-    // lists together, more than they save (one row of 130560: 15.3 us in 16, 16.9 in 64;
-    // 64 rows: 19.5 and 26).
     const uint32_t chunk = 16 / (uint32_t)es, off = aligned16(logits) && stride % chunk == 0 ? 0 : chunk - 1;
     const uint32_t chunks = (off + d->n_vocab + chunk - 1) / chunk;
-    if (chunks * chunk <= ROW_TOKENS) {
-        if (d->type == PF_TYPE_F32) hipLaunchKernelGGL(k_sample_row<PF_TYPE_F32>, dim3(rows), dim3(PICK), 0, c->stream, a);
-        else if (d->type == PF_TYPE_F16) hipLaunchKernelGGL(k_sample_row<PF_TYPE_F16>, dim3(rows), dim3(PICK), 0, c->stream, a);
-        else hipLaunchKernelGGL(k_sample_row<PF_TYPE_BF16>, dim3(rows), dim3(PICK), 0, c->stream, a);
+    if (chunks * chunk <= 32 * PICK) {
+        const uint32_t tokens = chunks * chunk <= 16 * PICK ? 16 : 32;
+        if (d->type == PF_TYPE_F32) sample_row<PF_TYPE_F32>(c->stream, tokens, a);
+        else if (d->type == PF_TYPE_F16) sample_row<PF_TYPE_F16>(c->stream, tokens, a);
+        else sample_row<PF_TYPE_BF16>(c->stream, tokens, a);
         PF_LAUNCHED(c);
         return PF_OK;
     }
-    uint32_t per = 32;
-    const auto slices = [&] { return (chunks + 256 * (per / chunk) - 1) / (256 * (per / chunk)); };
-    while (per > 8 && slices() <= 8 && (uint64_t)rows * slices() < 512) per /= 2;
-    a.slices = slices();
-    a.room = a.slices <= 4 ? 1024 : a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
+    // tokens of a thread of the slices' workgroups: 32, or 16 where a row has up to 8
+    // slices of 32 and all rows' are fewer than two for each compute unit (one row of 40000
+    // fp32 logits: 13.2 us, 15.3 with 32, 13.2 with 8; 64 of 40000: 15.2, 16.3 and 16.3).
+    // More slices cost the row's workgroup, that takes their lists together, more than
+    // they save (one row of 250000 bf16 logits: 15.4 us, 16.8 with 16, 21 with 8).
+    const auto cut = [&](uint32_t tokens) { return (chunks + 256 * (tokens / chunk) - 1) / (256 * (tokens / chunk)); };
+    const uint32_t per = cut(32) <= 8 && (uint64_t)rows * cut(32) < 512 ? 16 : 32;
+    a.slices = cut(per);
+    a.room = a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
     // as many rows at a time as keep their lists in SAMPLE_SCRATCH
     const size_t row_bytes = a.slices * (sizeof(Slice) + (size_t)a.room * 8);
     const uint32_t most = (uint32_t)std::min<size_t>(rows, std::max<size_t>(1, SAMPLE_SCRATCH / row_bytes));

@@ -438,6 +438,57 @@ def test_sample_many_sliced_rows(gpu):
         assert tokens[i] == token and abs(probs[i] - prob) <= 2.0 ** -23 * prob + 2.0 ** -44, i
 
 
+def test_sample_masked_long_rows(gpu):
+    """Masks, infinities and NaN in rows of two launches."""
+    V = 40003
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((8, V)).astype(np.float32)
+    x[0, rng.permutation(V)[:V - 3]] = -np.inf
+    x[1] = -np.inf
+    x[2] = -np.inf
+    x[2, V - 1] = -3e38
+    x[3, ::2] = np.nan
+    x[4, [7, 32000]] = np.inf
+    x[5] = np.nan
+    x[6] = np.where(np.arange(V) % 2, 3e38, -3e38)
+    x[7, 5:] = np.finfo(np.float32).min
+    sample_case(gpu, x, "f32", [0.0, 0.3, 0.7, 1 - 2.0 ** -24], SETTINGS)
+    y = rng.choice(np.array([1.0, 1.5, 1.5, 2.0, -3.0], np.float32), (1, V))
+    for t in ("f32", "bf16"):
+        sample_case(gpu, R.to_bits(y, t), t, [0.0, 0.2, 0.4, 0.6, 0.8, 0.97],
+                    [dict(), dict(top_k=3000), dict(top_k=9000, top_p=0.7), dict(top_p=0.3), dict(min_p=0.2, top_p=0.9), dict(top_k=1000)])
+
+
+def test_sample_many_long_rows(gpu):
+    """More rows of two launches than have room for their lists at a time, with settings of their own, rows that start anywhere."""
+    rng = np.random.default_rng(14)
+    rows, V, stride = 3700, 33001, 33003
+    x = logits_of(rng, 20, V, "bf16")
+    big = np.zeros((rows, stride), x.dtype)
+    big[:, :V] = np.tile(x, (rows // 20, 1))
+    u = rng.random(rows).astype(np.float32)
+    k = rng.integers(0, 60, rows).astype(np.int32)
+    temp = rng.choice(np.array([0, 0.5, 1], np.float32), rows)
+    b, tokens, probs = dev(gpu, big), gpu.empty((rows,), np.int32), gpu.empty((rows,), np.float32)
+    uu, kk, tt = dev(gpu, u), dev(gpu, k), dev(gpu, temp)
+    d = pf.SampleDesc(TYPE["bf16"], V, stride, 1.0, 0, 1.0, 0, tt.ptr, kk.ptr, None, None)
+    gpu.check(pf.lib().pf_sample_rows(gpu.h, C.byref(d), C.c_void_p(b.ptr), C.c_void_p(uu.ptr), rows, C.c_void_p(tokens.ptr),
+                                      C.c_void_p(probs.ptr)), "pf_sample_rows")
+    tokens, probs = tokens.numpy(), probs.numpy()
+    f = R.from_bits(x, "bf16")
+    for i in list(range(0, rows, 61)) + list(range(rows - 520, rows, 13)):
+        token, prob = S.sample(f[i % 20], u[i], temp[i], int(k[i]))
+        assert tokens[i] == token and abs(probs[i] - prob) <= 2.0 ** -23 * prob + 2.0 ** -44, i
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V,stride", [(16384, 16384), (16385, 16386), (24001, 24003), (32761, 32763), (32768, 32768), (32769, 32771)])
+def test_sample_around_one_workgroup(gpu, t, V, stride):
+    """Rows of 16 and of 32 tokens a thread, and the first that take two launches."""
+    for kind in ("zipf", "flat"):
+        sample_case(gpu, logits_of(np.random.default_rng(V), 2, V, t, kind), t, U, SETTINGS[:10], stride)
+
+
 def test_sample_equal_tails(gpu):
     """Far below the largest logit a row's weight lies in equal ones, which fp32 rounds alike: a weight 2^-o of the largest's,
     o up to 32, is off by half a step of o, ln 2 2^-20, and by what exp2 is, 2^-23."""
