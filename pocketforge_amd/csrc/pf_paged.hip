@@ -39,6 +39,11 @@ __host__ __device__ constexpr int paged_waves(int act, int ct, int dp, int nt) {
 // 128: 94 MB in 24 us; one round of workgroups with up to 9 tiles a wave, each a memory
 // round trip, the codes' way to bf16 and three products per piece of the rows.
 // One context of 700 keys: 5.8 us and the join's 3.5, both latency.
+//
+// 4-bit rows are a quarter of the bytes for the same products, after conversions of
+// two codes an instruction: 64 contexts of 4100 to 16000 keys, 16 heads of 128 over
+// 4: 349 MB in 70 us, 5.0 TB/s, vector units issuing 53% of the time, matrix units busy
+// 26%; the 16 verify passes: 50 MB in 19 us, nine tiles a wave one after another.
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
 __global__ __launch_bounds__(64 * W, paged_waves(ACT, CT, DP, NT)) void k_paged_attn(PagedArgs a) {
     // Weights over int8 rows take the rows' scales, whose range fp16 does not
@@ -480,7 +485,7 @@ static void paged_dim(hipStream_t st, const PageSplit& u, const PagedArgs& a) {
 // (PG_JOIN4; one context of 700, 16 heads: 9.5 us cut, 7.5 uncut), and a third
 // workgroup on each compute unit, which the registers allow, keeps more bytes
 // under way where a wave has many of them (PG_LONG or more; 64 contexts of up to
-// 16000: 72 us with three, 78.5 with two; two of 120000, 6 a wave: 21 and 19).
+// 16000: 72 us with three, 78.5 with two; two of 120000 and 64000, 6 a wave: 21 and 19).
 constexpr uint32_t PG_CUS = 256, PG_JOIN = 5, PG_JOIN4 = 10, PG_JOIN_ROWS = 512, PG_LONG = 24;
 struct PageShares {
     uint32_t chunk = 1, waves = 4;
