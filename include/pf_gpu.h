@@ -380,7 +380,10 @@ typedef struct {
 
 /* tokens [rows]; probs [rows] (may be NULL): the token's share of what stayed
  * (1 where the temperature is 0, 0 for a row without tokens).  Rows may start
- * anywhere that is a multiple of their type's size. */
+ * anywhere that is a multiple of their type's size.  Asynchronous on the
+ * context's stream; rows of over 32768 tokens list their largest in its scratch
+ * (64 MiB at most), and only a call that needs more of it than it has
+ * allocates. */
 pf_status pf_sample_rows(pf_ctx* ctx, const pf_sample_desc* desc, const void* logits_dev, const float* u_dev,
                          uint32_t rows, int32_t* tokens_dev, float* probs_dev);
 
