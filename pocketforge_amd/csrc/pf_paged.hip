@@ -42,7 +42,7 @@ __host__ __device__ constexpr int paged_waves(int act, int ct, int dp, int nt) {
 //
 // 4-bit rows are a quarter of the bytes for the same products, after conversions of
 // two codes an instruction: 64 contexts of 4100 to 16000 keys, 16 heads of 128 over
-// 4: 349 MB in 70 us, 5.0 TB/s, vector units issuing 53% of the time, matrix units busy
+// 4: 349 MB in 73 us, 4.8 TB/s, vector units issuing 53% of the time, matrix units busy
 // 26%; the 16 verify passes: 50 MB in 19 us, nine tiles a wave one after another.
 template <int ACT, int CT, int DP, int NT, bool EXACT, int W>
 __global__ __launch_bounds__(64 * W, paged_waves(ACT, CT, DP, NT)) void k_paged_attn(PagedArgs a) {

@@ -511,6 +511,32 @@ def test_sample_largest_vocabulary(gpu, kind):
         sample_case(gpu, x, "f32", [0.2, 0.8, 0.9999], [s])
 
 
+def test_two_contexts_at_once(gpu):
+    """Calls of two contexts under way together, each with its own scratch and stream: what each alone gives."""
+    rng = np.random.default_rng(15)
+    other = pf.Context(0)
+    rot = [pf.Rotary(c, 64, interleaved=False) for c in (gpu, other)]
+    want, runs = [], []
+    for i, c in enumerate((gpu, other)):
+        x, u = dev(c, logits_of(rng, 40, 40000, "bf16")), dev(c, rng.random(40).astype(np.float32))
+        y, p = dev(c, rng.standard_normal((300, 6, 64)).astype(np.float32)), dev(c, np.arange(300, dtype=np.int32) * 977)
+        out = c.empty((40,), np.int32), c.empty((40,), np.float32), c.empty((300, 6, 64), np.float32)
+        a, b = c.sample_rows(x, u, temperature=0.9, top_p=0.97)
+        want.append((a.numpy(), b.numpy(), rot[i].apply(y, p).numpy()))
+        runs.append((c, rot[i], x, u, y, p, out))
+    for _ in range(30):
+        for c, r, x, u, y, p, out in runs:
+            c.sample_rows(x, u, temperature=0.9, top_p=0.97, out=out[:2])
+            r.apply(y, p, out=out[2])
+    for (c, _, _, _, _, _, out), w in zip(runs, want):
+        c.synchronize()
+        for a, b in zip(out, w):
+            np.testing.assert_array_equal(a.numpy(), b)
+    for r in rot:
+        r.close()
+    other.close()
+
+
 def test_sample_refusals(gpu):
     L = pf.lib()
     x, u, o, p = gpu.empty((4, 100), np.float32), dev(gpu, np.zeros(4, np.float32)), gpu.empty((4,), np.int32), gpu.empty((4,), np.float32)
