@@ -147,6 +147,7 @@ struct Setting {
     uint32_t k;                   // 0: off
     double scale, p, least;       // log2(e) / T; p >= 1: off; min_p in steps, 0: off
     float to_bin, hi, lo;
+    float far;                    // distance to the largest at which nothing weighs any more
     bool plain;
     bool few;                     // top-k alone decides how far to look: no sums over the row
     __device__ __forceinline__ void of(const SampleArgs& a, uint32_t row) {
@@ -173,10 +174,15 @@ struct Setting {
     __device__ __forceinline__ void fp32() {
         hi = (float)scale;
         lo = (float)(scale - (double)hi);
+        far = -1024.0f / hi;
         plain = max < INFINITY && hi > 1e-30f && hi < 1e30f;
     }
+    // (1024 octaves and more, masked tokens among them, are 1024: beside a small
+    // temperature's hi a larger distance's product with lo would be an infinity, of
+    // either sign)
+    __device__ __forceinline__ float distance32(float l) const { return fmaxf(l - max, far); }
     __device__ __forceinline__ float octaves32(float l) const {
-        const float d = fmaxf(l - max, -3.4028234663852886e38f);       // (masked: no weight)
+        const float d = distance32(l);
         return fmaf(d, hi, d * lo);
     }
     // 2^43 2^x to the nearest whole number: 2^x = 2^n e^(f ln 2) with |f| <= 1/2, the
@@ -870,7 +876,7 @@ struct Tail {
     // (the exponent's product in two pieces: 16-bit logits have few values, whose
     // roundings would add up)
     __device__ __forceinline__ uint32_t weight(float x) const {
-        const float d = x - s.max, o = d * s.hi, more = fmaf(d, s.lo, fmaf(d, s.hi, -o));
+        const float d = s.distance32(x), o = d * s.hi, more = fmaf(d, s.lo, fmaf(d, s.hi, -o));
         const float w = __builtin_amdgcn_exp2f(o);
         return (uint32_t)(fmaf(w, more * 0.693147181f, w) * unit);
     }

@@ -374,6 +374,26 @@ def test_sample_settings_of_all_rows(gpu):
     assert a.numpy().tolist() == [S.sample(x[i].astype(np.float64), 0.8, temperature=1.1, top_k=max(0, int(k[i])))[0] for i in range(7)]
 
 
+# temperatures at which log2(e) / T has fp32 pieces far above 1, of either sign
+NEARLY_GREEDY = [dict(temperature=t) for t in (1e-6, 8e-8, 4e-8, 1e-8, 1e-9, 1e-10, 2e-10, 1e-12, 1e-15, 1e-20, 1e-30)]
+NEARLY_GREEDY += [dict(temperature=1e-10, top_p=0.6), dict(temperature=1e-10, min_p=0.3), dict(temperature=1e-10, top_k=2000)]
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [100, 5003, 16384, 32768, 40001, 130560])
+def test_sample_nearly_greedy(gpu, t, V):
+    """Small temperatures beside masked tokens (-infinity, NaN, the type's lowest value) and what lies past a row's end:
+    none of them weighs anything; of equal largest logits each weighs the same."""
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((5, V)).astype(np.float32)
+    x[:, ::3] = -np.inf
+    x[1, 1::5] = np.nan
+    x[2, 2::3] = R.from_bits(R.to_bits(np.float32(-3.3e38 if t != "f16" else -65504), t), t)
+    for r, n in ((1, 1), (2, 2), (3, 5), (4, 40)):              # this many largest logits, all equal
+        x[r, 1 + 3 * rng.permutation(V // 3 - 1)[:min(n, V // 6)]] = 6.5
+    sample_case(gpu, R.to_bits(x, t), t, [0.0, 0.3, 0.52, 0.56, 0.8, 1 - 2.0 ** -24], NEARLY_GREEDY)
+
+
 def test_sample_many_rows(gpu):
     """More rows than are taken at a time, with settings of their own."""
     rng = np.random.default_rng(12)
