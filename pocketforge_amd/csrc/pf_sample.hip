@@ -1110,10 +1110,14 @@ __device__ __forceinline__ void pick_token(const SampleArgs& a, PickLds& m, uint
                 done = q.all > 0;
                 kept = back(q.all);
                 if (done && p_below) {
+                    // (to either side: these weights' sum is not the slices' to the last bit)
                     const uint64_t w = reach(kept);
                     if (w > p.all) {
                         done = q.place(to(w), f);
                         kept = min(kept, back(f.upto));
+                    } else {
+                        done = p.place(w, false, f);
+                        kept = min(kept, f.upto);
                     }
                 }
                 if (done && m_below) kept = min(kept, back(q.least));

@@ -394,6 +394,51 @@ def test_sample_nearly_greedy(gpu, t, V):
     sample_case(gpu, R.to_bits(x, t), t, [0.0, 0.3, 0.52, 0.56, 0.8, 1 - 2.0 ** -24], NEARLY_GREEDY)
 
 
+def masses(l):
+    """Float64 logits' tokens in their order and cumulative weights (extended precision, the largest logit's 1) at temperature 1."""
+    order = np.lexsort((np.arange(len(l)), -l))
+    return order, np.cumsum(np.exp(l[order] - l[order[0]]).astype(np.longdouble))
+
+
+def kept_within(upto, top_p, off):
+    """The least and the largest mass that top_p may keep where the row's is known to `off` of itself."""
+    p = np.longdouble(np.float32(top_p))
+    at = [np.searchsorted(upto, p * upto[-1] * (1 + s * off)) for s in (-1, 1)]
+    return upto[at[0]], upto[min(at[1], len(upto) - 1)]
+
+
+@pytest.mark.parametrize("V,tail", [(16384, 4.0), (16384, 6.5), (32768, 5.0)])
+def test_sample_border_where_the_list_ends(gpu, V, tail):
+    """top_p whose border is the last of the listed tokens to fp32's last bit.  A thread of a row of one launch has one of
+    64 large logits of its wave, so the 41st of these (the 41 lanes that c = 64 (1 - e^(-1040 / 1024)) + 1 counts) is the
+    first listed value's bound in each of the 16 waves; below come the other 23 lanes' and equal ones, whose weights fp32
+    rounds alike.  Whatever side rounding puts the border on, what stays is top_p of the row's weight to 2^-19 of it, and
+    a token more."""
+    off = 2.0 ** -19
+    rows, ps, known = [], [], []
+    for i in range(64):
+        x = np.full((V // 4, 4), -tail - i / 37, np.float32)
+        for t in range(1024):
+            x[t, (t * 7) % 4] = 2 - (t % 64) / 64
+        x = x.reshape(-1)
+        order, upto = masses(x.astype(np.float64))
+        p = np.float32(upto[41 * 16 - 1] / upto[-1])
+        rows += 7 * [x]
+        known += 7 * [(order, upto)]
+        ps += [np.float32(p + k * np.spacing(p)) for k in range(-3, 4)]
+    print(f"sample border V {V} tail {tail}", flush=True)
+    b, pp = dev(gpu, np.stack(rows)), dev(gpu, np.array(ps, np.float32))
+    for u in (0.0, 0.5, 0.9, 0.99, 1 - 2.0 ** -24):
+        tokens, probs = (a.numpy() for a in gpu.sample_rows(b, dev(gpu, np.full(len(rows), u, np.float32)), top_p=pp))
+        for i, (order, upto) in enumerate(known):
+            least, most = kept_within(upto, ps[i], off)
+            at = int(np.flatnonzero(order == tokens[i])[0])
+            w = upto[at] - (upto[at - 1] if at else 0)
+            # (a probability rounds to fp32; cumulative weights are known to off as well)
+            assert w / most * (1 - off - 2.0 ** -24) <= probs[i] <= w / least * (1 + off + 2.0 ** -24), (i, u, tokens[i], probs[i], w / most, w / least)
+            assert upto[at] >= u * least * (1 - off) and upto[at] - w <= u * most * (1 + off), (i, u, tokens[i])
+
+
 def test_sample_many_rows(gpu):
     """More rows than are taken at a time, with settings of their own."""
     rng = np.random.default_rng(12)
