@@ -853,8 +853,10 @@ struct Listed {
     }
 };
 
-// What a row has below its listed tokens, in weights beside `bound`'s in steps of
-// 2^-30 or finer: a border or a token in flat rows.  One compute unit goes through the row:
+// What a row has below its listed tokens, in weights beside `bound`'s, to the nearest
+// of steps of 2^-42 of it (of 2^20 tokens far below it no more than 2^-23 is lost, and
+// the bound's own token stays; steps of 2^-30, all that 32 bits hold, would lose
+// 2^-15 of a row with 16 listed tokens): a border or a token in flat rows.  One compute unit goes through the row:
 // once for a histogram by value, kept 32 times so that a pair of lanes has one in
 // LDS banks of its own, and once for the tokens of the bin; these again by a finer
 // histogram, so that only a few have to be put in order, or all are equal.  Bound by
@@ -869,16 +871,18 @@ struct Tail {
     const Setting& s;
     PickLds& m;
     const float bound;
-    float unit, per_bin;          // weights to steps; values to bins
-    double by;                    // steps of 2^43 to these
+    float per_bin;                // values to bins
+    double unit, by;              // weights to steps; steps of 2^43 to these
     uint64_t all, least = 0;      // of all; of those that weigh min_p
 
     // (the exponent's product in two pieces: 16-bit logits have few values, whose
     // roundings would add up)
-    __device__ __forceinline__ uint32_t weight(float x) const {
+    __device__ __forceinline__ uint64_t weight(float x) const {
         const float d = s.distance32(x), o = d * s.hi, more = fmaf(d, s.lo, fmaf(d, s.hi, -o));
         const float w = __builtin_amdgcn_exp2f(o);
-        return (uint32_t)(fmaf(w, more * 0.693147181f, w) * unit);
+        // (below 2^52, and added to it whole in the last place)
+        const double y = fma((double)fmaf(w, more * 0.693147181f, w), unit, 4503599627370496.0);
+        return __builtin_bit_cast(uint64_t, y) - 0x4330000000000000ull;
     }
     // 0 .. TAIL_BINS - 1 (and what is left behind the point, up to the last); never falls as x falls
     __device__ __forceinline__ float place_of(float x) const { return __builtin_amdgcn_fmed3f((bound - x) * per_bin, 0.0f, TAIL_BINS - 0.001f); }
@@ -888,25 +892,27 @@ struct Tail {
         : r(a, row), s(s), m(m), bound(bound) {
         const uint32_t t = threadIdx.x;
         const float o = floorf(s.octaves32(bound));
-        unit = __builtin_amdgcn_ldexpf(1.0f, 30 - (int)o);
-        by = exp2(-13.0 - (double)o);
+        unit = exp2(42.0 - (double)o);
+        by = exp2(-1.0 - (double)o);
         per_bin = s.hi * (TAIL_BINS / TAIL_OCTAVES);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < TAIL_BINS * TAIL_COPIES / PICK; i++) m.wide[t + i * PICK] = 0;
         __syncthreads();
-        const uint32_t some = s.least > 0.0 ? (uint32_t)fmin(s.least * by, 4294967295.0) : ~0u;
+        // (min_p's weight, where it lies below the bound's)
+        const bool lightest = s.least > 0.0 && s.least * by < 8796093022208.0;
+        const uint64_t some = lightest ? (uint64_t)(s.least * by) : 0;
         uint64_t* own = m.wide + t % TAIL_COPIES;
         // (no branch: a masked token weighs nothing, nor does a listed one here)
         const auto add = [&](float x) {
-            const uint32_t w = x < bound ? weight(x) : 0;
+            const uint64_t w = x < bound ? weight(x) : 0;
             atomicAdd((unsigned long long*)&own[bin(x) * TAIL_COPIES], (unsigned long long)w);
             return w;
         };
-        if (some == ~0u) r.template each<PICK>([&](float x, int32_t) { add(x); });
+        if (!lightest) r.template each<PICK>([&](float x, int32_t) { add(x); });
         else
             r.template each<PICK>([&](float x, int32_t) {
-                const uint32_t w = add(x);
+                const uint64_t w = add(x);
                 least += w >= some ? w : 0;
             });
         __syncthreads();
@@ -977,7 +983,7 @@ struct Tail {
 #pragma unroll
         for (int i = 0; i < (int)(MOST / PICK); i++) {
             if (t + i * PICK >= n) continue;
-            const uint32_t w = weight(x[i]);
+            const uint64_t w = weight(x[i]);
             fine[i] = min((uint32_t)((place_of(x[i]) - (float)b) * (float)BINS), (uint32_t)BINS - 1);
             if (w) atomicAdd((unsigned long long*)&m.wide[fine[i]], (unsigned long long)w);
         }

@@ -439,6 +439,32 @@ def test_sample_border_where_the_list_ends(gpu, V, tail):
             assert upto[at] >= u * least * (1 - off) and upto[at] - w <= u * most * (1 + off), (i, u, tokens[i])
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_sample_light_tail(gpu, t):
+    """A million tokens of 2^-13 to 2^-33 of the largest's weight, below 16 that a slice lists (four lanes of each of its
+    waves, and c = 64 (1 - e^(-1700 / 128 / 256)) + 1 = 4): together a third of the row.  What stays is known to 2^-19."""
+    V, E, off = 1 << 20, 4 if t == "f32" else 8, 2.0 ** -19
+    rng = np.random.default_rng(31)
+    x = (1 - np.log(2) * rng.uniform(13, 33, V)).astype(np.float32)
+    x[[E * (64 * w + i) for w in range(4) for i in range(4)]] = 1
+    b = R.to_bits(x, t)
+    order, upto = masses(R.from_bits(b, t).astype(np.float64))
+    total = upto[-1]
+    print(f"sample light tail {t} mass {float(total)}", flush=True)
+    for settings, kept in ((dict(), (total, total)), (dict(top_p=0.95), kept_within(upto, 0.95, off))):
+        least, most = kept
+        for u in (0.0, 0.5, 0.8, 0.9, 0.99):
+            uu = dev(gpu, np.array([u], np.float32))
+            tokens, probs = (a.numpy() for a in gpu.sample_rows(dev(gpu, b[None]), uu, **settings))
+            at = int(np.flatnonzero(order == tokens[0])[0])
+            w = upto[at] - (upto[at - 1] if at else 0)
+            # (and the token's weight to half a step of 2^-43)
+            tol = w / total * (off + 2.0 ** -24) + 2.0 ** -44
+            assert w / most - tol <= probs[0] <= w / least + tol, (settings, u, tokens[0], probs[0], w / most)
+            u = float(np.float32(u))
+            assert upto[at] >= u * least * (1 - off) and upto[at] - w <= u * most * (1 + off), (settings, u, tokens[0])
+
+
 def test_sample_many_rows(gpu):
     """More rows than are taken at a time, with settings of their own."""
     rng = np.random.default_rng(12)
