@@ -361,8 +361,8 @@ pf_status pf_pages_compact(pf_pages* p, uint32_t* moved);
  * A logit of -infinity or NaN is masked; of infinities the infinities alone
  * weigh.  A row without any other gives -1.
  * The largest few weights of a row, a thousand or those of its top-k, are held
- * in steps of 2^-43 and their sums are exact; the others' are of fp32, off by
- * 2^-20 of what stays at most (of many equal ones; 2^-24 of different ones).
+ * in steps of 2^-43 and their sums are exact; the others' are of fp32, and
+ * their sums off by less than 2^-19 of what stays.
  * The same call gives the same tokens.  Of the same row among more or fewer
  * others these last sums may differ by their rounding. */
 typedef struct {

@@ -22,11 +22,14 @@
 // 2^20 tokens of up to 2^43 fit 64 bits, and what a step leaves of 2^20 sums is
 // 2^-24 of the largest weight, what sums of fp32 would lose of the first few.
 // The others', each below a thousandth of the row's or so, are fp32's: in fp64 they
-// would be most of a slice's time.  A thread adds its own 8 to 32 of them, and these
-// sums are added as whole numbers.  An exponent o is off by half a step, 2^-21 for
-// o in 8 .. 16, a weight by ln 2 times that and by exp2's 2^-23: of 2^20 equal
-// ones 2^-o of the largest's this is 2^-20 of all at most, of different ones it
-// averages out.
+// would be most of a slice's time.  A thread adds its own 16 or 32 of them, two by two
+// within a chunk, and these sums are added as whole numbers.  Where o octaves lie
+// between a weight and the largest, the logits' difference rounds and its product with
+// the scale does, by 2^-24 o each; a weight is off by ln 2 times that and by exp2's
+// 2^-23, a thread's sum by nine additions' 2^-24.  2^20 tokens that far down weigh
+// r = 2^(20 - o) of the largest, so that all is off by r / (1 + r) (1.39 o + 11) 2^-24,
+// which is 31.3 2^-24 at most (o = 16): less than 2^-19 of what stays.  (A slice's o
+// is from its own largest, of 8192 tokens, a one-launch row has 2^15: 25 2^-24.)
 #include "pf_attend.h"
 #include "pf_context.h"
 
@@ -170,11 +173,11 @@ struct Setting {
     __device__ __forceinline__ double octaves(float l) const {
         return l == max ? 0.0 : fmax(((double)l - (double)max) * scale, -60.0);
     }
-    // the same in fp32, where `plain`: off by 2^-19 at most where weights reach, to either side
+    // the same in fp32, where `plain`: off by 2^-23 of itself at most, to either side
     __device__ __forceinline__ void fp32() {
         hi = (float)scale;
         lo = (float)(scale - (double)hi);
-        far = -1024.0f / hi;
+        far = -1024.0f * __builtin_amdgcn_rcpf(hi);
         plain = max < INFINITY && hi > 1e-30f && hi < 1e30f;
     }
     // (1024 octaves and more, masked tokens among them, are 1024: beside a small
@@ -265,6 +268,16 @@ __device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
 }
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return lane64(wave_scan64(v), 63); }
 
+// Two by two: the sum of eight rounds three times, not seven.
+template <int N>
+__device__ __forceinline__ float sum_pairs(float (&v)[N]) {
+#pragma unroll
+    for (int w = 1; w < N; w *= 2)
+#pragma unroll
+        for (int i = 0; i + w < N; i += 2 * w) v[i] += v[i + w];
+    return v[0];
+}
+
 // A wave's c-th largest of its lanes' values, to 16 bits (the next lower such
 // value), as an integer that rises with it; 0 where fewer than c are above -infinity.
 __device__ __forceinline__ uint32_t nth_of_wave(float v, uint32_t c) {
@@ -350,20 +363,21 @@ __global__ __launch_bounds__(256) void k_sample_slice(SampleArgs a) {
         // a number picks one
         const float above = fmaxf(bound, -3.4028234663852886e38f);
         uint32_t hits = 0;
-        // The weights of the others in fp32, exponents too: the sum of a thousand different
-        // ones is off by some 2^-24 of itself, and it is a small part of the row's where that
-        // sum is used.
+        // (the others' weights in fp32)
         s.fp32();
         float rest = 0.0f;
 #pragma unroll
-        for (int n = 0; n < N; n++)
+        for (int n = 0; n < N; n++) {
+            float w[E];
 #pragma unroll
             for (int i = 0; i < E; i++) {
                 const bool hit = x[n][i] >= above;
                 hits |= (hit ? 1u : 0u) << (n * E + i);
                 s_x[n * E + i][t] = x[n][i];
-                if (!s.few) rest += __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
+                if (!s.few) w[i] = __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
             }
+            if (!s.few) rest += sum_pairs(w);
+        }
         const uint32_t upto = wave_scan((uint32_t)__popc(hits));
         uint32_t at = 0;
         if ((t & 63) == 63) at = atomicAdd(&s_listed, upto);
@@ -1231,13 +1245,16 @@ __global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
         uint32_t hits = 0;
         float others = 0.0f;
 #pragma unroll
-        for (int n = 0; n < N; n++)
+        for (int n = 0; n < N; n++) {
+            float w[E];
 #pragma unroll
             for (int i = 0; i < E; i++) {
                 const bool hit = x[n][i] >= above;
                 hits |= (hit ? 1u : 0u) << (n * E + i);
-                if (!s.few) others += __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
+                if (!s.few) w[i] = __builtin_amdgcn_exp2f(hit ? -INFINITY : s.octaves32(x[n][i]));
             }
+            if (!s.few) others += sum_pairs(w);
+        }
         if (!s.few) {
             rest = (uint64_t)((double)others * STEPS);
             if (!s.plain) {

@@ -465,6 +465,36 @@ def test_sample_light_tail(gpu, t):
             assert upto[at] >= u * least * (1 - off) and upto[at] - w <= u * most * (1 + off), (settings, u, tokens[0])
 
 
+def test_sample_equal_tails_below_lists(gpu):
+    """Thousands of equal tokens o = 9 to 13 octaves below the largest, with logits, temperatures and sums that round alike
+    for each, below 41 listed ones of each wave (test_sample_border_where_the_list_ends) that lie as little above as 16
+    bits tell.  The difference's and the product's rounding are ln 2 2^-24 o each, exp2's 2^-23; of a thread's eight chunks
+    of four, whose own sums are exact, the sums of 3, 5, 6 and 7 round, 21 / 8 2^-24, and in 41 threads of 64, whose last
+    chunk has three, the last two, (21 4 + 3 + 31) / 31: 3.4 on the average.  What is not in the tail is exact, the
+    probability rounds once more."""
+    V = 32768
+    cases = [(6.903881072998047, 0.5513023138046265, 2.8222405910491943), (3.1673521995544434, 0.5426825881004333, -0.8532230854034424),
+             (6.047861099243164, 1.0479786396026611, -1.9790167808532715), (8.076173782348633, 0.5354180932044983, 3.9715540409088135),
+             (7.283297538757324, 0.5564096570014954, 3.1821577548980713), (5.566736221313477, 0.5240152478218079, 1.5442888736724854),
+             (2.0830864906311035, 1.264405369758606, -6.6693010330200195), (0.5012397766113281, 1.1914342641830444, -7.728212833404541)]
+    x = np.zeros((len(cases), V), np.float32)
+    for i, (top, T, low) in enumerate(cases):
+        u = np.array([low], np.float32).view(np.uint32)
+        x[i] = low
+        x[i, [4 * (7 * 1024 + t) for t in range(1024) if t % 64 < 41]] = (u + (1 << 16) & 0xFFFF0000 if low > 0 else (u & 0xFFFF0000) - 1).view(np.float32)[0]
+        x[i, 0] = top
+    T = np.array([c[1] for c in cases], np.float32)
+    print("sample tails below lists", flush=True)
+    tokens, probs = (a.numpy() for a in gpu.sample_rows(dev(gpu, x), dev(gpu, np.zeros(len(cases), np.float32)), temperature=dev(gpu, T)))
+    for i in range(len(cases)):
+        l = x[i].astype(np.float64)
+        w = np.exp((l - l[0]) / float(T[i])).astype(np.longdouble)
+        share = float(w[x[i] == x[i, 1]].sum() / w.sum())
+        o = float(l[0] - l[1]) / float(T[i]) / np.log(2)
+        tol = (share * (2 * np.log(2) * o + 2 + 3.4) + 1) * 2.0 ** -24
+        assert tokens[i] == 0 and abs(probs[i] * w.sum() - 1) <= tol, (cases[i], probs[i], float(probs[i] * w.sum() - 1) * 2 ** 24, tol * 2 ** 24)
+
+
 def test_sample_many_rows(gpu):
     """More rows than are taken at a time, with settings of their own."""
     rng = np.random.default_rng(12)
