@@ -363,8 +363,9 @@ pf_status pf_pages_compact(pf_pages* p, uint32_t* moved);
  * The largest few weights of a row, a thousand or those of its top-k, are held
  * in steps of 2^-43 and their sums are exact; the others' are of fp32, and
  * their sums off by less than 2^-19 of what stays.
- * The same call gives the same tokens.  Of the same row among more or fewer
- * others these last sums may differ by their rounding. */
+ * The same row and settings give the same token, whatever other rows the call
+ * has; where the row starts at another place within 16 bytes these last sums
+ * may differ by their rounding. */
 typedef struct {
     int32_t type;              /* logits: PF_TYPE_F32, F16 or BF16 */
     uint32_t n_vocab;          /* 1 .. 2^20 */

@@ -1356,12 +1356,14 @@ extern "C" pf_status pf_sample_rows(pf_ctx* c, const pf_sample_desc* d, const vo
         return PF_OK;
     }
     // tokens of a thread of the slices' workgroups: 32, or 16 where a row has up to 8
-    // slices of 32 and all rows' are fewer than two for each compute unit (one row of 40000
-    // fp32 logits: 13.2 us, 15.3 with 32, 13.2 with 8; 64 of 40000: 15.2, 16.3 and 16.3).
+    // slices of 32 (one row of 40000 fp32 logits: 13.2 us, 15.4 with 32; 64 of them 15.5
+    // and 16.8, 512 41.0 and 43.5; 128 of 65536 bf16 ones 19.3 and 18.8, 512 46.4 and 46.2).
     // More slices cost the row's workgroup, that takes their lists together, more than
-    // they save (one row of 250000 bf16 logits: 15.4 us, 16.8 with 16, 21 with 8).
+    // they save (one row of 250000 bf16 logits: 15.4 us, 16.8 with 16, 21 with 8).  How
+    // many rows there are does not matter here, so that a row's sums, and its token, are
+    // the same among any others.
     const auto cut = [&](uint32_t tokens) { return (chunks + 256 * (tokens / chunk) - 1) / (256 * (tokens / chunk)); };
-    const uint32_t per = cut(32) <= 8 && (uint64_t)rows * cut(32) < 512 ? 16 : 32;
+    const uint32_t per = cut(32) <= 8 ? 16 : 32;
     a.slices = cut(per);
     a.room = a.slices <= 8 ? 512 : a.slices <= 16 ? 256 : 128;   // (1700 tokens in all, unevenly)
     // as many rows at a time as keep their lists in SAMPLE_SCRATCH

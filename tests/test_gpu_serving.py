@@ -495,6 +495,38 @@ def test_sample_equal_tails_below_lists(gpu):
         assert tokens[i] == 0 and abs(probs[i] * w.sum() - 1) <= tol, (cases[i], probs[i], float(probs[i] * w.sum() - 1) * 2 ** 24, tol * 2 ** 24)
 
 
+@pytest.mark.parametrize("t,V,stride", [("f32", 40000, 40000), ("bf16", 65536, 65536), ("f32", 33001, 33002), ("f16", 50001, 50003),
+                                        ("bf16", 20000, 20000), ("bf16", 100000, 100000)])
+def test_sample_rows_among_others(gpu, t, V, stride):
+    """A row's token and probability are the same, to the last bit, among many rows, among few and alone."""
+    rng = np.random.default_rng(V)
+    rows = 160
+    x = np.zeros((rows, stride), R.to_bits(np.zeros(1, np.float32), t).dtype)
+    x[::2, :V], x[1::2, :V] = (logits_of(rng, rows // 2, V, t, kind) for kind in ("zipf", "flat"))
+    # and equal tails, whose sums fp32 rounds all alike: 1300 tokens are listed
+    for i in range(0, rows, 4):
+        y = np.full(V, 1 - 7.5 - i / 97, np.float32)
+        y[rng.permutation(V)[:1300]] = -6
+        y[rng.integers(V)] = 1
+        x[i, :V] = R.to_bits(y, t)
+    b, u = dev(gpu, x), dev(gpu, (rng.random(rows) * (np.arange(rows) % 4 > 0)).astype(np.float32))
+    p = dev(gpu, rng.choice(np.array([1.0, 0.9, 0.97], np.float32), rows))
+    print(f"sample among others {t} {V}", flush=True)
+
+    def call(first, n):
+        tokens, probs = gpu.empty((n,), np.int32), gpu.empty((n,), np.float32)
+        d = pf.SampleDesc(TYPE[t], V, stride, 0.8, 0, 1.0, 0.0, None, None, p.ptr + 4 * first, None)
+        gpu.check(pf.lib().pf_sample_rows(gpu.h, C.byref(d), C.c_void_p(b.ptr + first * stride * x.itemsize), C.c_void_p(u.ptr + 4 * first), n,
+                                          C.c_void_p(tokens.ptr), C.c_void_p(probs.ptr)), "pf_sample_rows")
+        return tokens.numpy(), probs.numpy()
+
+    tokens, probs = call(0, rows)
+    for first, n in [(i, 1) for i in range(rows)] + [(0, 20), (20, 77), (97, 63)]:
+        a, q = call(first, n)
+        np.testing.assert_array_equal(a, tokens[first:first + n])
+        np.testing.assert_array_equal(q.view(np.uint32), probs[first:first + n].view(np.uint32))
+
+
 def test_sample_many_rows(gpu):
     """More rows than are taken at a time, with settings of their own."""
     rng = np.random.default_rng(12)
