@@ -305,11 +305,12 @@ pf_status pf_pages_append(pf_pages* p, const uint32_t* seqs, const uint32_t* row
  * quantized by KVCache::quantize_row (a row with an infinity or a NaN reads
  * back as NaN).  PF_TYPE_FP4: each block of 32 dims takes the smallest power of
  * two, 2^-125 .. 2^125, that brings its largest value to 7 or less, and its
- * values go to the nearest code (ties to even codes; over 6 to 6).  A block's
- * largest value may come out a fifth larger than it was or a seventh smaller;
- * fp16's above 57344 come out as 65536, an infinity where fp16 rows are read
- * back.  A block with an infinity or a NaN reads back as NaN.  Strides as in
- * pf_attn_desc; buffers of 16 bytes. */
+ * values go to the nearest code (ties to even codes; over 6 to 6).  Where that
+ * power is in range, a block's largest value may come out up to a fifth larger
+ * (from just above 5 powers to 6) or smaller (from 5 to 4); fp16's above 57344
+ * come out as 65536, an infinity where fp16 rows are read back.  A block with an
+ * infinity or a NaN reads back as NaN.  Strides as in pf_attn_desc; buffers of
+ * 16 bytes. */
 pf_status pf_pages_store(pf_pages* p, uint32_t layer, int32_t type, const void* k_dev, const void* v_dev,
                          uint32_t k_stride, uint32_t v_stride);
 /* pf_pages_store of a pass before its rotary positions: the key rows turned at

@@ -171,3 +171,17 @@ def test_reference_sample():
         token, prob = S.sample(l, u, **kw)
         assert token == order[at] and abs(prob - w[at] / sum(w)) < 1e-12
     assert S.sample(np.array([1, 3, 3.0]), 0.9, 0.0) == (1, 1.0) and S.sample(np.array([-np.inf, np.nan]), 0.5) == (-1, 0.0)
+
+
+def test_reference_bound_of_the_largest():
+    """A block's largest value comes out between four fifths (5 powers, a tie, go to 4) and below six fifths of itself (the
+    next value above 5 goes to 6), and no value is off by more than the block's power of two."""
+    x = np.zeros((3000, 32), np.float32)
+    x[:, 0] = np.geomspace(1, 64, 3000)
+    x[:3, 0] = 5, np.nextafter(np.float32(5), np.float32(6)), 7
+    x[:, 1:] = np.random.default_rng(3).uniform(-1, 1, (3000, 31)) * x[:, :1]
+    code, e = S.fp4_rows(x)
+    held = S.fp4_values(code, e, 32)
+    r = held[:, 0] / x[:, 0].astype(np.float64)
+    assert r.min() == r[0] == 0.8 and r.max() == r[1] < 1.2 and r[1] > 1.2 - 1e-6 and r[2] == 6 / 7
+    assert (np.abs(held - x) <= 2.0 ** (e.astype(np.float64) - 127)).all()
