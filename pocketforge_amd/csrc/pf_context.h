@@ -128,8 +128,11 @@ pf_status attn_desc_check(pf_ctx* c, const pf_attn_desc* d, AttnShape* s);
 // Which kernels a call takes, for tests that cover each of them (host only; not
 // part of the library's interface).  Prompts: query rows of a workgroup, parts of
 // the keys.  Pages (a pass of `rows` new rows of sequences of `lens`): waves of a
-// workgroup, key tiles of a share and of the longest sequence.
+// workgroup, key tiles of a share and of the longest sequence; `_of` pages of a
+// type, and also how many workgroups of 4 waves share a compute unit.
 extern "C" pf_status pf_test_prompt_plan(const pf_attn_desc* d, const uint32_t* q_lens, const uint32_t* k_lens,
                                          uint32_t n_seq, uint32_t* rows, uint32_t* parts);
+extern "C" pf_status pf_test_pages_plan_of(const pf_attn_desc* d, int32_t cache, const uint32_t* rows, const uint32_t* lens,
+                                           uint32_t n, uint32_t* waves, uint32_t* chunk, uint32_t* longest, uint32_t* held);
 extern "C" pf_status pf_test_pages_plan(const pf_attn_desc* d, const uint32_t* rows, const uint32_t* lens, uint32_t n,
                                         uint32_t* waves, uint32_t* chunk, uint32_t* longest);

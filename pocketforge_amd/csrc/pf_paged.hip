@@ -520,6 +520,7 @@ static void page_shares(const std::vector<uint32_t>& tiles, uint32_t longest, ui
 struct PagePlan {
     std::vector<uint32_t> tiles;
     uint32_t most = 0, longest = 0, keys = 0;   // rows, tiles and keys of a sequence at most
+    uint32_t held = 0;                          // workgroups of 4 waves on a compute unit
     PageShares shares;
 };
 static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc* d, int32_t ct, const AttnShape& s) {
@@ -535,7 +536,7 @@ static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc*
         rows += q.rows;
     }
     const uint64_t R = (uint64_t)n.most * (d->n_heads / d->n_kv_heads), per = (uint64_t)d->n_kv_heads * (R <= 16 ? 1 : (R + 31) / 32);
-    uint32_t held = (uint32_t)paged_waves(d->type, ct, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
+    uint32_t& held = n.held = (uint32_t)paged_waves(d->type, ct, d->head_dim <= 64 ? 64 : 128, R <= 16 ? 1 : 2);
     const bool fp4 = ct == PF_TYPE_FP4;
     if (fp4 && held == 3) {
         uint64_t all = 0;
@@ -547,19 +548,25 @@ static PagePlan paged_plan(const std::vector<PageSeq>& pass, const pf_attn_desc*
     if (held > 1) page_shares(n.tiles, n.longest, per, (uint64_t)PG_CUS * (held / 2), 8, join, &n.shares);
     return n;
 }
-extern "C" pf_status pf_test_pages_plan(const pf_attn_desc* d, const uint32_t* rows, const uint32_t* lens, uint32_t n,
-                                        uint32_t* waves, uint32_t* chunk, uint32_t* longest) {
+extern "C" pf_status pf_test_pages_plan_of(const pf_attn_desc* d, int32_t cache, const uint32_t* rows, const uint32_t* lens,
+                                           uint32_t n, uint32_t* waves, uint32_t* chunk, uint32_t* longest, uint32_t* held) {
     AttnShape s;
     if (pf_status st = attn_desc_check(nullptr, d, &s)) return st;
     return no_throw(nullptr, [&] {
         std::vector<PageSeq> pass;
         for (uint32_t i = 0; i < n; i++) pass.push_back({i, 0, rows[i], lens[i]});
-        const PagePlan plan = paged_plan(pass, d, d->type, s);
+        const PagePlan plan = paged_plan(pass, d, cache, s);
         *waves = plan.shares.waves;
         *chunk = plan.shares.chunk;
         *longest = plan.longest;
+        *held = plan.held;
         return (pf_status)PF_OK;
     });
+}
+extern "C" pf_status pf_test_pages_plan(const pf_attn_desc* d, const uint32_t* rows, const uint32_t* lens, uint32_t n,
+                                        uint32_t* waves, uint32_t* chunk, uint32_t* longest) {
+    uint32_t held;
+    return d ? pf_test_pages_plan_of(d, d->type, rows, lens, n, waves, chunk, longest, &held) : PF_ERR_ARG;
 }
 static pf_status paged_cut(pf_pages* p, const pf_attn_desc* d, const AttnShape& s) {
     PageSplit& u = p->cut;

@@ -7,6 +7,7 @@ import attention_ref as R
 import pocketforge_amd as pf
 import serving_ref as S
 import test_gpu_attention as A
+from test_serving_cpu import pages_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -232,6 +233,27 @@ def test_many_tiles_a_wave(gpu):
     y = R.from_bits(m.c.attention(0, dev(gpu, q)).numpy(), "bf16")
     for s in range(0, n, 9):
         want, tol = R.attend(R.from_bits(q[s:s + 1], "bf16"), *m.rows[s][0], R.visible(1, 1025), R.default_scale(128), "bf16")
+        R.check(y[s:s + 1], want, tol, f"sequence {s}")
+    m.c.close()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,held", [(62, 2), (63, 3)])
+def test_around_many_tiles(gpu, t, n, held):
+    """The last pass with two workgroups on a compute unit and the first with three (49152 tiles), its rule's choice asserted."""
+    G = 24
+    assert pages_plan(A.TYPE[t], pf.TYPE_FP4, G, G, 128, [1] * n, [1025] * n)[2] == held
+    m = Mirror(gpu, G, 128, 256, 4 + n, n, 1100, t=t)
+    m.append([0], [1024])
+    m.c.fork(0, list(range(1, n)))
+    for s in range(1, n):
+        m.rows[s] = list(m.rows[0])
+    m.append(list(range(n)), [1] * n)
+    q = R.rand(m.rng, (n, G, 128), t)
+    print(f"4 bits {t} {n} contexts of 1025", flush=True)
+    y = R.from_bits(m.c.attention(0, dev(gpu, q)).numpy(), t)
+    for s in range(0, n, 15):
+        want, tol = R.attend(R.from_bits(q[s:s + 1], t), *m.rows[s][0], R.visible(1, 1025), R.default_scale(128), t)
         R.check(y[s:s + 1], want, tol, f"sequence {s}")
     m.c.close()
 

@@ -185,3 +185,29 @@ def test_reference_bound_of_the_largest():
     r = held[:, 0] / x[:, 0].astype(np.float64)
     assert r.min() == r[0] == 0.8 and r.max() == r[1] < 1.2 and r[1] > 1.2 - 1e-6 and r[2] == 6 / 7
     assert (np.abs(held - x) <= 2.0 ** (e.astype(np.float64) - 127)).all()
+
+
+def pages_plan(t, cache, H, G, D, rows, lens):
+    """(waves of a workgroup, whether the keys are cut, workgroups on a compute unit) of a pass over pages of a type."""
+    d = pf.AttnDesc(t, H, G, D, 1, 0, 0, 0.0, 0, 0, 0, 0)
+    x = [C.c_uint32() for _ in range(4)]
+    a, b = ((C.c_uint32 * len(y))(*y) for y in (rows, lens))
+    assert pf.lib().pf_test_pages_plan_of(C.byref(d), cache, a, b, len(lens), *map(C.byref, x)) == 0
+    return x[0].value, x[1].value < x[2].value, x[3].value
+
+
+def test_plans_of_4_bit_pages():
+    """What 4-bit pages take otherwise than wider ones: a third workgroup on a compute unit from 24 tiles a wave of two on
+    (24 4 2 256 = 49152 tiles, 33 of each of 24 heads: 62 contexts are fewer, 63 more), and joins priced twice as high."""
+    bf, f32, i8, fp4 = pf.TYPE_BF16, pf.TYPE_F32, pf.TYPE_I8, pf.TYPE_FP4
+    for n, held in ((62, 2), (63, 3), (64, 3)):
+        assert pages_plan(bf, fp4, 24, 24, 128, [1] * n, [1025] * n) == (4, False, held)
+        assert pages_plan(bf, i8, 24, 24, 128, [1] * n, [1025] * n) == (4, False, 2)
+    many = [4100 + 187 * i for i in range(64)]
+    assert pages_plan(bf, fp4, 16, 4, 128, [1] * 64, many) == (4, True, 3)
+    assert pages_plan(bf, i8, 16, 4, 128, [1] * 64, many) == (4, True, 2)
+    assert pages_plan(pf.TYPE_F16, fp4, 16, 2, 128, [1, 1], [120000, 64000]) == (4, True, 2)
+    # two tiles of 16 rows: two workgroups, however many tiles
+    assert pages_plan(bf, fp4, 40, 2, 128, [1] * 64, [16000] * 64)[2] == 2
+    assert pages_plan(bf, fp4, 16, 16, 128, [1], [700]) == (8, False, 2) and pages_plan(bf, i8, 16, 16, 128, [1], [700]) == (4, True, 2)
+    assert pages_plan(bf, fp4, 16, 16, 128, [1], [4000])[1] and pages_plan(f32, fp4, 16, 16, 128, [5] * 16, [2100] * 16) == (8, False, 2)
