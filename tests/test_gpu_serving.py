@@ -192,6 +192,37 @@ def test_store_rotary(gpu, ct, t, interleaved, H, G, D, turn):
     rot.close()
 
 
+@pytest.mark.parametrize("t,ct", [("bf16", "f16"), ("f16", "bf16")])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("H,G,D,turn", [(4, 4, 64, 0), (16, 2, 128, 64), (6, 3, 80, 40), (1, 1, 16, 8)])
+def test_store_rotary_of_another_type(gpu, t, ct, interleaved, H, G, D, turn):
+    """16-bit rows into pages of the other 16-bit type, with positions (turned in fp32, rounded once) and without."""
+    rng = np.random.default_rng(H + D)
+    c = pf.PagedCache(gpu, 1, G, D, 12, 2, 90, 16, TYPE[ct])
+    rot = pf.Rotary(gpu, D, turn, interleaved, magnitude=1.25, **RAMP)
+    c.append([1], [21])
+    c.append([0, 1], [40, 7])
+    at = np.concatenate([np.arange(40), np.arange(21, 28)])
+    q, k, v = (R.rand(rng, (47, h, D), t) for h in (H, G, G))
+    print(f"store rotary {t} into {ct} interleaved {interleaved} H {H} G {G} D {D}", flush=True)
+    y = R.from_bits(c.store_rotary(0, rot, dev(gpu, q), dev(gpu, k), dev(gpu, v)).numpy(), t)
+    kw = dict(RAMP, magnitude=1.25)
+    want, size = S.turned(R.from_bits(q, t), at, turn or D, interleaved, **kw)
+    R.check(y, want.astype(np.float64), bound(want, size, t), "queries")
+    want, size = S.turned(R.from_bits(k, t), at, turn or D, interleaved, **kw)
+    new = np.r_[0:40, 61:68]
+    gk, gv = (g.numpy()[new] for g in c.gather(0, [0, 1]))
+    R.check(gk, want.astype(np.float64), bound(want, size, ct), "keys")
+    held = [R.from_bits(R.to_bits(R.from_bits(x, t).astype(np.float32), ct), ct) for x in (k, v)]
+    np.testing.assert_array_equal(gv, held[1])
+    c.store(0, dev(gpu, k), dev(gpu, v))
+    gk, gv = (g.numpy()[new] for g in c.gather(0, [0, 1]))
+    np.testing.assert_array_equal(gk, held[0])
+    np.testing.assert_array_equal(gv, held[1])
+    c.close()
+    rot.close()
+
+
 def test_store_rotary_in_place_and_refusals(gpu):
     """Queries of a fused row turned in place; and the calls that are refused, which change nothing."""
     H, G, D, n = 4, 2, 64, 9
