@@ -382,7 +382,10 @@ typedef struct {
 
 /* tokens [rows]; probs [rows] (may be NULL): the token's share of what stayed
  * (1 where the temperature is 0, 0 for a row without tokens).  Rows may start
- * anywhere that is a multiple of their type's size.  Asynchronous on the
+ * anywhere that is a multiple of their type's size.  A row whose border or token
+ * lies below its listed ones, a top_k above 1024, or a mask of a finite value (as
+ * the type's lowest) that leaves few tokens is right as well, and slower: one
+ * compute unit goes through that row again.  Asynchronous on the
  * context's stream; rows of over 32768 tokens list their largest in its scratch
  * (64 MiB at most), and only a call that needs more of it than it has
  * allocates. */

@@ -561,7 +561,8 @@ class Context:
         """A token from each row of logits [rows][n_vocab], by u [rows] (float32 in
         [0, 1)): (tokens int32, their probabilities float32).  Each setting is a
         number, or a device array of the rows' own (int32 for top_k, float32 for
-        the others).  With `out`, two arrays (the second may be None), the call is
+        the others).  top_k is off at 0 and from n_vocab on; an array's numbers below
+        0 are off too, a negative number is refused.  With `out`, two arrays (the second may be None), the call is
         asynchronous on the context's stream."""
         rows, V, stride = _matrix(logits, "logits", self)
         d = SampleDesc(_type(logits), V, stride, 1.0, 0, 1.0, 0.0)

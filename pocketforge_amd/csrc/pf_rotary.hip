@@ -137,10 +137,14 @@ struct Turn {
     }
 };
 
-// Past the caches: what a prompt's rows would leave in them costs the kernels that
-// follow their own (two batches in turn of 24 prompts of up to 700 rows turned into
-// 4-bit pages, and these read back: 32 us, 42 otherwise; with three batches, past
-// the 256 MB cache either way, 44 and 45; attention over the turned rows takes the same).
+// Past the caches: a prompt's rows would evict what the next calls read.  24 prompts of
+// up to 700 rows turned and stored into 4-bit pages, 1 / 2 / 3 / 4 batches in turn:
+// 20 / 20 / 20 / 29 us, 21 / 21 / 30 / 31 with plain stores; the pages read back as well 27.6 /
+// 27.6 / 33 / 39, 28 / 34 / 40 / 40.6; 8192 rows of 16 heads of 128, four in turn, 11.4 and 13.7.
+// A kernel that reads the turned rows at once pays a part of it back: prompt attention
+// after the store 71 / 71 / 78 / 82, 70 / 70 / 79 / 81; the 8192 rows turned again 25 and 23.
+// A decode step's few rows take the same either way (64 turned, stored and attended
+// over contexts of 300: 12.3 us).
 template <int T>
 __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
     if constexpr (T == PF_TYPE_F32) {

@@ -38,7 +38,10 @@ namespace pf {
 constexpr int BINS = 1024;
 constexpr float BIN_OCTAVES = 44.0f;   // of the weights, that the bins cover (the last one has the rest)
 constexpr uint32_t LIST = 2048;        // tokens that are sorted at once
-constexpr uint32_t FEW_K = 1024;       // top-k up to here needs no sums over the row
+// top-k up to here needs no sums over the row.  Beyond it a row lists no more tokens,
+// so its border takes the whole row (`Pick`), by one workgroup: one row of 130560 bf16
+// logits 94 us, 14 with a top-k of 1000; 5 of 16384 fp32 ones 28 and 11.
+constexpr uint32_t FEW_K = 1024;
 constexpr double STEPS = 8796093022208.0;   // 2^43
 constexpr double WHOLE = 6755399441055744.0;   // 2^52 + 2^51: what is added to it is whole, in its low bits
 
@@ -294,7 +297,7 @@ __device__ __forceinline__ uint32_t nth_of_wave(float v, uint32_t c) {
 // A slice: N chunks a thread.  The bound is the mean of the four waves' c-th
 // largest lanes: of n listed tokens over 256 threads a thread has one with the
 // probability 1 - e^(-n / 256), so c = 64 of that gives about n.  64 rows of 130560
-// bf16 logits: 17 MB in 10.7 us; some ten instructions and an exponential a token are
+// bf16 logits: 17 MB in 10 us; some ten instructions and an exponential a token are
 // half of it, the launch and the loads' round trip most of the rest.
 template <int T, int N>
 __global__ __launch_bounds__(256) void k_sample_slice(SampleArgs a) {
@@ -874,9 +877,9 @@ struct Listed {
 // once for a histogram by value, kept 32 times so that a pair of lanes has one in
 // LDS banks of its own, and once for the tokens of the bin; these again by a finer
 // histogram, so that only a few have to be put in order, or all are equal.  Bound by
-// that one compute unit: 25 us for each border or token in a row of 130560 bf16 logits
-// (drawn from a normal distribution, one row: 14 us without a tail, 50 at temperature
-// 1, 70 with top-p; the whole row instead, `Pick`, takes 133 and 160).
+// that one compute unit: 27 us for each border or token in a row of 130560 bf16 logits
+// (drawn from a normal distribution, one row: 14 us without a tail, 53 at temperature
+// 1, 72 with top-p; the whole row instead, `Pick`, takes 133 and 160).
 template <int T>
 struct Tail {
     static constexpr uint32_t MOST = 8192;   // tokens of a bin
@@ -1176,7 +1179,9 @@ __global__ __launch_bounds__(PICK) void k_sample_pick(SampleArgs a) {
 // A row of up to 32 tokens a thread, listed and picked by one workgroup, in one launch
 // (5 rows of 16384 fp32 logits, top-p: 10.3 us, 13.5 in two; 5 of 32000 bf16: 12.2 and
 // 13.3; 300 of 27000 fp32: 24.8 and 34).  Bound by one compute unit's instructions for
-// each token, then by a few barriers and LDS round trips a border, 1 us each.
+// each token, then by a few barriers and LDS round trips a border, 1 us each.  Its 16
+// waves leave a thread 128 registers, and 2 to 9 of a thread's values spill (12 to 40
+// bytes a lane; of k_sample_pick's 2 to 4).
 template <int T, int TOKENS>
 __global__ __launch_bounds__(PICK) void k_sample_row(SampleArgs a) {
     constexpr int E = Row<T>::E, N = TOKENS / E;
