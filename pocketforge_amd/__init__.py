@@ -867,12 +867,13 @@ class PagedCache:
         return lib().pf_pages_memory_usage(self.h)
 
     def close(self):
-        if self.h:
+        if self.h and self.ctx.h:               # (else its context is gone, and the memory goes with the process)
             lib().pf_pages_destroy(self.h)
-            self.h = None
+        self.h = None
 
     def __del__(self):
-        self.close()
+        if lib is not None:                     # (not where the program ends)
+            self.close()
 
 
 class Rotary:
@@ -905,12 +906,12 @@ class Rotary:
         return y
 
     def close(self):
-        if self.h:
+        if self.h and self.ctx.h:               # (else its context is gone, and the memory goes with the process)
             lib().pf_rotary_destroy(self.h)
-            self.h = None
+        self.h = None
 
     def __del__(self):
-        if lib is not None and self.ctx.h:      # (not where the program ends, or the context has)
+        if lib is not None:                     # (not where the program ends)
             self.close()
 
 

@@ -109,6 +109,26 @@ def test_calls_refused_by_the_binding():
             c.store_rotary(layer, rot, q, k, k, out=q)
 
 
+def test_closed_after_the_context(monkeypatch):
+    """A cache or a rotary handle that outlives its context does not reach into it."""
+    called = []
+
+    class Lib:
+        pf_pages_destroy = pf_rotary_destroy = staticmethod(lambda h: called.append(h))
+
+    monkeypatch.setattr(pf, "lib", Lib)
+    for kind in (pf.PagedCache, pf.Rotary):
+        for h, calls in ((None, []), (1234, [5678])):
+            x = kind.__new__(kind)
+            x.ctx, x.h = context(), 5678
+            x.ctx.h = h
+            del called[:]
+            x.close()
+            assert called == calls and x.h is None
+            x.close()
+            assert called == calls
+
+
 def test_reference_codes():
     """The search against the rule in bits, and ties."""
     rng = np.random.default_rng(0)
